@@ -470,6 +470,144 @@ WispError wisp_lm_head_forward(const wisp_half* final_norm, const wisp_half* lm_
                                WispErrCtx* err);
 
 /* ====================================================================== *
+ * 2d. A paged key/value cache for a batch of sequences (paged.cu,
+ *     paged_attn.cu, page_pool.cpp); no reference counterpart: the
+ *     reference decodes one sequence on one contiguous cache.
+ * ====================================================================== */
+typedef enum {
+    WISP_DTYPE_F32 = 0,
+    WISP_DTYPE_F16 = 1,
+    WISP_DTYPE_BF16 = 2,
+} WispDtype;
+
+/* One layer's pages: page p of the keys is k + p * page_stride elements,
+ * [page_size][n_kv_heads][head_dim] (a page is a slice of the contiguous
+ * cache's layout), the values the same.  fp16 or bf16; head_dim a multiple of
+ * 8 up to 256; page_size a multiple of 8; 16-byte aligned, page_stride a
+ * multiple of 8 and at least a page. */
+typedef struct WispKvPages {
+    void* k;
+    void* v;
+    size_t page_stride;
+    int n_pages, page_size, n_kv_heads, head_dim;
+    int dtype; /* WISP_DTYPE_F16 or WISP_DTYPE_BF16 */
+} WispKvPages;
+
+/* A batch's tokens, sequence after sequence.  Sequence s owns the tokens
+ * [q_start[s], q_start[s + 1]), the last ones of its kv_len[s] cached
+ * positions (its own tokens included): token i stands at position
+ * kv_len[s] - (q_start[s + 1] - i).  Position p lies in page
+ * table[s * table_stride + p / page_size].  All three arrays are on the
+ * device and are read there: no call synchronises, and a captured step may be
+ * replayed after they changed.  max_q: no sequence has more tokens (a bound
+ * for the choice of kernels).  A sequence with kv_len 0 (an unused slot) or
+ * with more tokens than positions has tokens that see nothing. */
+typedef struct WispTokenBatch {
+    const int* q_start; /* [n_seq + 1] */
+    const int* kv_len;  /* [n_seq] */
+    const int* table;   /* [n_seq][table_stride] */
+    int n_seq, n_tokens, max_q, table_stride;
+} WispTokenBatch;
+
+/* Rows of the batch's tokens: token t's head h starts at base + t * stride +
+ * h * head_dim elements.  16-byte aligned, stride a multiple of 8. */
+typedef struct WispRows {
+    void* base;
+    size_t stride;
+    int n_heads;
+    int dtype; /* WispDtype */
+} WispRows;
+
+/* Rotary positions.  Pair i of the window [offset, offset + dim) of a head is
+ * (x[i], x[i + dim/2]), or (x[2i], x[2i + 1]) when interleaved; it is turned by
+ * position * inv_freq[i] radians and scaled by gain.  inv_freq: device,
+ * [dim / 2] doubles; the angle is reduced in 64 bits, so positions of millions
+ * keep full 32-bit sines.  A scaled context is a matter of the frequencies
+ * (and gain).  dim a multiple of 16 (0: no rotation), offset of 8.
+ * positions: device [n_tokens], or NULL for the cache positions. */
+typedef struct WispRope {
+    const double* inv_freq;
+    const int* positions;
+    int dim, offset, interleaved;
+    float gain;
+} WispRope;
+
+/* q_out = rotated q; rotated k and v are stored at the tokens' positions of
+ * the pages.  q, k, v: one dtype; q_out: that dtype or the pages'.  q_out may
+ * be q itself.  A token without a position (an unused slot) stores nothing and
+ * its q_out row is zero; so does a token whose page number is outside the pool,
+ * with bit 0 of *status set.  status: one device word or NULL. */
+WispError wisp_rope_append(const WispRows* q, const WispRows* k, const WispRows* v,
+                           const WispRows* q_out, const WispKvPages* pages,
+                           const WispTokenBatch* batch, const WispRope* rope, int* status,
+                           cudaStream_t stream, WispErrCtx* err);
+
+/* out = softmax(scale q.K) V over the cached positions j <= i of each token's
+ * sequence, where window > 0 only those with i - j < window or j < sinks.  lse
+ * (optional, device [n_tokens][n_heads]): the log of the sum of exp(scale q.k).
+ * A row that sees nothing gets zeros and lse -infinity.  What a row does not
+ * see never reaches it, infinities and NaNs included.  q and out: fp32 (products
+ * to fp32 precision: the rows and weights are split into two 16-bit parts), or
+ * the pages' dtype; q.n_heads a multiple of n_kv_heads.
+ * wisp_prefix_attention: groups of consecutive sequences
+ * [groups[g], groups[g + 1]) whose first prefix_len[g] positions lie in the
+ * same pages: these are read once for all rows of the group (through the table
+ * row of its first sequence).  Device arrays [n_groups + 1] and [n_groups];
+ * sequences outside every group have no shared part.  The results are those of
+ * the plain call up to rounding.
+ * The workspace's first word is the call's status (wisp_moe_status reads it;
+ * bit 0: a page number outside the pool, its positions read as zeros; bit 1: a
+ * kv_len beyond the table, cut to it; bit 3: a bounded wait timed out). */
+size_t wisp_paged_attention_workspace_bytes(const WispKvPages* pages, const WispTokenBatch* batch,
+                                            int n_heads, int q_dtype, int n_groups);
+WispError wisp_paged_attention(const WispRows* q, const WispRows* out, float* lse,
+                               const WispKvPages* pages, const WispTokenBatch* batch, float scale,
+                               int window, int sinks, void* workspace, size_t workspace_bytes,
+                               cudaStream_t stream, WispErrCtx* err);
+WispError wisp_prefix_attention(const WispRows* q, const WispRows* out, float* lse,
+                                const WispKvPages* pages, const WispTokenBatch* batch,
+                                const int* groups, const int* prefix_len, int n_groups,
+                                float scale, int window, int sinks, void* workspace,
+                                size_t workspace_bytes, cudaStream_t stream, WispErrCtx* err);
+
+/* Pages src[i] -> dst[i] (host arrays, n pairs) in every layer: layer l's page
+ * p of the keys is k + l * layer_stride + p * page_stride elements.  All source
+ * pages are read as they were before the call: a page that is both a source and
+ * a destination, or twice a destination, is refused. */
+WispError wisp_pages_copy(const WispKvPages* pages, int n_layers, size_t layer_stride,
+                          const int* src, const int* dst, int n, cudaStream_t stream,
+                          WispErrCtx* err);
+
+/* Host-side owner of a pool's page numbers: which sequence holds which pages, shared pages
+ * counted.  Nothing here touches the device; moves that a call needs are queued and drained
+ * with wisp_page_pool_moves, to be given to wisp_pages_copy before the next kernel writes or
+ * reads the pages.  A queued move's source stays reserved until it is drained.  One thread at
+ * a time per pool. */
+typedef struct WispPagePool WispPagePool;
+WispPagePool* wisp_page_pool_create(int n_pages, int page_size, WispErrCtx* err);
+void wisp_page_pool_destroy(WispPagePool* pool);
+int wisp_page_pool_free_pages(const WispPagePool* pool);
+/* A new empty sequence; its id (>= 0), -1 on failure. */
+int wisp_page_pool_open(WispPagePool* pool, WispErrCtx* err);
+/* Make room for `length` positions (not fewer than the sequence has); positions from the
+ * present length on are about to be written, so a shared page among them is replaced by a copy
+ * of its own.  Fails with WISP_ERR_OOM, changing nothing, when pages run out. */
+WispError wisp_page_pool_extend(WispPagePool* pool, int seq, int length, WispErrCtx* err);
+/* Forget the positions from `length` on. */
+WispError wisp_page_pool_truncate(WispPagePool* pool, int seq, int length, WispErrCtx* err);
+/* A new sequence that shares all pages of `seq`; its id, -1 on failure. */
+int wisp_page_pool_fork(WispPagePool* pool, int seq, WispErrCtx* err);
+WispError wisp_page_pool_close(WispPagePool* pool, int seq, WispErrCtx* err);
+/* Renumber so that the pages in use are the first ones (queues the moves); refused while moves
+ * are queued.  The number of pages in use, -1 on failure. */
+int wisp_page_pool_compact(WispPagePool* pool, WispErrCtx* err);
+int wisp_page_pool_length(const WispPagePool* pool, int seq, WispErrCtx* err);
+/* The sequence's page numbers (at most cap); how many it has, -1 on failure. */
+int wisp_page_pool_pages(const WispPagePool* pool, int seq, int* pages, int cap, WispErrCtx* err);
+/* Drain up to cap queued moves; how many were written. */
+int wisp_page_pool_moves(WispPagePool* pool, int* src, int* dst, int cap);
+
+/* ====================================================================== *
  * 3. Engine ABI (reference: csrc/core/wisp_engine.h:472-543)
  * ====================================================================== */
 typedef struct WispEngine WispEngine;

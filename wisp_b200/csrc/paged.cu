@@ -1,0 +1,571 @@
+// paged.cu -- the paged cache's entry points: rotary positions with the append of k and v,
+// page copies, and the attention calls (argument checks, workspace, choice of kernels; the
+// kernels are in paged_plan.cu and paged_attn.cu).
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "internal.h"
+#include "paged.h"
+#include "paged_math.cuh"
+
+namespace wb {
+
+cudaError_t launch_paged_plan(const PagedArgs& A, cudaStream_t s);
+cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
+                              cudaStream_t s);
+cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s);
+int paged_attn_tile();
+int paged_attn_rw(int rows, bool split);
+int paged_attn_ctas(int hd);
+
+namespace {
+
+// ------------------------------------------------------------------------
+// Rotary positions and append.  CTA (token, block of heads): the token's sines and cosines go
+// to shared memory (the angle in turns is reduced in 64 bits, then sin and cos in 32), then
+// each thread turns 8 pairs (16 elements) or passes 8 elements on.
+// ------------------------------------------------------------------------
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+    const void *q, *k, *v;
+    void* q_out;
+    void *kp, *vp;
+    const int *q_start, *kv_len, *table, *positions;
+    const double* freq;
+    int* status;
+    size_t qs, ks, vs, qos, page_stride;
+    int n_seq, n_tokens, table_stride, n_pages, page_size, nh, nkv, hd;
+    int dim, off, interleaved, heads_per_cta;
+    float gain;
+};
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(p);
+        const float4 b = *(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = PMath<T>::unpack(u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *(reinterpret_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(PMath<T>::pack(v[0], v[1]), PMath<T>::pack(v[2], v[3]),
+                       PMath<T>::pack(v[4], v[5]), PMath<T>::pack(v[6], v[7]));
+    }
+}
+
+template <typename TI, typename TC, typename TQ>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs A) {
+    __shared__ float2 cs[128];  // (cos, sin) * gain of each pair
+    __shared__ int s_seq;
+    const int t = blockIdx.x, tid = threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tid == 0) s_seq = -1;
+    __syncthreads();
+    for (int s = tid; s < A.n_seq; s += kRopeThreads)
+        if (A.q_start[s] <= t && t < A.q_start[s + 1]) s_seq = s;
+    __syncthreads();
+    const int seq = s_seq;
+    int pos = -1, page = -1;
+    if (seq >= 0) {
+        const long long cap = (long long)A.table_stride * A.page_size;
+        pos = A.kv_len[seq] - (A.q_start[seq + 1] - t);
+        if (pos >= 0 && pos < cap) {
+            page = A.table[(size_t)seq * A.table_stride + pos / A.page_size];
+            if ((unsigned)page >= (unsigned)A.n_pages) page = -1;
+        }
+        if (page < 0 && pos >= 0 && tid == 0 && A.status) atomicOr(A.status, PG_BAD_PAGE);
+    }
+    const int half = A.dim / 2;
+    if (page >= 0) {
+        const int rp = A.positions ? A.positions[t] : pos;
+        for (int i = tid; i < half; i += kRopeThreads) {
+            const double turns = (double)rp * A.freq[i] * 0.15915494309189533577;
+            float s, c;
+            sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+            cs[i] = make_float2(c * A.gain, s * A.gain);
+        }
+    }
+    __syncthreads();
+    const size_t row = page >= 0 ? (size_t)page * A.page_stride +
+                                       (size_t)(pos % A.page_size) * A.nkv * A.hd
+                                 : 0;
+    // units of a head: its pairs by eights, then what passes through, by eights
+    const int pu = A.dim / 16, per = pu + (A.hd - A.dim) / 8;
+    const int heads = A.nh + 2 * A.nkv;
+    const int hbeg = blockIdx.y * A.heads_per_cta, hend = min(heads, hbeg + A.heads_per_cta);
+    for (int i = tid; i < (hend - hbeg) * per; i += kRopeThreads) {
+        const int h = hbeg + i / per, u = i % per;
+        const bool is_q = h < A.nh, is_k = !is_q && h < A.nh + A.nkv;
+        const int kh = is_q ? 0 : is_k ? h - A.nh : h - A.nh - A.nkv;
+        const TI* src = is_q ? reinterpret_cast<const TI*>(A.q) + (size_t)t * A.qs + (size_t)h * A.hd
+                        : is_k ? reinterpret_cast<const TI*>(A.k) + (size_t)t * A.ks + (size_t)kh * A.hd
+                               : reinterpret_cast<const TI*>(A.v) + (size_t)t * A.vs + (size_t)kh * A.hd;
+        TQ* qd = reinterpret_cast<TQ*>(A.q_out) + (size_t)t * A.qos + (size_t)h * A.hd;
+        TC* cd = reinterpret_cast<TC*>(is_k ? A.kp : A.vp) + row + (size_t)kh * A.hd;
+        if (page < 0 && !is_q) continue;
+        int d0, d1;  // the unit's two pieces of eight
+        float a[8], b[8];
+        if (u < pu) {
+            d0 = A.interleaved ? A.off + u * 16 : A.off + u * 8;
+            d1 = A.interleaved ? d0 + 8 : d0 + half;
+            load8(src + d0, a);
+            load8(src + d1, b);
+            if (is_q || is_k) {
+                if (page < 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.f;
+                } else if (A.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 ca = cs[u * 8 + e], cb = cs[u * 8 + 4 + e];
+                        const float x = a[2 * e], y = a[2 * e + 1];
+                        a[2 * e] = x * ca.x - y * ca.y;
+                        a[2 * e + 1] = y * ca.x + x * ca.y;
+                        const float z = b[2 * e], w = b[2 * e + 1];
+                        b[2 * e] = z * cb.x - w * cb.y;
+                        b[2 * e + 1] = w * cb.x + z * cb.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 c = cs[u * 8 + e];
+                        const float x = a[e], y = b[e];
+                        a[e] = x * c.x - y * c.y;
+                        b[e] = y * c.x + x * c.y;
+                    }
+                }
+            }
+            if (is_q) {
+                store8(qd + d0, a);
+                store8(qd + d1, b);
+            } else {
+                store8(cd + d0, a);
+                store8(cd + d1, b);
+            }
+        } else {
+            d0 = (u - pu) * 8;
+            if (d0 >= A.off) d0 += A.dim;
+            load8(src + d0, a);
+            if (is_q) {
+                if (page < 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) a[e] = 0.f;
+                }
+                store8(qd + d0, a);
+            } else {
+                store8(cd + d0, a);
+            }
+        }
+    }
+}
+
+template <typename TI, typename TC>
+cudaError_t launch_rope(const RopeArgs& A, bool q_as_cache, cudaStream_t s) {
+    const int heads = A.nh + 2 * A.nkv;
+    RopeArgs B = A;
+    // few tokens: their heads spread over CTAs
+    int parts = std::max(1, std::min(heads, 2 * sm_count() / std::max(1, A.n_tokens)));
+    B.heads_per_cta = (heads + parts - 1) / parts;
+    const dim3 grid(A.n_tokens, (heads + B.heads_per_cta - 1) / B.heads_per_cta);
+    if (q_as_cache)
+        return launch_pdl(rope_append_kernel<TI, TC, TC>, grid, dim3(kRopeThreads), 0, s, B);
+    return launch_pdl(rope_append_kernel<TI, TC, TI>, grid, dim3(kRopeThreads), 0, s, B);
+}
+
+// ------------------------------------------------------------------------
+// Page copies: CTA (piece of a page, layer and K / V, move); the moves travel in the launch's
+// parameters, so nothing is copied to the device and nothing is waited for.
+// ------------------------------------------------------------------------
+constexpr int kCopyThreads = 256;
+constexpr int kCopyVec = 8;  // 16-byte loads in flight per thread
+constexpr size_t kCopyPiece = (size_t)kCopyThreads * kCopyVec * 16;
+
+template <int N>
+struct CopyArgs {
+    char *k, *v;
+    size_t layer_bytes, page_stride_bytes, page_bytes;
+    int n_layers;
+    int2 move[N];
+};
+
+template <int N>
+__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_constant__ CopyArgs<N> A) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int2 mv = A.move[blockIdx.z];
+    const int l = blockIdx.y >> 1;
+    char* base = (blockIdx.y & 1 ? A.v : A.k) + (size_t)l * A.layer_bytes;
+    const uint4* src = reinterpret_cast<const uint4*>(base + (size_t)mv.x * A.page_stride_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(base + (size_t)mv.y * A.page_stride_bytes);
+    const size_t n = A.page_bytes / 16;
+    const size_t at = (size_t)blockIdx.x * kCopyThreads * kCopyVec + threadIdx.x;
+    uint4 r[kCopyVec];
+#pragma unroll
+    for (int i = 0; i < kCopyVec; ++i)
+        if (at + i * kCopyThreads < n) r[i] = __ldcs(src + at + i * kCopyThreads);
+#pragma unroll
+    for (int i = 0; i < kCopyVec; ++i)
+        if (at + i * kCopyThreads < n) __stcs(dst + at + i * kCopyThreads, r[i]);
+}
+
+template <int N>
+cudaError_t launch_copy(const WispKvPages* P, int n_layers, size_t layer_stride, const int* src,
+                        const int* dst, int n, cudaStream_t s) {
+    CopyArgs<N> A;
+    A.k = static_cast<char*>(P->k);
+    A.v = static_cast<char*>(P->v);
+    A.layer_bytes = layer_stride * 2;
+    A.page_stride_bytes = P->page_stride * 2;
+    A.page_bytes = (size_t)P->page_size * P->n_kv_heads * P->head_dim * 2;
+    A.n_layers = n_layers;
+    for (int i = 0; i < n; ++i) A.move[i] = make_int2(src[i], dst[i]);
+    const unsigned pieces = (unsigned)((A.page_bytes + kCopyPiece - 1) / kCopyPiece);
+    return launch_pdl(pages_copy_kernel<N>, dim3(pieces, 2 * n_layers, n), dim3(kCopyThreads), 0, s,
+                      A);
+}
+
+// ------------------------------------------------------------------------
+// Argument checks
+// ------------------------------------------------------------------------
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool known(int d) { return d == WISP_DTYPE_F32 || d == WISP_DTYPE_F16 || d == WISP_DTYPE_BF16; }
+
+#define PG_REFUSE(...)                                      \
+    do {                                                    \
+        WB_SET_ERR(err, WISP_ERR_INVALID_ARG, __VA_ARGS__); \
+        return WISP_ERR_INVALID_ARG;                        \
+    } while (0)
+
+WispError check_pages(const char* who, const WispKvPages* P, WispErrCtx* err) {
+    if (!P || !P->k || !P->v || !al16(P->k) || !al16(P->v))
+        PG_REFUSE("%s: pages NULL or not 16-byte aligned", who);
+    if (P->dtype != WISP_DTYPE_F16 && P->dtype != WISP_DTYPE_BF16)
+        PG_REFUSE("%s: pages of dtype %d (fp16 or bf16)", who, P->dtype);
+    if (P->n_pages <= 0 || P->page_size <= 0 || P->page_size % 8 || P->page_size > 65536 ||
+        P->n_kv_heads <= 0 || P->n_kv_heads > 1024 || P->head_dim <= 0 || P->head_dim % 8 ||
+        P->head_dim > 256)
+        PG_REFUSE("%s: unsupported pages: %d of %d positions, %d heads of %d (page_size a multiple "
+                  "of 8, head_dim a multiple of 8 up to 256)",
+                  who, P->n_pages, P->page_size, P->n_kv_heads, P->head_dim);
+    if (P->page_stride % 8 ||
+        P->page_stride < (size_t)P->page_size * P->n_kv_heads * P->head_dim)
+        PG_REFUSE("%s: page_stride %zu (a multiple of 8, at least a page)", who, P->page_stride);
+    return WISP_OK;
+}
+
+WispError check_batch(const char* who, const WispTokenBatch* B, WispErrCtx* err) {
+    if (!B || B->n_seq < 0 || B->n_tokens < 0 || B->max_q < 0 || B->table_stride < 0)
+        PG_REFUSE("%s: batch NULL or negative", who);
+    if (B->n_tokens > 0 &&
+        (B->n_seq == 0 || !B->q_start || !B->kv_len || !B->table || B->table_stride == 0 ||
+         B->max_q == 0))
+        PG_REFUSE("%s: a batch of %d tokens without sequences, table or max_q", who, B->n_tokens);
+    return WISP_OK;
+}
+
+WispError check_rows(const char* who, const char* name, const WispRows* R, int hd, WispErrCtx* err) {
+    if (!R || !R->base || !al16(R->base) || !known(R->dtype))
+        PG_REFUSE("%s: %s NULL, not 16-byte aligned or of unknown dtype", who, name);
+    if (R->n_heads <= 0 || R->n_heads > 65535 || R->stride % 8 ||
+        R->stride < (size_t)R->n_heads * hd)
+        PG_REFUSE("%s: %s has %d heads and stride %zu (a multiple of 8, at least its heads)", who,
+                  name, R->n_heads, R->stride);
+    return WISP_OK;
+}
+
+// ------------------------------------------------------------------------
+// Attention: what runs, and its workspace
+// ------------------------------------------------------------------------
+struct AttnShape {
+    int rw[2];  // 16-row MMA tiles of the two plans' row tiles
+    size_t bytes;
+};
+
+// Fills the geometry, plans and (with a workspace) pointers of a call.
+AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
+    const bool split = q_dtype == WISP_DTYPE_F32;
+    const int per = split ? 8 : 16;
+    AttnShape S{};
+    size_t at = 256;
+    auto take = [&](size_t bytes) {
+        char* p = ws ? ws + at : nullptr;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    };
+    A.status = reinterpret_cast<int*>(ws);
+    A.group = A.nh / A.nkv;
+    // rows of a row tile: the sequence's own, at most 4 MMA tiles; heads of a group beyond that
+    // become blocks of their own
+    A.gpb = std::min(A.group, 4 * per);
+    A.hblocks = (A.group + A.gpb - 1) / A.gpb;
+    const int n_plans = A.n_groups > 0 ? 2 : 1;
+    const int ctas = paged_attn_ctas(A.hd) * sm_count();
+    for (int w = 0; w < n_plans; ++w) {
+        PagedPlan& P = A.plan[w];
+        const int n_seg = w ? A.n_groups : A.n_seq;
+        const long long rows =
+            w ? (long long)((A.n_tokens + n_seg - 1) / n_seg) * A.gpb : (long long)max_q * A.gpb;
+        S.rw[w] = paged_attn_rw((int)std::min<long long>(rows, 4 * per), split);
+        P.tile = paged_attn_tile();
+        P.rows = S.rw[w] * per;
+        P.tpt = std::max(1, P.rows / A.gpb);
+        P.heads = A.nkv * A.hblocks;
+        P.lanes = std::max(1, ctas / P.heads);
+        P.max_items = A.n_tokens / P.tpt + n_seg;
+        P.n_items = reinterpret_cast<int*>(take(4));
+        P.item_off = reinterpret_cast<int*>(take((size_t)(n_seg + 1) * 4));
+        P.cum = reinterpret_cast<int*>(take((size_t)(P.max_items + 1) * 4));
+        P.items = reinterpret_cast<PagedItem*>(take((size_t)P.max_items * sizeof(PagedItem)));
+        const size_t recs = (size_t)P.lanes * P.heads * 2 * P.rows;
+        P.part_o = reinterpret_cast<float*>(take(recs * A.hd * 4));
+        P.part_ml = reinterpret_cast<float*>(take(recs * 8));
+    }
+    if (A.n_groups > 0) {
+        const size_t recs = (size_t)2 * A.n_tokens * A.nh;
+        A.full_o = reinterpret_cast<float*>(take(recs * A.hd * 4));
+        A.full_ml = reinterpret_cast<float*>(take(recs * 8));
+    }
+    S.bytes = at;
+    return S;
+}
+
+PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_heads, int n_groups) {
+    PagedArgs A{};
+    A.k = P->k;
+    A.v = P->v;
+    A.q_start = B->q_start;
+    A.kv_len = B->kv_len;
+    A.table = B->table;
+    A.page_stride = P->page_stride;
+    A.n_seq = B->n_seq;
+    A.n_tokens = B->n_tokens;
+    A.n_groups = n_groups;
+    A.table_stride = B->table_stride;
+    A.n_pages = P->n_pages;
+    A.page_size = P->page_size;
+    A.page_shift = (P->page_size & (P->page_size - 1)) ? -1 : __builtin_ctz(P->page_size);
+    A.nh = n_heads;
+    A.nkv = P->n_kv_heads;
+    A.hd = P->head_dim;
+    return A;
+}
+
+WispError attention_call(const char* who, const WispRows* q, const WispRows* out, float* lse,
+                         const WispKvPages* P, const WispTokenBatch* B, const int* groups,
+                         const int* prefix_len, int n_groups, float scale, int window, int sinks,
+                         void* ws, size_t ws_bytes, cudaStream_t s, WispErrCtx* err) {
+    WispError rc;
+    if ((rc = check_pages(who, P, err)) || (rc = check_batch(who, B, err))) return rc;
+    if (B->n_tokens == 0) return WISP_OK;
+    if ((rc = check_rows(who, "q", q, P->head_dim, err)) ||
+        (rc = check_rows(who, "out", out, P->head_dim, err)))
+        return rc;
+    if (q->dtype != out->dtype || (q->dtype != WISP_DTYPE_F32 && q->dtype != P->dtype))
+        PG_REFUSE("%s: q of dtype %d, out of %d (fp32 or the pages' %d, both the same)", who,
+                  q->dtype, out->dtype, P->dtype);
+    if (q->n_heads != out->n_heads || q->n_heads % P->n_kv_heads)
+        PG_REFUSE("%s: %d heads of q, %d of out (a multiple of the %d kv heads, both the same)", who,
+                  q->n_heads, out->n_heads, P->n_kv_heads);
+    if (!(fabsf(scale) <= 3e38f) || window < 0 || sinks < 0)
+        PG_REFUSE("%s: scale %g, window %d, sinks %d (finite; not negative)", who, (double)scale,
+                  window, sinks);
+    if (n_groups < 0 || (n_groups > 0 && (!groups || !prefix_len)))
+        PG_REFUSE("%s: %d groups without their arrays", who, n_groups);
+    PagedArgs A = attention_args(P, B, q->n_heads, n_groups);
+    A.q = q->base;
+    A.out = out->base;
+    A.lse = lse;
+    A.groups = groups;
+    A.prefix_len = prefix_len;
+    A.q_stride = q->stride;
+    A.out_stride = out->stride;
+    A.window = window >= (1 << 30) ? 0 : window;  // longer than any cache: none
+    A.sinks = sinks;
+    A.scale_log2 = scale * 1.4426950408889634f;
+    const AttnShape S = attention_layout(A, q->dtype, std::min(B->max_q, B->n_tokens),
+                                         static_cast<char*>(ws));
+    if (!ws || !al16(ws) || ws_bytes < S.bytes)
+        PG_REFUSE("%s: workspace of %zu bytes, need %zu (16-byte aligned)", who, ws ? ws_bytes : 0,
+                  S.bytes);
+    WB_CUDA_RET(launch_paged_plan(A, s), err);
+    if (n_groups > 0) WB_CUDA_RET(launch_paged_attn(A, 1, S.rw[1], q->dtype, P->dtype, s), err);
+    WB_CUDA_RET(launch_paged_attn(A, 0, S.rw[0], q->dtype, P->dtype, s), err);
+    WB_CUDA_RET(launch_paged_join(A, q->dtype, P->dtype, s), err);
+    return WISP_OK;
+}
+
+}  // namespace
+}  // namespace wb
+
+using namespace wb;
+
+extern "C" size_t wisp_paged_attention_workspace_bytes(const WispKvPages* P, const WispTokenBatch* B,
+                                                       int n_heads, int q_dtype, int n_groups) {
+    if (check_pages("paged_attention", P, nullptr) || check_batch("paged_attention", B, nullptr) ||
+        n_heads <= 0 || n_heads % P->n_kv_heads || n_groups < 0 || B->n_tokens == 0)
+        return 0;
+    PagedArgs A = attention_args(P, B, n_heads, n_groups);
+    return attention_layout(A, q_dtype, std::min(B->max_q, B->n_tokens), nullptr).bytes;
+}
+
+extern "C" WispError wisp_paged_attention(const WispRows* q, const WispRows* out, float* lse,
+                                          const WispKvPages* pages, const WispTokenBatch* batch,
+                                          float scale, int window, int sinks, void* workspace,
+                                          size_t workspace_bytes, cudaStream_t stream,
+                                          WispErrCtx* err) {
+    return attention_call("paged_attention", q, out, lse, pages, batch, nullptr, nullptr, 0, scale,
+                          window, sinks, workspace, workspace_bytes, stream, err);
+}
+
+extern "C" WispError wisp_prefix_attention(const WispRows* q, const WispRows* out, float* lse,
+                                           const WispKvPages* pages, const WispTokenBatch* batch,
+                                           const int* groups, const int* prefix_len, int n_groups,
+                                           float scale, int window, int sinks, void* workspace,
+                                           size_t workspace_bytes, cudaStream_t stream,
+                                           WispErrCtx* err) {
+    return attention_call("prefix_attention", q, out, lse, pages, batch, groups, prefix_len,
+                          n_groups, scale, window, sinks, workspace, workspace_bytes, stream, err);
+}
+
+extern "C" WispError wisp_rope_append(const WispRows* q, const WispRows* k, const WispRows* v,
+                                      const WispRows* q_out, const WispKvPages* P,
+                                      const WispTokenBatch* B, const WispRope* rope, int* status,
+                                      cudaStream_t s, WispErrCtx* err) {
+    const char* who = "rope_append";
+    WispError rc;
+    if ((rc = check_pages(who, P, err)) || (rc = check_batch(who, B, err))) return rc;
+    if (B->n_tokens == 0) return WISP_OK;
+    const int hd = P->head_dim;
+    if ((rc = check_rows(who, "q", q, hd, err)) || (rc = check_rows(who, "k", k, hd, err)) ||
+        (rc = check_rows(who, "v", v, hd, err)) || (rc = check_rows(who, "q_out", q_out, hd, err)))
+        return rc;
+    if (q->dtype != k->dtype || q->dtype != v->dtype ||
+        (q_out->dtype != q->dtype && q_out->dtype != P->dtype))
+        PG_REFUSE("%s: q, k, v of dtypes %d, %d, %d and q_out of %d (the first three the same, q_out "
+                  "theirs or the pages' %d)",
+                  who, q->dtype, k->dtype, v->dtype, q_out->dtype, P->dtype);
+    if (q_out->n_heads != q->n_heads || k->n_heads != P->n_kv_heads || v->n_heads != P->n_kv_heads)
+        PG_REFUSE("%s: %d heads of q, %d of q_out, %d of k, %d of v for %d kv heads", who, q->n_heads,
+                  q_out->n_heads, k->n_heads, v->n_heads, P->n_kv_heads);
+    if (!rope || rope->dim < 0 || rope->dim % 16 || rope->offset < 0 || rope->offset % 8 ||
+        rope->offset + rope->dim > hd || (rope->dim > 0 && !rope->inv_freq))
+        PG_REFUSE("%s: a window of %d at %d in heads of %d (a multiple of 16 at one of 8, with "
+                  "frequencies)",
+                  who, rope ? rope->dim : 0, rope ? rope->offset : 0, hd);
+    RopeArgs A{};
+    A.q = q->base;
+    A.k = k->base;
+    A.v = v->base;
+    A.q_out = q_out->base;
+    A.kp = P->k;
+    A.vp = P->v;
+    A.q_start = B->q_start;
+    A.kv_len = B->kv_len;
+    A.table = B->table;
+    A.positions = rope->positions;
+    A.freq = rope->inv_freq;
+    A.status = status;
+    A.qs = q->stride;
+    A.ks = k->stride;
+    A.vs = v->stride;
+    A.qos = q_out->stride;
+    A.page_stride = P->page_stride;
+    A.n_seq = B->n_seq;
+    A.n_tokens = B->n_tokens;
+    A.table_stride = B->table_stride;
+    A.n_pages = P->n_pages;
+    A.page_size = P->page_size;
+    A.nh = q->n_heads;
+    A.nkv = P->n_kv_heads;
+    A.hd = hd;
+    A.dim = rope->dim;
+    A.off = rope->offset;
+    A.interleaved = rope->interleaved != 0;
+    A.gain = rope->gain;
+    const bool h = P->dtype == WISP_DTYPE_F16, as_cache = q_out->dtype != q->dtype;
+    cudaError_t e;
+    if (q->dtype == WISP_DTYPE_F32)
+        e = h ? launch_rope<float, __half>(A, as_cache, s)
+              : launch_rope<float, __nv_bfloat16>(A, as_cache, s);
+    else if (q->dtype == WISP_DTYPE_F16)
+        e = h ? launch_rope<__half, __half>(A, as_cache, s)
+              : launch_rope<__half, __nv_bfloat16>(A, as_cache, s);
+    else
+        e = h ? launch_rope<__nv_bfloat16, __half>(A, as_cache, s)
+              : launch_rope<__nv_bfloat16, __nv_bfloat16>(A, as_cache, s);
+    WB_CUDA_RET(e, err);
+    return WISP_OK;
+}
+
+extern "C" WispError wisp_pages_copy(const WispKvPages* P, int n_layers, size_t layer_stride,
+                                     const int* src, const int* dst, int n, cudaStream_t s,
+                                     WispErrCtx* err) {
+    const char* who = "pages_copy";
+    WispError rc;
+    if ((rc = check_pages(who, P, err))) return rc;
+    if (n < 0 || (n > 0 && (!src || !dst)) || n_layers <= 0 || n_layers > 32767 || layer_stride % 8)
+        PG_REFUSE("%s: %d moves, %d layers, layer_stride %zu (a multiple of 8)", who, n, n_layers,
+                  layer_stride);
+    if (n == 0) return WISP_OK;
+    try {
+        // 1: a source, 2: a destination
+        std::vector<unsigned char> seen(P->n_pages, 0);
+        for (int i = 0; i < n; ++i) {
+            if (src[i] < 0 || src[i] >= P->n_pages || dst[i] < 0 || dst[i] >= P->n_pages)
+                PG_REFUSE("%s: move %d (%d -> %d) outside a pool of %d pages", who, i, src[i], dst[i],
+                          P->n_pages);
+            seen[src[i]] |= 1;
+        }
+        for (int i = 0; i < n; ++i) {
+            if (seen[dst[i]])
+                PG_REFUSE("%s: page %d is %s", who, dst[i],
+                          seen[dst[i]] & 1 ? "a source and a destination" : "twice a destination");
+            seen[dst[i]] |= 2;
+        }
+    } catch (const std::bad_alloc&) {
+        WB_SET_ERR(err, WISP_ERR_OOM, "%s: no host memory", who);
+        return WISP_ERR_OOM;
+    }
+    constexpr int kFew = 64, kMany = 1024;  // moves in a launch's parameters
+    for (int at = 0; at < n; at += kMany) {
+        const int m = std::min(kMany, n - at);
+        WB_CUDA_RET(m <= kFew ? launch_copy<kFew>(P, n_layers, layer_stride, src + at, dst + at, m, s)
+                              : launch_copy<kMany>(P, n_layers, layer_stride, src + at, dst + at, m, s),
+                    err);
+    }
+    return WISP_OK;
+}

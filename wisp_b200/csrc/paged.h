@@ -1,0 +1,66 @@
+// paged.h -- what the paged-cache sources share: tile plans, the argument block of the
+// attention kernels, status bits (not part of the ABI).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "wisp_b200.h"
+
+namespace wb {
+
+// Status bits of a paged call's workspace (wisp_paged_status).
+enum { PG_BAD_PAGE = 1, PG_BAD_LENGTH = 2, PG_TIMEOUT = 8 };
+
+// One row tile: consecutive tokens whose rows (token, query head of the kv head) go through
+// the same cached positions.  Positions come in tiles of `tile` from 0: the item's list is
+// [sink0, sink0 + n_sink) and then n_tiles - n_sink tiles from `first` on.
+struct PagedItem {
+    int tok0, ntok;      // tokens
+    int seq;             // row of the page table
+    int kv_lo, kv_hi;    // positions outside [kv_lo, kv_hi) belong to another item or to none
+    int pos0;            // position of tok0; the tokens' positions follow one another when
+    int pmin, pmax;      // `mixed` is 0, else each token's is looked up; their range
+    int sink0, n_sink, first, n_tiles;
+    int mixed;
+};
+
+// A plan covers all row tiles of one kind: n_items items, cum[i] KV tiles before item i.  The
+// line of all KV tiles is cut into `lanes` equal pieces; one CTA takes a piece for one head.
+struct PagedPlan {
+    int* n_items;
+    int* item_off;  // [segments + 1] items before each sequence (or group)
+    int* cum;       // [max_items + 1]
+    PagedItem* items;
+    float* part_o;   // [lanes][heads][2][rows][hd]: pieces of items that lanes share
+    float* part_ml;  // [lanes][heads][2][rows][2]: running maximum (log2) and sum
+    int tile;        // positions of a KV tile
+    int tpt;         // tokens of a row tile
+    int rows;        // rows of a row tile
+    int lanes, heads;
+    int max_items;
+};
+
+struct PagedArgs {
+    const void* q;
+    void* out;
+    float* lse;
+    const void* k;
+    const void* v;
+    const int* q_start;
+    const int* kv_len;
+    const int* table;
+    const int* groups;      // prefix mode: [n_groups + 1] first sequence of each group
+    const int* prefix_len;  // [n_groups]
+    float* full_o;          // prefix mode: [2][n_tokens * n_heads][hd], whole items' rows
+    float* full_ml;         // [2][n_tokens * n_heads][2]
+    int* status;
+    size_t q_stride, out_stride, page_stride;
+    int n_seq, n_tokens, n_groups, table_stride, n_pages, page_size, page_shift;
+    int nh, nkv, group, gpb, hblocks, hd, window, sinks;
+    float scale_log2;
+    PagedPlan plan[2];  // [0] the sequences (their own part), [1] the shared prefixes
+};
+
+}  // namespace wb

@@ -1,0 +1,541 @@
+// paged_attn.cu -- causal attention of a batch's tokens over a paged fp16 / bf16 cache, with
+// a sliding window and sinks, and its form for sequences that share a prefix.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j)
+//   over cached j <= i with (window == 0 or i - j < window or j < sinks)
+//
+// A row tile holds the rows (token, query head) of consecutive tokens that read one kv head;
+// it passes over the positions once with a running maximum and sum per row.  The line of all
+// (row tile, KV tile) pairs of the batch is cut into equal pieces (paged_plan.cu), one CTA
+// per piece and kv head: ragged batches balance by themselves, long sequences are split over
+// many CTAs, and at most two row tiles of a piece are shared with its neighbours, whose
+// partial results a second kernel joins in a fixed order (results do not depend on timing).
+//
+// Products run on mma.sync m16n8k16 with fp32 accumulators.  32-bit rows are split into two
+// 16-bit parts (x ~= hi + lo, 22 bits in fp16, 16 in bf16) that fill the two halves of a
+// 16-row tile, so 8 rows cost one instruction and their two sums meet in one thread; the
+// weights p are split the same way.  In fp16, p is scaled by 2^kPShift so that small weights
+// of long contexts stay above the subnormals (the factor cancels in the quotient).
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "internal.h"
+#include "paged.h"
+#include "paged_math.cuh"
+
+namespace wb {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kTile = 64;  // positions of a KV tile
+
+template <int HD>
+struct Cfg {
+    static constexpr int kStages = 3;
+    static constexpr int kCh = HD / 8;            // 16-byte pieces of a row
+    static constexpr int kStage = 2 * kTile * HD;  // elements: K then V
+};
+
+template <int HD, int RW>
+constexpr size_t attn_smem_bytes() {
+    return (size_t)Cfg<HD>::kStages * Cfg<HD>::kStage * 2 + (size_t)16 * RW * HD * 2;
+}
+
+// ------------------------------------------------------------------------
+// Row tile of 16 * RW MMA rows: warp w owns rows 16 * (w % RW) .. and the positions
+// (w / RW) * kTile * RW / 4 .. of every KV tile.  With RW == 1 the warps never wait for one
+// another inside the loop (each loads what it reads).
+// ------------------------------------------------------------------------
+template <typename T, bool SPLIT, int HD, int RW>
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int which) {
+    using C = Cfg<HD>;
+    constexpr int kCh = C::kCh, kS = C::kStages;
+    constexpr int kNP = kTile * RW / 4;       // positions per warp and tile
+    constexpr int kNT = kNP / 8;              // score tiles of 8 positions
+    constexpr int kRows = SPLIT ? 8 : 16;     // real rows per warp
+    constexpr bool kQRegs = HD <= 128;
+    extern __shared__ __align__(128) char smem[];
+    T* ring = reinterpret_cast<T*>(smem);
+    T* qs = ring + (size_t)kS * C::kStage;    // [16 * RW][HD], swizzled like the cache rows
+    __shared__ int s_pos[16 * RW];            // position of each real row (INT_MIN: no row)
+    __shared__ float s_fac[16 * RW];          // SPLIT: the row's power-of-two factor
+    const PagedPlan& P = A.plan[which];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c4 = lane & 3;
+    const int rw = warp % RW, pw = warp / RW;
+    const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
+    const int kvh = head_lane / A.hblocks, hb = head_lane - kvh * A.hblocks;
+    const int h0 = kvh * A.group + hb * A.gpb;             // first query head
+    const int gpb = min(A.gpb, A.group - hb * A.gpb);      // query heads of this block
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    const int n_items = *P.n_items;
+    if (n_items == 0) return;
+    const int total = P.cum[n_items];
+    int x = (int)((long long)piece * total / P.lanes);
+    const int x_end = (int)((long long)(piece + 1) * total / P.lanes);
+    if (x >= x_end) return;
+    // the item that holds KV tile x: the last with cum <= x
+    int lo = 0, span = n_items;
+    while (span > 1) {
+        const int step = (span + kThreads - 1) / kThreads;
+        const int at = lo + min(tid * step, span - 1);
+        const int hit = __syncthreads_count(tid * step < span && P.cum[at] <= x);
+        lo += (hit - 1) * step;
+        span = min(step, span - (hit - 1) * step);
+    }
+    int item = lo;
+
+    const T* __restrict__ Kc = reinterpret_cast<const T*>(A.k);
+    const T* __restrict__ Vc = reinterpret_cast<const T*>(A.v);
+    const float sl2 = A.scale_log2;
+    constexpr float kShift = PMath<T>::kPShift;
+
+    for (; x < x_end; ++item) {
+        const PagedItem it = P.items[item];
+        const int c0 = P.cum[item];
+        const int a = x - c0, b = min(it.n_tiles, x_end - c0);  // KV tiles [a, b) of the item
+        x = c0 + b;
+        const bool whole = a == 0 && b == it.n_tiles;
+        const int n_rows = it.ntok * gpb;
+
+        // rows of this tile: positions, and q as swizzled 16-bit rows in shared memory
+        __syncthreads();  // the previous item's readers of s_pos / qs / ring are done
+        for (int r = tid; r < 16 * RW; r += kThreads) {
+            const int wr = r / 16, rr = r & 15;
+            const int row = wr * kRows + rr;
+            int pos = INT_MIN;
+            if (rr < kRows && row < n_rows) {
+                const int t = it.tok0 + row / gpb;
+                pos = it.mixed ? token_position(A, t) : it.pos0 + row / gpb;
+            }
+            s_pos[r] = pos;
+        }
+        load_rows<T, SPLIT, HD, RW, kThreads>(A, it.tok0, n_rows, h0, gpb, qs, s_fac);
+        __syncthreads();
+
+        const int prow[2] = {s_pos[rw * 16 + g], SPLIT ? INT_MIN : s_pos[rw * 16 + g + 8]};
+        int hi_row[2], lo_row[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            hi_row[u] = prow[u] == INT_MIN ? 0 : min(it.kv_hi, prow[u] + 1);
+            lo_row[u] = A.window > 0 && prow[u] != INT_MIN ? prow[u] - A.window + 1 : INT_MIN;
+        }
+        const float fac = SPLIT ? s_fac[rw * 16 + g] * sl2 : sl2;
+        // what some row of the tile sees / what every row sees
+        const int any_hi = min(it.kv_hi, it.pmax + 1);
+        const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
+        const int all_hi = min(it.kv_hi, it.pmin + 1);
+        const int all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
+        const int sinks = A.window > 0 ? A.sinks : 0;
+
+        uint32_t qf[kQRegs ? HD / 16 : 1][4];
+        auto load_q = [&](int kk, uint32_t (&f)[4]) {
+            const int r = rw * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
+            ldsm4(f, qs + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+        };
+        if (kQRegs) {
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) load_q(kk, qf[kQRegs ? kk : 0]);
+        }
+
+        auto tile_at = [&](int i) { return i < it.n_sink ? it.sink0 + i : it.first + i - it.n_sink; };
+        // Where the 16 rows [16 * (warp)) of KV tile i start in the cache, one lane each
+        // (elements; -1: no row of the tile sees the position).
+        auto row_offset = [&](int i) -> long long {
+            const int j = tile_at(i) * kTile + warp * 16 + (lane & 15);
+            const bool seen = j >= it.kv_lo && j < any_hi && (j >= any_lo || j < sinks);
+            return seen ? page_offset(A, it.seq, j, kvh) : -1;
+        };
+        auto load_tile = [&](int st, long long off) {
+            T* kd = ring + (size_t)st * C::kStage;
+            T* vd = kd + kTile * HD;
+            constexpr int kPer = 32 / kCh > 0 ? 32 / kCh : 1;   // rows per pass of the warp
+            constexpr int kCol = kCh > 32 ? kCh / 32 : 1;
+#pragma unroll
+            for (int p = 0; p < 16 / kPer; ++p) {
+                const int r = p * kPer + (kCh >= 32 ? 0 : lane / kCh);
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                const int row = warp * 16 + r;
+#pragma unroll
+                for (int cc = 0; cc < kCol; ++cc) {
+                    const int c = (kCh >= 32 ? lane : lane % kCh) + cc * 32;
+                    const bool in = o >= 0 && c * 8 < A.hd;
+                    const size_t src = in ? (size_t)o + c * 8 : 0;
+                    const int dst = row * HD + ((c ^ (row & 7)) * 8);
+                    cp16(kd + dst, Kc + src, in);
+                    cp16(vd + dst, Vc + src, in);
+                }
+            }
+        };
+
+        float o[HD / 8][4];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[i][u] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+        // ring: kS - 1 tiles ahead; the page of the next tile to load is looked up one
+        // iteration before its copies are issued
+        long long off = -1;
+        for (int u = 0; u < kS - 1; ++u) {
+            if (a + u < b) load_tile(u, row_offset(a + u));
+            cp_commit();
+        }
+        if (a + kS - 1 < b) off = row_offset(a + kS - 1);
+        int st = 0;
+        for (int i = a; i < b; ++i) {
+            cp_wait<kS - 2>();
+            if (RW == 1) __syncwarp();
+            else __syncthreads();
+            {
+                const int ld = st == 0 ? kS - 1 : st - 1;
+                if (i + kS - 1 < b) load_tile(ld, off);
+                cp_commit();
+                if (i + kS < b) off = row_offset(i + kS);
+            }
+            const T* kd = ring + (size_t)st * C::kStage;
+            const T* vd = kd + kTile * HD;
+            st = st + 1 == kS ? 0 : st + 1;
+            const int j0 = tile_at(i) * kTile, jw = j0 + pw * kNP;
+            const bool full = jw >= it.kv_lo && jw + kNP <= all_hi &&
+                              (jw >= all_lo || jw + kNP <= sinks);
+
+            float s[kNT][4];
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[t][u] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                uint32_t qv[4];
+                if (!kQRegs) load_q(kk, qv);
+                const uint32_t(&qk)[4] = kQRegs ? qf[kQRegs ? kk : 0] : qv;
+#pragma unroll
+                for (int t = 0; t < kNT; t += 2) {
+                    const int r = pw * kNP + t * 8 + ((lane >> 4) & 1) * 8 + (lane & 7);
+                    const int c = kk * 2 + ((lane >> 3) & 1);
+                    uint32_t kf[4];
+                    ldsm4(kf, kd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+                    PMath<T>::mma(s[t], qk, kf[0], kf[1]);
+                    PMath<T>::mma(s[t + 1], qk, kf[2], kf[3]);
+                }
+            }
+            // scores in log2 units, masked; the row maxima
+            float mx[2] = {m[0], m[1]};
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (SPLIT && u >= 2) continue;
+                    float v = SPLIT ? (s[t][u] + s[t][u + 2 < 4 ? u + 2 : u]) * fac : s[t][u] * sl2;
+                    if (!full) {
+                        const int j = jw + t * 8 + c4 * 2 + (u & 1);
+                        if (!(j >= it.kv_lo && j < hi_row[u >> 1] &&
+                              (j >= lo_row[u >> 1] || j < sinks)))
+                            v = -INFINITY;
+                    }
+                    s[t][u] = v;
+                    mx[u >> 1] = fmaxf(mx[u >> 1], v);
+                }
+            float al[2], mb[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
+                mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
+                const float base = mx[u] == -INFINITY ? 0.f : mx[u];
+                al[u] = ex2(m[u] - base);
+                mb[u] = base - kShift;
+                m[u] = mx[u];
+                l[u] *= al[u];
+            }
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+#pragma unroll
+                for (int u = 0; u < (SPLIT ? 2 : 4); ++u) {
+                    s[t][u] = ex2(s[t][u] - mb[u >> 1]);
+                    l[u >> 1] += s[t][u];
+                }
+            if (al[0] != 1.f || (!SPLIT && al[1] != 1.f)) {
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) o[d][u] *= SPLIT ? al[0] : al[u >> 1];
+            }
+            // rows that see different positions of one tile: what is hidden from one may be
+            // an infinity or a NaN that another sees
+            const bool mixed_mask = !full && it.pmin != it.pmax;
+#pragma unroll
+            for (int kk = 0; kk < kNP / 16; ++kk) {
+                uint32_t pf[4];
+                if (SPLIT) {
+                    PMath<T>::split2(s[2 * kk][0], s[2 * kk][1], pf[0], pf[1]);
+                    PMath<T>::split2(s[2 * kk + 1][0], s[2 * kk + 1][1], pf[2], pf[3]);
+                } else {
+                    pf[0] = PMath<T>::pack(s[2 * kk][0], s[2 * kk][1]);
+                    pf[1] = PMath<T>::pack(s[2 * kk][2], s[2 * kk][3]);
+                    pf[2] = PMath<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+                    pf[3] = PMath<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+                }
+#pragma unroll
+                for (int d = 0; d < HD / 8; d += 2) {
+                    const int r = pw * kNP + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+                    const int c = d + (lane >> 4);
+                    uint32_t vf[4];
+                    ldsm4t(vf, vd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+                    if (mixed_mask) {
+                        bool bad = false;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) bad |= PMath<T>::not_finite(vf[u]);
+                        if (__any_sync(0xffffffffu, bad)) {
+                            // visible places of the 16 x 16 block of weights as ones
+                            uint32_t one[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const int row = u & 1;
+                                uint32_t w = 0;
+                                for (int e = 0; e < 2; ++e) {
+                                    const int j = jw + kk * 16 + (u >> 1) * 8 + c4 * 2 + e;
+                                    if (j >= it.kv_lo && j < hi_row[row] &&
+                                        (j >= lo_row[row] || j < sinks))
+                                        w |= PMath<T>::kOne << (16 * e);
+                                }
+                                one[u] = w;
+                            }
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                SpecialFrag f{{o[d + n][0], o[d + n][1], o[d + n][2], o[d + n][3]},
+                                              vf[2 * n], vf[2 * n + 1]};
+                                f = specials<T>(f, one[0], one[1], one[2], one[3]);
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) o[d + n][u] = f.o[u];
+                                vf[2 * n] = f.b0;
+                                vf[2 * n + 1] = f.b1;
+                            }
+                        }
+                    }
+                    PMath<T>::mma(o[d], pf, vf[0], vf[1]);
+                    PMath<T>::mma(o[d + 1], pf, vf[2], vf[3]);
+                }
+            }
+        }
+        cp_wait<0>();
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+            l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        }
+
+        // join the warps that read other positions of the same rows (shared memory, fp32)
+        if (RW < 4) {
+            __syncthreads();
+            float* xo = reinterpret_cast<float*>(smem);           // [4 / RW][16 * RW][HD]
+            float* xm = xo + (size_t)(4 / RW) * 16 * RW * HD;     // [4 / RW][16 * RW][2]
+#pragma unroll
+            for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
+                const int r = rw * 16 + g + 8 * u;
+                float* dst = xo + ((size_t)pw * 16 * RW + r) * HD;
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d) {
+                    const float2 v = SPLIT ? make_float2(o[d][0] + o[d][2], o[d][1] + o[d][3])
+                                           : make_float2(o[d][2 * u], o[d][2 * u + 1]);
+                    *reinterpret_cast<float2*>(dst + d * 8 + c4 * 2) = v;
+                }
+                if (c4 == 0) {
+                    xm[(pw * 16 * RW + r) * 2] = m[u];
+                    xm[(pw * 16 * RW + r) * 2 + 1] = l[u];
+                }
+            }
+            __syncthreads();
+            // warp w joins rows w, w + 4, ...
+            for (int r = warp; r < 16 * RW; r += 4) {
+                const int row = (r / 16) * kRows + (r & 15);
+                if ((r & 15) >= kRows || row >= n_rows) continue;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 4 / RW; ++w) M = fmaxf(M, xm[(w * 16 * RW + r) * 2]);
+                const float base = M == -INFINITY ? 0.f : M;
+                float e[4 / RW], L = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4 / RW; ++w) {
+                    e[w] = ex2(xm[(w * 16 * RW + r) * 2] - base);
+                    L += xm[(w * 16 * RW + r) * 2 + 1] * e[w];
+                }
+                RowOut<T, SPLIT> R(A, P, which, it, piece, head_lane, h0, gpb, row, a, whole);
+                for (int d = lane * 2; d < A.hd; d += 64) {
+                    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < 4 / RW; ++w) {
+                        const float2 v = *reinterpret_cast<const float2*>(
+                            xo + ((size_t)w * 16 * RW + r) * HD + d);
+                        acc.x = fmaf(v.x, e[w], acc.x);
+                        acc.y = fmaf(v.y, e[w], acc.y);
+                    }
+                    R.put2(d, acc, L);
+                }
+                if (lane == 0) R.put_ml(M, L);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
+                const int row = rw * kRows + g + 8 * u;
+                if (row >= n_rows) continue;
+                RowOut<T, SPLIT> R(A, P, which, it, piece, head_lane, h0, gpb, row, a, whole);
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d) {
+                    if (d * 8 >= A.hd) break;
+                    const float2 v = SPLIT ? make_float2(o[d][0] + o[d][2], o[d][1] + o[d][3])
+                                           : make_float2(o[d][2 * u], o[d][2 * u + 1]);
+                    R.put2(d * 8 + c4 * 2, v, l[u]);
+                }
+                if (c4 == 0) R.put_ml(m[u], l[u]);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------
+// Joins the pieces of split items: CTA (piece boundary, head, 4 rows), a warp per row.  The
+// CTA of piece p joins the item that begins in p and ends after it.
+// ------------------------------------------------------------------------
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs A) {
+    const PagedPlan& P = A.plan[0];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
+    const int n_items = *P.n_items;
+    if (n_items == 0) return;
+    const int total = P.cum[n_items];
+    const int x0 = (int)((long long)piece * total / P.lanes);
+    const int x1 = (int)((long long)(piece + 1) * total / P.lanes);
+    if (x0 >= x1 || x1 >= total) return;
+    int lo = 0, hi = n_items;  // the item of tile x1 - 1
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (P.cum[mid] <= x1 - 1) lo = mid;
+        else hi = mid;
+    }
+    if (P.cum[lo] < x0 || P.cum[lo + 1] == x1) return;
+    const PagedItem it = P.items[lo];
+    const int kvh = head_lane / A.hblocks, hb = head_lane - kvh * A.hblocks;
+    const int h0 = kvh * A.group + hb * A.gpb, gpb = min(A.gpb, A.group - hb * A.gpb);
+    const int row = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5);
+    if (row >= it.ntok * gpb) return;
+    const int last = (int)(((long long)P.cum[lo + 1] * P.lanes - 1) / total);
+    Joined J;
+    J.init();
+    J.add_range(A, P, piece, last, head_lane, row);
+    const int t = it.tok0 + row / gpb, h = h0 + row % gpb;
+    J.write<T, SPLIT>(A, t, h);
+}
+
+// Prefix mode: a warp per (token, head) joins its part of the shared prefix and its own part.
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) paged_join2_kernel(PagedArgs A) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const long long id = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (id >= (long long)A.n_tokens * A.nh) return;
+    const int t = (int)(id / A.nh), h = (int)(id - (long long)t * A.nh);
+    const int kvh = h / A.group, hg = h - kvh * A.group, hb = hg / A.gpb, hr = hg - hb * A.gpb;
+    const int gpb = min(A.gpb, A.group - hb * A.gpb);
+    const int head_lane = kvh * A.hblocks + hb;
+    const int seq = last_le(A.q_start, A.n_seq, t);
+    if (t < A.q_start[seq] || t >= A.q_start[seq + 1]) return;
+    Joined J;
+    J.init();
+    for (int which = 0; which < 2; ++which) {
+        const PagedPlan& P = A.plan[which];
+        int seg = seq;
+        if (which) {
+            seg = last_le(A.groups, A.n_groups, seq);
+            if (seq < A.groups[seg] || seq >= A.groups[seg + 1]) continue;
+        }
+        const int n_items = *P.n_items;
+        const int t0 = A.q_start[which ? A.groups[seg] : seg];
+        const int item = P.item_off[seg] + (t - t0) / P.tpt;
+        if (item >= n_items) continue;
+        const int row = ((t - t0) % P.tpt) * gpb + hr;
+        const int total = P.cum[n_items], a = P.cum[item], b = P.cum[item + 1];
+        const int first = (int)(((long long)(a + 1) * P.lanes - 1) / total);
+        const int last = (int)(((long long)b * P.lanes - 1) / total);
+        if (first == last) J.add_full(A, which, id);
+        else J.add_range(A, P, first, last, head_lane, row);
+    }
+    J.write<T, SPLIT>(A, t, h);
+}
+
+template <typename T, bool SPLIT, int HD, int RW>
+cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
+    auto kern = paged_attn_kernel<T, SPLIT, HD, RW>;
+    constexpr size_t smem = attn_smem_bytes<HD, RW>();
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    const PagedPlan& P = A.plan[which];
+    return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), smem, s, A, which);
+}
+
+template <typename T, bool SPLIT, int HD>
+cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
+    return rw == 1 ? launch_one<T, SPLIT, HD, 1>(A, which, s)
+           : rw == 2 ? launch_one<T, SPLIT, HD, 2>(A, which, s)
+                     : launch_one<T, SPLIT, HD, 4>(A, which, s);
+}
+
+template <typename T, bool SPLIT>
+cudaError_t launch_t(const PagedArgs& A, int which, int rw, cudaStream_t s) {
+    return A.hd <= 64    ? launch_rw<T, SPLIT, 64>(A, which, rw, s)
+           : A.hd <= 128 ? launch_rw<T, SPLIT, 128>(A, which, rw, s)
+                         : launch_rw<T, SPLIT, 256>(A, which, rw, s);
+}
+
+template <typename T, bool SPLIT>
+cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
+    if (A.n_groups > 0) {
+        const long long n = ((long long)A.n_tokens * A.nh + 3) / 4;
+        return launch_pdl(paged_join2_kernel<T, SPLIT>, dim3((unsigned)n), dim3(kThreads), 0, s, A);
+    }
+    const PagedPlan& P = A.plan[0];
+    return launch_pdl(paged_join_kernel<T, SPLIT>, dim3(P.heads * P.lanes, (P.rows + 3) / 4),
+                      dim3(kThreads), 0, s, A);
+}
+
+}  // namespace
+
+int paged_attn_tile() { return kTile; }
+
+// 16-row MMA tiles of a row tile with `rows` rows: 1, 2 or 4.
+int paged_attn_rw(int rows, bool split) {
+    const int per = split ? 8 : 16;
+    return rows <= per ? 1 : rows <= 2 * per ? 2 : 4;
+}
+
+// CTAs of one SM: what the ring leaves room for.
+int paged_attn_ctas(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
+
+cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
+                              cudaStream_t s) {
+    const bool split = q_dtype == WISP_DTYPE_F32;
+    if (kv_dtype == WISP_DTYPE_F16)
+        return split ? launch_t<__half, true>(A, which, rw, s)
+                     : launch_t<__half, false>(A, which, rw, s);
+    return split ? launch_t<__nv_bfloat16, true>(A, which, rw, s)
+                 : launch_t<__nv_bfloat16, false>(A, which, rw, s);
+}
+
+cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s) {
+    const bool split = q_dtype == WISP_DTYPE_F32;
+    if (kv_dtype == WISP_DTYPE_F16)
+        return split ? launch_join<__half, true>(A, s) : launch_join<__half, false>(A, s);
+    return split ? launch_join<__nv_bfloat16, true>(A, s)
+                 : launch_join<__nv_bfloat16, false>(A, s);
+}
+
+}  // namespace wb

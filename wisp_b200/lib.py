@@ -38,6 +38,28 @@ class WispAttnLayer(C.Structure):
                 ("rope_theta", C.c_float), ("rms_eps", C.c_float)]
 
 
+class WispKvPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_size_t),
+                ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("dtype", C.c_int)]
+
+
+class WispTokenBatch(C.Structure):
+    _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p),
+                ("n_seq", C.c_int), ("n_tokens", C.c_int), ("max_q", C.c_int),
+                ("table_stride", C.c_int)]
+
+
+class WispRows(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("stride", C.c_size_t), ("n_heads", C.c_int),
+                ("dtype", C.c_int)]
+
+
+class WispRope(C.Structure):
+    _fields_ = [("inv_freq", C.c_void_p), ("positions", C.c_void_p), ("dim", C.c_int),
+                ("offset", C.c_int), ("interleaved", C.c_int), ("gain", C.c_float)]
+
+
 class WispMoeLayer(C.Structure):
     _fields_ = [("meta", WispExpertMeta), ("expert_blobs", C.c_void_p), ("router_w", C.c_void_p),
                 ("router_bias", C.c_void_p), ("norm_w", C.c_void_p), ("shared_blob", C.c_void_p),
@@ -117,6 +139,32 @@ _SIGS = {
     "wisp_lm_head_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                        C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_void_p,
                                        C.POINTER(WispErrCtx)]),
+    # the paged cache
+    "wisp_paged_attention_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p, C.c_int,
+                                                          C.c_int, C.c_int]),
+    "wisp_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
+                                       C.c_void_p, C.c_void_p]),
+    "wisp_prefix_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_float,
+                                        C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
+                                        C.c_void_p]),
+    "wisp_rope_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "wisp_pages_copy": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p,
+                                  C.c_int, C.c_void_p, C.c_void_p]),
+    "wisp_page_pool_create": (C.c_void_p, [C.c_int, C.c_int, C.c_void_p]),
+    "wisp_page_pool_destroy": (None, [C.c_void_p]),
+    "wisp_page_pool_free_pages": (C.c_int, [C.c_void_p]),
+    "wisp_page_pool_open": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "wisp_page_pool_extend": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "wisp_page_pool_truncate": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "wisp_page_pool_fork": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
+    "wisp_page_pool_close": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
+    "wisp_page_pool_compact": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "wisp_page_pool_length": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
+    "wisp_page_pool_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
+    "wisp_page_pool_moves": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]),
     "wisp_gpu_embed_lookup": (None, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
     "wisp_gpu_rope": (None, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float,
                              C.c_void_p]),

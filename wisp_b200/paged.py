@@ -1,0 +1,373 @@
+"""A paged key/value cache for a batch of sequences, and the operators that work on it.
+
+* ``rope_append``       rotary positions on q and k, k and v appended to the cache's pages
+* ``attention``         causal attention over the pages: prompts, chunks and single tokens,
+  with a sliding window and a few first tokens (sinks) that stay visible
+* ``prefix_attention``  the same for sequences that share a long prefix (read once per group)
+* ``copy_pages``        pages copied inside the pool of all layers
+* ``PagePool``          the host-side owner of page numbers: open, extend, fork (copy on
+  write), truncate, close, compact
+* ``rope_frequencies``  rotary frequencies, plain or stretched for a long context
+
+Pages are ``[n_pages, page_size, n_kv_heads, head_dim]`` per layer (``[n_layers, ...]`` for
+the page operators), fp16 or bf16, one tensor for the keys and one for the values.  Every call
+runs on the caller's current CUDA stream and synchronises nothing; lengths and page tables are
+device tensors, so a captured step can be replayed after they changed.  torch is used for
+device memory and streams only; every kernel is in ``libwisp_b200.so``.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+from array import array
+
+import torch
+
+from .lib import (WispErrCtx, WispError, WispKvPages, WispRope, WispRows, WispTokenBatch, check,
+                  lib)
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _device_ints(name: str, t: torch.Tensor, dim: int) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != dim or not t.is_cuda or t.stride(-1) != 1:
+        raise ValueError(f"{name}: a contiguous int32 CUDA tensor of {dim} dimension(s) is wanted")
+    return t
+
+
+class TokenBatch:
+    """The tokens of one step, sequence after sequence (``WispTokenBatch``).
+
+    ``q_start`` int32 ``[n_seq + 1]``: first token of each sequence; ``kv_len`` int32
+    ``[n_seq]``: cached positions, the step's own tokens included; ``table`` int32
+    ``[n_seq, pages]``: the sequences' page numbers; ``max_q``: no sequence has more tokens.
+    One batch serves every layer of a step."""
+
+    __slots__ = ("q_start", "kv_len", "table", "max_q", "c", "device")
+
+    def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, table: torch.Tensor,
+                 max_q: int):
+        self.q_start = _device_ints("q_start", q_start, 1)
+        self.kv_len = _device_ints("kv_len", kv_len, 1)
+        self.table = _device_ints("table", table, 2)
+        n = kv_len.shape[0]
+        if q_start.shape[0] != n + 1 or table.shape[0] != n:
+            raise ValueError(f"{n} sequences: q_start has {q_start.shape[0]} entries, table "
+                             f"{table.shape[0]} rows")
+        self.device = kv_len.device
+        if q_start.device != self.device or table.device != self.device:
+            raise ValueError("q_start, kv_len and table are on different devices")
+        self.max_q = int(max_q)
+        self.c = WispTokenBatch(q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(), n, 0,
+                                self.max_q, table.stride(0) if n > 1 else table.shape[1])
+
+
+def _pages(k: torch.Tensor, v: torch.Tensor) -> WispKvPages:
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+        raise ValueError("k_pages and v_pages: two [n_pages, page_size, n_kv_heads, head_dim] "
+                         "tensors of one shape, layout and dtype are wanted")
+    n, page, heads, dim = k.shape
+    if k.stride()[1:] != (heads * dim, dim, 1):
+        raise ValueError("k_pages: a page's positions, heads and dims must be contiguous")
+    if not k.is_cuda or v.device != k.device:
+        raise ValueError("k_pages and v_pages must be on one CUDA device")
+    if k.dtype not in _DTYPES:
+        raise ValueError(f"k_pages of {k.dtype} (fp16 or bf16)")
+    stride = k.stride(0) if n > 1 else page * heads * dim
+    return WispKvPages(k.data_ptr(), v.data_ptr(), stride, n, page, heads, dim, _DTYPES[k.dtype])
+
+
+def _rows(name: str, x: torch.Tensor, n: int, dim: int, device) -> WispRows:
+    if x.dim() != 3 or x.shape[0] != n or x.shape[2] != dim:
+        raise ValueError(f"{name}: [{n}, heads, {dim}] is wanted, got {list(x.shape)}")
+    heads = x.shape[1]
+    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim):
+        raise ValueError(f"{name}: a row's heads must be contiguous")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, the pages on {device}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{name} of {x.dtype} (fp32, fp16 or bf16)")
+    return WispRows(x.data_ptr(), x.stride(0) if n > 1 else heads * dim, heads, _DTYPES[x.dtype])
+
+
+def _on(device):
+    """The device's current stream, with the device made current for the launch."""
+    if torch.cuda.current_device() != device.index:
+        raise ValueError(f"tensors on {device}, but the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def rope_frequencies(dim: int, theta: float = 10000.0, *, scaling: str | None = None,
+                     factor: float = 1.0, original: int = 4096, low: float = 1.0,
+                     high: float = 32.0, device=None) -> tuple[torch.Tensor, float]:
+    """(inverse frequencies ``[dim // 2]`` in float64, gain) of a rotary window of ``dim``.
+
+    ``scaling``: None; ``"linear"`` (every frequency / factor); ``"base"`` (theta raised so
+    that the slowest pair is stretched by factor and the fastest kept); ``"by_parts"``: pairs
+    that make fewer than ``low`` turns in ``original`` positions are divided by factor, those of
+    more than ``high`` kept, those between blended, and the rows scaled by
+    ``0.1 ln(factor) + 1``."""
+    if dim <= 0 or dim % 2 or factor < 1.0 or theta <= 0:
+        raise ValueError(f"rope_frequencies: dim {dim} (even), theta {theta}, factor {factor} (>= 1)")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    gain = 1.0
+    if scaling == "base":
+        theta = theta * factor ** (dim / (dim - 2)) if dim > 2 else theta
+    f = theta ** (-2.0 * i / dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "by_parts":
+        if not 0 <= low < high or original <= 0:
+            raise ValueError(f"rope_frequencies: turns {low} to {high} in {original} positions")
+        keep = ((original * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+        gain = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "base"):
+        raise ValueError(f"rope_frequencies: unknown scaling {scaling!r}")
+    return f.to(device) if device is not None else f, gain
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
+                v_pages: torch.Tensor, batch: TokenBatch, inv_freq: torch.Tensor, *,
+                q_out: torch.Tensor | None = None, offset: int = 0, interleaved: bool = False,
+                gain: float = 1.0, positions: torch.Tensor | None = None,
+                status: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate q ``[T, heads, dim]`` and k ``[T, kv_heads, dim]`` of the batch's tokens, store k
+    and v at the tokens' positions of the pages; returns the rotated q (``q_out``, by default a
+    new tensor of q's dtype; ``q`` itself is allowed).
+
+    The window of ``2 * len(inv_freq)`` dims at ``offset`` of each head is turned: pairs are
+    (i, i + half) or, ``interleaved``, neighbours.  ``inv_freq`` float64 on the device
+    (``rope_frequencies``); ``positions`` int32 ``[T]`` replaces the cache positions in the
+    angle.  ``status``: an int32 word that gets bit 0 set for a page number outside the pool."""
+    P = _pages(k_pages, v_pages)
+    T, dim, dev = q.shape[0], P.head_dim, k_pages.device
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != dev or \
+            not inv_freq.is_contiguous():
+        raise ValueError("inv_freq: a contiguous float64 vector on the pages' device is wanted")
+    if batch.device != dev:
+        raise ValueError(f"batch on {batch.device}, the pages on {dev}")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    rq, rk, rv = _rows("q", q, T, dim, dev), _rows("k", k, T, dim, dev), _rows("v", v, T, dim, dev)
+    ro = _rows("q_out", q_out, T, dim, dev)
+    for name, x, n in (("positions", positions, T), ("status", status, 1)):
+        if x is not None and (_device_ints(name, x, 1).shape[0] != n or x.device != dev):
+            raise ValueError(f"{name}: {n} int32 value(s) on {dev} are wanted")
+    R = WispRope(inv_freq.data_ptr(), positions.data_ptr() if positions is not None else None,
+                 2 * inv_freq.shape[0], offset, int(interleaved), gain)
+    b = batch.c
+    b.n_tokens = T
+    err = WispErrCtx()
+    rc = lib().wisp_rope_append(C.byref(rq), C.byref(rk), C.byref(rv), C.byref(ro), C.byref(P),
+                                C.byref(b), C.byref(R),
+                                status.data_ptr() if status is not None else None, _on(dev),
+                                C.byref(err))
+    check(rc, err)
+    return q_out
+
+
+def _attend(q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks, return_lse,
+            workspace):
+    P = _pages(k_pages, v_pages)
+    T, dim, dev = q.shape[0], P.head_dim, k_pages.device
+    if batch.device != dev:
+        raise ValueError(f"batch on {batch.device}, the pages on {dev}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    rq, ro = _rows("q", q, T, dim, dev), _rows("out", out, T, dim, dev)
+    lse = torch.empty((T, rq.n_heads), dtype=torch.float32, device=dev) if return_lse else None
+    b = batch.c
+    b.n_tokens = T
+    n_groups = prefix_len.shape[0] if prefix_len is not None else 0
+    L, err, pP, pb = lib(), WispErrCtx(), C.byref(P), C.byref(b)
+    if workspace is None:
+        need = L.wisp_paged_attention_workspace_bytes(pP, pb, rq.n_heads, rq.dtype, n_groups)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError("workspace: a contiguous uint8 tensor on the pages' device is wanted")
+    args = (C.c_float(scale if scale is not None else dim ** -0.5), window, sinks,
+            workspace.data_ptr(), workspace.numel(), _on(dev), C.byref(err))
+    lse_p = lse.data_ptr() if return_lse else None
+    if n_groups:
+        rc = L.wisp_prefix_attention(C.byref(rq), C.byref(ro), lse_p, pP, pb, groups.data_ptr(),
+                                     prefix_len.data_ptr(), n_groups, *args)
+    else:
+        rc = L.wisp_paged_attention(C.byref(rq), C.byref(ro), lse_p, pP, pb, *args)
+    check(rc, err)
+    return (out, lse) if return_lse else out
+
+
+def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, batch: TokenBatch, *,
+              out: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
+              sinks: int = 0, return_lse: bool = False, workspace: torch.Tensor | None = None):
+    """Causal attention of the batch's tokens over their sequences' cached positions.
+
+    q ``[T, heads, dim]`` in fp32 or the pages' dtype; the result has q's dtype.  ``window`` > 0:
+    token i sees position j when i - j < window or j < ``sinks``.  ``scale`` defaults to
+    dim ** -0.5.  ``return_lse``: also the rows' log-sum-exp, fp32 ``[T, heads]`` (-inf for a row
+    that sees nothing; its result is zero).  ``workspace``: uint8, at least
+    ``workspace_bytes``; by default taken from torch's allocator for the call."""
+    return _attend(q, k_pages, v_pages, batch, None, None, out, scale, window, sinks, return_lse,
+                   workspace)
+
+
+def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                     batch: TokenBatch, groups: torch.Tensor, prefix_len: torch.Tensor, *,
+                     out: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
+                     sinks: int = 0, return_lse: bool = False,
+                     workspace: torch.Tensor | None = None):
+    """``attention`` for sequences that share prefixes: the sequences ``groups[g]`` to
+    ``groups[g + 1]`` hold their first ``prefix_len[g]`` positions in the same pages, which are
+    read once for all of the group.  Both int32 on the device."""
+    _device_ints("groups", groups, 1)
+    _device_ints("prefix_len", prefix_len, 1)
+    if groups.shape[0] != prefix_len.shape[0] + 1 or prefix_len.shape[0] == 0 or \
+            groups.device != k_pages.device or prefix_len.device != k_pages.device:
+        raise ValueError(f"groups of {groups.shape[0]} entries, prefix_len of "
+                         f"{prefix_len.shape[0]} (one more and at least one, on the pages' device)")
+    return _attend(q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks,
+                   return_lse, workspace)
+
+
+def workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    batch: TokenBatch, n_groups: int = 0) -> int:
+    """Bytes of workspace an ``attention`` (or, with groups, ``prefix_attention``) call takes."""
+    P = _pages(k_pages, v_pages)
+    b = batch.c
+    b.n_tokens = q.shape[0]
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"q of {q.dtype}")
+    return int(lib().wisp_paged_attention_workspace_bytes(C.byref(P), C.byref(b), q.shape[1],
+                                                          _DTYPES[q.dtype], n_groups))
+
+
+def status(workspace: torch.Tensor) -> int:
+    """The status word of the last attention call on ``workspace`` (0: nothing wrong; bit 0: a
+    page number outside the pool; bit 1: a length beyond the page table; bit 3: a wait ran out).
+    Synchronises the current stream."""
+    return int(lib().wisp_moe_status(workspace.data_ptr(), _on(workspace.device)))
+
+
+def _ints(x) -> array:
+    return x if isinstance(x, array) and x.typecode == "i" else array("i", x)
+
+
+def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst) -> None:
+    """Copy pages ``src[i]`` to ``dst[i]`` (host integers) in every layer of pools
+    ``[n_layers, n_pages, page_size, n_kv_heads, head_dim]`` (or one layer's four dimensions).
+    No page may be both a source and a destination, or twice a destination."""
+    one = k_pages.dim() == 4
+    if not one and (k_pages.dim() != 5 or k_pages.stride() != v_pages.stride() or
+                    k_pages.shape != v_pages.shape or k_pages.shape[0] == 0):
+        raise ValueError("copy_pages: [n_layers, n_pages, page_size, n_kv_heads, head_dim] pools")
+    P = _pages(k_pages, v_pages) if one else _pages(k_pages[0], v_pages[0])
+    s, d = _ints(src), _ints(dst)
+    if len(s) != len(d):
+        raise ValueError(f"copy_pages: {len(s)} sources, {len(d)} destinations")
+    err = WispErrCtx()
+    check(lib().wisp_pages_copy(C.byref(P), 1 if one else k_pages.shape[0],
+                                0 if one else k_pages.stride(0), s.buffer_info()[0],
+                                d.buffer_info()[0], len(s), _on(k_pages.device), C.byref(err)),
+          err)
+
+
+class PagePool:
+    """Which sequence holds which pages of a pool (``wisp_page_pool_*``); host side only.
+
+    ``extend`` gives a sequence room and replaces a shared page that is about to be written by
+    one of its own; ``fork`` shares all pages of a sequence with a new one; ``compact`` renumbers
+    the pages in use to the lowest numbers.  The page copies that these need are queued:
+    ``apply`` runs them on the pools of all layers, and must be called before the pages are
+    next written or read."""
+
+    def __init__(self, n_pages: int, page_size: int):
+        err = WispErrCtx()
+        self.n_pages, self.page_size = n_pages, page_size
+        self._h = lib().wisp_page_pool_create(n_pages, page_size, C.byref(err))
+        if not self._h:
+            raise WispError(err)
+
+    def __del__(self):
+        h, self._h = getattr(self, "_h", None), None
+        if h:
+            lib().wisp_page_pool_destroy(h)
+
+    def _id(self, rc: int, err: WispErrCtx) -> int:
+        if rc < 0:
+            raise WispError(err)
+        return rc
+
+    @property
+    def free_pages(self) -> int:
+        return lib().wisp_page_pool_free_pages(self._h)
+
+    def open(self) -> int:
+        err = WispErrCtx()
+        return self._id(lib().wisp_page_pool_open(self._h, C.byref(err)), err)
+
+    def extend(self, seq: int, length: int) -> None:
+        err = WispErrCtx()
+        check(lib().wisp_page_pool_extend(self._h, seq, length, C.byref(err)), err)
+
+    def truncate(self, seq: int, length: int) -> None:
+        err = WispErrCtx()
+        check(lib().wisp_page_pool_truncate(self._h, seq, length, C.byref(err)), err)
+
+    def fork(self, seq: int) -> int:
+        err = WispErrCtx()
+        return self._id(lib().wisp_page_pool_fork(self._h, seq, C.byref(err)), err)
+
+    def close(self, seq: int) -> None:
+        err = WispErrCtx()
+        check(lib().wisp_page_pool_close(self._h, seq, C.byref(err)), err)
+
+    def compact(self) -> int:
+        err = WispErrCtx()
+        return self._id(lib().wisp_page_pool_compact(self._h, C.byref(err)), err)
+
+    def length(self, seq: int) -> int:
+        err = WispErrCtx()
+        return self._id(lib().wisp_page_pool_length(self._h, seq, C.byref(err)), err)
+
+    def pages(self, seq: int) -> list[int]:
+        err = WispErrCtx()
+        n = self._id(lib().wisp_page_pool_pages(self._h, seq, None, 0, C.byref(err)), err)
+        buf = (C.c_int * max(1, n))()
+        self._id(lib().wisp_page_pool_pages(self._h, seq, buf, n, C.byref(err)), err)
+        return list(buf[:n])
+
+    def moves(self) -> tuple[list[int], list[int]]:
+        """Drain the queued moves: (sources, destinations)."""
+        src, dst = (C.c_int * self.n_pages)(), (C.c_int * self.n_pages)()
+        s: list[int] = []
+        d: list[int] = []
+        while n := lib().wisp_page_pool_moves(self._h, src, dst, self.n_pages):
+            s += src[:n]
+            d += dst[:n]
+        return s, d
+
+    def apply(self, k_pages: torch.Tensor, v_pages: torch.Tensor) -> int:
+        """Run the queued moves on the pools of all layers; how many there were."""
+        s, d = self.moves()
+        at, touched, written = 0, set(), set()
+        for i, (a, b) in enumerate(zip(s, d)):
+            if b in touched or a in written:  # a page was freed and taken again in between
+                copy_pages(k_pages, v_pages, s[at:i], d[at:i])
+                at, touched, written = i, set(), set()
+            touched |= {a, b}
+            written.add(b)
+        if s:
+            copy_pages(k_pages, v_pages, s[at:], d[at:])
+        return len(s)
+
+    def table(self, seqs, width: int | None = None, device=None) -> torch.Tensor:
+        """The sequences' page numbers, int32 ``[len(seqs), width]`` (0 where a row is shorter)."""
+        rows = [self.pages(s) if s is not None else [] for s in seqs]
+        w = max([1] + [len(r) for r in rows]) if width is None else width
+        if any(len(r) > w for r in rows):
+            raise ValueError(f"table: a sequence has more than {w} pages")
+        t = torch.tensor([r + [0] * (w - len(r)) for r in rows], dtype=torch.int32).view(-1, w)
+        return t.to(device) if device is not None else t
