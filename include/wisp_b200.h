@@ -500,13 +500,15 @@ typedef struct WispKvPages {
  * table[s * table_stride + p / page_size].  All three arrays are on the
  * device and are read there: no call synchronises, and a captured step may be
  * replayed after they changed.  max_q: no sequence has more tokens (a bound
- * for the choice of kernels).  A sequence with kv_len 0 (an unused slot) or
+ * for the choice of kernels; tokens beyond it may be left out, with bit 1 of
+ * the status set).  A sequence with kv_len 0 (an unused slot) or
  * with more tokens than positions has tokens that see nothing. */
 typedef struct WispTokenBatch {
     const int* q_start; /* [n_seq + 1] */
     const int* kv_len;  /* [n_seq] */
-    const int* table;   /* [n_seq][table_stride] */
+    const int* table;   /* [n_seq][table_width], rows table_stride apart */
     int n_seq, n_tokens, max_q, table_stride;
+    int table_width; /* pages in a row of the table (0: table_stride) */
 } WispTokenBatch;
 
 /* Rows of the batch's tokens: token t's head h starts at base + t * stride +

@@ -29,6 +29,9 @@ LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libwisp_b200.so"
 OBJ_DIR = ROOT / "_build" / "obj"
 VERSION = "0.2.0"
+# the Python binding of the paged cache's calls: a module of its own, against torch
+BINDING_SRC = "torch_binding.cpp"
+BINDING = LIB_DIR / "_paged_torch.so"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -76,6 +79,7 @@ def _compile(src: Path, obj: Path, hdr_bytes: bytes, force: bool, ptxas_info: bo
 def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     LIB_DIR.mkdir(parents=True, exist_ok=True)
+    binding = ThreadPoolExecutor(max_workers=1).submit(build_binding, verbose)
     hdr_bytes = b"".join(p.read_bytes() for p in _headers())
     objs = [OBJ_DIR / (s + ".o") for s in SOURCES]
     with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 4)) as ex:
@@ -100,7 +104,37 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         lib_stamp.write_text(link_key)
+    binding.result()
     return LIB
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """``_paged_torch.so`` (host code only), rebuilt when its source, the ABI header, torch or
+    the flags change."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    src, torch_lib = CSRC / BINDING_SRC, Path(torch.__file__).parent / "lib"
+    inc = [*cpp_extension.include_paths(device_type="cuda"), sysconfig.get_paths()["include"],
+           str(ROOT / "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{i}" for i in inc), str(src), "-o", str(BINDING), f"-L{torch_lib}",
+           f"-Wl,-rpath,{torch_lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    key = hashlib.sha256(src.read_bytes() + (ROOT / "include" / "wisp_b200.h").read_bytes() +
+                         torch.__version__.encode() + " ".join(cmd).encode()).hexdigest()
+    stamp = BINDING.with_suffix(".so.sha256")
+    if BINDING.exists() and stamp.exists() and stamp.read_text() == key:
+        return BINDING
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(key)
+    return BINDING
 
 
 if __name__ == "__main__":

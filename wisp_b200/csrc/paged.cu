@@ -41,7 +41,7 @@ struct RopeArgs {
     const double* freq;
     int* status;
     size_t qs, ks, vs, qos, page_stride;
-    int n_seq, n_tokens, table_stride, n_pages, page_size, nh, nkv, hd;
+    int n_seq, n_tokens, table_stride, table_width, n_pages, page_size, nh, nkv, hd;
     int dim, off, interleaved, heads_per_cta;
     float gain;
 };
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs A) {
     const int seq = s_seq;
     int pos = -1, page = -1;
     if (seq >= 0) {
-        const long long cap = (long long)A.table_stride * A.page_size;
+        const long long cap = (long long)A.table_width * A.page_size;
         pos = A.kv_len[seq] - (A.q_start[seq + 1] - t);
         if (pos >= 0 && pos < cap) {
             page = A.table[(size_t)seq * A.table_stride + pos / A.page_size];
@@ -288,7 +288,8 @@ WispError check_pages(const char* who, const WispKvPages* P, WispErrCtx* err) {
 }
 
 WispError check_batch(const char* who, const WispTokenBatch* B, WispErrCtx* err) {
-    if (!B || B->n_seq < 0 || B->n_tokens < 0 || B->max_q < 0 || B->table_stride < 0)
+    if (!B || B->n_seq < 0 || B->n_tokens < 0 || B->max_q < 0 || B->table_stride < 0 ||
+        B->table_width < 0 || B->table_width > B->table_stride)
         PG_REFUSE("%s: batch NULL or negative", who);
     if (B->n_tokens > 0 &&
         (B->n_seq == 0 || !B->q_start || !B->kv_len || !B->table || B->table_stride == 0 ||
@@ -344,15 +345,21 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.rows = S.rw[w] * per;
         P.tpt = std::max(1, P.rows / A.gpb);
         P.heads = A.nkv * A.hblocks;
+        P.used_rows = w ? P.rows : (int)std::min<long long>(P.rows, rows);
         P.lanes = std::max(1, ctas / P.heads);
         P.max_items = A.n_tokens / P.tpt + n_seg;
+        P.inlined = n_seg <= kPagedInline && (w ? A.n_tokens : max_q) <= P.tpt;
         P.n_items = reinterpret_cast<int*>(take(4));
+        P.bad = reinterpret_cast<int*>(take(((size_t)P.lanes * P.heads + 1) * 4));
         P.item_off = reinterpret_cast<int*>(take((size_t)(n_seg + 1) * 4));
         P.cum = reinterpret_cast<int*>(take((size_t)(P.max_items + 1) * 4));
         P.items = reinterpret_cast<PagedItem*>(take((size_t)P.max_items * sizeof(PagedItem)));
         const size_t recs = (size_t)P.lanes * P.heads * 2 * P.rows;
         P.part_o = reinterpret_cast<float*>(take(recs * A.hd * 4));
         P.part_ml = reinterpret_cast<float*>(take(recs * 8));
+        P.split = reinterpret_cast<PagedSplit*>(take((size_t)P.lanes * sizeof(PagedSplit)));
+        if (A.n_groups > 0)
+            P.where = reinterpret_cast<PagedWhere*>(take((size_t)A.n_tokens * sizeof(PagedWhere)));
     }
     if (A.n_groups > 0) {
         const size_t recs = (size_t)2 * A.n_tokens * A.nh;
@@ -375,6 +382,7 @@ PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_he
     A.n_tokens = B->n_tokens;
     A.n_groups = n_groups;
     A.table_stride = B->table_stride;
+    A.table_width = B->table_width ? B->table_width : B->table_stride;
     A.n_pages = P->n_pages;
     A.page_size = P->page_size;
     A.page_shift = (P->page_size & (P->page_size - 1)) ? -1 : __builtin_ctz(P->page_size);
@@ -421,9 +429,14 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     if (!ws || !al16(ws) || ws_bytes < S.bytes)
         PG_REFUSE("%s: workspace of %zu bytes, need %zu (16-byte aligned)", who, ws ? ws_bytes : 0,
                   S.bytes);
-    WB_CUDA_RET(launch_paged_plan(A, s), err);
-    if (n_groups > 0) WB_CUDA_RET(launch_paged_attn(A, 1, S.rw[1], q->dtype, P->dtype, s), err);
-    WB_CUDA_RET(launch_paged_attn(A, 0, S.rw[0], q->dtype, P->dtype, s), err);
+    if (!A.plan[0].inlined || (n_groups > 0 && !A.plan[1].inlined))
+        WB_CUDA_RET(launch_paged_plan(A, s), err);
+    if (n_groups > 0 && S.rw[0] == S.rw[1]) {
+        WB_CUDA_RET(launch_paged_attn(A, -1, S.rw[0], q->dtype, P->dtype, s), err);
+    } else {
+        if (n_groups > 0) WB_CUDA_RET(launch_paged_attn(A, 1, S.rw[1], q->dtype, P->dtype, s), err);
+        WB_CUDA_RET(launch_paged_attn(A, 0, S.rw[0], q->dtype, P->dtype, s), err);
+    }
     WB_CUDA_RET(launch_paged_join(A, q->dtype, P->dtype, s), err);
     return WISP_OK;
 }
@@ -507,6 +520,7 @@ extern "C" WispError wisp_rope_append(const WispRows* q, const WispRows* k, cons
     A.n_seq = B->n_seq;
     A.n_tokens = B->n_tokens;
     A.table_stride = B->table_stride;
+    A.table_width = B->table_width ? B->table_width : B->table_stride;
     A.n_pages = P->n_pages;
     A.page_size = P->page_size;
     A.nh = q->n_heads;

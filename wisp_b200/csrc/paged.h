@@ -24,12 +24,26 @@ struct PagedItem {
     int pmin, pmax;      // `mixed` is 0, else each token's is looked up; their range
     int sink0, n_sink, first, n_tiles;
     int mixed;
+    int alone;  // prefix mode: the sequence is in no group
+};
+
+// What the join kernels read about a split row tile (written by the CTA of its first piece).
+struct PagedSplit {
+    int tok0, n_rows;  // n_rows 0: no split item begins in the piece
+    int last;          // the item's last piece
+    int pad;
+};
+struct PagedWhere {
+    int first, last;   // pieces (the same: a whole item)
+    int row0;          // the token's first row in the tile
+    int alone;         // the sequences' plan: no shared prefix comes before this part
 };
 
 // A plan covers all row tiles of one kind: n_items items, cum[i] KV tiles before item i.  The
 // line of all KV tiles is cut into `lanes` equal pieces; one CTA takes a piece for one head.
 struct PagedPlan {
     int* n_items;
+    int* bad;       // [lanes * heads + 1] status bits of each CTA, then of the plan
     int* item_off;  // [segments + 1] items before each sequence (or group)
     int* cum;       // [max_items + 1]
     PagedItem* items;
@@ -38,9 +52,16 @@ struct PagedPlan {
     int tile;        // positions of a KV tile
     int tpt;         // tokens of a row tile
     int rows;        // rows of a row tile
+    int used_rows;   // of them at most so many are used
     int lanes, heads;
+    PagedSplit* split;     // [lanes]: the item that begins in the piece and ends after it
+    PagedWhere* where;     // prefix mode: [n_tokens] the pieces of each token's row tile
     int max_items;
+    int inlined;     // item i is segment i: the attention CTAs find cum themselves
 };
+
+// Segments that an attention CTA counts by itself.
+constexpr int kPagedInline = 512;
 
 struct PagedArgs {
     const void* q;
@@ -57,7 +78,7 @@ struct PagedArgs {
     float* full_ml;         // [2][n_tokens * n_heads][2]
     int* status;
     size_t q_stride, out_stride, page_stride;
-    int n_seq, n_tokens, n_groups, table_stride, n_pages, page_size, page_shift;
+    int n_seq, n_tokens, n_groups, table_stride, table_width, n_pages, page_size, page_shift;
     int nh, nkv, group, gpb, hblocks, hd, window, sinks;
     float scale_log2;
     PagedPlan plan[2];  // [0] the sequences (their own part), [1] the shared prefixes

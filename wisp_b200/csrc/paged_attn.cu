@@ -31,6 +31,11 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kTile = 64;  // positions of a KV tile
+template <bool B>
+struct Bool {
+    static constexpr bool value = B;
+};
+constexpr int kInlineItems = kPagedInline;
 
 template <int HD>
 struct Cfg {
@@ -50,7 +55,7 @@ constexpr size_t attn_smem_bytes() {
 // another inside the loop (each loads what it reads).
 // ------------------------------------------------------------------------
 template <typename T, bool SPLIT, int HD, int RW>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int which) {
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int which0) {
     using C = Cfg<HD>;
     constexpr int kCh = C::kCh, kS = C::kStages;
     constexpr int kNP = kTile * RW / 4;       // positions per warp and tile
@@ -62,6 +67,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
     T* qs = ring + (size_t)kS * C::kStage;    // [16 * RW][HD], swizzled like the cache rows
     __shared__ int s_pos[16 * RW];            // position of each real row (INT_MIN: no row)
     __shared__ float s_fac[16 * RW];          // SPLIT: the row's power-of-two factor
+    __shared__ int s_cum[kInlineItems + 1];
+    __shared__ int s_sum[4];
+    __shared__ int s_bad;
+    const int which = which0 + blockIdx.y;
     const PagedPlan& P = A.plan[which];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c4 = lane & 3;
     const int rw = warp % RW, pw = warp / RW;
@@ -73,18 +82,62 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const int n_items = *P.n_items;
+    const bool inlined = P.inlined != 0;
+    if (tid == 0) {
+        s_bad = 0;
+        P.bad[blockIdx.x] = 0;
+        if (head_lane == 0) P.split[piece].n_rows = 0;
+        if (inlined && blockIdx.x == 0) P.bad[P.lanes * P.heads] = 0;
+    }
+    const int n_items = inlined ? (which ? A.n_groups : A.n_seq) : *P.n_items;
     if (n_items == 0) return;
-    const int total = P.cum[n_items];
-    int x = (int)((long long)piece * total / P.lanes);
-    const int x_end = (int)((long long)(piece + 1) * total / P.lanes);
-    if (x >= x_end) return;
+    const int* cum = inlined ? s_cum : P.cum;
+    if (inlined) {
+        // one row tile per segment: every CTA counts the KV tiles itself, which is shorter than
+        // a kernel of its own before this one (the join kernel reads what one CTA leaves)
+        __syncthreads();  // the words above are cleared
+        int carry = 0;
+        for (int base = 0; base < n_items; base += kThreads) {
+            const int i = base + tid;
+            int n = 0;
+            if (i < n_items) {
+                n = make_item(A, P, which != 0, i, 0).n_tiles;
+                if (blockIdx.x == 0 && which == 0 &&
+                    (length_too_long(A, i) || A.q_start[i + 1] - A.q_start[i] > P.tpt))
+                    P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
+            }
+            int v = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += y;
+            }
+            if (lane == 31) s_sum[warp] = v;
+            __syncthreads();
+            int before = carry;
+            for (int w = 0; w < 4; ++w) {
+                if (w < warp) before += s_sum[w];
+                carry += s_sum[w];
+            }
+            if (i < n_items) s_cum[i] = before + v - n;
+            __syncthreads();
+        }
+        if (tid == 0) s_cum[n_items] = carry;
+        __syncthreads();
+        if (blockIdx.x == 0)  // for the join kernel
+            for (int i = tid; i <= n_items; i += kThreads) P.cum[i] = s_cum[i];
+    }
+    const int total = cum[n_items];
+    const Pieces pieces(P, total);
+    if (piece >= pieces.n) return;
+    int x = pieces.start(piece);
+    const int x_end = pieces.start(piece + 1);
     // the item that holds KV tile x: the last with cum <= x
     int lo = 0, span = n_items;
     while (span > 1) {
         const int step = (span + kThreads - 1) / kThreads;
         const int at = lo + min(tid * step, span - 1);
-        const int hit = __syncthreads_count(tid * step < span && P.cum[at] <= x);
+        const int hit = __syncthreads_count(tid * step < span && cum[at] <= x);
         lo += (hit - 1) * step;
         span = min(step, span - (hit - 1) * step);
     }
@@ -96,36 +149,25 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
     constexpr float kShift = PMath<T>::kPShift;
 
     for (; x < x_end; ++item) {
-        const PagedItem it = P.items[item];
-        const int c0 = P.cum[item];
+        const PagedItem it = inlined ? make_item(A, P, which != 0, item, 0) : P.items[item];
+        const int c0 = cum[item];
+        if (it.n_tiles == 0) continue;
         const int a = x - c0, b = min(it.n_tiles, x_end - c0);  // KV tiles [a, b) of the item
         x = c0 + b;
         const bool whole = a == 0 && b == it.n_tiles;
         const int n_rows = it.ntok * gpb;
-
-        // rows of this tile: positions, and q as swizzled 16-bit rows in shared memory
-        __syncthreads();  // the previous item's readers of s_pos / qs / ring are done
-        for (int r = tid; r < 16 * RW; r += kThreads) {
-            const int wr = r / 16, rr = r & 15;
-            const int row = wr * kRows + rr;
-            int pos = INT_MIN;
-            if (rr < kRows && row < n_rows) {
-                const int t = it.tok0 + row / gpb;
-                pos = it.mixed ? token_position(A, t) : it.pos0 + row / gpb;
+        if (a == 0 && head_lane == 0) {  // what the join kernels need to know
+            if (A.n_groups > 0) {
+                const int last = pieces.of(c0 + it.n_tiles - 1);
+                for (int i = tid; i < it.ntok; i += kThreads)
+                    P.where[it.tok0 + i] = PagedWhere{piece, last, i * A.gpb, it.alone};
+            } else if (!whole && tid == 0) {
+                P.split[piece] =
+                    PagedSplit{it.tok0, it.ntok * A.gpb, pieces.of(c0 + it.n_tiles - 1), 0};
             }
-            s_pos[r] = pos;
         }
-        load_rows<T, SPLIT, HD, RW, kThreads>(A, it.tok0, n_rows, h0, gpb, qs, s_fac);
-        __syncthreads();
 
-        const int prow[2] = {s_pos[rw * 16 + g], SPLIT ? INT_MIN : s_pos[rw * 16 + g + 8]};
-        int hi_row[2], lo_row[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            hi_row[u] = prow[u] == INT_MIN ? 0 : min(it.kv_hi, prow[u] + 1);
-            lo_row[u] = A.window > 0 && prow[u] != INT_MIN ? prow[u] - A.window + 1 : INT_MIN;
-        }
-        const float fac = SPLIT ? s_fac[rw * 16 + g] * sl2 : sl2;
+        __syncthreads();  // the previous item's readers of s_pos / qs / ring are done
         // what some row of the tile sees / what every row sees
         const int any_hi = min(it.kv_hi, it.pmax + 1);
         const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
@@ -133,23 +175,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
         const int all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
         const int sinks = A.window > 0 ? A.sinks : 0;
 
-        uint32_t qf[kQRegs ? HD / 16 : 1][4];
-        auto load_q = [&](int kk, uint32_t (&f)[4]) {
-            const int r = rw * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
-            ldsm4(f, qs + (size_t)r * HD + ((c ^ (r & 7)) * 8));
-        };
-        if (kQRegs) {
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) load_q(kk, qf[kQRegs ? kk : 0]);
-        }
-
         auto tile_at = [&](int i) { return i < it.n_sink ? it.sink0 + i : it.first + i - it.n_sink; };
         // Where the 16 rows [16 * (warp)) of KV tile i start in the cache, one lane each
         // (elements; -1: no row of the tile sees the position).
         auto row_offset = [&](int i) -> long long {
             const int j = tile_at(i) * kTile + warp * 16 + (lane & 15);
             const bool seen = j >= it.kv_lo && j < any_hi && (j >= any_lo || j < sinks);
-            return seen ? page_offset(A, it.seq, j, kvh) : -1;
+            return seen ? page_offset(A, it.seq, j, kvh, &s_bad) : -1;
         };
         auto load_tile = [&](int st, long long off) {
             T* kd = ring + (size_t)st * C::kStage;
@@ -173,13 +205,6 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
             }
         };
 
-        float o[HD / 8][4];
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) o[i][u] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
         // ring: kS - 1 tiles ahead; the page of the next tile to load is looked up one
         // iteration before its copies are issued
         long long off = -1;
@@ -188,6 +213,45 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
             cp_commit();
         }
         if (a + kS - 1 < b) off = row_offset(a + kS - 1);
+        // rows of this tile: positions, and q as swizzled 16-bit rows in shared memory
+        for (int r = tid; r < 16 * RW; r += kThreads) {
+            const int wr = r / 16, rr = r & 15;
+            const int row = wr * kRows + rr;
+            int pos = INT_MIN;
+            if (rr < kRows && row < n_rows) {
+                const int t = it.tok0 + row / gpb;
+                pos = it.mixed ? token_position(A, t) : it.pos0 + row / gpb;
+            }
+            s_pos[r] = pos;
+        }
+        load_rows<T, SPLIT, HD, RW, kThreads>(A, it.tok0, n_rows, h0, gpb, qs, s_fac);
+        __syncthreads();
+
+        const int prow[2] = {s_pos[rw * 16 + g], SPLIT ? INT_MIN : s_pos[rw * 16 + g + 8]};
+        int hi_row[2], lo_row[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            hi_row[u] = prow[u] == INT_MIN ? 0 : min(it.kv_hi, prow[u] + 1);
+            lo_row[u] = A.window > 0 && prow[u] != INT_MIN ? prow[u] - A.window + 1 : INT_MIN;
+        }
+        const float fac = SPLIT ? s_fac[rw * 16 + g] * sl2 : sl2;
+        uint32_t qf[kQRegs ? HD / 16 : 1][4];
+        auto load_q = [&](int kk, uint32_t (&f)[4]) {
+            const int r = rw * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
+            ldsm4(f, qs + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+        };
+        if (kQRegs) {
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) load_q(kk, qf[kQRegs ? kk : 0]);
+        }
+
+        float o[HD / 8][4];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[i][u] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
         int st = 0;
         for (int i = a; i < b; ++i) {
             cp_wait<kS - 2>();
@@ -267,46 +331,52 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
 #pragma unroll
                     for (int u = 0; u < 4; ++u) o[d][u] *= SPLIT ? al[0] : al[u >> 1];
             }
-            // rows that see different positions of one tile: what is hidden from one may be
-            // an infinity or a NaN that another sees
-            const bool mixed_mask = !full && it.pmin != it.pmax;
-#pragma unroll
-            for (int kk = 0; kk < kNP / 16; ++kk) {
-                uint32_t pf[4];
-                if (SPLIT) {
-                    PMath<T>::split2(s[2 * kk][0], s[2 * kk][1], pf[0], pf[1]);
-                    PMath<T>::split2(s[2 * kk + 1][0], s[2 * kk + 1][1], pf[2], pf[3]);
-                } else {
-                    pf[0] = PMath<T>::pack(s[2 * kk][0], s[2 * kk][1]);
-                    pf[1] = PMath<T>::pack(s[2 * kk][2], s[2 * kk][3]);
-                    pf[2] = PMath<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-                    pf[3] = PMath<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+            // Rows that see different positions of one tile: what is hidden from one may be an
+            // infinity or a NaN that another sees.  Such values are looked for first (rare), so
+            // that the usual loop stays short.
+            bool odd = false;
+            if (!full && it.pmin != it.pmax) {
+                for (int i = lane; i < kNP * kCh; i += 32) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vd + (size_t)pw * kNP * HD + i * 8);
+                    odd |= PMath<T>::not_finite(w.x) || PMath<T>::not_finite(w.y) ||
+                           PMath<T>::not_finite(w.z) || PMath<T>::not_finite(w.w);
                 }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+            auto weigh = [&](auto special) {
 #pragma unroll
-                for (int d = 0; d < HD / 8; d += 2) {
-                    const int r = pw * kNP + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-                    const int c = d + (lane >> 4);
-                    uint32_t vf[4];
-                    ldsm4t(vf, vd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
-                    if (mixed_mask) {
-                        bool bad = false;
+                for (int kk = 0; kk < kNP / 16; ++kk) {
+                    uint32_t pf[4];
+                    if (SPLIT) {
+                        PMath<T>::split2(s[2 * kk][0], s[2 * kk][1], pf[0], pf[1]);
+                        PMath<T>::split2(s[2 * kk + 1][0], s[2 * kk + 1][1], pf[2], pf[3]);
+                    } else {
+                        pf[0] = PMath<T>::pack(s[2 * kk][0], s[2 * kk][1]);
+                        pf[1] = PMath<T>::pack(s[2 * kk][2], s[2 * kk][3]);
+                        pf[2] = PMath<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+                        pf[3] = PMath<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+                    }
+                    uint32_t one[4];  // visible places of the 16 x 16 block of weights as ones
+                    if (decltype(special)::value) {
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) bad |= PMath<T>::not_finite(vf[u]);
-                        if (__any_sync(0xffffffffu, bad)) {
-                            // visible places of the 16 x 16 block of weights as ones
-                            uint32_t one[4];
+                        for (int u = 0; u < 4; ++u) {
+                            one[u] = 0;
 #pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                const int row = u & 1;
-                                uint32_t w = 0;
-                                for (int e = 0; e < 2; ++e) {
-                                    const int j = jw + kk * 16 + (u >> 1) * 8 + c4 * 2 + e;
-                                    if (j >= it.kv_lo && j < hi_row[row] &&
-                                        (j >= lo_row[row] || j < sinks))
-                                        w |= PMath<T>::kOne << (16 * e);
-                                }
-                                one[u] = w;
+                            for (int e = 0; e < 2; ++e) {
+                                const int j = jw + kk * 16 + (u >> 1) * 8 + c4 * 2 + e;
+                                if (j >= it.kv_lo && j < hi_row[u & 1] &&
+                                    (j >= lo_row[u & 1] || j < sinks))
+                                    one[u] |= PMath<T>::kOne << (16 * e);
                             }
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < HD / 8; d += 2) {
+                        const int r = pw * kNP + kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+                        const int c = d + (lane >> 4);
+                        uint32_t vf[4];
+                        ldsm4t(vf, vd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+                        if (decltype(special)::value) {
 #pragma unroll
                             for (int n = 0; n < 2; ++n) {
                                 SpecialFrag f{{o[d + n][0], o[d + n][1], o[d + n][2], o[d + n][3]},
@@ -318,11 +388,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
                                 vf[2 * n + 1] = f.b1;
                             }
                         }
+                        PMath<T>::mma(o[d], pf, vf[0], vf[1]);
+                        PMath<T>::mma(o[d + 1], pf, vf[2], vf[3]);
                     }
-                    PMath<T>::mma(o[d], pf, vf[0], vf[1]);
-                    PMath<T>::mma(o[d + 1], pf, vf[2], vf[3]);
                 }
-            }
+            };
+            if (odd) weigh(Bool<true>());
+            else weigh(Bool<false>());
         }
         cp_wait<0>();
 #pragma unroll
@@ -397,78 +469,67 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
             }
         }
     }
+    __syncthreads();
+    if (tid == 0 && s_bad) P.bad[blockIdx.x] = s_bad;
 }
 
 // ------------------------------------------------------------------------
-// Joins the pieces of split items: CTA (piece boundary, head, 4 rows), a warp per row.  The
-// CTA of piece p joins the item that begins in p and ends after it.
+// Joins the pieces of split items.  CTA (piece, head, two rows): the item that begins in the
+// piece and ends after it.  Four warps per row take every fourth piece, in batches whose loads
+// are in flight together, and meet in shared memory in the order of the warps.
 // ------------------------------------------------------------------------
 template <typename T, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs A) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedArgs A) {
+    __shared__ JoinShared S;
     const PagedPlan& P = A.plan[0];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
     const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
-    const int n_items = *P.n_items;
-    if (n_items == 0) return;
-    const int total = P.cum[n_items];
-    const int x0 = (int)((long long)piece * total / P.lanes);
-    const int x1 = (int)((long long)(piece + 1) * total / P.lanes);
-    if (x0 >= x1 || x1 >= total) return;
-    int lo = 0, hi = n_items;  // the item of tile x1 - 1
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (P.cum[mid] <= x1 - 1) lo = mid;
-        else hi = mid;
-    }
-    if (P.cum[lo] < x0 || P.cum[lo + 1] == x1) return;
-    const PagedItem it = P.items[lo];
+    const PagedSplit sp = P.split[piece];
     const int kvh = head_lane / A.hblocks, hb = head_lane - kvh * A.hblocks;
     const int h0 = kvh * A.group + hb * A.gpb, gpb = min(A.gpb, A.group - hb * A.gpb);
-    const int row = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5);
-    if (row >= it.ntok * gpb) return;
-    const int last = (int)(((long long)P.cum[lo + 1] * P.lanes - 1) / total);
+    const int n_rows = sp.n_rows / A.gpb * gpb;  // n_rows counts full blocks of heads
+    if ((int)blockIdx.y * kJoinRows >= n_rows) return;
+    const int which_row = threadIdx.x / (32 * kJoinWarps);
+    const int row = blockIdx.y * kJoinRows + which_row;
     Joined J;
     J.init();
-    J.add_range(A, P, piece, last, head_lane, row);
-    const int t = it.tok0 + row / gpb, h = h0 + row % gpb;
-    J.write<T, SPLIT>(A, t, h);
+    if (row < n_rows) J.add_range(A, P, piece, sp.last, head_lane, row);
+    J.meet(S, which_row);
+    if (row < n_rows && (threadIdx.x / 32) % kJoinWarps == 0)
+        J.write<T, SPLIT>(A, sp.tok0 + row / gpb, h0 + row % gpb);
 }
 
-// Prefix mode: a warp per (token, head) joins its part of the shared prefix and its own part.
+// Prefix mode: the same for CTA (two of the token's heads), over the pieces of the shared
+// prefix and of the sequence's own part.
 template <typename T, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) paged_join2_kernel(PagedArgs A) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join2_kernel(PagedArgs A) {
+    __shared__ JoinShared S;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const long long id = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (id >= (long long)A.n_tokens * A.nh) return;
-    const int t = (int)(id / A.nh), h = (int)(id - (long long)t * A.nh);
-    const int kvh = h / A.group, hg = h - kvh * A.group, hb = hg / A.gpb, hr = hg - hb * A.gpb;
-    const int gpb = min(A.gpb, A.group - hb * A.gpb);
-    const int head_lane = kvh * A.hblocks + hb;
-    const int seq = last_le(A.q_start, A.n_seq, t);
-    if (t < A.q_start[seq] || t >= A.q_start[seq + 1]) return;
+    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
+    const int t = blockIdx.x, which_row = threadIdx.x / (32 * kJoinWarps);
+    const int h = blockIdx.y * kJoinRows + which_row;
+    if (t < A.q_start[0] || t >= A.q_start[A.n_seq]) return;  // nobody's token
     Joined J;
     J.init();
-    for (int which = 0; which < 2; ++which) {
-        const PagedPlan& P = A.plan[which];
-        int seg = seq;
-        if (which) {
-            seg = last_le(A.groups, A.n_groups, seq);
-            if (seq < A.groups[seg] || seq >= A.groups[seg + 1]) continue;
+    if (h < A.nh) {
+        const int kvh = h / A.group, hg = h - kvh * A.group, hb = hg / A.gpb, hr = hg - hb * A.gpb;
+        const int head_lane = kvh * A.hblocks + hb;
+        const PagedWhere own = A.plan[0].where[t];
+        for (int which = 0; which < (own.alone ? 1 : 2); ++which) {
+            const PagedPlan& P = A.plan[which];
+            const PagedWhere w = which ? P.where[t] : own;
+            if (w.first == w.last) J.add_full(A, which, (size_t)t * A.nh + h);
+            else {
+                const int gpb = min(A.gpb, A.group - hb * A.gpb);
+                J.add_range(A, P, w.first, w.last, head_lane, w.row0 / A.gpb * gpb + hr);
+            }
         }
-        const int n_items = *P.n_items;
-        const int t0 = A.q_start[which ? A.groups[seg] : seg];
-        const int item = P.item_off[seg] + (t - t0) / P.tpt;
-        if (item >= n_items) continue;
-        const int row = ((t - t0) % P.tpt) * gpb + hr;
-        const int total = P.cum[n_items], a = P.cum[item], b = P.cum[item + 1];
-        const int first = (int)(((long long)(a + 1) * P.lanes - 1) / total);
-        const int last = (int)(((long long)b * P.lanes - 1) / total);
-        if (first == last) J.add_full(A, which, id);
-        else J.add_range(A, P, first, last, head_lane, row);
     }
-    J.write<T, SPLIT>(A, t, h);
+    J.meet(S, which_row);
+    if (h < A.nh && (threadIdx.x / 32) % kJoinWarps == 0) J.write<T, SPLIT>(A, t, h);
 }
 
 template <typename T, bool SPLIT, int HD, int RW>
@@ -478,8 +539,10 @@ cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    const PagedPlan& P = A.plan[which];
-    return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), smem, s, A, which);
+    // which < 0: both plans in one launch
+    const PagedPlan& P = A.plan[which < 0 ? 0 : which];
+    return launch_pdl(kern, dim3(P.heads * P.lanes, which < 0 ? 2 : 1), dim3(kThreads), smem, s, A,
+                      which < 0 ? 0 : which);
 }
 
 template <typename T, bool SPLIT, int HD>
@@ -499,12 +562,14 @@ cudaError_t launch_t(const PagedArgs& A, int which, int rw, cudaStream_t s) {
 template <typename T, bool SPLIT>
 cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
     if (A.n_groups > 0) {
-        const long long n = ((long long)A.n_tokens * A.nh + 3) / 4;
-        return launch_pdl(paged_join2_kernel<T, SPLIT>, dim3((unsigned)n), dim3(kThreads), 0, s, A);
+        return launch_pdl(paged_join2_kernel<T, SPLIT>,
+                          dim3(A.n_tokens, (A.nh + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads),
+                          0, s, A);
     }
     const PagedPlan& P = A.plan[0];
-    return launch_pdl(paged_join_kernel<T, SPLIT>, dim3(P.heads * P.lanes, (P.rows + 3) / 4),
-                      dim3(kThreads), 0, s, A);
+    return launch_pdl(paged_join_kernel<T, SPLIT>,
+                      dim3(P.heads * P.lanes, (P.used_rows + kJoinRows - 1) / kJoinRows),
+                      dim3(kJoinThreads), 0, s, A);
 }
 
 }  // namespace

@@ -154,9 +154,94 @@ __device__ __forceinline__ int last_le(const int* __restrict__ a, int n, int x) 
 }
 
 __device__ __forceinline__ int cached_positions(const PagedArgs& A, int s) {
-    const long long cap = (long long)A.table_stride * A.page_size;
+    const long long cap = (long long)A.table_width * A.page_size;
     const int n = max(A.kv_len[s], 0);
     return n > cap ? (int)cap : n;
+}
+
+// Does the sequence claim more positions than its table row holds?
+__device__ __forceinline__ bool length_too_long(const PagedArgs& A, int s) {
+    return A.kv_len[s] > (long long)A.table_width * A.page_size;
+}
+
+struct PagedSeg {
+    int t0, t1;  // tokens
+    int s0, s1;  // sequences
+};
+// Sequence i, or group i of sequences.
+__device__ __forceinline__ PagedSeg paged_segment(const PagedArgs& A, bool prefix, int i) {
+    PagedSeg g;
+    g.s0 = prefix ? min(max(A.groups[i], 0), A.n_seq) : i;
+    g.s1 = prefix ? min(max(A.groups[i + 1], g.s0), A.n_seq) : i + 1;
+    g.t0 = min(max(A.q_start[g.s0], 0), A.n_tokens);
+    g.t1 = min(max(A.q_start[g.s1], g.t0), A.n_tokens);
+    if (g.s0 == g.s1) g.t1 = g.t0;
+    return g;
+}
+
+// Row tile `nth` of segment `seg`.
+__device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bool prefix, int seg,
+                                      int nth) {
+    const PagedSeg g = paged_segment(A, prefix, seg);
+    PagedItem it;
+    it.tok0 = g.t0 + nth * P.tpt;
+    it.ntok = min(P.tpt, g.t1 - it.tok0);
+    it.seq = min(g.s0, A.n_seq - 1);
+    it.mixed = prefix && g.s1 - g.s0 > 1;
+    int reach;  // the most that any sequence of the segment has cached
+    if (!it.mixed) {
+        reach = cached_positions(A, it.seq);
+        it.pos0 = reach - (g.t1 - it.tok0);
+        it.pmin = it.pos0;
+        it.pmax = it.pos0 + it.ntok - 1;
+    } else {
+        it.pos0 = 0;
+        it.pmin = 0x7fffffff;
+        it.pmax = -0x7fffffff;
+        reach = 0;
+        int s = g.s0;
+        for (int t = it.tok0; t < it.tok0 + it.ntok; ++t) {
+            while (s + 1 < g.s1 && A.q_start[s + 1] <= t) ++s;
+            const int n = cached_positions(A, s), p = n - (A.q_start[s + 1] - t);
+            it.pmin = min(it.pmin, p);
+            it.pmax = max(it.pmax, p);
+            reach = max(reach, n);
+        }
+    }
+    it.kv_lo = 0;
+    it.alone = 1;
+    it.kv_hi = reach;
+    if (A.n_groups > 0) {
+        int gr = seg;
+        if (!prefix) {  // the sequence's group
+            gr = last_le(A.groups, A.n_groups, g.s0);
+            if (g.s0 < A.groups[gr] || g.s0 >= A.groups[gr + 1]) gr = -1;
+        }
+        const int pl = gr >= 0 ? max(A.prefix_len[gr], 0) : 0;
+        it.alone = gr < 0;
+        if (prefix) it.kv_hi = min(reach, pl);
+        else it.kv_lo = min(reach, pl);
+    }
+    const int end = min(it.kv_hi, it.pmax + 1), begin = it.kv_lo;
+    const int wlo = A.window > 0 ? max(begin, it.pmin - A.window + 1) : begin;
+    it.sink0 = it.n_sink = 0;
+    it.first = begin / P.tile;
+    it.n_tiles = 1;
+    if (end > begin) {
+        const int last = (end + P.tile - 1) / P.tile;  // exclusive
+        int f = min(wlo, end - 1) / P.tile;
+        const int send = min(A.window > 0 ? A.sinks : 0, end);
+        if (send > begin) {
+            it.sink0 = begin / P.tile;
+            const int se = (send + P.tile - 1) / P.tile;
+            if (se >= f) f = it.sink0;  // they meet: one list
+            else it.n_sink = se - it.sink0;
+        }
+        it.first = f;
+        it.n_tiles = it.n_sink + last - f;
+    }
+    if (it.ntok <= 0) it.n_tiles = 0;
+    return it;
 }
 
 __device__ __forceinline__ int token_position(const PagedArgs& A, int t) {
@@ -164,13 +249,14 @@ __device__ __forceinline__ int token_position(const PagedArgs& A, int t) {
     return cached_positions(A, s) - (A.q_start[s + 1] - t);
 }
 
-// Element offset of position j's row for kv head h; -1 (and a status bit) where the table
-// names no page of the pool.
-__device__ __forceinline__ long long page_offset(const PagedArgs& A, int seq, int j, int h) {
+// Element offset of position j's row for kv head h; -1 (and a status bit in shared memory) where
+// the table names no page of the pool.
+__device__ __forceinline__ long long page_offset(const PagedArgs& A, int seq, int j, int h,
+                                                 int* bad) {
     const int p = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size;
     const int page = __ldg(A.table + (size_t)seq * A.table_stride + p);
     if ((unsigned)page >= (unsigned)A.n_pages) {
-        atomicOr(A.status, PG_BAD_PAGE);
+        atomicOr(bad, PG_BAD_PAGE);
         return -1;
     }
     return (long long)page * (long long)A.page_stride +
@@ -238,6 +324,36 @@ __device__ __forceinline__ float row_lse(float M, float L, float shift) {
     return L == 0.f ? -INFINITY : (M + log2f(L) - shift) * 0.69314718055994531f;
 }
 
+// The status word of the call: the CTAs' and the plans' bits, gathered by the last kernel's
+// first CTA.
+__device__ __forceinline__ void gather_status(const PagedArgs& A) {
+    int bits = 0;
+    for (int w = 0; w < (A.n_groups > 0 ? 2 : 1); ++w) {
+        const PagedPlan& P = A.plan[w];
+        for (int i = threadIdx.x; i <= P.lanes * P.heads; i += blockDim.x) bits |= P.bad[i];
+    }
+    const int any = __syncthreads_or(bits & PG_BAD_PAGE) ? PG_BAD_PAGE : 0;
+    const int len = __syncthreads_or(bits & PG_BAD_LENGTH) ? PG_BAD_LENGTH : 0;
+    const int late = __syncthreads_or(bits & PG_TIMEOUT) ? PG_TIMEOUT : 0;
+    if (threadIdx.x == 0) *A.status = any | len | late;
+}
+
+// The line of `total` KV tiles in pieces: as many as there are lanes, each with a tile at least.
+// Piece p starts at tile piece_start(p); tile x lies in piece piece_of(x).
+struct Pieces {
+    int total, n;
+    __device__ Pieces(const PagedPlan& P, int total_) : total(total_), n(min(P.lanes, total_)) {}
+    __device__ __forceinline__ int start(int p) const {
+        if (total <= 1 << 20) return (int)((unsigned)p * (unsigned)total / (unsigned)n);
+        return (int)((unsigned long long)p * total / n);
+    }
+    __device__ __forceinline__ int of(int x) const {
+        if (total <= 1 << 20)
+            return (int)((((unsigned)x + 1) * (unsigned)n - 1) / (unsigned)total);
+        return (int)((((unsigned long long)x + 1) * n - 1) / total);
+    }
+};
+
 __device__ __forceinline__ size_t part_row(const PagedPlan& P, int piece, int head_lane, int slot,
                                            int row) {
     return (((size_t)piece * P.heads + head_lane) * 2 + slot) * P.rows + row;
@@ -292,7 +408,12 @@ struct RowOut {
     }
 };
 
-// A warp's join of one row's partial records, in the order of the pieces.
+// The join of one row's partial records by kJoinWarps warps.
+constexpr int kJoinRows = 2, kJoinWarps = 4, kJoinThreads = 32 * kJoinRows * kJoinWarps;
+struct JoinShared {
+    float2 acc[kJoinRows][kJoinWarps][128];
+    float m[kJoinRows][kJoinWarps], l[kJoinRows][kJoinWarps];
+};
 struct Joined {
     float M, L;
     float2 acc[4];  // dims (i * 32 + lane) * 2
@@ -313,45 +434,89 @@ struct Joined {
             acc[i].y *= e;
         }
     }
-    __device__ __forceinline__ void add(const PagedArgs& A, const float* o, float2 ml) {
-        const float base = M == -INFINITY ? 0.f : M;
-        const float e = ex2(ml.x - base);
-        L = fmaf(ml.y, e, L);
+    // kBatch records whose loads are issued together; `ok` marks those that exist
+    template <int N>
+    __device__ __forceinline__ void add(const PagedArgs& A, const float* const (&o)[N],
+                                        const float* const (&ml)[N], int n) {
         const int lane = threadIdx.x & 31;
+        float2 v[N][4], w[N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = (i * 32 + lane) * 2;
-            if (d >= A.hd) break;
-            const float2 v = *reinterpret_cast<const float2*>(o + d);
-            acc[i].x = fmaf(v.x, e, acc[i].x);
-            acc[i].y = fmaf(v.y, e, acc[i].y);
+        for (int k = 0; k < N; ++k) {
+            w[k] = k < n ? __ldcg(reinterpret_cast<const float2*>(ml[k]))
+                         : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = (i * 32 + lane) * 2;
+                v[k][i] = k < n && d < A.hd ? __ldcg(reinterpret_cast<const float2*>(o[k] + d))
+                                            : make_float2(0.f, 0.f);
+            }
         }
-    }
-    __device__ void add_full(const PagedArgs& A, int which, size_t id) {
-        id += (size_t)which * A.n_tokens * A.nh;
-        const float2 ml = *reinterpret_cast<const float2*>(A.full_ml + id * 2);
-        rebase(fmaxf(M, ml.x));
-        add(A, A.full_o + id * A.hd, ml);
-    }
-    __device__ void add_range(const PagedArgs& A, const PagedPlan& P, int first, int last,
-                              int head_lane, int row) {
-        const int lane = threadIdx.x & 31, total = P.cum[*P.n_items];
         float m = M;
-        for (int p = first + lane; p <= last; p += 32)
-            if (used(P, p, total))
-                m = fmaxf(m, P.part_ml[part_row(P, p, head_lane, p == first, row) * 2]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int k = 0; k < N; ++k) m = fmaxf(m, w[k].x);
         rebase(m);
-#pragma unroll 4
-        for (int p = first; p <= last; ++p) {
-            if (!used(P, p, total)) continue;
-            const size_t id = part_row(P, p, head_lane, p == first, row);
-            add(A, P.part_o + id * A.hd, *reinterpret_cast<const float2*>(P.part_ml + id * 2));
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (k >= n) break;
+            const float e = ex2(w[k].x - base);
+            L = fmaf(w[k].y, e, L);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[i].x = fmaf(v[k][i].x, e, acc[i].x);
+                acc[i].y = fmaf(v[k][i].y, e, acc[i].y);
+            }
         }
     }
-    static __device__ __forceinline__ bool used(const PagedPlan& P, int p, int total) {
-        return (long long)p * total / P.lanes < (long long)(p + 1) * total / P.lanes;
+    __device__ __forceinline__ void add_full(const PagedArgs& A, int which, size_t id) {
+        if ((threadIdx.x / 32) % kJoinWarps != 0) return;
+        id += (size_t)which * A.n_tokens * A.nh;
+        const float* const o[1] = {A.full_o + id * A.hd};
+        const float* const ml[1] = {A.full_ml + id * 2};
+        add<1>(A, o, ml, 1);
+    }
+    __device__ __forceinline__ void add_range(const PagedArgs& A, const PagedPlan& P, int first,
+                                              int last, int head_lane, int row) {
+        constexpr int kBatch = 4;
+        const int warp = (threadIdx.x / 32) % kJoinWarps;
+        for (int p = first + warp; p <= last; p += kBatch * kJoinWarps) {
+            const float *o[kBatch], *ml[kBatch];
+            int n = 0;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int pp = min(p + k * kJoinWarps, last);
+                const size_t id = part_row(P, pp, head_lane, pp == first, row);
+                o[k] = P.part_o + id * A.hd;
+                ml[k] = P.part_ml + id * 2;
+                n += p + k * kJoinWarps <= last;
+            }
+            add<kBatch>(A, o, ml, n);
+        }
+    }
+    // All warps of the block: the row's warps hand their sums to its first one.
+    __device__ __forceinline__ void meet(JoinShared& S, int r) {
+        const int lane = threadIdx.x & 31, warp = (threadIdx.x / 32) % kJoinWarps;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S.acc[r][warp][i * 32 + lane] = acc[i];
+        if (lane == 0) {
+            S.m[r][warp] = M;
+            S.l[r][warp] = L;
+        }
+        __syncthreads();
+        if (warp != 0) return;
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) {
+            const float m = S.m[r][w];
+            rebase(fmaxf(M, m));
+            const float e = ex2(m - (M == -INFINITY ? 0.f : M));
+            L = fmaf(S.l[r][w], e, L);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = S.acc[r][w][i * 32 + lane];
+                acc[i].x = fmaf(v.x, e, acc[i].x);
+                acc[i].y = fmaf(v.y, e, acc[i].y);
+            }
+        }
     }
     template <typename T, bool SPLIT>
     __device__ void write(const PagedArgs& A, int t, int h) {

@@ -19,21 +19,37 @@ device memory and streams only; every kernel is in ``libwisp_b200.so``.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import math
-from array import array
 
 import torch
 
-from .lib import (WispErrCtx, WispError, WispKvPages, WispRope, WispRows, WispTokenBatch, check,
-                  lib)
+from .lib import LIB_PATH, WispErrCtx, WispError, check, lib
 
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_binding = None
 
 
-def _device_ints(name: str, t: torch.Tensor, dim: int) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != dim or not t.is_cuda or t.stride(-1) != 1:
-        raise ValueError(f"{name}: a contiguous int32 CUDA tensor of {dim} dimension(s) is wanted")
-    return t
+def _fail(code: int, message: str, file: bytes, line: int) -> None:
+    err = WispErrCtx(code, message.encode(), file or None, line)
+    raise WispError(err, code)
+
+
+def _torch():
+    """The binding module (raises if it has not been built)."""
+    global _binding
+    if _binding is None:
+        path = LIB_PATH.parent / "_paged_torch.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: run `python -m wisp_b200.build`")
+        spec = importlib.util.spec_from_file_location("_paged_torch", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        L = lib()
+        m.init(*(C.cast(f, C.c_void_p).value for f in
+                 (L.wisp_paged_attention_workspace_bytes, L.wisp_paged_attention,
+                  L.wisp_prefix_attention, L.wisp_rope_append, L.wisp_pages_copy)), _fail)
+        _binding = m
+    return _binding
 
 
 class TokenBatch:
@@ -44,59 +60,12 @@ class TokenBatch:
     ``[n_seq, pages]``: the sequences' page numbers; ``max_q``: no sequence has more tokens.
     One batch serves every layer of a step."""
 
-    __slots__ = ("q_start", "kv_len", "table", "max_q", "c", "device")
+    __slots__ = ("q_start", "kv_len", "table", "max_q")
 
     def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, table: torch.Tensor,
                  max_q: int):
-        self.q_start = _device_ints("q_start", q_start, 1)
-        self.kv_len = _device_ints("kv_len", kv_len, 1)
-        self.table = _device_ints("table", table, 2)
-        n = kv_len.shape[0]
-        if q_start.shape[0] != n + 1 or table.shape[0] != n:
-            raise ValueError(f"{n} sequences: q_start has {q_start.shape[0]} entries, table "
-                             f"{table.shape[0]} rows")
-        self.device = kv_len.device
-        if q_start.device != self.device or table.device != self.device:
-            raise ValueError("q_start, kv_len and table are on different devices")
-        self.max_q = int(max_q)
-        self.c = WispTokenBatch(q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(), n, 0,
-                                self.max_q, table.stride(0) if n > 1 else table.shape[1])
-
-
-def _pages(k: torch.Tensor, v: torch.Tensor) -> WispKvPages:
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
-        raise ValueError("k_pages and v_pages: two [n_pages, page_size, n_kv_heads, head_dim] "
-                         "tensors of one shape, layout and dtype are wanted")
-    n, page, heads, dim = k.shape
-    if k.stride()[1:] != (heads * dim, dim, 1):
-        raise ValueError("k_pages: a page's positions, heads and dims must be contiguous")
-    if not k.is_cuda or v.device != k.device:
-        raise ValueError("k_pages and v_pages must be on one CUDA device")
-    if k.dtype not in _DTYPES:
-        raise ValueError(f"k_pages of {k.dtype} (fp16 or bf16)")
-    stride = k.stride(0) if n > 1 else page * heads * dim
-    return WispKvPages(k.data_ptr(), v.data_ptr(), stride, n, page, heads, dim, _DTYPES[k.dtype])
-
-
-def _rows(name: str, x: torch.Tensor, n: int, dim: int, device) -> WispRows:
-    if x.dim() != 3 or x.shape[0] != n or x.shape[2] != dim:
-        raise ValueError(f"{name}: [{n}, heads, {dim}] is wanted, got {list(x.shape)}")
-    heads = x.shape[1]
-    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim):
-        raise ValueError(f"{name}: a row's heads must be contiguous")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the pages on {device}")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"{name} of {x.dtype} (fp32, fp16 or bf16)")
-    return WispRows(x.data_ptr(), x.stride(0) if n > 1 else heads * dim, heads, _DTYPES[x.dtype])
-
-
-def _on(device):
-    """The device's current stream, with the device made current for the launch."""
-    if torch.cuda.current_device() != device.index:
-        raise ValueError(f"tensors on {device}, but the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream
+        (_binding or _torch()).check_batch(q_start, kv_len, table, max_q)
+        self.q_start, self.kv_len, self.table, self.max_q = q_start, kv_len, table, max_q
 
 
 def rope_frequencies(dim: int, theta: float = 10000.0, *, scaling: str | None = None,
@@ -142,62 +111,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
     (i, i + half) or, ``interleaved``, neighbours.  ``inv_freq`` float64 on the device
     (``rope_frequencies``); ``positions`` int32 ``[T]`` replaces the cache positions in the
     angle.  ``status``: an int32 word that gets bit 0 set for a page number outside the pool."""
-    P = _pages(k_pages, v_pages)
-    T, dim, dev = q.shape[0], P.head_dim, k_pages.device
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != dev or \
-            not inv_freq.is_contiguous():
-        raise ValueError("inv_freq: a contiguous float64 vector on the pages' device is wanted")
-    if batch.device != dev:
-        raise ValueError(f"batch on {batch.device}, the pages on {dev}")
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    rq, rk, rv = _rows("q", q, T, dim, dev), _rows("k", k, T, dim, dev), _rows("v", v, T, dim, dev)
-    ro = _rows("q_out", q_out, T, dim, dev)
-    for name, x, n in (("positions", positions, T), ("status", status, 1)):
-        if x is not None and (_device_ints(name, x, 1).shape[0] != n or x.device != dev):
-            raise ValueError(f"{name}: {n} int32 value(s) on {dev} are wanted")
-    R = WispRope(inv_freq.data_ptr(), positions.data_ptr() if positions is not None else None,
-                 2 * inv_freq.shape[0], offset, int(interleaved), gain)
-    b = batch.c
-    b.n_tokens = T
-    err = WispErrCtx()
-    rc = lib().wisp_rope_append(C.byref(rq), C.byref(rk), C.byref(rv), C.byref(ro), C.byref(P),
-                                C.byref(b), C.byref(R),
-                                status.data_ptr() if status is not None else None, _on(dev),
-                                C.byref(err))
-    check(rc, err)
-    return q_out
-
-
-def _attend(q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks, return_lse,
-            workspace):
-    P = _pages(k_pages, v_pages)
-    T, dim, dev = q.shape[0], P.head_dim, k_pages.device
-    if batch.device != dev:
-        raise ValueError(f"batch on {batch.device}, the pages on {dev}")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    rq, ro = _rows("q", q, T, dim, dev), _rows("out", out, T, dim, dev)
-    lse = torch.empty((T, rq.n_heads), dtype=torch.float32, device=dev) if return_lse else None
-    b = batch.c
-    b.n_tokens = T
-    n_groups = prefix_len.shape[0] if prefix_len is not None else 0
-    L, err, pP, pb = lib(), WispErrCtx(), C.byref(P), C.byref(b)
-    if workspace is None:
-        need = L.wisp_paged_attention_workspace_bytes(pP, pb, rq.n_heads, rq.dtype, n_groups)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError("workspace: a contiguous uint8 tensor on the pages' device is wanted")
-    args = (C.c_float(scale if scale is not None else dim ** -0.5), window, sinks,
-            workspace.data_ptr(), workspace.numel(), _on(dev), C.byref(err))
-    lse_p = lse.data_ptr() if return_lse else None
-    if n_groups:
-        rc = L.wisp_prefix_attention(C.byref(rq), C.byref(ro), lse_p, pP, pb, groups.data_ptr(),
-                                     prefix_len.data_ptr(), n_groups, *args)
-    else:
-        rc = L.wisp_paged_attention(C.byref(rq), C.byref(ro), lse_p, pP, pb, *args)
-    check(rc, err)
-    return (out, lse) if return_lse else out
+    return (_binding or _torch()).rope_append(
+        q, k, v, k_pages, v_pages, batch, inv_freq, q_out, offset, interleaved, gain, positions,
+        status)
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, batch: TokenBatch, *,
@@ -210,8 +126,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bat
     dim ** -0.5.  ``return_lse``: also the rows' log-sum-exp, fp32 ``[T, heads]`` (-inf for a row
     that sees nothing; its result is zero).  ``workspace``: uint8, at least
     ``workspace_bytes``; by default taken from torch's allocator for the call."""
-    return _attend(q, k_pages, v_pages, batch, None, None, out, scale, window, sinks, return_lse,
-                   workspace)
+    return (_binding or _torch()).attend(
+        q, k_pages, v_pages, batch, None, None, out, scale, window, sinks, return_lse, workspace)
 
 
 def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -222,56 +138,29 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     """``attention`` for sequences that share prefixes: the sequences ``groups[g]`` to
     ``groups[g + 1]`` hold their first ``prefix_len[g]`` positions in the same pages, which are
     read once for all of the group.  Both int32 on the device."""
-    _device_ints("groups", groups, 1)
-    _device_ints("prefix_len", prefix_len, 1)
-    if groups.shape[0] != prefix_len.shape[0] + 1 or prefix_len.shape[0] == 0 or \
-            groups.device != k_pages.device or prefix_len.device != k_pages.device:
-        raise ValueError(f"groups of {groups.shape[0]} entries, prefix_len of "
-                         f"{prefix_len.shape[0]} (one more and at least one, on the pages' device)")
-    return _attend(q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks,
-                   return_lse, workspace)
+    return (_binding or _torch()).attend(
+        q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks, return_lse, workspace)
 
 
 def workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     batch: TokenBatch, n_groups: int = 0) -> int:
     """Bytes of workspace an ``attention`` (or, with groups, ``prefix_attention``) call takes."""
-    P = _pages(k_pages, v_pages)
-    b = batch.c
-    b.n_tokens = q.shape[0]
-    if q.dtype not in _DTYPES:
-        raise ValueError(f"q of {q.dtype}")
-    return int(lib().wisp_paged_attention_workspace_bytes(C.byref(P), C.byref(b), q.shape[1],
-                                                          _DTYPES[q.dtype], n_groups))
+    return (_binding or _torch()).workspace_bytes(q, k_pages, v_pages, batch, n_groups)
 
 
 def status(workspace: torch.Tensor) -> int:
     """The status word of the last attention call on ``workspace`` (0: nothing wrong; bit 0: a
     page number outside the pool; bit 1: a length beyond the page table; bit 3: a wait ran out).
     Synchronises the current stream."""
-    return int(lib().wisp_moe_status(workspace.data_ptr(), _on(workspace.device)))
-
-
-def _ints(x) -> array:
-    return x if isinstance(x, array) and x.typecode == "i" else array("i", x)
+    return int(lib().wisp_moe_status(workspace.data_ptr(),
+                                     torch.cuda.current_stream(workspace.device).cuda_stream))
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst) -> None:
     """Copy pages ``src[i]`` to ``dst[i]`` (host integers) in every layer of pools
     ``[n_layers, n_pages, page_size, n_kv_heads, head_dim]`` (or one layer's four dimensions).
     No page may be both a source and a destination, or twice a destination."""
-    one = k_pages.dim() == 4
-    if not one and (k_pages.dim() != 5 or k_pages.stride() != v_pages.stride() or
-                    k_pages.shape != v_pages.shape or k_pages.shape[0] == 0):
-        raise ValueError("copy_pages: [n_layers, n_pages, page_size, n_kv_heads, head_dim] pools")
-    P = _pages(k_pages, v_pages) if one else _pages(k_pages[0], v_pages[0])
-    s, d = _ints(src), _ints(dst)
-    if len(s) != len(d):
-        raise ValueError(f"copy_pages: {len(s)} sources, {len(d)} destinations")
-    err = WispErrCtx()
-    check(lib().wisp_pages_copy(C.byref(P), 1 if one else k_pages.shape[0],
-                                0 if one else k_pages.stride(0), s.buffer_info()[0],
-                                d.buffer_info()[0], len(s), _on(k_pages.device), C.byref(err)),
-          err)
+    (_binding or _torch()).copy_pages(k_pages, v_pages, src, dst)
 
 
 class PagePool:
