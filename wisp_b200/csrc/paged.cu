@@ -17,8 +17,13 @@
 namespace wb {
 
 cudaError_t launch_paged_plan(const PagedArgs& A, cudaStream_t s);
-cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
-                              cudaStream_t s);
+cudaError_t launch_paged_attn(const PagedArgs& A, int which, bool both, int rw, int q_dtype,
+                              int kv_dtype, cudaStream_t s);
+cudaError_t launch_paged_mma(const PagedArgs& A, int which, int q_dtype, int kv_dtype,
+                             cudaStream_t s);
+bool paged_mma_takes(int hd);
+int paged_mma_tile();
+int paged_mma_rows(bool split);
 cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s);
 int paged_attn_tile();
 int paged_attn_rw(int rows, bool split);
@@ -312,11 +317,15 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
 // Attention: what runs, and its workspace
 // ------------------------------------------------------------------------
 struct AttnShape {
-    int rw[2];  // 16-row MMA tiles of the two plans' row tiles
+    int rw[PLANS];  // 16-row MMA tiles of the plan's row tiles; 0: the tensor-core kernel
     size_t bytes;
 };
 
 // Fills the geometry, plans and (with a workspace) pointers of a call.
+//
+// Which kernel: a sequence (or group) whose rows for one kv head fit one 16-row tile of
+// mma.sync (8 rows in fp32) goes through paged_attn_kernel, whose CTAs are bound by HBM; more
+// rows go to tcgen05 where it takes the head dim, else to row tiles of two or four 16-row tiles.
 AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     const int per = split ? 8 : 16;
@@ -329,26 +338,46 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     };
     A.status = reinterpret_cast<int*>(ws);
     A.group = A.nh / A.nkv;
-    // rows of a row tile: the sequence's own, at most 4 MMA tiles; heads of a group beyond that
-    // become blocks of their own
-    A.gpb = std::min(A.group, 4 * per);
-    A.hblocks = (A.group + A.gpb - 1) / A.gpb;
-    const int n_plans = A.n_groups > 0 ? 2 : 1;
-    const int ctas = paged_attn_ctas(A.hd) * sm_count();
-    for (int w = 0; w < n_plans; ++w) {
+    const bool mma = paged_mma_takes(A.hd);
+    const int few = per / A.group;  // tokens whose rows fit one 16-row tile
+    const bool even = A.n_seq == 1 || (long long)A.n_seq * max_q == A.n_tokens;
+    PagedWhere* where = nullptr;
+    for (int w = 0; w < PLANS; ++w) {
         PagedPlan& P = A.plan[w];
-        const int n_seg = w ? A.n_groups : A.n_seq;
-        const long long rows =
-            w ? (long long)((A.n_tokens + n_seg - 1) / n_seg) * A.gpb : (long long)max_q * A.gpb;
-        S.rw[w] = paged_attn_rw((int)std::min<long long>(rows, 4 * per), split);
-        P.tile = paged_attn_tile();
-        P.rows = S.rw[w] * per;
-        P.tpt = std::max(1, P.rows / A.gpb);
-        P.heads = A.nkv * A.hblocks;
-        P.used_rows = w ? P.rows : (int)std::min<long long>(P.rows, rows);
-        P.lanes = std::max(1, ctas / P.heads);
+        P = PagedPlan{};
+        const int n_seg = w == PLAN_PREFIX ? A.n_groups : A.n_seq;
+        long long tokens = max_q;  // of the plan's largest segment (a guess for a prefix)
+        bool on_mma = false;
+        P.max_tok = 0x7fffffff;
+        if (w == PLAN_PREFIX) {
+            if (A.n_groups == 0) continue;
+            tokens = (A.n_tokens + n_seg - 1) / n_seg;
+            on_mma = mma && tokens > few;
+        } else if (w == PLAN_MANY) {
+            if (!mma || max_q <= few) continue;
+            P.min_tok = A.plan[PLAN_FEW].used ? few + 1 : 0;
+            on_mma = true;
+        } else if (mma) {
+            if (few == 0 || (even && max_q > few)) continue;
+            if (max_q > few) P.max_tok = few;
+            tokens = std::min<long long>(tokens, few);
+        }
+        P.used = 1;
+        const int most = on_mma ? paged_mma_rows(split) : 4 * per;
+        P.gpb = std::min(A.group, most);
+        P.hblocks = (A.group + P.gpb - 1) / P.gpb;
+        P.heads = A.nkv * P.hblocks;
+        const int rows = (int)std::min<long long>(tokens * P.gpb, most);
+        S.rw[w] = on_mma ? 0 : paged_attn_rw(rows, split);
+        P.tile = on_mma ? paged_mma_tile() : paged_attn_tile();
+        P.rows = on_mma ? most : S.rw[w] * per;
+        P.tpt = std::max(1, P.rows / P.gpb);
+        P.used_rows = w == PLAN_PREFIX ? P.rows : std::min(rows, P.rows);
+        const int ctas = (on_mma ? 1 : paged_attn_ctas(A.hd)) * sm_count();
+        P.lanes = std::min(4095, std::max(1, ctas / P.heads));
         P.max_items = A.n_tokens / P.tpt + n_seg;
-        P.inlined = n_seg <= kPagedInline && (w ? A.n_tokens : max_q) <= P.tpt;
+        P.inlined = !on_mma && n_seg <= kPagedInline &&
+                    (w == PLAN_PREFIX ? A.n_tokens : std::min(max_q, P.max_tok)) <= P.tpt;
         P.n_items = reinterpret_cast<int*>(take(4));
         P.bad = reinterpret_cast<int*>(take(((size_t)P.lanes * P.heads + 1) * 4));
         P.item_off = reinterpret_cast<int*>(take((size_t)(n_seg + 1) * 4));
@@ -358,8 +387,12 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.part_o = reinterpret_cast<float*>(take(recs * A.hd * 4));
         P.part_ml = reinterpret_cast<float*>(take(recs * 8));
         P.split = reinterpret_cast<PagedSplit*>(take((size_t)P.lanes * sizeof(PagedSplit)));
-        if (A.n_groups > 0)
-            P.where = reinterpret_cast<PagedWhere*>(take((size_t)A.n_tokens * sizeof(PagedWhere)));
+        if (on_mma) P.redo = reinterpret_cast<int*>(take((size_t)P.max_items * P.heads * 4));
+        if (A.n_groups > 0) {
+            const size_t bytes = (size_t)A.n_tokens * sizeof(PagedWhere);
+            if (w == PLAN_PREFIX) P.where = reinterpret_cast<PagedWhere*>(take(bytes));
+            else P.where = where = where ? where : reinterpret_cast<PagedWhere*>(take(bytes));
+        }
     }
     if (A.n_groups > 0) {
         const size_t recs = (size_t)2 * A.n_tokens * A.nh;
@@ -368,6 +401,12 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     }
     S.bytes = at;
     return S;
+}
+
+cudaError_t launch_plan_kernel(const PagedArgs& A, const AttnShape& S, int which, bool both,
+                               int q_dtype, int kv_dtype, cudaStream_t s) {
+    return S.rw[which] ? launch_paged_attn(A, which, both, S.rw[which], q_dtype, kv_dtype, s)
+                       : launch_paged_mma(A, which, q_dtype, kv_dtype, s);
 }
 
 PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_heads, int n_groups) {
@@ -429,13 +468,16 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     if (!ws || !al16(ws) || ws_bytes < S.bytes)
         PG_REFUSE("%s: workspace of %zu bytes, need %zu (16-byte aligned)", who, ws ? ws_bytes : 0,
                   S.bytes);
-    if (!A.plan[0].inlined || (n_groups > 0 && !A.plan[1].inlined))
-        WB_CUDA_RET(launch_paged_plan(A, s), err);
-    if (n_groups > 0 && S.rw[0] == S.rw[1]) {
-        WB_CUDA_RET(launch_paged_attn(A, -1, S.rw[0], q->dtype, P->dtype, s), err);
-    } else {
-        if (n_groups > 0) WB_CUDA_RET(launch_paged_attn(A, 1, S.rw[1], q->dtype, P->dtype, s), err);
-        WB_CUDA_RET(launch_paged_attn(A, 0, S.rw[0], q->dtype, P->dtype, s), err);
+    bool plan = false;
+    for (int w = 0; w < PLANS; ++w) plan |= A.plan[w].used && !A.plan[w].inlined;
+    if (plan) WB_CUDA_RET(launch_paged_plan(A, s), err);
+    // the shared prefixes go with the sequences' own parts where one kernel takes both
+    const bool both = A.plan[PLAN_PREFIX].used && A.plan[PLAN_FEW].used && S.rw[PLAN_PREFIX] &&
+                      S.rw[PLAN_PREFIX] == S.rw[PLAN_FEW];
+    const int order[PLANS] = {PLAN_PREFIX, PLAN_MANY, PLAN_FEW};
+    for (int w : order) {
+        if (!A.plan[w].used || (w == PLAN_PREFIX && both)) continue;
+        WB_CUDA_RET(launch_plan_kernel(A, S, w, both && w == PLAN_FEW, q->dtype, P->dtype, s), err);
     }
     WB_CUDA_RET(launch_paged_join(A, q->dtype, P->dtype, s), err);
     return WISP_OK;

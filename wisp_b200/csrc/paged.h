@@ -10,58 +10,68 @@
 
 namespace wb {
 
-// Status bits of a paged call's workspace (wisp_paged_status).
+// Status bits of a paged call's workspace.
 enum { PG_BAD_PAGE = 1, PG_BAD_LENGTH = 2, PG_TIMEOUT = 8 };
 
 // One row tile: consecutive tokens whose rows (token, query head of the kv head) go through
 // the same cached positions.  Positions come in tiles of `tile` from 0: the item's list is
 // [sink0, sink0 + n_sink) and then n_tiles - n_sink tiles from `first` on.
 struct PagedItem {
-    int tok0, ntok;      // tokens
-    int seq;             // row of the page table
-    int kv_lo, kv_hi;    // positions outside [kv_lo, kv_hi) belong to another item or to none
-    int pos0;            // position of tok0; the tokens' positions follow one another when
-    int pmin, pmax;      // `mixed` is 0, else each token's is looked up; their range
+    int tok0, ntok;    // tokens
+    int seq;           // row of the page table
+    int kv_lo, kv_hi;  // positions outside [kv_lo, kv_hi) belong to another item or to none
+    int pos0;          // position of tok0; the tokens' positions follow one another when
+    int pmin, pmax;    // `mixed` is 0, else each token's is looked up; their range
     int sink0, n_sink, first, n_tiles;
     int mixed;
     int alone;  // prefix mode: the sequence is in no group
 };
 
-// What the join kernels read about a split row tile (written by the CTA of its first piece).
+// What the join kernels read about a piece (written by the attention CTA of its first head).
 struct PagedSplit {
-    int tok0, n_rows;  // n_rows 0: no split item begins in the piece
-    int last;          // the item's last piece
-    int pad;
+    int tok0, n_rows;  // the item that begins in the piece and ends after it (n_rows 0: none)
+    int last;          // its last piece
+    int item;
+    int item0, item1;  // the items that begin in the piece
 };
+// Prefix mode: where the parts of a token's rows are.
 struct PagedWhere {
-    int first, last;   // pieces (the same: a whole item)
-    int row0;          // the token's first row in the tile
-    int alone;         // the sequences' plan: no shared prefix comes before this part
+    int first, last;  // pieces (the same: a whole item)
+    int row0;         // the token's first row in the tile
+    int alone;        // its own part: no shared prefix comes before it
+    int plan, item;
 };
 
-// A plan covers all row tiles of one kind: n_items items, cum[i] KV tiles before item i.  The
-// line of all KV tiles is cut into `lanes` equal pieces; one CTA takes a piece for one head.
+// A plan covers the row tiles of one kind: n_items items, cum[i] KV tiles before item i.  The
+// line of all KV tiles is cut into at most `lanes` equal pieces; one CTA takes a piece for one
+// block of query heads.
 struct PagedPlan {
     int* n_items;
     int* bad;       // [lanes * heads + 1] status bits of each CTA, then of the plan
     int* item_off;  // [segments + 1] items before each sequence (or group)
     int* cum;       // [max_items + 1]
     PagedItem* items;
-    float* part_o;   // [lanes][heads][2][rows][hd]: pieces of items that lanes share
-    float* part_ml;  // [lanes][heads][2][rows][2]: running maximum (log2) and sum
-    int tile;        // positions of a KV tile
-    int tpt;         // tokens of a row tile
-    int rows;        // rows of a row tile
-    int used_rows;   // of them at most so many are used
-    int lanes, heads;
-    PagedSplit* split;     // [lanes]: the item that begins in the piece and ends after it
-    PagedWhere* where;     // prefix mode: [n_tokens] the pieces of each token's row tile
+    float* part_o;      // [lanes][heads][2][rows][hd]: pieces of items that lanes share
+    float* part_ml;     // [lanes][heads][2][rows][2]: see PagedArgs.full_ml
+    PagedSplit* split;  // [lanes]
+    PagedWhere* where;  // prefix mode: [n_tokens]
+    int* redo;          // [max_items][heads], set for items to be worked out without tiles
+    int tile;           // positions of a KV tile
+    int tpt;            // tokens of a row tile
+    int rows;           // rows of a row tile
+    int used_rows;      // of them at most so many are used
+    int gpb, hblocks;   // query heads of a block, blocks of a kv head
+    int lanes, heads;   // heads = kv heads * hblocks
     int max_items;
-    int inlined;     // item i is segment i: the attention CTAs find cum themselves
+    int min_tok, max_tok;  // sequences with fewer or more tokens are another plan's
+    int inlined;           // item i is segment i: the attention CTAs find cum themselves
+    int used;              // the call has this plan
 };
 
 // Segments that an attention CTA counts by itself.
 constexpr int kPagedInline = 512;
+
+enum { PLAN_FEW = 0, PLAN_PREFIX = 1, PLAN_MANY = 2, PLANS = 3 };
 
 struct PagedArgs {
     const void* q;
@@ -74,14 +84,16 @@ struct PagedArgs {
     const int* table;
     const int* groups;      // prefix mode: [n_groups + 1] first sequence of each group
     const int* prefix_len;  // [n_groups]
-    float* full_o;          // prefix mode: [2][n_tokens * n_heads][hd], whole items' rows
-    float* full_ml;         // [2][n_tokens * n_heads][2]
+    float* full_o;          // prefix mode: [own, shared][n_tokens * n_heads][hd], whole items
+    float* full_ml;  // the same [2]: M and the sum of weights 2^(score - M), score in log2 units
     int* status;
     size_t q_stride, out_stride, page_stride;
     int n_seq, n_tokens, n_groups, table_stride, table_width, n_pages, page_size, page_shift;
-    int nh, nkv, group, gpb, hblocks, hd, window, sinks;
+    int nh, nkv, group, hd, window, sinks;
     float scale_log2;
-    PagedPlan plan[2];  // [0] the sequences (their own part), [1] the shared prefixes
+    // [PLAN_FEW] sequences of few rows (their own part), [PLAN_PREFIX] the shared prefixes,
+    // [PLAN_MANY] sequences of many rows
+    PagedPlan plan[PLANS];
 };
 
 }  // namespace wb

@@ -12,9 +12,10 @@
 // partial results a second kernel joins in a fixed order (results do not depend on timing).
 //
 // Products run on mma.sync m16n8k16 with fp32 accumulators.  32-bit rows are split into two
-// 16-bit parts (x ~= hi + lo, 22 bits in fp16, 16 in bf16) that fill the two halves of a
+// 16-bit parts (x ~= hi + lo, 22 bits in fp16) that fill the two halves of a
 // 16-row tile, so 8 rows cost one instruction and their two sums meet in one thread; the
-// weights p are split the same way.  In fp16, p is scaled by 2^kPShift so that small weights
+// weights p are split the same way.  bf16 parts hold 8 bits each, so there it takes three and a
+// second instruction (two parts left the results 2.8e-6 off, ten times the fp32 rounding).  In fp16, p is scaled by 2^kPShift so that small weights
 // of long contexts stay above the subnormals (the factor cancels in the quotient).
 
 #include <cuda_bf16.h>
@@ -39,14 +40,14 @@ constexpr int kInlineItems = kPagedInline;
 
 template <int HD>
 struct Cfg {
-    static constexpr int kStages = 3;
+    static constexpr int kStages = HD <= 128 ? 3 : 2;
     static constexpr int kCh = HD / 8;            // 16-byte pieces of a row
     static constexpr int kStage = 2 * kTile * HD;  // elements: K then V
 };
 
-template <int HD, int RW>
+template <int HD, int RW, int FRAGS>
 constexpr size_t attn_smem_bytes() {
-    return (size_t)Cfg<HD>::kStages * Cfg<HD>::kStage * 2 + (size_t)16 * RW * HD * 2;
+    return (size_t)Cfg<HD>::kStages * Cfg<HD>::kStage * 2 + (size_t)16 * RW * HD * 2 * FRAGS;
 }
 
 // ------------------------------------------------------------------------
@@ -55,29 +56,30 @@ constexpr size_t attn_smem_bytes() {
 // another inside the loop (each loads what it reads).
 // ------------------------------------------------------------------------
 template <typename T, bool SPLIT, int HD, int RW>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int which0) {
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs A, int which0) {
     using C = Cfg<HD>;
     constexpr int kCh = C::kCh, kS = C::kStages;
     constexpr int kNP = kTile * RW / 4;       // positions per warp and tile
     constexpr int kNT = kNP / 8;              // score tiles of 8 positions
     constexpr int kRows = SPLIT ? 8 : 16;     // real rows per warp
-    constexpr bool kQRegs = HD <= 128;
+    constexpr int kF = SPLIT ? PMath<T>::kFrags : 1;  // 16-row fragments that hold a row's parts
+    constexpr bool kQRegs = HD <= 128 && kF == 1;
     extern __shared__ __align__(128) char smem[];
     T* ring = reinterpret_cast<T*>(smem);
-    T* qs = ring + (size_t)kS * C::kStage;    // [16 * RW][HD], swizzled like the cache rows
+    T* qs = ring + (size_t)kS * C::kStage;    // [kF][16 * RW][HD], swizzled like the cache rows
     __shared__ int s_pos[16 * RW];            // position of each real row (INT_MIN: no row)
     __shared__ float s_fac[16 * RW];          // SPLIT: the row's power-of-two factor
     __shared__ int s_cum[kInlineItems + 1];
     __shared__ int s_sum[4];
     __shared__ int s_bad;
-    const int which = which0 + blockIdx.y;
+    const int which = blockIdx.y ? PLAN_PREFIX : which0;
     const PagedPlan& P = A.plan[which];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c4 = lane & 3;
     const int rw = warp % RW, pw = warp / RW;
     const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
-    const int kvh = head_lane / A.hblocks, hb = head_lane - kvh * A.hblocks;
-    const int h0 = kvh * A.group + hb * A.gpb;             // first query head
-    const int gpb = min(A.gpb, A.group - hb * A.gpb);      // query heads of this block
+    const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
+    const int h0 = kvh * A.group + hb * P.gpb;             // first query head
+    const int gpb = min(P.gpb, A.group - hb * P.gpb);      // query heads of this block
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -86,10 +88,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
     if (tid == 0) {
         s_bad = 0;
         P.bad[blockIdx.x] = 0;
-        if (head_lane == 0) P.split[piece].n_rows = 0;
+        if (head_lane == 0) P.split[piece] = PagedSplit{0, 0, 0, 0, 0, 0};
         if (inlined && blockIdx.x == 0) P.bad[P.lanes * P.heads] = 0;
     }
-    const int n_items = inlined ? (which ? A.n_groups : A.n_seq) : *P.n_items;
+    const int n_items = inlined ? (which == PLAN_PREFIX ? A.n_groups : A.n_seq) : *P.n_items;
     if (n_items == 0) return;
     const int* cum = inlined ? s_cum : P.cum;
     if (inlined) {
@@ -101,10 +103,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
             const int i = base + tid;
             int n = 0;
             if (i < n_items) {
-                n = make_item(A, P, which != 0, i, 0).n_tiles;
-                if (blockIdx.x == 0 && which == 0 &&
-                    (length_too_long(A, i) || A.q_start[i + 1] - A.q_start[i] > P.tpt))
-                    P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
+                n = make_item(A, P, which == PLAN_PREFIX, i, 0).n_tiles;
+                if (blockIdx.x == 0 && which != PLAN_PREFIX) {
+                    const int t = A.q_start[i + 1] - A.q_start[i];
+                    if (length_too_long(A, i) || (t > P.tpt && t <= P.max_tok))
+                        P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
+                }
             }
             int v = n;
 #pragma unroll
@@ -149,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
     constexpr float kShift = PMath<T>::kPShift;
 
     for (; x < x_end; ++item) {
-        const PagedItem it = inlined ? make_item(A, P, which != 0, item, 0) : P.items[item];
+        const PagedItem it = inlined ? make_item(A, P, which == PLAN_PREFIX, item, 0) : P.items[item];
         const int c0 = cum[item];
         if (it.n_tiles == 0) continue;
         const int a = x - c0, b = min(it.n_tiles, x_end - c0);  // KV tiles [a, b) of the item
@@ -160,10 +164,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
             if (A.n_groups > 0) {
                 const int last = pieces.of(c0 + it.n_tiles - 1);
                 for (int i = tid; i < it.ntok; i += kThreads)
-                    P.where[it.tok0 + i] = PagedWhere{piece, last, i * A.gpb, it.alone};
+                    P.where[it.tok0 + i] = PagedWhere{piece, last, i * P.gpb, it.alone, which, item};
             } else if (!whole && tid == 0) {
-                P.split[piece] =
-                    PagedSplit{it.tok0, it.ntok * A.gpb, pieces.of(c0 + it.n_tiles - 1), 0};
+                P.split[piece] = PagedSplit{it.tok0, it.ntok * P.gpb,
+                                            pieces.of(c0 + it.n_tiles - 1), item, 0, 0};
             }
         }
 
@@ -236,13 +240,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
         }
         const float fac = SPLIT ? s_fac[rw * 16 + g] * sl2 : sl2;
         uint32_t qf[kQRegs ? HD / 16 : 1][4];
-        auto load_q = [&](int kk, uint32_t (&f)[4]) {
+        auto load_q = [&](int n, int kk, uint32_t (&f)[4]) {
             const int r = rw * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
-            ldsm4(f, qs + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+            ldsm4(f, qs + (size_t)(n * 16 * RW + r) * HD + ((c ^ (r & 7)) * 8));
         };
         if (kQRegs) {
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) load_q(kk, qf[kQRegs ? kk : 0]);
+            for (int kk = 0; kk < HD / 16; ++kk) load_q(0, kk, qf[kQRegs ? kk : 0]);
         }
 
         float o[HD / 8][4];
@@ -277,17 +281,25 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
                 for (int u = 0; u < 4; ++u) s[t][u] = 0.f;
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) {
-                uint32_t qv[4];
-                if (!kQRegs) load_q(kk, qv);
-                const uint32_t(&qk)[4] = kQRegs ? qf[kQRegs ? kk : 0] : qv;
+                uint32_t qv[kF][4];
+#pragma unroll
+                for (int n = 0; n < kF; ++n) {
+                    if (!kQRegs) load_q(n, kk, qv[n]);
+                    else
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) qv[n][u] = qf[kQRegs ? kk : 0][u];
+                }
 #pragma unroll
                 for (int t = 0; t < kNT; t += 2) {
                     const int r = pw * kNP + t * 8 + ((lane >> 4) & 1) * 8 + (lane & 7);
                     const int c = kk * 2 + ((lane >> 3) & 1);
                     uint32_t kf[4];
                     ldsm4(kf, kd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
-                    PMath<T>::mma(s[t], qk, kf[0], kf[1]);
-                    PMath<T>::mma(s[t + 1], qk, kf[2], kf[3]);
+#pragma unroll
+                    for (int n = 0; n < kF; ++n) {
+                        PMath<T>::mma(s[t], qv[n], kf[0], kf[1]);
+                        PMath<T>::mma(s[t + 1], qv[n], kf[2], kf[3]);
+                    }
                 }
             }
             // scores in log2 units, masked; the row maxima
@@ -346,15 +358,18 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
             auto weigh = [&](auto special) {
 #pragma unroll
                 for (int kk = 0; kk < kNP / 16; ++kk) {
-                    uint32_t pf[4];
-                    if (SPLIT) {
-                        PMath<T>::split2(s[2 * kk][0], s[2 * kk][1], pf[0], pf[1]);
-                        PMath<T>::split2(s[2 * kk + 1][0], s[2 * kk + 1][1], pf[2], pf[3]);
-                    } else {
-                        pf[0] = PMath<T>::pack(s[2 * kk][0], s[2 * kk][1]);
-                        pf[1] = PMath<T>::pack(s[2 * kk][2], s[2 * kk][3]);
-                        pf[2] = PMath<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-                        pf[3] = PMath<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+                    uint32_t pf[kF][4];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        float(&w)[4] = s[2 * kk + t];
+                        if (!SPLIT) {
+                            pf[0][2 * t] = PMath<T>::pack(w[0], w[1]);
+                            pf[0][2 * t + 1] = PMath<T>::pack(w[2], w[3]);
+                        } else {
+                            PMath<T>::split(w[0], w[1], pf[0][2 * t], pf[0][2 * t + 1],
+                                            pf[kF - 1][2 * t]);
+                            if (kF == 2) pf[kF - 1][2 * t + 1] = 0;
+                        }
                     }
                     uint32_t one[4];  // visible places of the 16 x 16 block of weights as ones
                     if (decltype(special)::value) {
@@ -388,8 +403,11 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
                                 vf[2 * n + 1] = f.b1;
                             }
                         }
-                        PMath<T>::mma(o[d], pf, vf[0], vf[1]);
-                        PMath<T>::mma(o[d + 1], pf, vf[2], vf[3]);
+#pragma unroll
+                        for (int n = 0; n < kF; ++n) {
+                            PMath<T>::mma(o[d], pf[n], vf[0], vf[1]);
+                            PMath<T>::mma(o[d + 1], pf[n], vf[2], vf[3]);
+                        }
                     }
                 }
             };
@@ -450,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
                     }
                     R.put2(d, acc, L);
                 }
-                if (lane == 0) R.put_ml(M, L);
+                if (lane == 0) R.put_ml(M - kShift, L);
             }
         } else {
 #pragma unroll
@@ -465,7 +483,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
                                            : make_float2(o[d][2 * u], o[d][2 * u + 1]);
                     R.put2(d * 8 + c4 * 2, v, l[u]);
                 }
-                if (c4 == 0) R.put_ml(m[u], l[u]);
+                if (c4 == 0) R.put_ml(m[u] - kShift, l[u]);
             }
         }
     }
@@ -474,102 +492,136 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs A, int w
 }
 
 // ------------------------------------------------------------------------
-// Joins the pieces of split items.  CTA (piece, head, two rows): the item that begins in the
-// piece and ends after it.  Four warps per row take every fourth piece, in batches whose loads
-// are in flight together, and meet in shared memory in the order of the warps.
+// Joins the pieces of split items.  CTA (piece, block of heads, 8 / WARPS rows): the item that
+// begins in the piece and ends after it.  WARPS warps per row take every WARPS-th piece, in
+// batches whose loads are in flight together, and meet in shared memory in their order.
+// Items that the tensor-core kernel marked are worked out here without tiles.
 // ------------------------------------------------------------------------
-template <typename T, bool SPLIT>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedArgs A) {
+template <typename T, bool SPLIT, int WARPS>
+__global__ void __launch_bounds__(kJoinThreads)
+paged_join_kernel(const __grid_constant__ PagedArgs A, int which, int last_plan) {
     __shared__ JoinShared S;
-    const PagedPlan& P = A.plan[0];
+    constexpr int kRows = 8 / WARPS;
+    const PagedPlan& P = A.plan[which];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
+    if (last_plan && blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
     const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
     const PagedSplit sp = P.split[piece];
-    const int kvh = head_lane / A.hblocks, hb = head_lane - kvh * A.hblocks;
-    const int h0 = kvh * A.group + hb * A.gpb, gpb = min(A.gpb, A.group - hb * A.gpb);
-    const int n_rows = sp.n_rows / A.gpb * gpb;  // n_rows counts full blocks of heads
-    if ((int)blockIdx.y * kJoinRows >= n_rows) return;
-    const int which_row = threadIdx.x / (32 * kJoinWarps);
-    const int row = blockIdx.y * kJoinRows + which_row;
+    const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
+    const int h0 = kvh * A.group + hb * P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
+    const int warp = threadIdx.x / 32;
     Joined J;
-    J.init();
-    if (row < n_rows) J.add_range(A, P, piece, sp.last, head_lane, row);
-    J.meet(S, which_row);
-    if (row < n_rows && (threadIdx.x / 32) % kJoinWarps == 0)
-        J.write<T, SPLIT>(A, sp.tok0 + row / gpb, h0 + row % gpb);
-}
-
-// Prefix mode: the same for CTA (two of the token's heads), over the pieces of the shared
-// prefix and of the sequence's own part.
-template <typename T, bool SPLIT>
-__global__ void __launch_bounds__(kJoinThreads) paged_join2_kernel(PagedArgs A) {
-    __shared__ JoinShared S;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
-    const int t = blockIdx.x, which_row = threadIdx.x / (32 * kJoinWarps);
-    const int h = blockIdx.y * kJoinRows + which_row;
-    if (t < A.q_start[0] || t >= A.q_start[A.n_seq]) return;  // nobody's token
-    Joined J;
-    J.init();
-    if (h < A.nh) {
-        const int kvh = h / A.group, hg = h - kvh * A.group, hb = hg / A.gpb, hr = hg - hb * A.gpb;
-        const int head_lane = kvh * A.hblocks + hb;
-        const PagedWhere own = A.plan[0].where[t];
-        for (int which = 0; which < (own.alone ? 1 : 2); ++which) {
-            const PagedPlan& P = A.plan[which];
-            const PagedWhere w = which ? P.where[t] : own;
-            if (w.first == w.last) J.add_full(A, which, (size_t)t * A.nh + h);
-            else {
-                const int gpb = min(A.gpb, A.group - hb * A.gpb);
-                J.add_range(A, P, w.first, w.last, head_lane, w.row0 / A.gpb * gpb + hr);
+    if (P.redo && blockIdx.y == 0) {
+        for (int i = sp.item0; i < sp.item1; ++i) {
+            if (!P.redo[(size_t)i * P.heads + head_lane]) continue;
+            const PagedItem it = P.items[i];
+            for (int r = warp; r < it.ntok * gpb; r += kJoinThreads / 32) {
+                J.restate<T, SPLIT>(A, it.tok0 + r / gpb, h0 + r % gpb);
+                J.write<T, SPLIT>(A, it.tok0 + r / gpb, h0 + r % gpb);
             }
         }
     }
-    J.meet(S, which_row);
-    if (h < A.nh && (threadIdx.x / 32) % kJoinWarps == 0) J.write<T, SPLIT>(A, t, h);
+    const int n_rows = sp.n_rows / P.gpb * gpb;  // (counted with full blocks of heads)
+    if ((int)blockIdx.y * kRows >= n_rows) return;
+    if (P.redo && P.redo[(size_t)sp.item * P.heads + head_lane]) return;
+    const int row = blockIdx.y * kRows + warp / WARPS;
+    J.init();
+    if (row < n_rows) J.add_range(A, P, piece, sp.last, head_lane, row, warp % WARPS, WARPS);
+    J.meet(S, warp % WARPS, WARPS);
+    if (row < n_rows && warp % WARPS == 0)
+        J.write<T, SPLIT>(A, sp.tok0 + row / gpb, h0 + row % gpb);
+}
+
+// Prefix mode: the same for CTA (token, two of its heads), over the pieces of the shared prefix
+// and of the sequence's own part.
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kJoinThreads)
+paged_join2_kernel(const __grid_constant__ PagedArgs A) {
+    __shared__ JoinShared S;
+    constexpr int kWarps = 4, kRows = 2;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
+    const int t = blockIdx.x, warp = threadIdx.x / 32;
+    const int h = blockIdx.y * kRows + warp / kWarps;
+    if (t < A.q_start[0] || t >= A.q_start[A.n_seq]) return;  // nobody's token
+    Joined J;
+    J.init();
+    bool redo = false;
+    if (h < A.nh) {
+        // both sequence plans write the same array
+        const PagedWhere own = (A.plan[PLAN_FEW].used ? A.plan[PLAN_FEW] : A.plan[PLAN_MANY]).where[t];
+        const int kvh = h / A.group, hg = h - kvh * A.group;
+        for (int part = 0; part < (own.alone ? 1 : 2); ++part) {
+            const PagedWhere w = part ? A.plan[PLAN_PREFIX].where[t] : own;
+            if (w.plan < 0 || w.plan >= PLANS) continue;
+            const PagedPlan& P = A.plan[w.plan];
+            const int hb = hg / P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
+            const int head_lane = kvh * P.hblocks + hb, row = w.row0 / P.gpb * gpb + hg - hb * P.gpb;
+            // (a malformed q_start leaves tokens without a record)
+            if (w.first < 0 || w.last < w.first || w.last >= P.lanes || row < 0 || row >= P.rows ||
+                w.item < 0 || w.item >= P.max_items)
+                continue;
+            if (P.redo && P.redo[(size_t)w.item * P.heads + head_lane]) redo = true;
+            if (w.first == w.last) J.add_full(A, part != 0, (size_t)t * A.nh + h, warp % kWarps);
+            else J.add_range(A, P, w.first, w.last, head_lane, row, warp % kWarps, kWarps);
+        }
+    }
+    J.meet(S, warp % kWarps, kWarps);
+    if (h < A.nh && warp % kWarps == 0) {
+        if (redo) J.restate<T, SPLIT>(A, t, h);
+        J.write<T, SPLIT>(A, t, h);
+    }
 }
 
 template <typename T, bool SPLIT, int HD, int RW>
-cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
+cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, cudaStream_t s) {
     auto kern = paged_attn_kernel<T, SPLIT, HD, RW>;
-    constexpr size_t smem = attn_smem_bytes<HD, RW>();
+    constexpr size_t smem = attn_smem_bytes<HD, RW, SPLIT ? PMath<T>::kFrags : 1>();
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    // which < 0: both plans in one launch
-    const PagedPlan& P = A.plan[which < 0 ? 0 : which];
-    return launch_pdl(kern, dim3(P.heads * P.lanes, which < 0 ? 2 : 1), dim3(kThreads), smem, s, A,
-                      which < 0 ? 0 : which);
+    const PagedPlan& P = A.plan[which];
+    return launch_pdl(kern, dim3(P.heads * P.lanes, with_prefix ? 2 : 1), dim3(kThreads), smem, s, A,
+                      which);
 }
 
 template <typename T, bool SPLIT, int HD>
-cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
-    return rw == 1 ? launch_one<T, SPLIT, HD, 1>(A, which, s)
-           : rw == 2 ? launch_one<T, SPLIT, HD, 2>(A, which, s)
-                     : launch_one<T, SPLIT, HD, 4>(A, which, s);
+cudaError_t launch_rw(const PagedArgs& A, int which, bool both, int rw, cudaStream_t s) {
+    return rw == 1 ? launch_one<T, SPLIT, HD, 1>(A, which, both, s)
+           : rw == 2 ? launch_one<T, SPLIT, HD, 2>(A, which, both, s)
+                     : launch_one<T, SPLIT, HD, 4>(A, which, both, s);
 }
 
 template <typename T, bool SPLIT>
-cudaError_t launch_t(const PagedArgs& A, int which, int rw, cudaStream_t s) {
-    return A.hd <= 64    ? launch_rw<T, SPLIT, 64>(A, which, rw, s)
-           : A.hd <= 128 ? launch_rw<T, SPLIT, 128>(A, which, rw, s)
-                         : launch_rw<T, SPLIT, 256>(A, which, rw, s);
+cudaError_t launch_t(const PagedArgs& A, int which, bool both, int rw, cudaStream_t s) {
+    return A.hd <= 64    ? launch_rw<T, SPLIT, 64>(A, which, both, rw, s)
+           : A.hd <= 128 ? launch_rw<T, SPLIT, 128>(A, which, both, rw, s)
+                         : launch_rw<T, SPLIT, 256>(A, which, both, rw, s);
 }
 
 template <typename T, bool SPLIT>
 cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
-    if (A.n_groups > 0) {
-        return launch_pdl(paged_join2_kernel<T, SPLIT>,
-                          dim3(A.n_tokens, (A.nh + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads),
-                          0, s, A);
+    if (A.n_groups > 0)
+        return launch_pdl(paged_join2_kernel<T, SPLIT>, dim3(A.n_tokens, (A.nh + 1) / 2),
+                          dim3(kJoinThreads), 0, s, A);
+    for (int w = PLAN_FEW; w <= PLAN_MANY; w += PLAN_MANY - PLAN_FEW) {
+        const PagedPlan& P = A.plan[w];
+        if (!P.used) continue;
+        const int last = w == PLAN_MANY || !A.plan[PLAN_MANY].used;
+        // few rows: four warps each; many: as many rows as warps, most items are in few pieces
+        cudaError_t e =
+            P.used_rows <= 32
+                ? launch_pdl(paged_join_kernel<T, SPLIT, 4>,
+                             dim3(P.heads * P.lanes, (P.used_rows + 1) / 2), dim3(kJoinThreads), 0,
+                             s, A, w, last)
+                : launch_pdl(paged_join_kernel<T, SPLIT, 1>,
+                             dim3(P.heads * P.lanes, (P.used_rows + 7) / 8), dim3(kJoinThreads), 0,
+                             s, A, w, last);
+        if (e != cudaSuccess) return e;
     }
-    const PagedPlan& P = A.plan[0];
-    return launch_pdl(paged_join_kernel<T, SPLIT>,
-                      dim3(P.heads * P.lanes, (P.used_rows + kJoinRows - 1) / kJoinRows),
-                      dim3(kJoinThreads), 0, s, A);
+    return cudaSuccess;
 }
 
 }  // namespace
@@ -585,14 +637,14 @@ int paged_attn_rw(int rows, bool split) {
 // CTAs of one SM: what the ring leaves room for.
 int paged_attn_ctas(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
 
-cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
-                              cudaStream_t s) {
+cudaError_t launch_paged_attn(const PagedArgs& A, int which, bool both, int rw, int q_dtype,
+                              int kv_dtype, cudaStream_t s) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     if (kv_dtype == WISP_DTYPE_F16)
-        return split ? launch_t<__half, true>(A, which, rw, s)
-                     : launch_t<__half, false>(A, which, rw, s);
-    return split ? launch_t<__nv_bfloat16, true>(A, which, rw, s)
-                 : launch_t<__nv_bfloat16, false>(A, which, rw, s);
+        return split ? launch_t<__half, true>(A, which, both, rw, s)
+                     : launch_t<__half, false>(A, which, both, rw, s);
+    return split ? launch_t<__nv_bfloat16, true>(A, which, both, rw, s)
+                 : launch_t<__nv_bfloat16, false>(A, which, both, rw, s);
 }
 
 cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s) {

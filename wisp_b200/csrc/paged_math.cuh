@@ -57,7 +57,10 @@ struct PMath<__half> {
     static __device__ __forceinline__ float2 unpack(uint32_t v) {
         return __half22float2(*reinterpret_cast<const __half2*>(&v));
     }
-    static __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    // a, b in parts: two here (`third` is not written)
+    static constexpr int kFrags = 1;
+    static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo,
+                                                 uint32_t&) {
         hi = pack(a, b);
         const float2 f = unpack(hi);
         lo = pack(a - f.x, b - f.y);
@@ -86,10 +89,14 @@ struct PMath<__nv_bfloat16> {
     static __device__ __forceinline__ float2 unpack(uint32_t v) {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     }
-    static __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    static constexpr int kFrags = 2;
+    static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& mid,
+                                                 uint32_t& third) {
         hi = pack(a, b);
         const float2 f = unpack(hi);
-        lo = pack(a - f.x, b - f.y);
+        mid = pack(a - f.x, b - f.y);
+        const float2 g = unpack(mid);
+        third = pack(a - f.x - g.x, b - f.y - g.y);
     }
     static __device__ __forceinline__ bool not_finite(uint32_t v) {
         return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
@@ -240,7 +247,8 @@ __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bo
         it.first = f;
         it.n_tiles = it.n_sink + last - f;
     }
-    if (it.ntok <= 0) it.n_tiles = 0;
+    if (it.ntok <= 0 || (!prefix && (g.t1 - g.t0 < P.min_tok || g.t1 - g.t0 > P.max_tok)))
+        it.n_tiles = 0;
     return it;
 }
 
@@ -264,8 +272,8 @@ __device__ __forceinline__ long long page_offset(const PagedArgs& A, int seq, in
 }
 
 // q rows of a tile into shared memory: row r of MMA tile wr at line wr * 16 + r, 16-byte pieces
-// XORed with the line number.  SPLIT: 8 fp32 rows per MMA tile, hi parts in lines 0-7 and lo
-// parts in 8-15; fp16 parts are of q / 2^e with 2^e the row's largest exponent (s_fac).
+// XORed with the line number.  SPLIT: 8 fp32 rows per MMA tile, first parts in lines 0-7 and
+// second ones in 8-15 (third ones in lines 0-7 of a second set of tiles); fp16 parts are of q / 2^e with 2^e the row's largest exponent (s_fac).
 template <typename T, bool SPLIT, int HD, int RW, int THREADS>
 __device__ void load_rows(const PagedArgs& A, int tok0, int n_rows, int h0, int gpb, T* qs,
                           float* s_fac) {
@@ -308,28 +316,33 @@ __device__ void load_rows(const PagedArgs& A, int tok0, int n_rows, int h0, int 
 #pragma unroll
             for (int u = 0; u < kN; ++u) {
                 const int d = (u * 32 + lane) * 2, c = d / 8;
-                uint32_t hi, lo;
-                PMath<T>::split2(v[u].x * inv, v[u].y * inv, hi, lo);
+                uint32_t hi, lo, third = 0;
+                PMath<T>::split(v[u].x * inv, v[u].y * inv, hi, lo, third);
                 const int at = ((c ^ (line & 7)) * 8) + (d & 7);  // line + 8 has the same key
                 *reinterpret_cast<uint32_t*>(qs + (size_t)line * HD + at) = hi;
                 *reinterpret_cast<uint32_t*>(qs + (size_t)(line + 8) * HD + at) = lo;
+                if (PMath<T>::kFrags == 2) {
+                    T* q2 = qs + (size_t)16 * RW * HD;
+                    *reinterpret_cast<uint32_t*>(q2 + (size_t)line * HD + at) = third;
+                    *reinterpret_cast<uint32_t*>(q2 + (size_t)(line + 8) * HD + at) = 0;
+                }
             }
         }
     }
 }
 
-// log-sum-exp (natural) of a row with running maximum M (log2 units) and sum L, whose
-// weights carry the factor 2^shift.
-__device__ __forceinline__ float row_lse(float M, float L, float shift) {
-    return L == 0.f ? -INFINITY : (M + log2f(L) - shift) * 0.69314718055994531f;
+// log-sum-exp (natural) of a row whose weights 2^(score - M), score in log2 units, sum to L.
+__device__ __forceinline__ float row_lse(float M, float L) {
+    return L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
 
 // The status word of the call: the CTAs' and the plans' bits, gathered by the last kernel's
 // first CTA.
 __device__ __forceinline__ void gather_status(const PagedArgs& A) {
     int bits = 0;
-    for (int w = 0; w < (A.n_groups > 0 ? 2 : 1); ++w) {
+    for (int w = 0; w < PLANS; ++w) {
         const PagedPlan& P = A.plan[w];
+        if (!P.used) continue;
         for (int i = threadIdx.x; i <= P.lanes * P.heads; i += blockDim.x) bits |= P.bad[i];
     }
     const int any = __syncthreads_or(bits & PG_BAD_PAGE) ? PG_BAD_PAGE : 0;
@@ -379,7 +392,7 @@ struct RowOut {
             else o16 = reinterpret_cast<T*>(A.out) + t * A.out_stride + h * A.hd;
             if (A.lse) lse = A.lse + t * A.nh + h;
         } else if (whole) {
-            const size_t id = (size_t)which * A.n_tokens * A.nh + t * A.nh + h;
+            const size_t id = (size_t)(which == PLAN_PREFIX) * A.n_tokens * A.nh + t * A.nh + h;
             o32 = A.full_o + id * A.hd;
             ml = A.full_ml + id * 2;
         } else {
@@ -401,18 +414,18 @@ struct RowOut {
     }
     __device__ __forceinline__ void put_ml(float M, float L) {
         if (final) {
-            if (lse) *lse = row_lse(M, L, PMath<T>::kPShift);
+            if (lse) *lse = row_lse(M, L);
         } else {
             *reinterpret_cast<float2*>(ml) = make_float2(M, L);
         }
     }
 };
 
-// The join of one row's partial records by kJoinWarps warps.
-constexpr int kJoinRows = 2, kJoinWarps = 4, kJoinThreads = 32 * kJoinRows * kJoinWarps;
+// The join of one row's partial records by W warps.
+constexpr int kJoinThreads = 256;
 struct JoinShared {
-    float2 acc[kJoinRows][kJoinWarps][128];
-    float m[kJoinRows][kJoinWarps], l[kJoinRows][kJoinWarps];
+    float2 acc[8][128];
+    float m[8], l[8];
 };
 struct Joined {
     float M, L;
@@ -468,53 +481,106 @@ struct Joined {
             }
         }
     }
-    __device__ __forceinline__ void add_full(const PagedArgs& A, int which, size_t id) {
-        if ((threadIdx.x / 32) % kJoinWarps != 0) return;
-        id += (size_t)which * A.n_tokens * A.nh;
+    __device__ __forceinline__ void add_full(const PagedArgs& A, bool prefix, size_t id, int warp) {
+        if (warp != 0) return;
+        id += (size_t)prefix * A.n_tokens * A.nh;
         const float* const o[1] = {A.full_o + id * A.hd};
         const float* const ml[1] = {A.full_ml + id * 2};
         add<1>(A, o, ml, 1);
     }
     __device__ __forceinline__ void add_range(const PagedArgs& A, const PagedPlan& P, int first,
-                                              int last, int head_lane, int row) {
+                                              int last, int head_lane, int row, int warp,
+                                              int warps) {
         constexpr int kBatch = 4;
-        const int warp = (threadIdx.x / 32) % kJoinWarps;
-        for (int p = first + warp; p <= last; p += kBatch * kJoinWarps) {
+        for (int p = first + warp; p <= last; p += kBatch * warps) {
             const float *o[kBatch], *ml[kBatch];
             int n = 0;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                const int pp = min(p + k * kJoinWarps, last);
+                const int pp = min(p + k * warps, last);
                 const size_t id = part_row(P, pp, head_lane, pp == first, row);
                 o[k] = P.part_o + id * A.hd;
                 ml[k] = P.part_ml + id * 2;
-                n += p + k * kJoinWarps <= last;
+                n += p + k * warps <= last;
             }
             add<kBatch>(A, o, ml, n);
         }
     }
-    // All warps of the block: the row's warps hand their sums to its first one.
-    __device__ __forceinline__ void meet(JoinShared& S, int r) {
-        const int lane = threadIdx.x & 31, warp = (threadIdx.x / 32) % kJoinWarps;
+    // All warps of the block: a row's warps (consecutive ones) hand their sums to the first.
+    __device__ __forceinline__ void meet(JoinShared& S, int warp, int warps) {
+        if (warps == 1) return;
+        const int lane = threadIdx.x & 31, me = threadIdx.x / 32;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S.acc[r][warp][i * 32 + lane] = acc[i];
+        for (int i = 0; i < 4; ++i) S.acc[me][i * 32 + lane] = acc[i];
         if (lane == 0) {
-            S.m[r][warp] = M;
-            S.l[r][warp] = L;
+            S.m[me] = M;
+            S.l[me] = L;
         }
         __syncthreads();
         if (warp != 0) return;
-#pragma unroll
-        for (int w = 1; w < kJoinWarps; ++w) {
-            const float m = S.m[r][w];
+        for (int w = me + 1; w < me + warps; ++w) {
+            const float m = S.m[w];
             rebase(fmaxf(M, m));
             const float e = ex2(m - (M == -INFINITY ? 0.f : M));
-            L = fmaf(S.l[r][w], e, L);
+            L = fmaf(S.l[w], e, L);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float2 v = S.acc[r][w][i * 32 + lane];
+                const float2 v = S.acc[w][i * 32 + lane];
                 acc[i].x = fmaf(v.x, e, acc[i].x);
                 acc[i].y = fmaf(v.y, e, acc[i].y);
+            }
+        }
+    }
+    // One row without tiles, position by position: what it does not see is never touched.
+    template <typename T, bool SPLIT>
+    __device__ __noinline__ void restate(const PagedArgs& A, int t, int h) {
+        init();
+        const int lane = threadIdx.x & 31;
+        const int s = last_le(A.q_start, A.n_seq, t);
+        const int pos = cached_positions(A, s) - (A.q_start[s + 1] - t), kvh = h / A.group;
+        const int sinks = A.window > 0 ? A.sinks : 0;
+        const int lo = A.window > 0 ? max(0, pos - A.window + 1) : 0;
+        const size_t at = (size_t)t * A.q_stride + (size_t)h * A.hd;
+        float2 q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = (i * 32 + lane) * 2;
+            q[i] = make_float2(0.f, 0.f);
+            if (d >= A.hd) continue;
+            q[i] = SPLIT ? *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(A.q) + at + d)
+                         : PMath<T>::unpack(*reinterpret_cast<const uint32_t*>(
+                               reinterpret_cast<const T*>(A.q) + at + d));
+        }
+        for (int j = min(sinks, lo) > 0 ? 0 : lo; j <= pos; ++j) {
+            if (j >= sinks && j < lo) j = lo;
+            const int p = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size;
+            const int page = A.table[(size_t)s * A.table_stride + p];
+            if ((unsigned)page >= (unsigned)A.n_pages) continue;
+            const size_t row = (size_t)page * A.page_stride +
+                               ((size_t)(j - p * A.page_size) * A.nkv + kvh) * A.hd;
+            float dot = 0.f;
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = (i * 32 + lane) * 2;
+                v[i] = make_float2(0.f, 0.f);
+                if (d >= A.hd) continue;
+                const float2 k = PMath<T>::unpack(*reinterpret_cast<const uint32_t*>(
+                    reinterpret_cast<const T*>(A.k) + row + d));
+                v[i] = PMath<T>::unpack(*reinterpret_cast<const uint32_t*>(
+                    reinterpret_cast<const T*>(A.v) + row + d));
+                dot = fmaf(q[i].x, k.x, fmaf(q[i].y, k.y, dot));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            const float x = dot * A.scale_log2;
+            rebase(fmaxf(M, x));
+            const float e = ex2(x - (M == -INFINITY ? 0.f : M));
+            L += e;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[i].x = fmaf(v[i].x, e, acc[i].x);
+                acc[i].y = fmaf(v[i].y, e, acc[i].y);
             }
         }
     }
@@ -533,7 +599,7 @@ struct Joined {
             else *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(A.out) + at) = PMath<T>::pack(v.x, v.y);
         }
         if (lane == 0 && A.lse)
-            A.lse[(size_t)t * A.nh + h] = row_lse(M, L, PMath<T>::kPShift);
+            A.lse[(size_t)t * A.nh + h] = row_lse(M, L);
     }
 };
 

@@ -1,0 +1,808 @@
+// paged_mma.cu -- attention of row tiles with many rows (prompts, chunks, drafted tokens, the
+// sequences of a shared prefix) on tcgen05, over the pages.
+//
+// One persistent CTA per SM takes a piece of the line of (row tile, KV tile) pairs for one kv
+// head.  Per KV tile of 64 positions and 128 rows:
+//   S = Q K^T   tcgen05.mma M=128 N=64, Q and K from shared memory, S in tensor memory
+//   P = 2^(S fac - m)  one thread per row; P back to tensor memory as 16-bit pairs
+//   O += P V    tcgen05.mma M=128 N=head_dim, P from tensor memory, V from shared memory
+// Two tiles of 128 rows share each K / V tile.  S is double buffered, so the tensor core works
+// on tile j + 1 while the softmax warps work on tile j.  Roles:
+//   warps 0-3 (and 4-7)  softmax of row tile 0 (and 1): rows 32 * (warp & 3) + lane
+//   warp 8               issues the MMAs (one thread)
+//   warp 9               loads K and V: TMA boxes of up to 64 positions out of one page, lane
+//                        per box, 128-byte swizzle, ring of 16-KB slots
+// A row's running maximum is only moved when a score passes it by more than 2^8 (the weights
+// then still fit 16 bits and the sums are fp32), so that O is rarely rescaled; the warp that
+// needs it does so itself, behind the previous product.
+//
+// 32-bit rows: q and p are split into PARTS 16-bit parts (two in fp16, three in bf16) with one
+// product each into the same accumulator; one tile of 128 rows then.
+//
+// Hidden values.  A box outside what the tile's rows see is loaded from outside the tensor map
+// (zeros).  In tiles that are partly hidden the softmax warps look V through for infinities and
+// NaNs before the product: those that no row sees are zeroed in shared memory; where some row
+// sees one, the row tile is marked and the join kernel works it out again without tiles.
+//
+// TMEM (512 columns): S buffers of 64 columns, P over them (or beside them when it has several
+// parts), O of head_dim columns per row tile.  Every wait is bounded; on a timeout all roles
+// leave, copies and products in flight are drained and TMEM is freed.
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "internal.h"
+#include "paged.h"
+#include "paged_math.cuh"
+
+namespace wb {
+namespace {
+
+constexpr int kN = 64;          // positions of a KV tile
+constexpr int kM = 128;         // rows of a row tile
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr unsigned kAll = 0xffffffffu;
+
+template <int HD, int PARTS>
+struct MCfg {
+    static constexpr int kRT = PARTS == 1 ? 2 : 1;       // row tiles
+    static constexpr int kHalves = HD / 64;
+    static constexpr int kSlot = kN * HD * 2;            // bytes of a K or V tile
+    static constexpr int kQ = kM * HD * 2;               // bytes of one part of Q
+    static constexpr int kSlots = HD == 64 ? 12 : PARTS == 3 ? 7 : 9;
+    static constexpr int kSmem = 1024 + kRT * PARTS * kQ + kSlots * kSlot;
+    // TMEM columns
+    static constexpr int kPCols = 32 * PARTS;
+    static __host__ __device__ constexpr int s_col(int x, int b) { return (x * 2 + b) * 64; }
+    static __host__ __device__ constexpr int p_col(int x, int b) {
+        return PARTS == 1 ? s_col(x, b) : 128 + b * kPCols;
+    }
+    static __host__ __device__ constexpr int o_col(int x) { return 512 - (kRT - x) * HD; }
+};
+
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait; false when it ran out here or in another role.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+    if (bar_try(b, parity)) return true;
+    uint64_t t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        if (bar_try(b, parity)) return true;
+        if ((it & 63) == 63) {
+            if (*abort_flag) return false;
+            const uint64_t t = now_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > kWaitNs) {
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, uint32_t parity,
+                                              volatile int* abort_flag) {
+    return __all_sync(kAll, bar_wait(b, parity, abort_flag));
+}
+__device__ __forceinline__ void bar_drain(uint64_t* b, uint32_t parity) {
+    const uint64_t t0 = now_ns();
+    while (!bar_try(b, parity))
+        if (now_ns() - t0 > kWaitNs) return;
+}
+
+__device__ __forceinline__ void tma4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                      int c3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
+        "r"(smem_addr(bar))
+        : "memory");
+}
+
+// Shared-memory descriptors, 128-byte swizzle.  K-major (Q, K): 64 elements per row of 128 B,
+// atoms of 8 rows 1024 B apart.  MN-major (V: positions are K, head dims N): blocks of 64 dims
+// `lead` bytes apart, groups of 8 positions 1024 B apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptor of kind::f16: A and B fp16 (0) or bf16 (1), fp32 accumulator, M = 128,
+// N = n, A K-major, B K-major or (b_mn) MN-major.
+__host__ __device__ constexpr uint32_t idesc(int type, int n, int b_mn) {
+    return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                       uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                       uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+            smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tc_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void async_fence() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// 32 or 64 columns of this thread's TMEM lane.  The wait is part of the statement: the
+// registers are not valid before it, and nothing may be scheduled in between that reads them.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+        "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
+          "=f"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,"
+        "%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,"
+        "%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
+          "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]),
+          "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]),
+          "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]),
+          "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]),
+          "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]),
+          "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+        "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+struct KvMaps {
+    CUtensorMap k, v;  // (dim, kv head, position in page, page), boxes of 64 dims
+};
+
+// Weights of 16-bit pairs stay below 2^15 with the maximum up to 2^8 behind (fp16).
+template <typename T>
+struct MShift {
+    static constexpr float value = std::is_same<T, __half>::value ? 6.f : 0.f;
+};
+
+// The shared state of a piece's walk: which item and tiles come next.  Every role walks alike.
+struct Walk {
+    int item, x, x_end;
+    int a, b;  // KV tiles [a, b) of the item
+    int c0;    // the item's first tile on the line
+    PagedItem it;
+    __device__ __forceinline__ bool next(const PagedPlan& P) {
+        while (x < x_end) {
+            it = P.items[item];
+            c0 = P.cum[item];
+            ++item;
+            if (it.n_tiles == 0) continue;
+            a = x - c0;
+            b = min(it.n_tiles, x_end - c0);
+            x = c0 + b;
+            return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ int tile(int i) const {
+        return i < it.n_sink ? it.sink0 + i : it.first + i - it.n_sink;
+    }
+};
+
+template <typename T, int PARTS, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ KvMaps maps, int which,
+                 int box_rows) {
+    using C = MCfg<HD, PARTS>;
+    constexpr int kRT = C::kRT, kSlots = C::kSlots, kH = C::kHalves;
+    constexpr bool SPLIT = PARTS > 1;
+    constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    extern __shared__ char raw[];
+    char* base = reinterpret_cast<char*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    char* sQ = base;                                  // [kRT][PARTS][kH][128 rows][128 B]
+    char* sKV = base + kRT * PARTS * C::kQ;           // [kSlots][kH][64 rows][128 B]
+    __shared__ uint64_t full[kSlots], empty[kSlots];
+    __shared__ uint64_t q_full[kRT], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_abort;
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const PagedPlan& P = A.plan[which];
+    const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
+    const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
+    const int h0 = kvh * A.group + hb * P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
+
+    if (tid == 0) {
+        for (int i = 0; i < kSlots; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 1);
+        }
+        for (int x = 0; x < kRT; ++x) {
+            bar_init(&q_full[x], 4);
+            for (int b = 0; b < 2; ++b) {
+                bar_init(&o_done[x][b], 1);
+                bar_init(&s_full[x][b], 1);
+                bar_init(&p_full[x][b], 4);
+            }
+        }
+        bar_init(&drain, 1);
+        s_abort = 0;
+        s_bad = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                         smem_addr(&s_tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = s_tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    Walk W;
+    {
+        const int n_items = *P.n_items, total = n_items ? P.cum[n_items] : 0;
+        const Pieces pieces(P, max(total, 1));
+        W.x = W.x_end = 0;
+        if (total > 0 && piece < pieces.n) {
+            W.x = pieces.start(piece);
+            W.x_end = pieces.start(piece + 1);
+        }
+        W.item = n_items ? last_le(P.cum, n_items, W.x) : 0;
+        if (tid == 0) {
+            P.bad[blockIdx.x] = 0;
+            if (head_lane == 0) {
+                PagedSplit sp{0, 0, 0, -1, 0, 0};
+                // the items that begin in this piece
+                sp.item0 = W.item + (n_items && W.x < W.x_end && P.cum[W.item] < W.x);
+                sp.item1 = sp.item0;
+                if (W.x < W.x_end) {
+                    int last = last_le(P.cum, n_items, W.x_end - 1);
+                    sp.item1 = last + 1;
+                    if (last >= sp.item0 && P.cum[last + 1] > W.x_end && A.n_groups == 0) {
+                        const PagedItem it = P.items[last];
+                        sp.tok0 = it.tok0;
+                        sp.n_rows = it.ntok * P.gpb;
+                        sp.last = pieces.of(P.cum[last + 1] - 1);
+                        sp.item = last;
+                    }
+                }
+                P.split[piece] = sp;
+            }
+        }
+    }
+
+    // The product with V of row tile x's c-th KV tile is done.  (A barrier for odd and one for
+    // even tiles: a waiter may be two tiles ahead, where one barrier's parity would repeat.)
+    auto pv_done = [&](int x, uint32_t c) {
+        return bar_wait(&o_done[x][c & 1], (c >> 1) & 1, &s_abort);
+    };
+    uint32_t ring = 0;  // K / V tiles so far: slot ring % kSlots, phase (ring / kSlots) & 1
+    if (warp == kLoadWarp) {
+        // ------------------------------------------------------------- K / V tiles
+        const int per_half = kN / box_rows, boxes = per_half * kH;
+        const int half = lane / per_half, rb = lane - half * per_half;
+        bool ok = true;
+        while (ok && W.next(P)) {
+            const PagedItem& it = W.it;
+            const int any_hi = min(it.kv_hi, it.pmax + 1);
+            const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
+            const int sinks = A.window > 0 ? A.sinks : 0;
+            // this lane's page and row of a tile's box (outside the pool: zeros)
+            auto place = [&](int i) {
+                int2 at = make_int2(A.n_pages, 0);
+                const int j = W.tile(i) * kN + rb * box_rows, je = j + box_rows;
+                if (lane < boxes && j < any_hi && je > it.kv_lo && (je > any_lo || j < sinks)) {
+                    const int p = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size;
+                    const int page = __ldg(A.table + (size_t)it.seq * A.table_stride + p);
+                    if ((unsigned)page < (unsigned)A.n_pages)
+                        at = make_int2(page, j - p * A.page_size);
+                    else
+                        atomicOr(&s_bad, PG_BAD_PAGE);
+                }
+                return at;
+            };
+            int2 at = place(W.a);
+            for (int i = W.a; ok && i < W.b; ++i) {
+                const int2 cur = at;
+                if (i + 1 < W.b) at = place(i + 1);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++ring) {
+                    const int s = ring % kSlots;
+                    if (!bar_wait_warp(&empty[s], ((ring / kSlots) & 1) ^ 1, &s_abort)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) bar_expect(&full[s], C::kSlot);
+                    __syncwarp();
+                    if (lane < boxes)
+                        tma4d(smem_addr(sKV + s * C::kSlot + half * (kN * 128) + rb * box_rows * 128),
+                              kv ? &maps.v : &maps.k, half * 64, kvh, cur.y, cur.x, &full[s]);
+                }
+            }
+        }
+        __syncwarp();
+        // (only after a timeout can some of these still be in flight)
+        if (lane == 0)
+            for (uint32_t i = ring > kSlots ? ring - kSlots : 0; i < ring; ++i)
+                bar_drain(&full[i % kSlots], (i / kSlots) & 1);
+    } else if (warp == kMmaWarp) {
+        // ------------------------------------------------------------- products
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t seg[kRT] = {}, cnt[kRT] = {};  // segments, tiles of each row tile so far
+            const uint32_t q0 = smem_addr(sQ), kv0 = smem_addr(sKV);
+            auto issue_s = [&](int x, uint32_t ks, uint32_t c) {
+                const uint32_t d = tmem + C::s_col(x, c & 1);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint32_t qa = q0 + (x * PARTS + p) * C::kQ + (k / 4) * (kM * 128) +
+                                            (k % 4) * 32;
+                        const uint32_t ka = kv0 + ks * C::kSlot + (k / 4) * (kN * 128) + (k % 4) * 32;
+                        mma_ss(d, desc_k(qa), desc_k(ka), idesc(kType, kN, 0), (p | k) ? 1u : 0u);
+                    }
+                mma_commit(&s_full[x][c & 1]);
+            };
+            while (ok && W.next(P)) {
+                const int n = W.b - W.a, nx = kRT == 2 && W.it.ntok * gpb > kM ? 2 : 1;
+                for (int x = 0; ok && x < nx; ++x) {
+                    ok = bar_wait(&q_full[x], seg[x] & 1, &s_abort) &&
+                         bar_wait(&full[ring % kSlots], (ring / kSlots) & 1, &s_abort);
+                    if (!ok) break;
+                    ++seg[x];
+                    tc_after();
+                    issue_s(x, ring % kSlots, cnt[x]);
+                }
+                if (!ok) break;
+                mma_commit(&empty[ring % kSlots]);
+                for (int j = 0; ok && j < n; ++j, ring += 2) {
+                    const uint32_t rv = ring + 1, rk = ring + 2;
+                    for (int x = 0; x < nx; ++x) {
+                        if (j + 1 < n) {
+                            // S of the next tile takes the buffer of the last one's P
+                            ok = (j == 0 || pv_done(x, cnt[x] - 1)) &&
+                                 bar_wait(&full[rk % kSlots], (rk / kSlots) & 1, &s_abort);
+                            if (!ok) break;
+                            tc_after();
+                            issue_s(x, rk % kSlots, cnt[x] + 1);
+                            if (x == nx - 1) mma_commit(&empty[rk % kSlots]);
+                        }
+                        ok = bar_wait(&p_full[x][cnt[x] & 1], (cnt[x] >> 1) & 1, &s_abort) &&
+                             bar_wait(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort);
+                        if (!ok) break;
+                        tc_after();
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                            for (int k = 0; k < kN / 16; ++k)
+                                mma_ts(tmem + C::o_col(x),
+                                       tmem + C::p_col(x, cnt[x] & 1) + p * 32 + k * 8,
+                                       desc_mn(kv0 + (rv % kSlots) * C::kSlot + k * 16 * 128, kN * 128),
+                                       idesc(kType, HD, 1), (j | p | k) ? 1u : 0u);
+                        mma_commit(&o_done[x][cnt[x] & 1]);
+                        if (x == nx - 1) mma_commit(&empty[rv % kSlots]);
+                        ++cnt[x];
+                    }
+                }
+            }
+            mma_commit(&drain);
+            bar_drain(&drain, 0);
+        }
+    } else if (warp < 4 * kRT) {
+        // ------------------------------------------------------------- softmax of a row tile
+        const int x = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const bool flip = A.scale_log2 < 0.f;  // q takes the sign, so that fac >= 0
+        constexpr float kShift = MShift<T>::value;
+        uint32_t cnt = 0;
+        bool ok = true;
+        while (ok && W.next(P)) {
+            const PagedItem& it = W.it;
+            const int n_rows = it.ntok * gpb, n = W.b - W.a;
+            if (x * kM >= n_rows) {
+                ring += 2 * n;
+                continue;
+            }
+            const int row = x * kM + r;
+            const bool real = row < n_rows;
+            const int tok = it.tok0 + row / gpb, h = h0 + row % gpb;
+            int pos = INT_MIN;
+            if (real) pos = it.mixed ? token_position(A, tok) : it.pos0 + row / gpb;
+            float fac = fabsf(A.scale_log2);
+            {
+                // this thread's row of Q (the previous item's products have read theirs: the
+                // last S of this row tile has been waited for)
+                char* dst = sQ + x * PARTS * C::kQ + r * 128;
+                const size_t src = (size_t)tok * A.q_stride + (size_t)h * A.hd;
+                if (!SPLIT) {
+                    const T* q = reinterpret_cast<const T*>(A.q) + src;
+                    const uint32_t sign = flip ? 0x80008000u : 0u;
+#pragma unroll
+                    for (int c = 0; c < HD / 8; ++c) {
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (real && c * 8 < A.hd) w = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
+                        w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
+                        *reinterpret_cast<uint4*>(dst + (c / 8) * (kM * 128) +
+                                                  (((c & 7) ^ (r & 7)) * 16)) = w;
+                    }
+                } else {
+                    const float* q = reinterpret_cast<const float*>(A.q) + src;
+                    float mx = 0.f;
+                    for (int d = 0; real && d < A.hd; d += 4) {
+                        const float4 w = __ldg(reinterpret_cast<const float4*>(q + d));
+                        mx = fmaxf(fmaxf(mx, fmaxf(fabsf(w.x), fabsf(w.y))),
+                                   fmaxf(fabsf(w.z), fabsf(w.w)));
+                    }
+                    const uint32_t e = (__float_as_uint(mx) >> 23) & 255u;
+                    const bool scaled = kType == 0 && e > 0 && e < 254;
+                    const float inv = (scaled ? __uint_as_float((254u - e) << 23) : 1.f) *
+                                      (flip ? -1.f : 1.f);
+                    if (scaled) fac *= __uint_as_float(e << 23);
+                    for (int c = 0; c < HD / 8; ++c) {
+                        float v[8] = {};
+                        if (real && c * 8 < A.hd) {
+                            const float4 u = __ldg(reinterpret_cast<const float4*>(q + c * 8));
+                            const float4 w = __ldg(reinterpret_cast<const float4*>(q + c * 8 + 4));
+                            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+                            v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] *= inv;
+                        char* to = dst + (c / 8) * (kM * 128) + (((c & 7) ^ (r & 7)) * 16);
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                w[i] = PMath<T>::pack(v[2 * i], v[2 * i + 1]);
+                                const float2 f = PMath<T>::unpack(w[i]);
+                                v[2 * i] -= f.x;
+                                v[2 * i + 1] -= f.y;
+                            }
+                            *reinterpret_cast<uint4*>(to + p * C::kQ) =
+                                make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&q_full[x]);
+            }
+            const int hi_row = real ? min(it.kv_hi, pos + 1) : 0;
+            const int lo_row = real && A.window > 0 ? pos - A.window + 1 : INT_MIN;
+            const int sinks = A.window > 0 ? A.sinks : 0;
+            const int any_hi = min(it.kv_hi, it.pmax + 1);
+            const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
+            const int all_hi = min(it.kv_hi, it.pmin + 1);
+            const int all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < n; ++j, ++cnt, ring += 2) {
+                const int b = cnt & 1, j0 = W.tile(W.a + j) * kN;
+                const bool whole = j0 >= it.kv_lo && j0 + kN <= all_hi &&
+                                   (j0 >= all_lo || j0 + kN <= sinks);
+                if (!bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort)) {
+                    ok = false;
+                    break;
+                }
+                tc_after();
+                float s[kN];
+                tmem_ld64(lanes + C::s_col(x, b), s);
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) {
+                        const int p = j0 + i;
+                        if (!(p >= it.kv_lo && p < hi_row && (p >= lo_row || p < sinks)))
+                            s[i] = -INFINITY;
+                    }
+                    // V of a partly hidden tile: no infinity or NaN may meet a zero weight
+                    const uint32_t rv = ring + 1;
+                    if (!bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort)) {
+                        ok = false;
+                        break;
+                    }
+                    char* vt = sKV + (rv % kSlots) * C::kSlot;
+                    bool changed = false;
+                    for (int c = r; c < kN * HD / 8; c += kM) {
+                        uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
+                        const uint4 w = *at;
+                        if (PMath<T>::not_finite(w.x) || PMath<T>::not_finite(w.y) ||
+                            PMath<T>::not_finite(w.z) || PMath<T>::not_finite(w.w)) {
+                            const int p = j0 + ((c / 8) & (kN - 1));
+                            if (p >= it.kv_lo && p < any_hi && (p >= any_lo || p < sinks))
+                                P.redo[(size_t)(W.item - 1) * P.heads + head_lane] = 1;
+                            *at = make_uint4(0, 0, 0, 0);
+                            changed = true;
+                        }
+                    }
+                    if (changed) async_fence();
+                }
+                float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+#pragma unroll
+                for (int i = 4; i < kN; i += 4) {
+                    mx0 = fmaxf(mx0, s[i]);
+                    mx1 = fmaxf(mx1, s[i + 1]);
+                    mx2 = fmaxf(mx2, s[i + 2]);
+                    mx3 = fmaxf(mx3, s[i + 3]);
+                }
+                const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * fac;
+                if (__any_sync(kAll, mx > m + 8.f)) {
+                    const float to = fmaxf(m, mx);
+                    const float al = ex2(m - (to == -INFINITY ? 0.f : to));
+                    m = to;
+                    l *= al;
+                    if (j > 0) {
+                        if (!__all_sync(kAll, pv_done(x, cnt - 1))) {
+                            ok = false;
+                            break;
+                        }
+                        tc_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            float o[32];
+                            tmem_ld32(lanes + C::o_col(x) + c, o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= al;
+                            tmem_st32(lanes + C::o_col(x) + c, reinterpret_cast<uint32_t*>(o));
+                        }
+                    }
+                }
+                const float mb = (m == -INFINITY ? 0.f : m) - kShift;
+                float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+#pragma unroll
+                for (int i = 0; i < kN; i += 4) {
+                    s[i] = ex2(fmaf(s[i], fac, -mb));
+                    s[i + 1] = ex2(fmaf(s[i + 1], fac, -mb));
+                    s[i + 2] = ex2(fmaf(s[i + 2], fac, -mb));
+                    s[i + 3] = ex2(fmaf(s[i + 3], fac, -mb));
+                    l0 += s[i];
+                    l1 += s[i + 1];
+                    l2 += s[i + 2];
+                    l3 += s[i + 3];
+                }
+                l += (l0 + l1) + (l2 + l3);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        w[i] = PMath<T>::pack(s[2 * i], s[2 * i + 1]);
+                        if (p + 1 < PARTS) {
+                            const float2 f = PMath<T>::unpack(w[i]);
+                            s[2 * i] -= f.x;
+                            s[2 * i + 1] -= f.y;
+                        }
+                    }
+                    tmem_st32(lanes + C::p_col(x, b) + p * 32, w);
+                }
+                tmem_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&p_full[x][b]);
+            }
+            if (!ok) break;
+            // the rows of this piece of the item
+            if (!__all_sync(kAll, pv_done(x, cnt - 1))) {
+                ok = false;
+                break;
+            }
+            tc_after();
+            const bool complete = W.a == 0 && W.b == it.n_tiles;
+            const bool last_word = complete && A.n_groups == 0;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float M = m - kShift;
+            float* o32 = nullptr;
+            T* o16 = nullptr;
+            if (last_word) {
+                const size_t at = (size_t)tok * A.out_stride + (size_t)h * A.hd;
+                if (SPLIT) o32 = reinterpret_cast<float*>(A.out) + at;
+                else o16 = reinterpret_cast<T*>(A.out) + at;
+                if (real && A.lse) A.lse[(size_t)tok * A.nh + h] = row_lse(M, l);
+            } else {
+                const size_t id = complete ? (size_t)(which == 1) * A.n_tokens * A.nh +
+                                                 (size_t)tok * A.nh + h
+                                           : part_row(P, piece, head_lane, W.a > 0 ? 0 : 1, row);
+                o32 = (complete ? A.full_o : P.part_o) + id * A.hd;
+                if (real)
+                    *reinterpret_cast<float2*>((complete ? A.full_ml : P.part_ml) + id * 2) =
+                        make_float2(M, l);
+            }
+            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && h == h0)
+                P.where[tok] = PagedWhere{piece, 0, row, it.alone, which, W.item - 1};
+            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && h == h0)
+                P.where[tok].last = Pieces(P, P.cum[*P.n_items]).of(W.c0 + it.n_tiles - 1);
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                float o[32];
+                tmem_ld32(lanes + C::o_col(x) + c, o);
+                if (!real) continue;
+                if (last_word) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (c + i >= A.hd) break;
+                    if (o16) {
+                        *reinterpret_cast<uint4*>(o16 + c + i) =
+                            make_uint4(PMath<T>::pack(o[i], o[i + 1]), PMath<T>::pack(o[i + 2], o[i + 3]),
+                                       PMath<T>::pack(o[i + 4], o[i + 5]),
+                                       PMath<T>::pack(o[i + 6], o[i + 7]));
+                    } else {
+                        *reinterpret_cast<float4*>(o32 + c + i) =
+                            make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<float4*>(o32 + c + i + 4) =
+                            make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
+                    }
+                }
+            }
+            tc_before();
+        }
+    }
+
+    tc_before();
+    __syncthreads();
+    if (tid == 0 && (s_bad || s_abort)) P.bad[blockIdx.x] = s_bad | (s_abort ? PG_TIMEOUT : 0);
+    if (warp == kMmaWarp) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem)
+                     : "memory");
+    }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                             const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static EncodeFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                             &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(p);
+    });
+    return fn;
+}
+
+bool encode(CUtensorMap* map, const void* addr, const PagedArgs& A, bool bf16, int rows) {
+    EncodeFn fn = encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)A.hd, (cuuint64_t)A.nkv, (cuuint64_t)A.page_size,
+                                (cuuint64_t)A.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)A.hd * 2, (cuuint64_t)A.nkv * A.hd * 2,
+                                   (cuuint64_t)A.page_stride * 2};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, one[4] = {1, 1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+              const_cast<void*>(addr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int PARTS, int HD>
+cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
+    auto kern = paged_mma_kernel<T, PARTS, HD>;
+    constexpr int smem = MCfg<HD, PARTS>::kSmem;
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    int rows = kN;  // positions of a box: they lie in one page
+    while (A.page_size % rows) rows /= 2;
+    KvMaps maps;
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    if (!encode(&maps.k, A.k, A, bf16, rows) || !encode(&maps.v, A.v, A, bf16, rows))
+        return cudaErrorInvalidValue;
+    const PagedPlan& P = A.plan[which];
+    return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), (size_t)smem, s, A, maps, which,
+                      rows);
+}
+
+template <typename T, int PARTS>
+cudaError_t launch_hd(const PagedArgs& A, int which, cudaStream_t s) {
+    return A.hd == 64 ? launch_one<T, PARTS, 64>(A, which, s) : launch_one<T, PARTS, 128>(A, which, s);
+}
+
+}  // namespace
+
+// Head dims that the tensor-core kernel takes: one or two boxes of 64, the second possibly cut.
+bool paged_mma_takes(int hd) { return hd >= 64 && hd <= 128; }
+int paged_mma_tile() { return kN; }
+int paged_mma_rows(bool split) { return split ? kM : 2 * kM; }
+
+cudaError_t launch_paged_mma(const PagedArgs& A, int which, int q_dtype, int kv_dtype,
+                             cudaStream_t s) {
+    const bool split = q_dtype == WISP_DTYPE_F32;
+    if (kv_dtype == WISP_DTYPE_F16)
+        return split ? launch_hd<__half, 2>(A, which, s) : launch_hd<__half, 1>(A, which, s);
+    return split ? launch_hd<__nv_bfloat16, 3>(A, which, s)
+                 : launch_hd<__nv_bfloat16, 1>(A, which, s);
+}
+
+}  // namespace wb

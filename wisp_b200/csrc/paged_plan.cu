@@ -1,7 +1,7 @@
 // paged_plan.cu -- the row tiles of a paged attention call, found on the device: sequence
 // lengths stay there, so a step needs no host synchronisation and can be captured once.
 //
-// One CTA per plan (the sequences' own parts; the shared prefixes).  It counts the row tiles
+// One CTA per plan (sequences of few rows, shared prefixes, sequences of many rows).  It counts the row tiles
 // of every sequence, then for each row tile the KV tiles that its mask leaves (the window's
 // and the sinks'), and keeps running sums of both; the attention kernels cut the line of all
 // KV tiles into equal pieces.  A sequence without cached positions keeps one (fully hidden)
@@ -44,12 +44,13 @@ __device__ int block_scan(int v, int* total, int* warp_sums) {
     return x - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedArgs A) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PagedArgs A) {
     __shared__ int sums[32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const bool prefix = blockIdx.x == 1;
+    const bool prefix = blockIdx.x == PLAN_PREFIX;
     const PagedPlan& P = A.plan[blockIdx.x];
+    if (!P.used || P.inlined) return;
     const int n_seg = prefix ? A.n_groups : A.n_seq, tid = threadIdx.x;
     int carry = 0, total, bad = 0;
     for (int base = 0; base < n_seg; base += kPlanThreads) {
@@ -57,7 +58,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedArgs A) {
         int n = 0;
         if (i < n_seg) {
             const PagedSeg g = paged_segment(A, prefix, i);
-            n = (g.t1 - g.t0 + P.tpt - 1) / P.tpt;
+            n = g.t1 - g.t0 >= P.min_tok && g.t1 - g.t0 <= P.max_tok
+                    ? (g.t1 - g.t0 + P.tpt - 1) / P.tpt
+                    : 0;
             bad |= !prefix && length_too_long(A, i);
         }
         const int at = carry + block_scan(n, &total, sums);
@@ -92,12 +95,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedArgs A) {
         carry += total;
     }
     if (tid == 0) P.cum[n_items] = carry;
+    if (P.redo)
+        for (int i = tid; i < n_items * P.heads; i += kPlanThreads) P.redo[i] = 0;
 }
 
 }  // namespace
 
 cudaError_t launch_paged_plan(const PagedArgs& A, cudaStream_t s) {
-    return launch_pdl(plan_kernel, dim3(A.n_groups > 0 ? 2 : 1), dim3(kPlanThreads), 0, s, A);
+    return launch_pdl(plan_kernel, dim3(PLANS), dim3(kPlanThreads), 0, s, A);
 }
 
 }  // namespace wb
