@@ -9,8 +9,8 @@
 // Two tiles of 128 rows share each K / V tile.  S is double buffered, so the tensor core works
 // on tile j + 1 while the softmax warps work on tile j.  Roles:
 //   warps 0-3 (and 4-7)  softmax of row tile 0 (and 1): rows 32 * (warp & 3) + lane
-//   warp 8               issues the MMAs (one thread)
-//   warp 9               loads K and V: TMA boxes of up to 64 positions out of one page, lane
+//   warps 8 and 9        issue the MMAs of one row tile each (an elected thread)
+//   warp 10              loads K and V: TMA boxes of up to 64 positions out of one page, lane
 //                        per box, 128-byte swizzle, ring of 16-KB slots
 // A row's running maximum is only moved when a score passes it by more than 2^8 (the weights
 // then still fit 16 bits and the sums are fp32), so that O is rarely rescaled; the warp that
@@ -44,8 +44,8 @@ namespace {
 
 constexpr int kN = 64;          // positions of a KV tile
 constexpr int kM = 128;         // rows of a row tile
-constexpr int kThreads = 320;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 352;
+constexpr int kMmaWarp = 8, kLoadWarp = 10;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -133,13 +133,11 @@ __device__ __forceinline__ void tma4d(uint32_t dst, const CUtensorMap* map, int 
 // Shared-memory descriptors, 128-byte swizzle.  K-major (Q, K): 64 elements per row of 128 B,
 // atoms of 8 rows 1024 B apart.  MN-major (V: positions are K, head dims N): blocks of 64 dims
 // `lead` bytes apart, groups of 8 positions 1024 B apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
-           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// (Both as the low word of `addr` with a constant high word: an address step is one addition.)
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr, uint32_t lead) {
+    return (addr >> 4) | ((lead >> 4) << 16);
 }
 // Instruction descriptor of kind::f16: A and B fp16 (0) or bf16 (1), fp32 accumulator, M = 128,
 // N = n, A K-major, B K-major or (b_mn) MN-major.
@@ -147,21 +145,33 @@ __host__ __device__ constexpr uint32_t idesc(int type, int n, int b_mn) {
     return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
-                                       uint32_t acc) {
+// By the whole warp with the same operands; the thread with `leader` set issues.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc,
+                                       uint32_t leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"(acc), "r"(kDescHi), "r"(leader)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
-                                       uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc,
+                                       uint32_t leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"(acc), "r"(kDescHi), "r"(leader)
         : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t is;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(is));
+    return is;
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile(
@@ -280,11 +290,12 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     char* sQ = base;                                  // [kRT][PARTS][kH][128 rows][128 B]
     char* sKV = base + kRT * PARTS * C::kQ;           // [kSlots][kH][64 rows][128 B]
     __shared__ uint64_t full[kSlots], empty[kSlots];
-    __shared__ uint64_t q_full[kRT], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain;
+    __shared__ uint64_t q_full[kRT], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain[kRT];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ int s_bad;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (the shuffle tells the compiler that the warp number is the same for all lanes)
+    const int tid = threadIdx.x, warp = __shfl_sync(kAll, tid >> 5, 0), lane = tid & 31;
     const PagedPlan& P = A.plan[which];
     const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
     const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
@@ -293,7 +304,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     if (tid == 0) {
         for (int i = 0; i < kSlots; ++i) {
             bar_init(&full[i], 1);
-            bar_init(&empty[i], 1);
+            bar_init(&empty[i], kRT);
         }
         for (int x = 0; x < kRT; ++x) {
             bar_init(&q_full[x], 4);
@@ -303,7 +314,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 bar_init(&p_full[x][b], 4);
             }
         }
-        bar_init(&drain, 1);
+        for (int x = 0; x < kRT; ++x) bar_init(&drain[x], 1);
         s_abort = 0;
         s_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -408,70 +419,76 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         if (lane == 0)
             for (uint32_t i = ring > kSlots ? ring - kSlots : 0; i < ring; ++i)
                 bar_drain(&full[i % kSlots], (i / kSlots) & 1);
-    } else if (warp == kMmaWarp) {
-        // ------------------------------------------------------------- products
-        if (lane == 0) {
-            bool ok = true;
-            uint32_t seg[kRT] = {}, cnt[kRT] = {};  // segments, tiles of each row tile so far
-            const uint32_t q0 = smem_addr(sQ), kv0 = smem_addr(sKV);
-            auto issue_s = [&](int x, uint32_t ks, uint32_t c) {
-                const uint32_t d = tmem + C::s_col(x, c & 1);
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + kRT) {
+        // ------------------------------------------------------------- products of a row tile
+        const int x = warp - kMmaWarp;
+        const uint32_t leader = elect_one();
+        const uint32_t qd = desc_k(smem_addr(sQ) + x * PARTS * C::kQ);
+        const uint32_t kd = desc_k(smem_addr(sKV)), vd = desc_mn(smem_addr(sKV), kN * 128);
+        bool ok = true;
+        uint32_t seg = 0, cnt = 0;  // segments, KV tiles of this row tile so far
+        auto arrive_full = [&](uint32_t i) {
+            return bar_wait_warp(&full[i % kSlots], (i / kSlots) & 1, &s_abort);
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (leader) mma_commit(bar);
+            __syncwarp();
+        };
+        auto issue_s = [&](uint32_t slot, uint32_t c) {
+            const uint32_t d = tmem + C::s_col(x, c & 1), k0 = kd + slot * (C::kSlot >> 4);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)
+                    mma_ss(d, qd + ((p * C::kQ + (k / 4) * (kM * 128) + (k % 4) * 32) >> 4),
+                           k0 + (((k / 4) * (kN * 128) + (k % 4) * 32) >> 4), idesc(kType, kN, 0),
+                           (p | k) ? 1u : 0u, leader);
+            commit(&s_full[x][c & 1]);
+        };
+        while (ok && W.next(P)) {
+            const int n = W.b - W.a;
+            if (x * kM >= W.it.ntok * gpb) {  // no rows here: only give the slots back
+                for (int i = 0; ok && i < 2 * n; ++i, ++ring) {
+                    ok = arrive_full(ring);
+                    if (ok && lane == 0) bar_arrive(&empty[ring % kSlots]);
+                }
+                continue;
+            }
+            ok = bar_wait_warp(&q_full[x], seg & 1, &s_abort) && arrive_full(ring);
+            if (!ok) break;
+            ++seg;
+            tc_after();
+            issue_s(ring % kSlots, cnt);
+            commit(&empty[ring % kSlots]);
+            for (int j = 0; j < n; ++j, ++cnt, ring += 2) {
+                const uint32_t rv = ring + 1, rk = ring + 2;
+                if (j + 1 < n) {
+                    // S of the next tile takes the buffer of the last one's P
+                    ok = (j == 0 || __all_sync(kAll, pv_done(x, cnt - 1))) && arrive_full(rk);
+                    if (!ok) break;
+                    tc_after();
+                    issue_s(rk % kSlots, cnt + 1);
+                    commit(&empty[rk % kSlots]);
+                }
+                ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) && arrive_full(rv);
+                if (!ok) break;
+                tc_after();
+                const uint32_t d = tmem + C::o_col(x), a0 = tmem + C::p_col(x, 0) +
+                                                            (cnt & 1) * (C::p_col(x, 1) - C::p_col(x, 0));
+                const uint32_t v0 = vd + (rv % kSlots) * (C::kSlot >> 4);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        const uint32_t qa = q0 + (x * PARTS + p) * C::kQ + (k / 4) * (kM * 128) +
-                                            (k % 4) * 32;
-                        const uint32_t ka = kv0 + ks * C::kSlot + (k / 4) * (kN * 128) + (k % 4) * 32;
-                        mma_ss(d, desc_k(qa), desc_k(ka), idesc(kType, kN, 0), (p | k) ? 1u : 0u);
-                    }
-                mma_commit(&s_full[x][c & 1]);
-            };
-            while (ok && W.next(P)) {
-                const int n = W.b - W.a, nx = kRT == 2 && W.it.ntok * gpb > kM ? 2 : 1;
-                for (int x = 0; ok && x < nx; ++x) {
-                    ok = bar_wait(&q_full[x], seg[x] & 1, &s_abort) &&
-                         bar_wait(&full[ring % kSlots], (ring / kSlots) & 1, &s_abort);
-                    if (!ok) break;
-                    ++seg[x];
-                    tc_after();
-                    issue_s(x, ring % kSlots, cnt[x]);
-                }
-                if (!ok) break;
-                mma_commit(&empty[ring % kSlots]);
-                for (int j = 0; ok && j < n; ++j, ring += 2) {
-                    const uint32_t rv = ring + 1, rk = ring + 2;
-                    for (int x = 0; x < nx; ++x) {
-                        if (j + 1 < n) {
-                            // S of the next tile takes the buffer of the last one's P
-                            ok = (j == 0 || pv_done(x, cnt[x] - 1)) &&
-                                 bar_wait(&full[rk % kSlots], (rk / kSlots) & 1, &s_abort);
-                            if (!ok) break;
-                            tc_after();
-                            issue_s(x, rk % kSlots, cnt[x] + 1);
-                            if (x == nx - 1) mma_commit(&empty[rk % kSlots]);
-                        }
-                        ok = bar_wait(&p_full[x][cnt[x] & 1], (cnt[x] >> 1) & 1, &s_abort) &&
-                             bar_wait(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort);
-                        if (!ok) break;
-                        tc_after();
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                            for (int k = 0; k < kN / 16; ++k)
-                                mma_ts(tmem + C::o_col(x),
-                                       tmem + C::p_col(x, cnt[x] & 1) + p * 32 + k * 8,
-                                       desc_mn(kv0 + (rv % kSlots) * C::kSlot + k * 16 * 128, kN * 128),
-                                       idesc(kType, HD, 1), (j | p | k) ? 1u : 0u);
-                        mma_commit(&o_done[x][cnt[x] & 1]);
-                        if (x == nx - 1) mma_commit(&empty[rv % kSlots]);
-                        ++cnt[x];
-                    }
-                }
+                    for (int k = 0; k < kN / 16; ++k)
+                        mma_ts(d, a0 + p * 32 + k * 8, v0 + ((k * 16 * 128) >> 4),
+                               idesc(kType, HD, 1), p || k ? 1u : (uint32_t)(j > 0), leader);
+                commit(&o_done[x][cnt & 1]);
+                commit(&empty[rv % kSlots]);
             }
-            mma_commit(&drain);
-            bar_drain(&drain, 0);
         }
+        commit(&drain[x]);
+        if (lane == 0) bar_drain(&drain[x], 0);
+        __syncwarp();
     } else if (warp < 4 * kRT) {
         // ------------------------------------------------------------- softmax of a row tile
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;
