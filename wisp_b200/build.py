@@ -38,7 +38,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3,-Wall,-Wno-unused-function",
           f"-I{ROOT / 'include'}", f"-I{CSRC}"]
 SOURCES = ["moe_kernels.cu", "dense_ffn.cu", "prefill.cu", "expert_layout.cu", "quantize.cu",
-           "ref_launchers.cu", "decoder.cu", "paged.cu", "paged_plan.cu", "paged_attn.cu", "paged_mma.cu",
+           "ref_launchers.cu", "decoder.cu", "paged.cu", "paged_plan.cu", "paged_attn.cu", "paged_mma.cu", "paged_few.cu",
            "page_pool.cpp", "engine.cpp", "tiers.cpp", "stream_cache.cpp", "multi_gpu.cpp"]
 HEADERS = ["internal.h", "tiers.h", "route_common.cuh", "dense_ffn.h", "paged.h", "paged_math.cuh"]
 

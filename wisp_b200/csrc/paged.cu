@@ -17,8 +17,12 @@
 namespace wb {
 
 cudaError_t launch_paged_plan(const PagedArgs& A, cudaStream_t s);
-cudaError_t launch_paged_attn(const PagedArgs& A, int which, bool both, int rw, int q_dtype,
-                              int kv_dtype, cudaStream_t s);
+cudaError_t launch_paged_few(const PagedArgs& A, int which, bool both, int q_dtype, int kv_dtype,
+                             cudaStream_t s);
+int paged_few_tile();
+int paged_few_ctas(int hd);
+cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
+                              cudaStream_t s);
 cudaError_t launch_paged_mma(const PagedArgs& A, int which, int q_dtype, int kv_dtype,
                              cudaStream_t s);
 bool paged_mma_takes(int hd);
@@ -316,16 +320,20 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
 // ------------------------------------------------------------------------
 // Attention: what runs, and its workspace
 // ------------------------------------------------------------------------
+// What a row tile costs before its first KV tile, in KV tiles.
+constexpr int kLeadMma = 4, kLeadFew = 1;
+
 struct AttnShape {
-    int rw[PLANS];  // 16-row MMA tiles of the plan's row tiles; 0: the tensor-core kernel
+    int rw[PLANS];  // 16-row tiles of the plan's row tiles; 0: the tensor-core kernel
     size_t bytes;
 };
 
 // Fills the geometry, plans and (with a workspace) pointers of a call.
 //
 // Which kernel: a sequence (or group) whose rows for one kv head fit one 16-row tile of
-// mma.sync (8 rows in fp32) goes through paged_attn_kernel, whose CTAs are bound by HBM; more
-// rows go to tcgen05 where it takes the head dim, else to row tiles of two or four 16-row tiles.
+// mma.sync (8 rows in fp32) goes through paged_few_kernel, whose CTAs are bound by HBM; more
+// rows go to tcgen05 where it takes the head dim, else to paged_attn_kernel's row tiles of two
+// or four 16-row tiles.
 AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     const int per = split ? 8 : 16;
@@ -368,15 +376,18 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.hblocks = (A.group + P.gpb - 1) / P.gpb;
         P.heads = A.nkv * P.hblocks;
         const int rows = (int)std::min<long long>(tokens * P.gpb, most);
-        S.rw[w] = on_mma ? 0 : paged_attn_rw(rows, split);
-        P.tile = on_mma ? paged_mma_tile() : paged_attn_tile();
+        const bool is_few = !on_mma && rows <= per;
+        S.rw[w] = on_mma ? 0 : is_few ? 1 : paged_attn_rw(rows, split);
+        P.tile = on_mma ? paged_mma_tile() : is_few ? paged_few_tile() : paged_attn_tile();
         P.rows = on_mma ? most : S.rw[w] * per;
         P.tpt = std::max(1, P.rows / P.gpb);
         P.used_rows = w == PLAN_PREFIX ? P.rows : std::min(rows, P.rows);
-        const int ctas = (on_mma ? 1 : paged_attn_ctas(A.hd)) * sm_count();
+        const int ctas =
+            (on_mma ? 1 : is_few ? paged_few_ctas(A.hd) : paged_attn_ctas(A.hd)) * sm_count();
+        P.lead = on_mma ? kLeadMma : kLeadFew;
         P.lanes = std::min(4095, std::max(1, ctas / P.heads));
         P.max_items = A.n_tokens / P.tpt + n_seg;
-        P.inlined = !on_mma && n_seg <= kPagedInline &&
+        P.inlined = is_few && n_seg <= kPagedInline &&
                     (w == PLAN_PREFIX ? A.n_tokens : std::min(max_q, P.max_tok)) <= P.tpt;
         P.n_items = reinterpret_cast<int*>(take(4));
         P.bad = reinterpret_cast<int*>(take(((size_t)P.lanes * P.heads + 1) * 4));
@@ -405,8 +416,9 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
 
 cudaError_t launch_plan_kernel(const PagedArgs& A, const AttnShape& S, int which, bool both,
                                int q_dtype, int kv_dtype, cudaStream_t s) {
-    return S.rw[which] ? launch_paged_attn(A, which, both, S.rw[which], q_dtype, kv_dtype, s)
-                       : launch_paged_mma(A, which, q_dtype, kv_dtype, s);
+    return S.rw[which] == 0   ? launch_paged_mma(A, which, q_dtype, kv_dtype, s)
+           : S.rw[which] == 1 ? launch_paged_few(A, which, both, q_dtype, kv_dtype, s)
+                              : launch_paged_attn(A, which, S.rw[which], q_dtype, kv_dtype, s);
 }
 
 PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_heads, int n_groups) {
@@ -472,8 +484,8 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     for (int w = 0; w < PLANS; ++w) plan |= A.plan[w].used && !A.plan[w].inlined;
     if (plan) WB_CUDA_RET(launch_paged_plan(A, s), err);
     // the shared prefixes go with the sequences' own parts where one kernel takes both
-    const bool both = A.plan[PLAN_PREFIX].used && A.plan[PLAN_FEW].used && S.rw[PLAN_PREFIX] &&
-                      S.rw[PLAN_PREFIX] == S.rw[PLAN_FEW];
+    const bool both = A.plan[PLAN_PREFIX].used && A.plan[PLAN_FEW].used &&
+                      S.rw[PLAN_PREFIX] == 1 && S.rw[PLAN_FEW] == 1;
     const int order[PLANS] = {PLAN_PREFIX, PLAN_MANY, PLAN_FEW};
     for (int w : order) {
         if (!A.plan[w].used || (w == PLAN_PREFIX && both)) continue;

@@ -42,9 +42,10 @@ struct PagedWhere {
     int plan, item;
 };
 
-// A plan covers the row tiles of one kind: n_items items, cum[i] KV tiles before item i.  The
-// line of all KV tiles is cut into at most `lanes` equal pieces; one CTA takes a piece for one
-// block of query heads.
+// A plan covers the row tiles of one kind.  On the line of their work an item is `lead` units
+// (what it costs to begin one, in KV tiles) and its KV tiles; cum[i] units lie before item i.
+// The line is cut into at most `lanes` equal pieces; one CTA takes a piece for one block of
+// query heads.
 struct PagedPlan {
     int* n_items;
     int* bad;       // [lanes * heads + 1] status bits of each CTA, then of the plan
@@ -57,6 +58,7 @@ struct PagedPlan {
     PagedWhere* where;  // prefix mode: [n_tokens]
     int* redo;          // [max_items][heads], set for items to be worked out without tiles
     int tile;           // positions of a KV tile
+    int lead;
     int tpt;            // tokens of a row tile
     int rows;           // rows of a row tile
     int used_rows;      // of them at most so many are used

@@ -32,11 +32,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kTile = 64;  // positions of a KV tile
-template <bool B>
-struct Bool {
-    static constexpr bool value = B;
-};
-constexpr int kInlineItems = kPagedInline;
 
 template <int HD>
 struct Cfg {
@@ -56,7 +51,7 @@ constexpr size_t attn_smem_bytes() {
 // another inside the loop (each loads what it reads).
 // ------------------------------------------------------------------------
 template <typename T, bool SPLIT, int HD, int RW>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs A, int which0) {
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs A, int which) {
     using C = Cfg<HD>;
     constexpr int kCh = C::kCh, kS = C::kStages;
     constexpr int kNP = kTile * RW / 4;       // positions per warp and tile
@@ -69,10 +64,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     T* qs = ring + (size_t)kS * C::kStage;    // [kF][16 * RW][HD], swizzled like the cache rows
     __shared__ int s_pos[16 * RW];            // position of each real row (INT_MIN: no row)
     __shared__ float s_fac[16 * RW];          // SPLIT: the row's power-of-two factor
-    __shared__ int s_cum[kInlineItems + 1];
-    __shared__ int s_sum[4];
     __shared__ int s_bad;
-    const int which = blockIdx.y ? PLAN_PREFIX : which0;
     const PagedPlan& P = A.plan[which];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c4 = lane & 3;
     const int rw = warp % RW, pw = warp / RW;
@@ -84,68 +76,20 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const bool inlined = P.inlined != 0;
     if (tid == 0) {
         s_bad = 0;
         P.bad[blockIdx.x] = 0;
         if (head_lane == 0) P.split[piece] = PagedSplit{0, 0, 0, 0, 0, 0};
-        if (inlined && blockIdx.x == 0) P.bad[P.lanes * P.heads] = 0;
     }
-    const int n_items = inlined ? (which == PLAN_PREFIX ? A.n_groups : A.n_seq) : *P.n_items;
+    const int n_items = *P.n_items;
     if (n_items == 0) return;
-    const int* cum = inlined ? s_cum : P.cum;
-    if (inlined) {
-        // one row tile per segment: every CTA counts the KV tiles itself, which is shorter than
-        // a kernel of its own before this one (the join kernel reads what one CTA leaves)
-        __syncthreads();  // the words above are cleared
-        int carry = 0;
-        for (int base = 0; base < n_items; base += kThreads) {
-            const int i = base + tid;
-            int n = 0;
-            if (i < n_items) {
-                n = make_item(A, P, which == PLAN_PREFIX, i, 0).n_tiles;
-                if (blockIdx.x == 0 && which != PLAN_PREFIX) {
-                    const int t = A.q_start[i + 1] - A.q_start[i];
-                    if (length_too_long(A, i) || (t > P.tpt && t <= P.max_tok))
-                        P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
-                }
-            }
-            int v = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += y;
-            }
-            if (lane == 31) s_sum[warp] = v;
-            __syncthreads();
-            int before = carry;
-            for (int w = 0; w < 4; ++w) {
-                if (w < warp) before += s_sum[w];
-                carry += s_sum[w];
-            }
-            if (i < n_items) s_cum[i] = before + v - n;
-            __syncthreads();
-        }
-        if (tid == 0) s_cum[n_items] = carry;
-        __syncthreads();
-        if (blockIdx.x == 0)  // for the join kernel
-            for (int i = tid; i <= n_items; i += kThreads) P.cum[i] = s_cum[i];
-    }
+    const int* cum = P.cum;
     const int total = cum[n_items];
     const Pieces pieces(P, total);
     if (piece >= pieces.n) return;
     int x = pieces.start(piece);
     const int x_end = pieces.start(piece + 1);
-    // the item that holds KV tile x: the last with cum <= x
-    int lo = 0, span = n_items;
-    while (span > 1) {
-        const int step = (span + kThreads - 1) / kThreads;
-        const int at = lo + min(tid * step, span - 1);
-        const int hit = __syncthreads_count(tid * step < span && cum[at] <= x);
-        lo += (hit - 1) * step;
-        span = min(step, span - (hit - 1) * step);
-    }
-    int item = lo;
+    int item = block_last_le(cum, n_items, x);  // the item of unit x
 
     const T* __restrict__ Kc = reinterpret_cast<const T*>(A.k);
     const T* __restrict__ Vc = reinterpret_cast<const T*>(A.v);
@@ -153,11 +97,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     constexpr float kShift = PMath<T>::kPShift;
 
     for (; x < x_end; ++item) {
-        const PagedItem it = inlined ? make_item(A, P, which == PLAN_PREFIX, item, 0) : P.items[item];
-        const int c0 = cum[item];
+        const PagedItem it = P.items[item];
+        const int c0 = cum[item] + P.lead;
         if (it.n_tiles == 0) continue;
-        const int a = x - c0, b = min(it.n_tiles, x_end - c0);  // KV tiles [a, b) of the item
-        x = c0 + b;
+        const int a = max(0, x - c0), b = min(it.n_tiles, x_end - c0);  // KV tiles [a, b)
+        x = c0 + max(b, 0);
+        if (b <= 0) break;  // the piece ends before the item's first tile
         const bool whole = a == 0 && b == it.n_tiles;
         const int n_rows = it.ntok * gpb;
         if (a == 0 && head_lane == 0) {  // what the join kernels need to know
@@ -259,8 +204,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
         int st = 0;
         for (int i = a; i < b; ++i) {
             cp_wait<kS - 2>();
-            if (RW == 1) __syncwarp();
-            else __syncthreads();
+            __syncthreads();
             {
                 const int ld = st == 0 ? kS - 1 : st - 1;
                 if (i + kS - 1 < b) load_tile(ld, off);
@@ -411,8 +355,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
                     }
                 }
             };
-            if (odd) weigh(Bool<true>());
-            else weigh(Bool<false>());
+            if (odd) weigh(Flag<true>());
+            else weigh(Flag<false>());
         }
         cp_wait<0>();
 #pragma unroll
@@ -512,7 +456,11 @@ paged_join_kernel(const __grid_constant__ PagedArgs A, int which, int last_plan)
     const int h0 = kvh * A.group + hb * P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
     const int warp = threadIdx.x / 32;
     Joined J;
-    if (P.redo && blockIdx.y == 0) {
+    int marked = 0;
+    if (P.redo && blockIdx.y == 0)
+        for (int i = sp.item0 + (int)threadIdx.x; i < sp.item1; i += kJoinThreads)
+            marked |= P.redo[(size_t)i * P.heads + head_lane];
+    if (P.redo && blockIdx.y == 0 && __syncthreads_or(marked)) {
         for (int i = sp.item0; i < sp.item1; ++i) {
             if (!P.redo[(size_t)i * P.heads + head_lane]) continue;
             const PagedItem it = P.items[i];
@@ -576,29 +524,27 @@ paged_join2_kernel(const __grid_constant__ PagedArgs A) {
 }
 
 template <typename T, bool SPLIT, int HD, int RW>
-cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, cudaStream_t s) {
+cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     auto kern = paged_attn_kernel<T, SPLIT, HD, RW>;
     constexpr size_t smem = attn_smem_bytes<HD, RW, SPLIT ? PMath<T>::kFrags : 1>();
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const PagedPlan& P = A.plan[which];
-    return launch_pdl(kern, dim3(P.heads * P.lanes, with_prefix ? 2 : 1), dim3(kThreads), smem, s, A,
-                      which);
+    return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), smem, s, A, which);
 }
 
 template <typename T, bool SPLIT, int HD>
-cudaError_t launch_rw(const PagedArgs& A, int which, bool both, int rw, cudaStream_t s) {
-    return rw == 1 ? launch_one<T, SPLIT, HD, 1>(A, which, both, s)
-           : rw == 2 ? launch_one<T, SPLIT, HD, 2>(A, which, both, s)
-                     : launch_one<T, SPLIT, HD, 4>(A, which, both, s);
+cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
+    return rw == 2 ? launch_one<T, SPLIT, HD, 2>(A, which, s)
+                   : launch_one<T, SPLIT, HD, 4>(A, which, s);
 }
 
 template <typename T, bool SPLIT>
-cudaError_t launch_t(const PagedArgs& A, int which, bool both, int rw, cudaStream_t s) {
-    return A.hd <= 64    ? launch_rw<T, SPLIT, 64>(A, which, both, rw, s)
-           : A.hd <= 128 ? launch_rw<T, SPLIT, 128>(A, which, both, rw, s)
-                         : launch_rw<T, SPLIT, 256>(A, which, both, rw, s);
+cudaError_t launch_t(const PagedArgs& A, int which, int rw, cudaStream_t s) {
+    // (64 to 128 dims are the tensor-core kernel's)
+    return A.hd < 64 ? launch_rw<T, SPLIT, 64>(A, which, rw, s)
+                     : launch_rw<T, SPLIT, 256>(A, which, rw, s);
 }
 
 template <typename T, bool SPLIT>
@@ -628,23 +574,20 @@ cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
 
 int paged_attn_tile() { return kTile; }
 
-// 16-row MMA tiles of a row tile with `rows` rows: 1, 2 or 4.
-int paged_attn_rw(int rows, bool split) {
-    const int per = split ? 8 : 16;
-    return rows <= per ? 1 : rows <= 2 * per ? 2 : 4;
-}
+// 16-row MMA tiles of a row tile with `rows` rows.
+int paged_attn_rw(int rows, bool split) { return rows <= (split ? 16 : 32) ? 2 : 4; }
 
 // CTAs of one SM: what the ring leaves room for.
-int paged_attn_ctas(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
+int paged_attn_ctas(int hd) { return hd <= 64 ? 3 : 1; }
 
-cudaError_t launch_paged_attn(const PagedArgs& A, int which, bool both, int rw, int q_dtype,
-                              int kv_dtype, cudaStream_t s) {
+cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
+                              cudaStream_t s) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     if (kv_dtype == WISP_DTYPE_F16)
-        return split ? launch_t<__half, true>(A, which, both, rw, s)
-                     : launch_t<__half, false>(A, which, both, rw, s);
-    return split ? launch_t<__nv_bfloat16, true>(A, which, both, rw, s)
-                 : launch_t<__nv_bfloat16, false>(A, which, both, rw, s);
+        return split ? launch_t<__half, true>(A, which, rw, s)
+                     : launch_t<__half, false>(A, which, rw, s);
+    return split ? launch_t<__nv_bfloat16, true>(A, which, rw, s)
+                 : launch_t<__nv_bfloat16, false>(A, which, rw, s);
 }
 
 cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s) {

@@ -43,6 +43,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
                  : "memory");
 }
 
+template <bool B>
+struct Flag {
+    static constexpr bool value = B;
+};
+
 template <typename T>
 struct PMath;
 
@@ -206,12 +211,13 @@ __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bo
         it.pmin = 0x7fffffff;
         it.pmax = -0x7fffffff;
         reach = 0;
-        int s = g.s0;
-        for (int t = it.tok0; t < it.tok0 + it.ntok; ++t) {
-            while (s + 1 < g.s1 && A.q_start[s + 1] <= t) ++s;
-            const int n = cached_positions(A, s), p = n - (A.q_start[s + 1] - t);
-            it.pmin = min(it.pmin, p);
-            it.pmax = max(it.pmax, p);
+#pragma unroll 4
+        for (int s = g.s0; s < g.s1; ++s) {  // the tile's tokens of each sequence
+            const int end = A.q_start[s + 1], n = cached_positions(A, s);
+            const int a = max(A.q_start[s], it.tok0), b = min(end, it.tok0 + it.ntok);
+            if (a >= b) continue;
+            it.pmin = min(it.pmin, n - (end - a));
+            it.pmax = max(it.pmax, n - (end - b) - 1);
             reach = max(reach, n);
         }
     }
@@ -331,6 +337,44 @@ __device__ void load_rows(const PagedArgs& A, int tok0, int n_rows, int h0, int 
     }
 }
 
+// The same from up to 8 fp32 rows that lie in shared memory ([row][HD]), by a block of 128
+// threads: parts into `out` ([fragment][16][HD], swizzled), factors by row.
+template <typename T, int HD>
+__device__ __forceinline__ void split_rows(const PagedArgs& A, const float* rows, int n_rows, T* out,
+                                           float* s_fac) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kN = HD / 64;
+    for (int r = threadIdx.x >> 5; r < 8; r += 4) {
+        float2 v[kN];
+        float mx = 0.f;
+#pragma unroll
+        for (int u = 0; u < kN; ++u) {
+            v[u] = r < n_rows ? *reinterpret_cast<const float2*>(rows + r * HD + (u * 32 + lane) * 2)
+                              : make_float2(0.f, 0.f);
+            mx = fmaxf(mx, fmaxf(fabsf(v[u].x), fabsf(v[u].y)));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const uint32_t e = (__float_as_uint(mx) >> 23) & 255u;
+        const bool scaled = PMath<T>::kPShift != 0.f && e > 0 && e < 254;
+        const float inv = scaled ? __uint_as_float((254u - e) << 23) : 1.f;
+        if (lane == 0) s_fac[r] = scaled ? __uint_as_float(e << 23) : 1.f;
+#pragma unroll
+        for (int u = 0; u < kN; ++u) {
+            const int d = (u * 32 + lane) * 2;
+            uint32_t p[3] = {0, 0, 0};
+            PMath<T>::split(v[u].x * inv, v[u].y * inv, p[0], p[1], p[2]);
+            T* to = out + ((((d / 8) ^ (r & 7)) * 8) + (d & 7));  // rows r and r + 8 share the key
+            *reinterpret_cast<uint32_t*>(to + r * HD) = p[0];
+            *reinterpret_cast<uint32_t*>(to + (r + 8) * HD) = p[1];
+            if (PMath<T>::kFrags == 2) {
+                *reinterpret_cast<uint32_t*>(to + (16 + r) * HD) = p[2];
+                *reinterpret_cast<uint32_t*>(to + (24 + r) * HD) = 0;
+            }
+        }
+    }
+}
+
 // log-sum-exp (natural) of a row whose weights 2^(score - M), score in log2 units, sum to L.
 __device__ __forceinline__ float row_lse(float M, float L) {
     return L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
@@ -351,8 +395,25 @@ __device__ __forceinline__ void gather_status(const PagedArgs& A) {
     if (threadIdx.x == 0) *A.status = any | len | late;
 }
 
-// The line of `total` KV tiles in pieces: as many as there are lanes, each with a tile at least.
-// Piece p starts at tile piece_start(p); tile x lies in piece piece_of(x).
+__device__ __forceinline__ int item_units(const PagedPlan& P, int tiles) {
+    return tiles ? tiles + P.lead : 0;
+}
+
+// The last i in [0, n) with cum[i] <= x (cum[0] <= x), by the whole block.
+__device__ __forceinline__ int block_last_le(const int* cum, int n, int x) {
+    int lo = 0, span = n;
+    while (span > 1) {
+        const int step = (span + (int)blockDim.x - 1) / (int)blockDim.x;
+        const int at = (int)threadIdx.x * step;
+        const int hit = __syncthreads_count(at < span && cum[lo + min(at, span - 1)] <= x) - 1;
+        lo += hit * step;
+        span = min(step, span - hit * step);
+    }
+    return lo;
+}
+
+// The line of `total` units in pieces: as many as there are lanes, each with a unit at least.
+// Piece p starts at unit start(p); unit x lies in piece of(x).
 struct Pieces {
     int total, n;
     __device__ Pieces(const PagedPlan& P, int total_) : total(total_), n(min(P.lanes, total_)) {}

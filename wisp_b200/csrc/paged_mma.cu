@@ -257,18 +257,18 @@ struct MShift {
 struct Walk {
     int item, x, x_end;
     int a, b;  // KV tiles [a, b) of the item
-    int c0;    // the item's first tile on the line
+    int c0;    // the item's first KV tile on the line
     PagedItem it;
     __device__ __forceinline__ bool next(const PagedPlan& P) {
         while (x < x_end) {
             it = P.items[item];
-            c0 = P.cum[item];
+            c0 = P.cum[item] + P.lead;
             ++item;
             if (it.n_tiles == 0) continue;
-            a = x - c0;
+            a = max(0, x - c0);
             b = min(it.n_tiles, x_end - c0);
-            x = c0 + b;
-            return true;
+            x = c0 + max(b, 0);
+            return b > 0;  // (not: the piece ends before the item's first tile)
         }
         return false;
     }
@@ -341,17 +341,18 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             W.x = pieces.start(piece);
             W.x_end = pieces.start(piece + 1);
         }
-        W.item = n_items ? last_le(P.cum, n_items, W.x) : 0;
+        W.item = n_items ? block_last_le(P.cum, n_items, W.x) : 0;
         if (tid == 0) {
             P.bad[blockIdx.x] = 0;
             if (head_lane == 0) {
                 PagedSplit sp{0, 0, 0, -1, 0, 0};
-                // the items that begin in this piece
-                sp.item0 = W.item + (n_items && W.x < W.x_end && P.cum[W.item] < W.x);
+                // the items whose first KV tile lies in this piece
+                sp.item0 = W.item + (n_items && W.x < W.x_end && P.cum[W.item] + P.lead < W.x);
                 sp.item1 = sp.item0;
                 if (W.x < W.x_end) {
                     int last = last_le(P.cum, n_items, W.x_end - 1);
-                    sp.item1 = last + 1;
+                    last -= P.cum[last] + P.lead >= W.x_end;
+                    sp.item1 = max(sp.item0, last + 1);
                     if (last >= sp.item0 && P.cum[last + 1] > W.x_end && A.n_groups == 0) {
                         const PagedItem it = P.items[last];
                         sp.tok0 = it.tok0;

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
                 else hi = mid;
             }
             const PagedItem it = make_item(A, P, prefix, lo, i - P.item_off[lo]);
-            tiles = it.n_tiles;
+            tiles = item_units(P, it.n_tiles);
             P.items[i] = it;
         }
         const int at = carry + block_scan(tiles, &total, sums);
