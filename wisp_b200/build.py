@@ -40,7 +40,7 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3,-Wall,-Wno-
 SOURCES = ["moe_kernels.cu", "dense_ffn.cu", "prefill.cu", "expert_layout.cu", "quantize.cu",
            "ref_launchers.cu", "decoder.cu", "paged.cu", "paged_plan.cu", "paged_attn.cu", "paged_mma.cu", "paged_few.cu",
            "page_pool.cpp", "engine.cpp", "tiers.cpp", "stream_cache.cpp", "multi_gpu.cpp"]
-HEADERS = ["internal.h", "tiers.h", "route_common.cuh", "dense_ffn.h", "paged.h", "paged_math.cuh"]
+HEADERS = ["internal.h", "tiers.h", "route_common.cuh", "dense_ffn.h", "paged.h", "paged_math.cuh", "paged_tma.cuh"]
 
 
 def _headers() -> list[Path]:

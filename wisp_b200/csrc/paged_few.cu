@@ -4,13 +4,16 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(log2(e) scale q_i . k_j - m_i)
 //
-// A CTA streams its piece of the line of KV tiles (64 positions, one kv head) through a ring of
-// cp.async stages that does not stop at the end of a row tile: the next one's rows of q and its
-// first positions are on their way while the last tiles of this one are worked on.  Per tile,
-// each of the four warps scores 16 of the positions; the row maxima and the weights go through
-// shared memory, and then each warp adds all 64 weighted positions to a quarter of the head's
-// dims.  (The first form had each warp keep all dims for its own positions: 64 accumulators a
-// thread, a join of four 16 x head_dim tiles per row tile, and a ring that drained there.)
+// A CTA streams its piece of the line of KV tiles (64 positions, one kv head).  A loading warp
+// walks the piece's row tiles, looks their pages up and issues the TMA boxes (128-byte swizzle)
+// and the rows of q into rings that do not stop at the end of a row tile.  Four warps work: each
+// scores 16 of a tile's positions; the row maxima and the weights go through shared memory, and
+// then each warp adds all 64 weighted positions to a quarter of the head's dims.
+//
+// Before: each warp kept all dims for its own positions (64 accumulators a thread, a join of four
+// 16 x head_dim tiles and an empty ring at the end of every row tile: 39.7 us for 14 ragged
+// sequences of up to 4096 positions); the same split with cp.async issued by the working warps
+// (486 instructions a warp and tile: 35.7 us, but long windows fell from 6.4 to 5.6 TB/s).
 //
 // 32-bit rows are split into 16-bit parts (two in fp16, 22 bits, three in bf16) that share the
 // 16 rows of a fragment, 8 rows each; their sums meet in one thread.  The weights are split the
@@ -21,28 +24,32 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
 #include "paged.h"
 #include "paged_math.cuh"
+#include "paged_tma.cuh"
 
 namespace wb {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kWork = 128;             // working threads
+constexpr int kThreads = kWork + 32;  // and the loading warp
 constexpr int kTile = 64;
-constexpr int kRecs = 16;
+constexpr int kRecs = 32;
 
 template <typename T, bool SPLIT, int HD>
 struct FCfg {
     static constexpr int kF = SPLIT ? PMath<T>::kFrags : 1;  // 16-row fragments of a row's parts
     static constexpr int kStages = HD == 64 ? 4 : HD == 128 && kF == 1 ? 3 : 2;
     static constexpr int kCtas = HD == 64 ? 3 : HD == 128 ? 2 : 1;
-    static constexpr int kStage = 2 * kTile * HD;                  // elements: K then V
+    static constexpr int kHalves = HD / 64;
+    static constexpr int kTen = kTile * HD * 2;      // bytes of a K or V tile
     static constexpr int kQBytes = SPLIT ? 8 * HD * 4 : 16 * HD * 2;  // a row tile's q as it is
-    // converted q (fp32 rows only) or the tile's weights
-    static constexpr int kWork = std::max(kF * 16 * kTile, SPLIT ? kF * 16 * HD : 0);
-    static constexpr size_t kSmem = (size_t)kStages * kStage * 2 + 2 * kQBytes + (size_t)kWork * 2;
+    // converted q (fp32 rows only) or the tile's weights, elements
+    static constexpr int kBuf = std::max(kF * 16 * kTile, SPLIT ? kF * 16 * HD : 0);
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kTen + 2 * kQBytes + kBuf * 2;
 };
 
 struct Rec {  // a row tile of this piece and its KV tiles [a, b); b < 0: there are no more
@@ -51,28 +58,46 @@ struct Rec {  // a row tile of this piece and its KV tiles [a, b); b < 0: there 
     int item, c0;
 };
 
+__device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
 template <typename T, bool SPLIT, int HD>
 __global__ void __launch_bounds__(kThreads, (FCfg<T, SPLIT, HD>::kCtas))
-paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
+paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ KvMaps maps, int which0,
+                 int box_rows) {
     using C = FCfg<T, SPLIT, HD>;
-    constexpr int kF = C::kF, kS = C::kStages, kCh = HD / 8, kRows = SPLIT ? 8 : 16;
+    constexpr int kF = C::kF, kS = C::kStages, kRows = SPLIT ? 8 : 16;
     constexpr int kDW = HD / 4;  // dims of a warp
     constexpr float kShift = PMath<T>::kPShift;
-    extern __shared__ __align__(128) char smem[];
-    T* ring = reinterpret_cast<T*>(smem);
-    char* qraw = smem + (size_t)kS * C::kStage * 2;
+    extern __shared__ char raw[];
+    char* ring = reinterpret_cast<char*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    char* qraw = ring + kS * 2 * C::kTen;  // [2] rows of q as they are
     T* work = reinterpret_cast<T*>(qraw + 2 * C::kQBytes);
+    __shared__ uint64_t full[kS], empty[kS], q_full[2], q_empty[2];
+    __shared__ volatile int s_abort;
     __shared__ Rec s_rec[kRecs], s_cur[2];
     __shared__ int s_cum[kPagedInline + 1];
-    __shared__ int s_sum[4], s_bad, s_pos[16];
+    __shared__ int s_sum[kThreads / 32], s_bad, s_pos[16];
     __shared__ float s_fac[16], s_max[4][16], s_l[4][16];
     const int which = blockIdx.y ? PLAN_PREFIX : which0;
     const PagedPlan& P = A.plan[which];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c4 = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kAll, tid >> 5, 0);
+    const int g = lane >> 2, c4 = lane & 3;
     const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
     const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
     const int h0 = kvh * A.group + hb * P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
 
+    if (tid == 0) {
+        for (int i = 0; i < kS; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&q_full[i], 33);
+            bar_init(&q_empty[i], 4);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -111,7 +136,8 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
             if (lane == 31) s_sum[warp] = v;
             __syncthreads();
             int before = carry;
-            for (int w = 0; w < 4; ++w) {
+#pragma unroll
+            for (int w = 0; w < kThreads / 32; ++w) {
                 if (w < warp) before += s_sum[w];
                 carry += s_sum[w];
             }
@@ -127,62 +153,27 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
     const int x0 = pieces.start(piece), x_end = pieces.start(piece + 1);
     const int item0 = block_last_le(cum, n_items, x0);
 
-    const T* __restrict__ Kc = reinterpret_cast<const T*>(A.k);
-    const T* __restrict__ Vc = reinterpret_cast<const T*>(A.v);
+    __syncthreads();  // the barriers are there (a plan that is not inlined had no barrier yet)
     const int sinks = A.window > 0 ? A.sinks : 0;
 
-    // ---------------------------------------------------------------- what comes next
-    // Records of this piece, kRecs at a time; the loading side walks them (all threads alike).
-    int lk = 0, li = 0, lq = 0;  // record, next tile of it, row tiles begun
-    int issued = 0;              // tiles whose copies were issued
-    bool have = false;           // there is a next tile, with
-    long long off = -1;          // the cache offset of this lane's row of it (-1: unseen)
-    auto fill = [&]() {
-        if (tid < kRecs) {
-            Rec r;
-            r.b = -1;
-            r.a = 0;
-            r.item = item0 + lk + tid;
-            if (r.item < n_items && cum[r.item] < x_end) {
-                r.it = inlined ? make_item(A, P, prefix, r.item, 0) : P.items[r.item];
-                r.c0 = cum[r.item] + P.lead;
-                r.a = max(0, x0 - r.c0);
-                r.b = max(0, min(r.it.n_tiles, x_end - r.c0));
+    if (warp == kWork / 32) {
+        // ------------------------------------------------------------ loads
+        const int per_half = kTile / box_rows, boxes = per_half * C::kHalves;
+        uint32_t tiles = 0, rows = 0;  // KV tiles and row tiles so far
+        bool ok = true;
+        // hands a record (and with it the rows of q) over
+        auto hand = [&](const Rec& r) {
+            const int b = rows & 1;
+            if (!bar_wait_warp(&q_empty[b], ((rows >> 1) & 1) ^ 1, &s_abort)) return false;
+            ++rows;
+            if (lane == 0) {
+                s_cur[b] = r;
+                bar_arrive(&q_full[b]);
             }
-            s_rec[tid] = r;
-        }
-        __syncthreads();
-    };
-    auto look = [&]() {  // to the next tile that exists
-        const Rec* r = &s_rec[lk % kRecs];
-        while (r->b >= 0 && li >= r->b) {
-            ++lk;
-            if (lk % kRecs == 0) {
-                __syncthreads();
-                fill();
-            }
-            r = &s_rec[lk % kRecs];
-            li = r->a;
-            if (r->b > r->a) ++lq;
-        }
-        have = r->b >= 0;
-        if (!have) return;
-        const PagedItem& it = r->it;
-        const int t = li < it.n_sink ? it.sink0 + li : it.first + li - it.n_sink;
-        const int j = t * kTile + warp * 16 + (lane & 15);
-        const int any_hi = min(it.kv_hi, it.pmax + 1);
-        const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
-        const bool seen = j >= it.kv_lo && j < any_hi && (j >= any_lo || j < sinks);
-        off = seen ? page_offset(A, it.seq, j, kvh, &s_bad) : -1;
-    };
-    auto issue = [&]() {
-        const Rec& r = s_rec[lk % kRecs];
-        if (li == r.a) {  // the row tile's record and rows travel with its first positions
-            if (tid == 0) s_cur[lq & 1] = r;
-            char* dst = qraw + (lq & 1) * C::kQBytes;
+            char* dst = qraw + b * C::kQBytes;
             constexpr int kPer = SPLIT ? HD / 4 : HD / 8;  // 16-byte pieces of a row
-            const int n_rows = r.it.ntok * gpb;
-            for (int i = tid; i < n_rows * kPer; i += kThreads) {
+            const int n = r.b < 0 ? 0 : r.it.ntok * gpb * kPer;
+            for (int i = lane; i < n; i += 32) {
                 const int row = i / kPer, c = i - row * kPer;
                 const size_t at = (size_t)(r.it.tok0 + row / gpb) * A.q_stride +
                                   (size_t)(h0 + row % gpb) * A.hd;
@@ -196,70 +187,85 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
                          reinterpret_cast<const T*>(A.q) + (in ? at + c * 8 : 0), in);
                 }
             }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                             smem_addr(&q_full[b]))
+                         : "memory");
+            return true;
+        };
+        for (int k = 0; ok; ++k) {
+            if (k % kRecs == 0) {  // the next records, one a lane
+                __syncwarp();
+                Rec r;
+                r.a = 0;
+                r.b = -1;
+                r.item = item0 + k + lane;
+                if (r.item < n_items && cum[r.item] < x_end) {
+                    r.it = inlined ? make_item(A, P, prefix, r.item, 0) : P.items[r.item];
+                    r.c0 = cum[r.item] + P.lead;
+                    r.a = max(0, x0 - r.c0);
+                    r.b = max(0, min(r.it.n_tiles, x_end - r.c0));
+                }
+                s_rec[lane] = r;
+                __syncwarp();
+            }
+            const Rec& r = s_rec[k % kRecs];
+            if (r.b >= 0 && r.a >= r.b) continue;
+            auto place = [&](int i) {
+                const int t = i < r.it.n_sink ? r.it.sink0 + i : r.it.first + i - r.it.n_sink;
+                return lane < boxes
+                           ? box_place(A, r.it, t * kTile, lane % per_half, box_rows, &s_bad)
+                           : make_int2(0, 0);
+            };
+            int2 at = r.b < 0 ? make_int2(0, 0) : place(r.a);
+            for (int i = r.a; ok && i < r.b; ++i, ++tiles) {
+                const int2 cur = at;
+                if (i + 1 < r.b) at = place(i + 1);
+                const int st = tiles % kS;
+                ok = bar_wait_warp(&empty[st], ((tiles / kS) & 1) ^ 1, &s_abort);
+                if (!ok) break;
+                if (lane == 0) bar_expect(&full[st], 2 * C::kTen);
+                __syncwarp();
+                const uint32_t dst = smem_addr(ring + st * 2 * C::kTen);
+                if (lane < boxes) {
+                    const int half = lane / per_half, rb = lane % per_half;
+                    const uint32_t to = dst + half * (kTile * 128) + rb * box_rows * 128;
+                    tma4d(to, &maps.k, half * 64, kvh, cur.y, cur.x, &full[st]);
+                    tma4d(to + C::kTen, &maps.v, half * 64, kvh, cur.y, cur.x, &full[st]);
+                }
+                if (i == r.a) ok = hand(r);
+            }
+            if (r.b < 0) {  // the end
+                if (ok) hand(r);
+                break;
+            }
         }
-        T* kd = ring + (size_t)(issued % kS) * C::kStage;
-        T* vd = kd + kTile * HD;
-        constexpr int kPer = kCh >= 32 ? 1 : 32 / kCh;  // rows per pass of the warp
-#pragma unroll
-        for (int p = 0; p < 16 / kPer; ++p) {
-            const int rr = p * kPer + (kCh >= 32 ? 0 : lane / kCh);
-            const long long o = __shfl_sync(0xffffffffu, off, rr);
-            const int row = warp * 16 + rr, c = kCh >= 32 ? lane : lane % kCh;
-            const bool in = o >= 0 && c * 8 < A.hd;
-            const size_t src = in ? (size_t)o + c * 8 : 0;
-            const int to = row * HD + ((c ^ (row & 7)) * 8);
-            cp16(kd + to, Kc + src, in);
-            cp16(vd + to, Vc + src, in);
-        }
-        ++issued;
-        ++li;
-        look();
-    };
-
-    fill();
-    li = s_rec[0].a;
-    if (s_rec[0].b > s_rec[0].a) lq = 1;
-    look();
-    int cq = 0, done = 0, end = 0;  // row tiles begun, tiles worked on, tile that ends this one
-    // Copy group c holds tile c while one tile is issued per iteration; where it was not (at most
-    // one row tile is fetched ahead), the next `loose` iterations wait for all groups.
-    int loose = 0;
-#pragma unroll
-    for (int u = 0; u < kS - 1; ++u) {
-        if (have && lq <= cq + 1) issue();
-        else if (have) loose = kS;
         cp_commit();
-    }
-
+        cp_wait<0>();
+        __syncwarp();
+        if (lane == 0)  // (only after a timeout can some of these still be in flight)
+            for (uint32_t i = tiles > (uint32_t)kS ? tiles - kS : 0; i < tiles; ++i)
+                bar_drain(&full[i % kS], (i / kS) & 1);
+    } else {
+    // ---------------------------------------------------------------- work
     Rec cur;
     int hi_row[2] = {0, 0}, lo_row[2] = {INT_MIN, INT_MIN};
     int all_hi = 0, all_lo = 0, n_rows = 0;
     float fac = A.scale_log2;
     uint32_t qf[kF][HD / 16][4];
     float o[kDW / 8][4], m[2], l[2];
-    int ci = 0;  // tile of the current row tile
+    uint32_t done = 0, rows = 0;  // KV tiles, row tiles so far
+    int ci = 0;                   // tile of the current row tile
+    bool begins = true;
 
-    while (done < issued || have) {
-        if (loose > 0) {
-            cp_wait<0>();
-            --loose;
-        } else {
-            cp_wait<kS - 2>();
-        }
-        __syncthreads();  // this tile is here, the last one's stage, weights and maxima are free
-        const bool begins = done == end;
+    for (;;) {
         if (begins) {
-            ++cq;
-            cur = s_cur[cq & 1];
-            end = done + cur.b - cur.a;
+            const int b = rows & 1;
+            if (!__all_sync(kAll, bar_wait(&q_full[b], (rows >> 1) & 1, &s_abort))) break;
+            cur = s_cur[b];
+            if (cur.b < 0) break;
             ci = cur.a;
         }
-        {
-            int n = 0;
-            for (; have && lq <= cq + 1 && issued < done + kS; ++n) issue();
-            if (n > 1 || (n == 0 && have)) loose = kS;
-            cp_commit();
-        }
+        if (!__all_sync(kAll, bar_wait(&full[done % kS], (done / kS) & 1, &s_abort))) break;
         const PagedItem& it = cur.it;
         if (begins) {
             n_rows = it.ntok * gpb;
@@ -271,12 +277,13 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
                     pos = it.mixed ? token_position(A, it.tok0 + tid / gpb) : it.pos0 + tid / gpb;
                 s_pos[tid] = pos;
             }
-            const T* q = reinterpret_cast<const T*>(qraw + (cq & 1) * C::kQBytes);
+            const T* q = reinterpret_cast<const T*>(qraw + (rows & 1) * C::kQBytes);
             if (SPLIT) {
+                work_sync();  // the last tile's weights have been read
                 split_rows<T, HD>(A, reinterpret_cast<const float*>(q), n_rows, work, s_fac);
                 q = work;
             }
-            __syncthreads();
+            work_sync();
 #pragma unroll
             for (int n = 0; n < kF; ++n)
 #pragma unroll
@@ -284,6 +291,10 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
                     const int r = lane & 15, c = kk * 2 + (lane >> 4);
                     ldsm4(qf[n][kk], q + (size_t)(n * 16 + r) * HD + ((c ^ (r & 7)) * 8));
                 }
+            __syncwarp();
+            if (lane == 0) bar_arrive(&q_empty[rows & 1]);
+            ++rows;
+            begins = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int pos = SPLIT && u ? INT_MIN : s_pos[g + 8 * u];
@@ -299,8 +310,12 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
                 for (int u = 0; u < 4; ++u) o[d][u] = 0.f;
         }
 
-        const T* kd = ring + (size_t)(done % kS) * C::kStage;
-        const T* vd = kd + kTile * HD;
+        // [half][position][64 dims], 16-byte pieces XORed with the position's low bits
+        const char* kd = ring + (done % kS) * 2 * C::kTen;
+        const char* vd = kd + C::kTen;
+        auto piece_at = [&](const char* tile, int row, int c) {
+            return tile + (c / 8) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) * 16);
+        };
         const int j0 = (ci < it.n_sink ? it.sink0 + ci : it.first + ci - it.n_sink) * kTile;
         const bool full = j0 >= it.kv_lo && j0 + kTile <= all_hi &&
                           (j0 >= all_lo || j0 + kTile <= sinks);
@@ -320,7 +335,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
             const int r = warp * 16 + ((lane >> 4) & 1) * 8 + (lane & 7);
             const int c = kk * 2 + ((lane >> 3) & 1);
             uint32_t kf[4];
-            ldsm4(kf, kd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+            ldsm4(kf, piece_at(kd, r, c));
 #pragma unroll
             for (int n = 0; n < kF; ++n) {
                 PMath<T>::mma(s[0], qf[n][kk], kf[0], kf[1]);
@@ -343,7 +358,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
             mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
             if (c4 == 0) s_max[warp][g + 8 * u] = mx[u];
         }
-        __syncthreads();
+        work_sync();
         float al[2] = {1.f, 1.f};
 #pragma unroll
         for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
@@ -391,20 +406,20 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) o[d][u] *= SPLIT ? al[0] : al[u >> 1];
         }
-        // Rows that see different positions of one tile: what is hidden from one may be an
-        // infinity or a NaN that another sees.  Looked for first (rare), so that the usual loop
+        // What a partly hidden tile hides (a page's end that nobody wrote, another row's future)
+        // may hold infinities and NaNs.  They are looked for first (rare), so that the usual loop
         // stays short.
         bool odd = false;
-        if (!full && it.pmin != it.pmax) {
+        if (!full) {
             for (int i = lane; i < kTile * kDW / 8; i += 32) {
                 const int r = i / (kDW / 8), c = warp * (kDW / 8) + i % (kDW / 8);
-                const uint4 w = *reinterpret_cast<const uint4*>(vd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+                const uint4 w = *reinterpret_cast<const uint4*>(piece_at(vd, r, c));
                 odd |= PMath<T>::not_finite(w.x) || PMath<T>::not_finite(w.y) ||
                        PMath<T>::not_finite(w.z) || PMath<T>::not_finite(w.w);
             }
             odd = __any_sync(0xffffffffu, odd);
         }
-        __syncthreads();  // the weights are there
+        work_sync();  // the weights are there
         auto weigh = [&](auto special) {
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk) {
@@ -429,7 +444,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
                     const int r = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
                     const int c = warp * (kDW / 8) + d + (lane >> 4);
                     uint32_t vf[4];
-                    ldsm4t(vf, vd + (size_t)r * HD + ((c ^ (r & 7)) * 8));
+                    ldsm4t(vf, piece_at(vd, r, c));
                     if (decltype(special)::value) {
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
@@ -452,16 +467,18 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
         };
         if (odd) weigh(Flag<true>());
         else weigh(Flag<false>());
+        __syncwarp();
+        if (lane == 0) bar_arrive(&empty[done % kS]);
         ++done;
-        ++ci;
-        if (done != end) continue;
+        if (++ci < cur.b) continue;
+        begins = true;
 
         // ------------------------------------------------------------ the row tile's piece ends
         const bool whole = cur.a == 0 && cur.b == it.n_tiles;
         if (cur.a == 0 && head_lane == 0) {  // what the join kernels need to know
             const int last = pieces.of(cur.c0 + it.n_tiles - 1);
             if (A.n_groups > 0) {
-                for (int i = tid; i < it.ntok; i += kThreads)
+                for (int i = tid; i < it.ntok; i += kWork)
                     P.where[it.tok0 + i] =
                         PagedWhere{piece, last, i * P.gpb, it.alone, which, cur.item};
             } else if (!whole && tid == 0) {
@@ -474,7 +491,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
             if (c4 == 0) s_l[warp][g + 8 * u] = l[u];
         }
-        __syncthreads();
+        work_sync();
 #pragma unroll
         for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
             const int row = g + 8 * u;
@@ -491,9 +508,9 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, int which0) {
             if (warp == 0 && c4 == 0) R.put_ml(m[u] - kShift, L);
         }
     }
-    cp_wait<0>();
+    }
     __syncthreads();
-    if (tid == 0 && s_bad) P.bad[blockIdx.x] = s_bad;
+    if (tid == 0 && (s_bad || s_abort)) P.bad[blockIdx.x] = s_bad | (s_abort ? PG_TIMEOUT : 0);
 }
 
 template <typename T, bool SPLIT, int HD>
@@ -503,9 +520,13 @@ cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, cudaStre
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
+    KvMaps maps;
+    const int rows = kv_maps(&maps, A, std::is_same<T, __nv_bfloat16>::value,
+                             kTile);
+    if (rows == 0) return cudaErrorInvalidValue;
     const PagedPlan& P = A.plan[which];
     return launch_pdl(kern, dim3(P.heads * P.lanes, with_prefix ? 2 : 1), dim3(kThreads), smem, s, A,
-                      which);
+                      maps, which, rows);
 }
 
 template <typename T, bool SPLIT>

@@ -28,16 +28,15 @@
 // parts), O of head_dim columns per row tile.  Every wait is bounded; on a timeout all roles
 // leave, copies and products in flight are drained and TMEM is freed.
 
-#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <mutex>
 #include <type_traits>
 
 #include "internal.h"
 #include "paged.h"
 #include "paged_math.cuh"
+#include "paged_tma.cuh"
 
 namespace wb {
 namespace {
@@ -46,8 +45,6 @@ constexpr int kN = 64;          // positions of a KV tile
 constexpr int kM = 128;         // rows of a row tile
 constexpr int kThreads = 352;
 constexpr int kMmaWarp = 8, kLoadWarp = 10;
-constexpr unsigned long long kWaitNs = 2000000000ull;
-constexpr unsigned kAll = 0xffffffffu;
 
 template <int HD, int PARTS>
 struct MCfg {
@@ -65,70 +62,6 @@ struct MCfg {
     }
     static __host__ __device__ constexpr int o_col(int x) { return 512 - (kRT - x) * HD; }
 };
-
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_addr(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait; false when it ran out here or in another role.
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
-    if (bar_try(b, parity)) return true;
-    uint64_t t0 = 0;
-    for (uint32_t it = 0;; ++it) {
-        if (bar_try(b, parity)) return true;
-        if ((it & 63) == 63) {
-            if (*abort_flag) return false;
-            const uint64_t t = now_ns();
-            if (t0 == 0) t0 = t;
-            else if (t - t0 > kWaitNs) {
-                *abort_flag = 1;
-                return false;
-            }
-        }
-    }
-}
-__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, uint32_t parity,
-                                              volatile int* abort_flag) {
-    return __all_sync(kAll, bar_wait(b, parity, abort_flag));
-}
-__device__ __forceinline__ void bar_drain(uint64_t* b, uint32_t parity) {
-    const uint64_t t0 = now_ns();
-    while (!bar_try(b, parity))
-        if (now_ns() - t0 > kWaitNs) return;
-}
-
-__device__ __forceinline__ void tma4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
-                                      int c3, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
-        "r"(smem_addr(bar))
-        : "memory");
-}
 
 // Shared-memory descriptors, 128-byte swizzle.  K-major (Q, K): 64 elements per row of 128 B,
 // atoms of 8 rows 1024 B apart.  MN-major (V: positions are K, head dims N): blocks of 64 dims
@@ -242,10 +175,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-
-struct KvMaps {
-    CUtensorMap k, v;  // (dim, kv head, position in page, page), boxes of 64 dims
-};
 
 // Weights of 16-bit pairs stay below 2^15 with the maximum up to 2^8 behind (fp16).
 template <typename T>
@@ -378,23 +307,11 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         const int half = lane / per_half, rb = lane - half * per_half;
         bool ok = true;
         while (ok && W.next(P)) {
-            const PagedItem& it = W.it;
-            const int any_hi = min(it.kv_hi, it.pmax + 1);
-            const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
-            const int sinks = A.window > 0 ? A.sinks : 0;
-            // this lane's page and row of a tile's box (outside the pool: zeros)
+            // this lane's page and row of a tile's box
             auto place = [&](int i) {
-                int2 at = make_int2(A.n_pages, 0);
-                const int j = W.tile(i) * kN + rb * box_rows, je = j + box_rows;
-                if (lane < boxes && j < any_hi && je > it.kv_lo && (je > any_lo || j < sinks)) {
-                    const int p = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size;
-                    const int page = __ldg(A.table + (size_t)it.seq * A.table_stride + p);
-                    if ((unsigned)page < (unsigned)A.n_pages)
-                        at = make_int2(page, j - p * A.page_size);
-                    else
-                        atomicOr(&s_bad, PG_BAD_PAGE);
-                }
-                return at;
+                return lane < boxes
+                           ? box_place(A, W.it, W.tile(i) * kN, rb, box_rows, &s_bad)
+                           : make_int2(0, 0);
             };
             int2 at = place(W.a);
             for (int i = W.a; ok && i < W.b; ++i) {
@@ -751,39 +668,6 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     }
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                             const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encoder() {
-    static EncodeFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
-                                             &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeFn>(p);
-    });
-    return fn;
-}
-
-bool encode(CUtensorMap* map, const void* addr, const PagedArgs& A, bool bf16, int rows) {
-    EncodeFn fn = encoder();
-    if (!fn) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)A.hd, (cuuint64_t)A.nkv, (cuuint64_t)A.page_size,
-                                (cuuint64_t)A.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)A.hd * 2, (cuuint64_t)A.nkv * A.hd * 2,
-                                   (cuuint64_t)A.page_stride * 2};
-    const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, one[4] = {1, 1, 1, 1};
-    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-              const_cast<void*>(addr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int PARTS, int HD>
 cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     auto kern = paged_mma_kernel<T, PARTS, HD>;
@@ -791,12 +675,9 @@ cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    int rows = kN;  // positions of a box: they lie in one page
-    while (A.page_size % rows) rows /= 2;
     KvMaps maps;
-    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    if (!encode(&maps.k, A.k, A, bf16, rows) || !encode(&maps.v, A.v, A, bf16, rows))
-        return cudaErrorInvalidValue;
+    const int rows = kv_maps(&maps, A, std::is_same<T, __nv_bfloat16>::value, kN);
+    if (rows == 0) return cudaErrorInvalidValue;
     const PagedPlan& P = A.plan[which];
     return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), (size_t)smem, s, A, maps, which,
                       rows);
