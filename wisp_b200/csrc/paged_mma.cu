@@ -12,6 +12,7 @@
 //   warps 8 and 9        issue the MMAs of one row tile each (an elected thread)
 //   warp 10              loads K and V: TMA boxes of up to 64 positions out of one page, lane
 //                        per box, 128-byte swizzle, ring of 16-KB slots
+//   warp 11              loads the rows of Q, one row tile ahead
 // A row's running maximum is only moved when a score passes it by more than 2^8 (the weights
 // then still fit 16 bits and the sums are fp32), so that O is rarely rescaled; the warp that
 // needs it does so itself, behind the previous product.
@@ -43,8 +44,8 @@ namespace {
 
 constexpr int kN = 64;          // positions of a KV tile
 constexpr int kM = 128;         // rows of a row tile
-constexpr int kThreads = 352;
-constexpr int kMmaWarp = 8, kLoadWarp = 10;
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 10, kRowWarp = 11;
 
 template <int HD, int PARTS>
 struct MCfg {
@@ -52,8 +53,11 @@ struct MCfg {
     static constexpr int kHalves = HD / 64;
     static constexpr int kSlot = kN * HD * 2;            // bytes of a K or V tile
     static constexpr int kQ = kM * HD * 2;               // bytes of one part of Q
-    static constexpr int kSlots = HD == 64 ? 12 : PARTS == 3 ? 7 : 9;
-    static constexpr int kSmem = 1024 + kRT * PARTS * kQ + kSlots * kSlot;
+    // Q of this and the next row tile where the ring keeps four KV tiles beside them (with 128
+    // dims it does not: a ring of three tiles cost more than Q's early loads gave)
+    static constexpr int kQBufs = HD == 64 ? 2 : 1;
+    static constexpr int kSlots = HD == 64 ? (PARTS == 3 ? 8 : 12) : PARTS == 3 ? 7 : 9;
+    static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot;
     // TMEM columns
     static constexpr int kPCols = 32 * PARTS;
     static __host__ __device__ constexpr int s_col(int x, int b) { return (x * 2 + b) * 64; }
@@ -182,6 +186,18 @@ struct MShift {
     static constexpr float value = std::is_same<T, __half>::value ? 6.f : 0.f;
 };
 
+// The low n bits (none for n <= 0, all for n >= 64).
+__device__ __forceinline__ uint64_t below(int n) {
+    return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+// Nonzero when a half of v is an infinity or a NaN: adding one to a full exponent carries.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t v) {
+    constexpr uint32_t e = PMath<T>::kExp * 0x10001u;
+    constexpr uint32_t one = (PMath<T>::kExp & (0u - PMath<T>::kExp)) * 0x10001u;
+    return ((v & e) + one) & 0x80008000u;
+}
+
 // The shared state of a piece's walk: which item and tiles come next.  Every role walks alike.
 struct Walk {
     int item, x, x_end;
@@ -206,21 +222,103 @@ struct Walk {
     }
 };
 
+// By one warp: n rows of Q from row `row0` of the item on into a 128-row tile (zeros below them).
+template <typename T, int PARTS, int HD>
+__device__ __forceinline__ void load_q_tile(const PagedArgs& A, int tok0, int row0, int n, int h0,
+                                            int gpb, bool flip, char* tile, float* s_fac) {
+    const int lane = threadIdx.x & 31;
+    using C = MCfg<HD, PARTS>;
+    auto source = [&](int r) {
+        const int row = row0 + r, t = row / gpb;
+        return (size_t)(tok0 + t) * A.q_stride + (size_t)(h0 + row - t * gpb) * A.hd;
+    };
+    if constexpr (PARTS == 1) {
+        constexpr int kCh = HD / 8, kPer = 32 / kCh;  // rows per pass
+        const int c = lane % kCh;
+        const T* q = reinterpret_cast<const T*>(A.q) + c * 8;
+        char* dst = tile + (c / 8) * (kM * 128);
+        const bool in_row = c * 8 < A.hd;
+#pragma unroll 8
+        for (int r = lane / kCh; r < kM; r += kPer) {
+            const bool in = r < n && in_row;
+            char* to = dst + r * 128 + (((c & 7) ^ (r & 7)) * 16);
+            const T* from = in ? q + source(r) : reinterpret_cast<const T*>(A.q);
+            if (!flip) {
+                cp16(to, from, in);
+            } else {
+                uint4 w = in ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+                w.x ^= 0x80008000u, w.y ^= 0x80008000u, w.z ^= 0x80008000u, w.w ^= 0x80008000u;
+                *reinterpret_cast<uint4*>(to) = w;
+            }
+        }
+        cp_commit();
+        cp_wait<0>();
+    } else {
+        // fp32 rows, HD / 32 floats a lane: parts of 16 bits, in fp16 of q / 2^e with 2^e the row's
+        // largest exponent
+        constexpr int kV = HD / 32;  // 2 or 4
+        const int d = lane * kV, c = d / 8;
+#pragma unroll 4
+        for (int r = 0; r < kM; ++r) {
+            const bool in = r < n && d < A.hd;
+            const float* from = reinterpret_cast<const float*>(A.q) + (in ? source(r) + d : 0);
+            float v[kV], mx = 0.f;
+            if constexpr (kV == 4) {
+                const float4 w = in ? __ldg(reinterpret_cast<const float4*>(from))
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+            } else {
+                const float2 w = in ? __ldg(reinterpret_cast<const float2*>(from))
+                                    : make_float2(0.f, 0.f);
+                v[0] = w.x, v[1] = w.y;
+            }
+#pragma unroll
+            for (int i = 0; i < kV; ++i) mx = fmaxf(mx, fabsf(v[i]));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
+            const uint32_t e = (__float_as_uint(mx) >> 23) & 255u;
+            const bool scaled = std::is_same<T, __half>::value && e > 0 && e < 254;
+            const float inv = (scaled ? __uint_as_float((254u - e) << 23) : 1.f) * (flip ? -1.f : 1.f);
+            if (lane == 0) s_fac[r] = scaled ? __uint_as_float(e << 23) : 1.f;
+            char* to = tile + (c / 8) * (kM * 128) + r * 128 + (((c & 7) ^ (r & 7)) * 16) + (d & 7) * 2;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) v[i] *= inv;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                uint32_t w[kV / 2];
+#pragma unroll
+                for (int i = 0; i < kV / 2; ++i) {
+                    w[i] = PMath<T>::pack(v[2 * i], v[2 * i + 1]);
+                    const float2 f = PMath<T>::unpack(w[i]);
+                    v[2 * i] -= f.x;
+                    v[2 * i + 1] -= f.y;
+                }
+                if constexpr (kV == 4)
+                    *reinterpret_cast<uint2*>(to + p * C::kQ) = make_uint2(w[0], w[1]);
+                else
+                    *reinterpret_cast<uint32_t*>(to + p * C::kQ) = w[0];
+            }
+        }
+    }
+}
+
 template <typename T, int PARTS, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ KvMaps maps, int which,
-                 int box_rows) {
+paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ KvMaps maps,
+                 const __grid_constant__ CUtensorMap q_map, int which, int box_rows, int q_boxes) {
     using C = MCfg<HD, PARTS>;
     constexpr int kRT = C::kRT, kSlots = C::kSlots, kH = C::kHalves;
     constexpr bool SPLIT = PARTS > 1;
     constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     extern __shared__ char raw[];
     char* base = reinterpret_cast<char*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    char* sQ = base;                                  // [kRT][PARTS][kH][128 rows][128 B]
-    char* sKV = base + kRT * PARTS * C::kQ;           // [kSlots][kH][64 rows][128 B]
+    constexpr int kQB = C::kQBufs;
+    char* sQ = base;                                // [kQB][kRT][PARTS][kH][128 rows][128 B]
+    char* sKV = base + kQB * kRT * PARTS * C::kQ;   // [kSlots][kH][64 rows][128 B]
     __shared__ uint64_t full[kSlots], empty[kSlots];
-    __shared__ uint64_t q_full[kRT], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain[kRT];
+    __shared__ uint64_t q_full[kRT][kQB], q_empty[kRT][kQB], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain[kRT];
     __shared__ uint32_t s_tmem;
+    __shared__ float s_fac[kRT][kQB][kM];  // fp32 rows: score factors
     __shared__ volatile int s_abort;
     __shared__ int s_bad;
     // (the shuffle tells the compiler that the warp number is the same for all lanes)
@@ -236,7 +334,10 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             bar_init(&empty[i], kRT);
         }
         for (int x = 0; x < kRT; ++x) {
-            bar_init(&q_full[x], 4);
+            for (int b = 0; b < kQB; ++b) {
+                bar_init(&q_full[x][b], 1);
+                bar_init(&q_empty[x][b], SPLIT ? 5 : 1);
+            }
             for (int b = 0; b < 2; ++b) {
                 bar_init(&o_done[x][b], 1);
                 bar_init(&s_full[x][b], 1);
@@ -341,7 +442,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         // ------------------------------------------------------------- products of a row tile
         const int x = warp - kMmaWarp;
         const uint32_t leader = elect_one();
-        const uint32_t qd = desc_k(smem_addr(sQ) + x * PARTS * C::kQ);
+        const uint32_t qd0 = desc_k(smem_addr(sQ) + x * PARTS * C::kQ);
         const uint32_t kd = desc_k(smem_addr(sKV)), vd = desc_mn(smem_addr(sKV), kN * 128);
         bool ok = true;
         uint32_t seg = 0, cnt = 0;  // segments, KV tiles of this row tile so far
@@ -352,7 +453,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             if (leader) mma_commit(bar);
             __syncwarp();
         };
-        auto issue_s = [&](uint32_t slot, uint32_t c) {
+        auto issue_s = [&](uint32_t slot, uint32_t c, uint32_t qb) {
+            const uint32_t qd = qd0 + qb * (kRT * PARTS * C::kQ >> 4);
             const uint32_t d = tmem + C::s_col(x, c & 1), k0 = kd + slot * (C::kSlot >> 4);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
@@ -372,21 +474,25 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 }
                 continue;
             }
-            ok = bar_wait_warp(&q_full[x], seg & 1, &s_abort) && arrive_full(ring);
+            const uint32_t qb = seg % kQB;
+            // S of tile c takes the buffer of tile c - 2's P
+            ok = bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_abort) && arrive_full(ring) &&
+                 (cnt < 2 || __all_sync(kAll, pv_done(x, cnt - 2)));
             if (!ok) break;
             ++seg;
             tc_after();
-            issue_s(ring % kSlots, cnt);
+            issue_s(ring % kSlots, cnt, qb);
             commit(&empty[ring % kSlots]);
+            if (n == 1) commit(&q_empty[x][qb]);
             for (int j = 0; j < n; ++j, ++cnt, ring += 2) {
                 const uint32_t rv = ring + 1, rk = ring + 2;
                 if (j + 1 < n) {
-                    // S of the next tile takes the buffer of the last one's P
-                    ok = (j == 0 || __all_sync(kAll, pv_done(x, cnt - 1))) && arrive_full(rk);
+                    ok = (cnt == 0 || __all_sync(kAll, pv_done(x, cnt - 1))) && arrive_full(rk);
                     if (!ok) break;
                     tc_after();
-                    issue_s(rk % kSlots, cnt + 1);
+                    issue_s(rk % kSlots, cnt + 1, qb);
                     commit(&empty[rk % kSlots]);
+                    if (j + 2 == n) commit(&q_empty[x][qb]);
                 }
                 ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) && arrive_full(rv);
                 if (!ok) break;
@@ -407,13 +513,50 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         commit(&drain[x]);
         if (lane == 0) bar_drain(&drain[x], 0);
         __syncwarp();
+    } else if (warp == kRowWarp) {
+        // ------------------------------------------------------------- rows of Q
+        const bool flip = A.scale_log2 < 0.f;  // q takes the sign, so that the factor is >= 0
+        uint32_t seg[kRT] = {};
+        bool ok = true;
+        while (ok && W.next(P)) {
+            const int n_rows = W.it.ntok * gpb;
+#pragma unroll
+            for (int x = 0; x < kRT; ++x) {
+                if (!ok || x * kM >= n_rows) continue;
+                const uint32_t qb = seg[x] % kQB;
+                ok = bar_wait_warp(&q_empty[x][qb], ((seg[x] / kQB) & 1) ^ 1, &s_abort);
+                if (!ok) continue;
+                ++seg[x];
+                if (q_boxes) {
+                    if (lane == 0) {
+                        bar_expect(&q_full[x][qb], C::kQ);
+#pragma unroll
+                        for (int h = 0; h < kH; ++h)
+                            tma3d(smem_addr(sQ + (qb * kRT + x) * C::kQ + h * (kM * 128)), &q_map,
+                                  h * 64, h0, W.it.tok0 + x * (kM / gpb), &q_full[x][qb]);
+                    }
+                    continue;
+                }
+                const int n = min(kM, n_rows - x * kM);
+                load_q_tile<T, PARTS, HD>(A, W.it.tok0, x * kM, n, h0, gpb, flip,
+                                          sQ + (qb * kRT + x) * PARTS * C::kQ, s_fac[x][qb]);
+                async_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&q_full[x][qb]);
+            }
+        }
+        if (q_boxes && lane == 0)  // (only after a timeout can some of these still be in flight)
+#pragma unroll
+            for (int x = 0; x < kRT; ++x)
+                for (uint32_t i = seg[x] > (uint32_t)kQB ? seg[x] - kQB : 0; i < seg[x]; ++i)
+                    bar_drain(&q_full[x][i % kQB], (i / kQB) & 1);
+        __syncwarp();
     } else if (warp < 4 * kRT) {
         // ------------------------------------------------------------- softmax of a row tile
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const bool flip = A.scale_log2 < 0.f;  // q takes the sign, so that fac >= 0
         constexpr float kShift = MShift<T>::value;
-        uint32_t cnt = 0;
+        uint32_t cnt = 0, seg = 0;
         bool ok = true;
         while (ok && W.next(P)) {
             const PagedItem& it = W.it;
@@ -428,65 +571,18 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             int pos = INT_MIN;
             if (real) pos = it.mixed ? token_position(A, tok) : it.pos0 + row / gpb;
             float fac = fabsf(A.scale_log2);
-            {
-                // this thread's row of Q (the previous item's products have read theirs: the
-                // last S of this row tile has been waited for)
-                char* dst = sQ + x * PARTS * C::kQ + r * 128;
-                const size_t src = (size_t)tok * A.q_stride + (size_t)h * A.hd;
-                if (!SPLIT) {
-                    const T* q = reinterpret_cast<const T*>(A.q) + src;
-                    const uint32_t sign = flip ? 0x80008000u : 0u;
-#pragma unroll
-                    for (int c = 0; c < HD / 8; ++c) {
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (real && c * 8 < A.hd) w = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
-                        w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
-                        *reinterpret_cast<uint4*>(dst + (c / 8) * (kM * 128) +
-                                                  (((c & 7) ^ (r & 7)) * 16)) = w;
-                    }
-                } else {
-                    const float* q = reinterpret_cast<const float*>(A.q) + src;
-                    float mx = 0.f;
-                    for (int d = 0; real && d < A.hd; d += 4) {
-                        const float4 w = __ldg(reinterpret_cast<const float4*>(q + d));
-                        mx = fmaxf(fmaxf(mx, fmaxf(fabsf(w.x), fabsf(w.y))),
-                                   fmaxf(fabsf(w.z), fabsf(w.w)));
-                    }
-                    const uint32_t e = (__float_as_uint(mx) >> 23) & 255u;
-                    const bool scaled = kType == 0 && e > 0 && e < 254;
-                    const float inv = (scaled ? __uint_as_float((254u - e) << 23) : 1.f) *
-                                      (flip ? -1.f : 1.f);
-                    if (scaled) fac *= __uint_as_float(e << 23);
-                    for (int c = 0; c < HD / 8; ++c) {
-                        float v[8] = {};
-                        if (real && c * 8 < A.hd) {
-                            const float4 u = __ldg(reinterpret_cast<const float4*>(q + c * 8));
-                            const float4 w = __ldg(reinterpret_cast<const float4*>(q + c * 8 + 4));
-                            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-                            v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] *= inv;
-                        char* to = dst + (c / 8) * (kM * 128) + (((c & 7) ^ (r & 7)) * 16);
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                w[i] = PMath<T>::pack(v[2 * i], v[2 * i + 1]);
-                                const float2 f = PMath<T>::unpack(w[i]);
-                                v[2 * i] -= f.x;
-                                v[2 * i + 1] -= f.y;
-                            }
-                            *reinterpret_cast<uint4*>(to + p * C::kQ) =
-                                make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
+            if (SPLIT) {
+                const uint32_t qb = seg % kQB;
+                if (!bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_abort)) {
+                    ok = false;
+                    break;
                 }
-                async_fence();
+                fac *= s_fac[x][qb][r];
                 __syncwarp();
-                if (lane == 0) bar_arrive(&q_full[x]);
+                if (lane == 0) bar_arrive(&q_empty[x][qb]);
             }
+            ++seg;
+            fac = fmaxf(fac, 1e-37f);  // (0 would make NaNs of hidden scores)
             const int hi_row = real ? min(it.kv_hi, pos + 1) : 0;
             const int lo_row = real && A.window > 0 ? pos - A.window + 1 : INT_MIN;
             const int sinks = A.window > 0 ? A.sinks : 0;
@@ -507,12 +603,14 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 float s[kN];
                 tmem_ld64(lanes + C::s_col(x, b), s);
                 if (!whole) {
+                    // this row's visible places as bits
+                    uint64_t seen = below(hi_row - j0) & ~below(lo_row == INT_MIN ? 0 : lo_row - j0);
+                    if (sinks) seen |= below(min(sinks, hi_row) - j0);
+                    seen &= ~below(it.kv_lo - j0);
+                    const uint32_t w[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
-                    for (int i = 0; i < kN; ++i) {
-                        const int p = j0 + i;
-                        if (!(p >= it.kv_lo && p < hi_row && (p >= lo_row || p < sinks)))
-                            s[i] = -INFINITY;
-                    }
+                    for (int i = 0; i < kN; ++i)
+                        if (!((w[i / 32] >> (i % 32)) & 1u)) s[i] = -INFINITY;
                     // V of a partly hidden tile: no infinity or NaN may meet a zero weight
                     const uint32_t rv = ring + 1;
                     if (!bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort)) {
@@ -520,20 +618,27 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                         break;
                     }
                     char* vt = sKV + (rv % kSlots) * C::kSlot;
-                    bool changed = false;
-                    for (int c = r; c < kN * HD / 8; c += kM) {
-                        uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
-                        const uint4 w = *at;
-                        if (PMath<T>::not_finite(w.x) || PMath<T>::not_finite(w.y) ||
-                            PMath<T>::not_finite(w.z) || PMath<T>::not_finite(w.w)) {
+                    uint32_t found = 0;
+#pragma unroll
+                    for (int c = 0; c < kN * HD / 8 / kM; ++c) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(vt + (c * kM + r) * 16);
+                        found |= odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
+                                 odd_halves<T>(v.w);
+                    }
+                    if (found) {
+                        for (int c = r; c < kN * HD / 8; c += kM) {
+                            uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
+                            const uint4 v = *at;
+                            if (!(odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
+                                  odd_halves<T>(v.w)))
+                                continue;
                             const int p = j0 + ((c / 8) & (kN - 1));
                             if (p >= it.kv_lo && p < any_hi && (p >= any_lo || p < sinks))
                                 P.redo[(size_t)(W.item - 1) * P.heads + head_lane] = 1;
                             *at = make_uint4(0, 0, 0, 0);
-                            changed = true;
                         }
+                        async_fence();
                     }
-                    if (changed) async_fence();
                 }
                 float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
 #pragma unroll
@@ -676,11 +781,16 @@ cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     KvMaps maps;
-    const int rows = kv_maps(&maps, A, std::is_same<T, __nv_bfloat16>::value, kN);
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    const int rows = kv_maps(&maps, A, bf16, kN);
     if (rows == 0) return cudaErrorInvalidValue;
     const PagedPlan& P = A.plan[which];
-    return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), (size_t)smem, s, A, maps, which,
-                      rows);
+    // Q by TMA where a row tile is whole tokens of whole blocks of heads
+    const bool q_boxes = PARTS == 1 && kM % P.gpb == 0 && A.group % P.gpb == 0 && A.scale_log2 >= 0.f;
+    CUtensorMap q_map = maps.k;
+    if (q_boxes && !encode_rows(&q_map, A, bf16, P.gpb, kM / P.gpb)) return cudaErrorInvalidValue;
+    return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), (size_t)smem, s, A, maps, q_map,
+                      which, rows, (int)q_boxes);
 }
 
 template <typename T, int PARTS>

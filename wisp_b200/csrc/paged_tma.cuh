@@ -79,6 +79,15 @@ __device__ __forceinline__ void tma4d(uint32_t dst, const CUtensorMap* map, int 
         : "memory");
 }
 
+__device__ __forceinline__ void tma3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                      uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
+        : "memory");
+}
+
 struct KvMaps {
     CUtensorMap k, v;  // (dim, kv head, position in page, page), boxes of 64 dims
 };
@@ -112,6 +121,19 @@ bool encode(CUtensorMap* map, const void* addr, const PagedArgs& A, bool bf16, i
     const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1}, one[4] = {1, 1, 1, 1};
     return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
               const_cast<void*>(addr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 16-bit rows of q, (dim, head, token), boxes of 64 dims, `heads` heads and `tokens` tokens.
+bool encode_rows(CUtensorMap* map, const PagedArgs& A, bool bf16, int heads, int tokens) {
+    EncodeFn fn = encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)A.hd, (cuuint64_t)A.nh, (cuuint64_t)A.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)A.hd * 2, (cuuint64_t)A.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens}, one[3] = {1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+              const_cast<void*>(A.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
