@@ -57,7 +57,8 @@ struct MCfg {
     // dims it does not: a ring of three tiles cost more than Q's early loads gave)
     static constexpr int kQBufs = HD == 64 ? 2 : 1;
     static constexpr int kSlots = HD == 64 ? (PARTS == 3 ? 8 : 12) : PARTS == 3 ? 7 : 9;
-    static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot;
+    static constexpr int kStage = 4 * kRT * 2048;  // 64 bytes of each row on their way out
+    static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot + kStage;
     // TMEM columns
     static constexpr int kPCols = 32 * PARTS;
     static __host__ __device__ constexpr int s_col(int x, int b) { return (x * 2 + b) * 64; }
@@ -185,6 +186,30 @@ template <typename T>
 struct MShift {
     static constexpr float value = std::is_same<T, __half>::value ? 6.f : 0.f;
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 // The low n bits (none for n <= 0, all for n >= 64).
 __device__ __forceinline__ uint64_t below(int n) {
@@ -640,15 +665,16 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                         async_fence();
                     }
                 }
-                float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+                float mx4[4];
 #pragma unroll
-                for (int i = 4; i < kN; i += 4) {
-                    mx0 = fmaxf(mx0, s[i]);
-                    mx1 = fmaxf(mx1, s[i + 1]);
-                    mx2 = fmaxf(mx2, s[i + 2]);
-                    mx3 = fmaxf(mx3, s[i + 3]);
-                }
-                const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * fac;
+                for (int i = 0; i < 4; ++i) mx4[i] = max3(s[i], s[i + 4], s[i + 8]);
+#pragma unroll
+                for (int i = 12; i < kN - 4; i += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) mx4[u] = max3(mx4[u], s[i + u], s[i + 4 + u]);
+                const float mx =
+                    max3(max3(mx4[0], s[kN - 4], s[kN - 3]), max3(mx4[1], s[kN - 2], s[kN - 1]),
+                         fmaxf(mx4[2], mx4[3])) * fac;
                 if (__any_sync(kAll, mx > m + 8.f)) {
                     const float to = fmaxf(m, mx);
                     const float al = ex2(m - (to == -INFINITY ? 0.f : to));
@@ -671,19 +697,21 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                     }
                 }
                 const float mb = (m == -INFINITY ? 0.f : m) - kShift;
-                float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+                // (pairs of fp32 in one instruction: these warps are short of issue slots)
+                const uint64_t fac2 = pair(fac, fac), mb2 = pair(-mb, -mb);
+                uint64_t l2[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < kN; i += 4) {
-                    s[i] = ex2(fmaf(s[i], fac, -mb));
-                    s[i + 1] = ex2(fmaf(s[i + 1], fac, -mb));
-                    s[i + 2] = ex2(fmaf(s[i + 2], fac, -mb));
-                    s[i + 3] = ex2(fmaf(s[i + 3], fac, -mb));
-                    l0 += s[i];
-                    l1 += s[i + 1];
-                    l2 += s[i + 2];
-                    l3 += s[i + 3];
+                for (int i = 0; i < kN; i += 2) {
+                    unpair(fma2(pair(s[i], s[i + 1]), fac2, mb2), s[i], s[i + 1]);
+                    s[i] = ex2(s[i]);
+                    s[i + 1] = ex2(s[i + 1]);
+                    l2[(i / 2) & 1] = add2(l2[(i / 2) & 1], pair(s[i], s[i + 1]));
                 }
-                l += (l0 + l1) + (l2 + l3);
+                {
+                    float a, b;
+                    unpair(add2(l2[0], l2[1]), a, b);
+                    l += a + b;
+                }
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
                     uint32_t w[32];
@@ -714,49 +742,64 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             const bool last_word = complete && A.n_groups == 0;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float M = m - kShift;
-            float* o32 = nullptr;
-            T* o16 = nullptr;
+            char* dst;  // this row's place
             if (last_word) {
                 const size_t at = (size_t)tok * A.out_stride + (size_t)h * A.hd;
-                if (SPLIT) o32 = reinterpret_cast<float*>(A.out) + at;
-                else o16 = reinterpret_cast<T*>(A.out) + at;
+                dst = reinterpret_cast<char*>(A.out) + at * (SPLIT ? 4 : 2);
                 if (real && A.lse) A.lse[(size_t)tok * A.nh + h] = row_lse(M, l);
             } else {
-                const size_t id = complete ? (size_t)(which == 1) * A.n_tokens * A.nh +
+                const size_t id = complete ? (size_t)(which == PLAN_PREFIX) * A.n_tokens * A.nh +
                                                  (size_t)tok * A.nh + h
                                            : part_row(P, piece, head_lane, W.a > 0 ? 0 : 1, row);
-                o32 = (complete ? A.full_o : P.part_o) + id * A.hd;
+                dst = reinterpret_cast<char*>((complete ? A.full_o : P.part_o) + id * A.hd);
                 if (real)
                     *reinterpret_cast<float2*>((complete ? A.full_ml : P.part_ml) + id * 2) =
                         make_float2(M, l);
             }
-            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && h == h0)
-                P.where[tok] = PagedWhere{piece, 0, row, it.alone, which, W.item - 1};
-            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && h == h0)
-                P.where[tok].last = Pieces(P, P.cum[*P.n_items]).of(W.c0 + it.n_tiles - 1);
+            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && h == h0) {
+                const int last = Pieces(P, P.cum[*P.n_items]).of(W.c0 + it.n_tiles - 1);
+                P.where[tok] = PagedWhere{piece, last, row, it.alone, which, W.item - 1};
+            }
+            // 64 bytes of each row at a time through shared memory, so that four lanes write a row's
+            // whole sectors (a lane per row wrote halves of 32 sectors at once: 4 us a row tile).
+            // The 16-byte pieces are XORed with the row to keep both sides free of bank conflicts.
+            char* stage = sKV + kSlots * C::kSlot + warp * 2048;
+            const bool halves = !SPLIT && last_word;
+            auto send = [&](int col, const uint32_t* w) {  // 16 words of this row from dim `col` on
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
+                        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rr = k * 8 + lane / 4, c = lane & 3;
+                    char* to = reinterpret_cast<char*>(
+                        __shfl_sync(kAll, reinterpret_cast<unsigned long long>(dst), rr));
+                    const int d = col + c * (halves ? 8 : 4);
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 +
+                                                                    ((c ^ ((rr >> 1) & 3)) * 16));
+                    if (x * kM + (warp & 3) * 32 + rr < n_rows && d < A.hd)
+                        *reinterpret_cast<uint4*>(to + d * (halves ? 2 : 4)) = v;
+                }
+                __syncwarp();
+            };
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 float o[32];
                 tmem_ld32(lanes + C::o_col(x) + c, o);
-                if (!real) continue;
                 if (last_word) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
                 }
+                if (halves) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (c + i >= A.hd) break;
-                    if (o16) {
-                        *reinterpret_cast<uint4*>(o16 + c + i) =
-                            make_uint4(PMath<T>::pack(o[i], o[i + 1]), PMath<T>::pack(o[i + 2], o[i + 3]),
-                                       PMath<T>::pack(o[i + 4], o[i + 5]),
-                                       PMath<T>::pack(o[i + 6], o[i + 7]));
-                    } else {
-                        *reinterpret_cast<float4*>(o32 + c + i) =
-                            make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        *reinterpret_cast<float4*>(o32 + c + i + 4) =
-                            make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
-                    }
+                    for (int i = 0; i < 16; ++i) w[i] = PMath<T>::pack(o[2 * i], o[2 * i + 1]);
+                    send(c, w);
+                } else {
+                    send(c, reinterpret_cast<const uint32_t*>(o));
+                    send(c + 16, reinterpret_cast<const uint32_t*>(o + 16));
                 }
             }
             tc_before();
