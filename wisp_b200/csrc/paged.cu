@@ -366,7 +366,7 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
 // Attention: what runs, and its workspace
 // ------------------------------------------------------------------------
 // What a row tile costs before its first KV tile, in KV tiles.
-constexpr int kLeadMma = 4, kLeadFew = 1;
+constexpr int kLeadMma = 4, kLeadFew = 2;
 
 struct AttnShape {
     int rw[PLANS];  // 16-row tiles of the plan's row tiles; 0: the tensor-core kernel
@@ -378,7 +378,9 @@ struct AttnShape {
 // Which kernel: a sequence (or group) whose rows for one kv head fit one 16-row tile of
 // mma.sync (8 rows in fp32) goes through paged_few_kernel, whose CTAs are bound by HBM; more
 // rows go to tcgen05 where it takes the head dim, else to paged_attn_kernel's row tiles of two
-// or four 16-row tiles.
+// or four 16-row tiles.  A batch goes by its longest sequence: single tokens beside a prompt
+// take its kernel too (they read the cache at 80% of HBM there instead of 95%; a second pair of
+// launches for them cost 12 us a call).
 AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     const int per = split ? 8 : 16;
@@ -393,27 +395,19 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     A.group = A.nh / A.nkv;
     const bool mma = paged_mma_takes(A.hd);
     const int few = per / A.group;  // tokens whose rows fit one 16-row tile
-    const bool even = A.n_seq == 1 || (long long)A.n_seq * max_q == A.n_tokens;
-    PagedWhere* where = nullptr;
     for (int w = 0; w < PLANS; ++w) {
         PagedPlan& P = A.plan[w];
         P = PagedPlan{};
         const int n_seg = w == PLAN_PREFIX ? A.n_groups : A.n_seq;
         long long tokens = max_q;  // of the plan's largest segment (a guess for a prefix)
         bool on_mma = false;
-        P.max_tok = 0x7fffffff;
         if (w == PLAN_PREFIX) {
             if (A.n_groups == 0) continue;
             tokens = (A.n_tokens + n_seg - 1) / n_seg;
             on_mma = mma && tokens > few;
-        } else if (w == PLAN_MANY) {
-            if (!mma || max_q <= few) continue;
-            P.min_tok = A.plan[PLAN_FEW].used ? few + 1 : 0;
-            on_mma = true;
-        } else if (mma) {
-            if (few == 0 || (even && max_q > few)) continue;
-            if (max_q > few) P.max_tok = few;
-            tokens = std::min<long long>(tokens, few);
+        } else {
+            on_mma = mma && max_q > few;
+            if (on_mma != (w == PLAN_MANY)) continue;
         }
         P.used = 1;
         const int most = on_mma ? paged_mma_rows(split) : 4 * per;
@@ -433,7 +427,7 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.lanes = std::min(4095, std::max(1, ctas / P.heads));
         P.max_items = A.n_tokens / P.tpt + n_seg;
         P.inlined = is_few && n_seg <= kPagedInline &&
-                    (w == PLAN_PREFIX ? A.n_tokens : std::min(max_q, P.max_tok)) <= P.tpt;
+                    (w == PLAN_PREFIX ? A.n_tokens : max_q) <= P.tpt;
         P.n_items = reinterpret_cast<int*>(take(4));
         P.bad = reinterpret_cast<int*>(take(((size_t)P.lanes * P.heads + 1) * 4));
         P.item_off = reinterpret_cast<int*>(take((size_t)(n_seg + 1) * 4));
@@ -444,11 +438,8 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.part_ml = reinterpret_cast<float*>(take(recs * 8));
         P.split = reinterpret_cast<PagedSplit*>(take((size_t)P.lanes * sizeof(PagedSplit)));
         if (on_mma) P.redo = reinterpret_cast<int*>(take((size_t)P.max_items * P.heads * 4));
-        if (A.n_groups > 0) {
-            const size_t bytes = (size_t)A.n_tokens * sizeof(PagedWhere);
-            if (w == PLAN_PREFIX) P.where = reinterpret_cast<PagedWhere*>(take(bytes));
-            else P.where = where = where ? where : reinterpret_cast<PagedWhere*>(take(bytes));
-        }
+        if (A.n_groups > 0)
+            P.where = reinterpret_cast<PagedWhere*>(take((size_t)A.n_tokens * sizeof(PagedWhere)));
     }
     if (A.n_groups > 0) {
         const size_t recs = (size_t)2 * A.n_tokens * A.nh;

@@ -65,7 +65,6 @@ struct PagedPlan {
     int gpb, hblocks;   // query heads of a block, blocks of a kv head
     int lanes, heads;   // heads = kv heads * hblocks
     int max_items;
-    int min_tok, max_tok;  // sequences with fewer or more tokens are another plan's
     int inlined;           // item i is segment i: the attention CTAs find cum themselves
     int used;              // the call has this plan
 };
@@ -93,8 +92,7 @@ struct PagedArgs {
     int n_seq, n_tokens, n_groups, table_stride, table_width, n_pages, page_size, page_shift;
     int nh, nkv, group, hd, window, sinks;
     float scale_log2;
-    // [PLAN_FEW] sequences of few rows (their own part), [PLAN_PREFIX] the shared prefixes,
-    // [PLAN_MANY] sequences of many rows
+    // the sequences' own part, of few or of many rows (one of the two), and the shared prefixes
     PagedPlan plan[PLANS];
 };
 

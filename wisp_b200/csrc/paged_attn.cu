@@ -443,13 +443,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
 // ------------------------------------------------------------------------
 template <typename T, bool SPLIT, int WARPS>
 __global__ void __launch_bounds__(kJoinThreads)
-paged_join_kernel(const __grid_constant__ PagedArgs A, int which, int last_plan) {
+paged_join_kernel(const __grid_constant__ PagedArgs A, int which) {
     __shared__ JoinShared S;
     constexpr int kRows = 8 / WARPS;
     const PagedPlan& P = A.plan[which];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (last_plan && blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
+    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
     const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
     const PagedSplit sp = P.split[piece];
     const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
@@ -498,8 +498,7 @@ paged_join2_kernel(const __grid_constant__ PagedArgs A) {
     J.init();
     bool redo = false;
     if (h < A.nh) {
-        // both sequence plans write the same array
-        const PagedWhere own = (A.plan[PLAN_FEW].used ? A.plan[PLAN_FEW] : A.plan[PLAN_MANY]).where[t];
+        const PagedWhere own = A.plan[A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY].where[t];
         const int kvh = h / A.group, hg = h - kvh * A.group;
         for (int part = 0; part < (own.alone ? 1 : 2); ++part) {
             const PagedWhere w = part ? A.plan[PLAN_PREFIX].where[t] : own;
@@ -552,22 +551,15 @@ cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
     if (A.n_groups > 0)
         return launch_pdl(paged_join2_kernel<T, SPLIT>, dim3(A.n_tokens, (A.nh + 1) / 2),
                           dim3(kJoinThreads), 0, s, A);
-    for (int w = PLAN_FEW; w <= PLAN_MANY; w += PLAN_MANY - PLAN_FEW) {
-        const PagedPlan& P = A.plan[w];
-        if (!P.used) continue;
-        const int last = w == PLAN_MANY || !A.plan[PLAN_MANY].used;
-        // few rows: four warps each; many: as many rows as warps, most items are in few pieces
-        cudaError_t e =
-            P.used_rows <= 32
-                ? launch_pdl(paged_join_kernel<T, SPLIT, 4>,
-                             dim3(P.heads * P.lanes, (P.used_rows + 1) / 2), dim3(kJoinThreads), 0,
-                             s, A, w, last)
-                : launch_pdl(paged_join_kernel<T, SPLIT, 1>,
-                             dim3(P.heads * P.lanes, (P.used_rows + 7) / 8), dim3(kJoinThreads), 0,
-                             s, A, w, last);
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+    const int w = A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY;
+    const PagedPlan& P = A.plan[w];
+    // few rows: four warps each; many: as many rows as warps, most items are in few pieces
+    if (P.used_rows <= 32)
+        return launch_pdl(paged_join_kernel<T, SPLIT, 4>,
+                          dim3(P.heads * P.lanes, (P.used_rows + 1) / 2), dim3(kJoinThreads), 0, s, A,
+                          w);
+    return launch_pdl(paged_join_kernel<T, SPLIT, 1>,
+                      dim3(P.heads * P.lanes, (P.used_rows + 7) / 8), dim3(kJoinThreads), 0, s, A, w);
 }
 
 }  // namespace

@@ -123,7 +123,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 n = item_units(P, make_item(A, P, prefix, i, 0).n_tiles);
                 if (blockIdx.x == 0 && !prefix) {
                     const int t = A.q_start[i + 1] - A.q_start[i];
-                    if (length_too_long(A, i) || (t > P.tpt && t <= P.max_tok))
+                    if (length_too_long(A, i) || t > P.tpt)
                         P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
                 }
             }

@@ -253,8 +253,7 @@ __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bo
         it.first = f;
         it.n_tiles = it.n_sink + last - f;
     }
-    if (it.ntok <= 0 || (!prefix && (g.t1 - g.t0 < P.min_tok || g.t1 - g.t0 > P.max_tok)))
-        it.n_tiles = 0;
+    if (it.ntok <= 0) it.n_tiles = 0;
     return it;
 }
 

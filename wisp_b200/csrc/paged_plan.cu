@@ -1,7 +1,7 @@
 // paged_plan.cu -- the row tiles of a paged attention call, found on the device: sequence
 // lengths stay there, so a step needs no host synchronisation and can be captured once.
 //
-// One CTA per plan (sequences of few rows, shared prefixes, sequences of many rows).  It counts the row tiles
+// One CTA per plan (the sequences' own parts; the shared prefixes).  It counts the row tiles
 // of every sequence, then for each row tile the KV tiles that its mask leaves (the window's
 // and the sinks'), and keeps running sums of both; the attention kernels cut the line of all
 // KV tiles into equal pieces.  A sequence without cached positions keeps one (fully hidden)
@@ -58,9 +58,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         int n = 0;
         if (i < n_seg) {
             const PagedSeg g = paged_segment(A, prefix, i);
-            n = g.t1 - g.t0 >= P.min_tok && g.t1 - g.t0 <= P.max_tok
-                    ? (g.t1 - g.t0 + P.tpt - 1) / P.tpt
-                    : 0;
+            n = (g.t1 - g.t0 + P.tpt - 1) / P.tpt;
             bad |= !prefix && length_too_long(A, i);
         }
         const int at = carry + block_scan(n, &total, sums);
