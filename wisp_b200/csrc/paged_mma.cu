@@ -6,7 +6,10 @@
 //   S = Q K^T   tcgen05.mma M=128 N=64, Q and K from shared memory, S in tensor memory
 //   P = 2^(S fac - m)  one thread per row; P back to tensor memory as 16-bit pairs
 //   O += P V    tcgen05.mma M=128 N=head_dim, P from tensor memory, V from shared memory
-// Two tiles of 128 rows share each K / V tile.  S is double buffered, so the tensor core works
+// Two tiles of 128 rows share each K / V tile; an item with at most 128 rows (drafted tokens, a
+// group behind a prefix) takes both for itself, one for its even and one for its odd KV tiles,
+// and joins them at the end (each thread reads both O's: one tile's softmax alone kept such
+// items at 75% of HBM).  S is double buffered, so the tensor core works
 // on tile j + 1 while the softmax warps work on tile j.  Roles:
 //   warps 0-3 (and 4-7)  softmax of row tile 0 (and 1): rows 32 * (warp & 3) + lane
 //   warps 8 and 9        issue the MMAs of one row tile each (an elected thread)
@@ -57,7 +60,7 @@ struct MCfg {
     // dims it does not: a ring of three tiles cost more than Q's early loads gave)
     static constexpr int kQBufs = HD == 64 ? 2 : 1;
     static constexpr int kSlots = HD == 64 ? (PARTS == 3 ? 8 : 12) : PARTS == 3 ? 7 : 9;
-    static constexpr int kStage = 4 * kRT * 2048;  // 64 bytes of each row on their way out
+    static constexpr int kStage = 4 * kRT * 1024;  // 32 bytes of each row on their way out
     static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot + kStage;
     // TMEM columns
     static constexpr int kPCols = 32 * PARTS;
@@ -343,6 +346,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     __shared__ uint64_t full[kSlots], empty[kSlots];
     __shared__ uint64_t q_full[kRT][kQB], q_empty[kRT][kQB], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain[kRT];
     __shared__ uint32_t s_tmem;
+    __shared__ uint64_t x_done[2], x_read[2];  // both halves of an item: sums there, O read
+    __shared__ float2 s_ml[2][kM];
     __shared__ float s_fac[kRT][kQB][kM];  // fp32 rows: score factors
     __shared__ volatile int s_abort;
     __shared__ int s_bad;
@@ -370,6 +375,10 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             }
         }
         for (int x = 0; x < kRT; ++x) bar_init(&drain[x], 1);
+        for (int x = 0; x < 2; ++x) {
+            bar_init(&x_done[x], 4);
+            bar_init(&x_read[x], 4);
+        }
         s_abort = 0;
         s_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -426,6 +435,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     auto pv_done = [&](int x, uint32_t c) {
         return bar_wait(&o_done[x][c & 1], (c >> 1) & 1, &s_abort);
     };
+    // Whether both row tiles' roles work on one item of at most kM rows (even and odd KV tiles).
+    auto halved = [&]() { return kRT == 2 && W.it.ntok * gpb <= kM && W.b - W.a >= 2; };
     uint32_t ring = 0;  // K / V tiles so far: slot ring % kSlots, phase (ring / kSlots) & 1
     if (warp == kLoadWarp) {
         // ------------------------------------------------------------- K / V tiles
@@ -490,34 +501,42 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                            (p | k) ? 1u : 0u, leader);
             commit(&s_full[x][c & 1]);
         };
-        while (ok && W.next(P)) {
+        auto release = [&](uint32_t first, uint32_t slots) {  // what the other row tile reads
+            for (uint32_t i = first; i < first + slots; ++i) {
+                if (!arrive_full(i)) return false;
+                if (lane == 0) bar_arrive(&empty[i % kSlots]);
+            }
+            return true;
+        };
+        for (; ok && W.next(P); ring += 2 * (W.b - W.a)) {
             const int n = W.b - W.a;
-            if (x * kM >= W.it.ntok * gpb) {  // no rows here: only give the slots back
-                for (int i = 0; ok && i < 2 * n; ++i, ++ring) {
-                    ok = arrive_full(ring);
-                    if (ok && lane == 0) bar_arrive(&empty[ring % kSlots]);
-                }
+            const bool half = halved();
+            if (!half && x * kM >= W.it.ntok * gpb) {  // no rows here
+                ok = release(ring, 2 * n);
                 continue;
             }
-            const uint32_t qb = seg % kQB;
+            const int step = half ? 2 : 1, first = half ? x : 0, own = half ? (n - x + 1) / 2 : n;
+            const uint32_t qb = seg % kQB, r0 = ring + 2 * first;
             // S of tile c takes the buffer of tile c - 2's P
-            ok = bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_abort) && arrive_full(ring) &&
+            ok = (first == 0 || release(ring, 2)) &&
+                 bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_abort) && arrive_full(r0) &&
                  (cnt < 2 || __all_sync(kAll, pv_done(x, cnt - 2)));
             if (!ok) break;
             ++seg;
             tc_after();
-            issue_s(ring % kSlots, cnt, qb);
-            commit(&empty[ring % kSlots]);
-            if (n == 1) commit(&q_empty[x][qb]);
-            for (int j = 0; j < n; ++j, ++cnt, ring += 2) {
-                const uint32_t rv = ring + 1, rk = ring + 2;
-                if (j + 1 < n) {
-                    ok = (cnt == 0 || __all_sync(kAll, pv_done(x, cnt - 1))) && arrive_full(rk);
+            issue_s(r0 % kSlots, cnt, qb);
+            commit(&empty[r0 % kSlots]);
+            if (own == 1) commit(&q_empty[x][qb]);
+            for (int j = 0; j < own; ++j, ++cnt) {
+                const uint32_t rv = r0 + 2 * j * step + 1, rk = rv + 2 * step - 1;
+                if (j + 1 < own) {
+                    ok = (cnt == 0 || __all_sync(kAll, pv_done(x, cnt - 1))) &&
+                         (!half || release(rv + 1, 2)) && arrive_full(rk);
                     if (!ok) break;
                     tc_after();
                     issue_s(rk % kSlots, cnt + 1, qb);
                     commit(&empty[rk % kSlots]);
-                    if (j + 2 == n) commit(&q_empty[x][qb]);
+                    if (j + 2 == own) commit(&q_empty[x][qb]);
                 }
                 ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) && arrive_full(rv);
                 if (!ok) break;
@@ -534,6 +553,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 commit(&o_done[x][cnt & 1]);
                 commit(&empty[rv % kSlots]);
             }
+            if (ok && half && (first + own * 2 - 1) < n) ok = release(ring + 2 * (first + own * 2 - 1), 2);
         }
         commit(&drain[x]);
         if (lane == 0) bar_drain(&drain[x], 0);
@@ -547,7 +567,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             const int n_rows = W.it.ntok * gpb;
 #pragma unroll
             for (int x = 0; x < kRT; ++x) {
-                if (!ok || x * kM >= n_rows) continue;
+                const int row0 = halved() ? 0 : x * kM;
+                if (!ok || row0 >= n_rows) continue;
                 const uint32_t qb = seg[x] % kQB;
                 ok = bar_wait_warp(&q_empty[x][qb], ((seg[x] / kQB) & 1) ^ 1, &s_abort);
                 if (!ok) continue;
@@ -558,12 +579,12 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 #pragma unroll
                         for (int h = 0; h < kH; ++h)
                             tma3d(smem_addr(sQ + (qb * kRT + x) * C::kQ + h * (kM * 128)), &q_map,
-                                  h * 64, h0, W.it.tok0 + x * (kM / gpb), &q_full[x][qb]);
+                                  h * 64, h0, W.it.tok0 + row0 / gpb, &q_full[x][qb]);
                     }
                     continue;
                 }
-                const int n = min(kM, n_rows - x * kM);
-                load_q_tile<T, PARTS, HD>(A, W.it.tok0, x * kM, n, h0, gpb, flip,
+                const int n = min(kM, n_rows - row0);
+                load_q_tile<T, PARTS, HD>(A, W.it.tok0, row0, n, h0, gpb, flip,
                                           sQ + (qb * kRT + x) * PARTS * C::kQ, s_fac[x][qb]);
                 async_fence();
                 __syncwarp();
@@ -581,16 +602,15 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         constexpr float kShift = MShift<T>::value;
-        uint32_t cnt = 0, seg = 0;
+        uint32_t cnt = 0, seg = 0, pairs = 0;
         bool ok = true;
-        while (ok && W.next(P)) {
+        for (; ok && W.next(P); ring += 2 * (W.b - W.a)) {
             const PagedItem& it = W.it;
             const int n_rows = it.ntok * gpb, n = W.b - W.a;
-            if (x * kM >= n_rows) {
-                ring += 2 * n;
-                continue;
-            }
-            const int row = x * kM + r;
+            const bool half = halved();
+            if (!half && x * kM >= n_rows) continue;
+            const int step = half ? 2 : 1, first = half ? x : 0, own = half ? (n - x + 1) / 2 : n;
+            const int row0 = half ? 0 : x * kM, row = row0 + r;
             const bool real = row < n_rows;
             const int tok = it.tok0 + row / gpb, h = h0 + row % gpb;
             int pos = INT_MIN;
@@ -616,8 +636,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             const int all_hi = min(it.kv_hi, it.pmin + 1);
             const int all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < n; ++j, ++cnt, ring += 2) {
-                const int b = cnt & 1, j0 = W.tile(W.a + j) * kN;
+            for (int j = 0; j < own; ++j, ++cnt) {
+                const int b = cnt & 1, j0 = W.tile(W.a + first + j * step) * kN;
                 const bool whole = j0 >= it.kv_lo && j0 + kN <= all_hi &&
                                    (j0 >= all_lo || j0 + kN <= sinks);
                 if (!bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort)) {
@@ -637,7 +657,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                     for (int i = 0; i < kN; ++i)
                         if (!((w[i / 32] >> (i % 32)) & 1u)) s[i] = -INFINITY;
                     // V of a partly hidden tile: no infinity or NaN may meet a zero weight
-                    const uint32_t rv = ring + 1;
+                    const uint32_t rv = ring + 2 * (first + j * step) + 1;
                     if (!bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort)) {
                         ok = false;
                         break;
@@ -740,54 +760,79 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             tc_after();
             const bool complete = W.a == 0 && W.b == it.n_tiles;
             const bool last_word = complete && A.n_groups == 0;
+            float mine = 1.f, other = 0.f;  // factors of this row tile's O and of the other one's
+            if (half) {
+                s_ml[x][r] = make_float2(m, l);
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&x_done[x]);
+                if (!bar_wait_warp(&x_done[1 - x], pairs & 1, &s_abort)) {
+                    ok = false;
+                    break;
+                }
+                tc_after();
+                const float2 o = s_ml[1 - x][r];
+                const float to = fmaxf(m, o.x), base = to == -INFINITY ? 0.f : to;
+                mine = ex2(m - base);
+                other = ex2(o.x - base);
+                m = to;
+                l = l * mine + o.y * other;
+            }
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float M = m - kShift;
+            const bool tells = !half || x == 0;  // one of two halves writes what is per row
             char* dst;  // this row's place
             if (last_word) {
                 const size_t at = (size_t)tok * A.out_stride + (size_t)h * A.hd;
                 dst = reinterpret_cast<char*>(A.out) + at * (SPLIT ? 4 : 2);
-                if (real && A.lse) A.lse[(size_t)tok * A.nh + h] = row_lse(M, l);
+                if (real && tells && A.lse) A.lse[(size_t)tok * A.nh + h] = row_lse(M, l);
             } else {
                 const size_t id = complete ? (size_t)(which == PLAN_PREFIX) * A.n_tokens * A.nh +
                                                  (size_t)tok * A.nh + h
                                            : part_row(P, piece, head_lane, W.a > 0 ? 0 : 1, row);
                 dst = reinterpret_cast<char*>((complete ? A.full_o : P.part_o) + id * A.hd);
-                if (real)
+                if (real && tells)
                     *reinterpret_cast<float2*>((complete ? A.full_ml : P.part_ml) + id * 2) =
                         make_float2(M, l);
             }
-            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && h == h0) {
+            if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && tells && h == h0) {
                 const int last = Pieces(P, P.cum[*P.n_items]).of(W.c0 + it.n_tiles - 1);
                 P.where[tok] = PagedWhere{piece, last, row, it.alone, which, W.item - 1};
             }
-            // 64 bytes of each row at a time through shared memory, so that four lanes write a row's
-            // whole sectors (a lane per row wrote halves of 32 sectors at once: 4 us a row tile).
-            // The 16-byte pieces are XORed with the row to keep both sides free of bank conflicts.
-            char* stage = sKV + kSlots * C::kSlot + warp * 2048;
+            // 32 bytes of each row at a time through shared memory, so that two lanes write a row's
+            // whole sectors.  The 16-byte pieces are XORed with the row to keep both sides free of
+            // bank conflicts.
+            char* stage = sKV + kSlots * C::kSlot + warp * 1024;
             const bool halves = !SPLIT && last_word;
-            auto send = [&](int col, const uint32_t* w) {  // 16 words of this row from dim `col` on
+            auto send = [&](int col, const uint32_t* w) {  // 8 words of this row from dim `col` on
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
+                for (int c = 0; c < 2; ++c)
+                    *reinterpret_cast<uint4*>(stage + lane * 32 + ((c ^ ((lane >> 2) & 1)) * 16)) =
                         make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
                 __syncwarp();
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int rr = k * 8 + lane / 4, c = lane & 3;
+                for (int k = 0; k < 2; ++k) {
+                    const int rr = k * 16 + lane / 2, c = lane & 1;
                     char* to = reinterpret_cast<char*>(
                         __shfl_sync(kAll, reinterpret_cast<unsigned long long>(dst), rr));
                     const int d = col + c * (halves ? 8 : 4);
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 +
-                                                                    ((c ^ ((rr >> 1) & 3)) * 16));
-                    if (x * kM + (warp & 3) * 32 + rr < n_rows && d < A.hd)
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 32 +
+                                                                    ((c ^ ((rr >> 2) & 1)) * 16));
+                    if (row0 + (warp & 3) * 32 + rr < n_rows && d < A.hd)
                         *reinterpret_cast<uint4*>(to + d * (halves ? 2 : 4)) = v;
                 }
                 __syncwarp();
             };
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
+            for (int c = half ? x * (HD / 2) : 0; c < (half ? (x + 1) * (HD / 2) : HD); c += 32) {
                 float o[32];
                 tmem_ld32(lanes + C::o_col(x) + c, o);
+                if (half) {
+                    float p[32];
+                    tmem_ld32(lanes + C::o_col(kRT - 1 - x) + c, p);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = fmaf(o[i], mine, p[i] * other);
+                }
                 if (last_word) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
@@ -797,12 +842,23 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = PMath<T>::pack(o[2 * i], o[2 * i + 1]);
                     send(c, w);
+                    send(c + 16, w + 8);
                 } else {
-                    send(c, reinterpret_cast<const uint32_t*>(o));
-                    send(c + 16, reinterpret_cast<const uint32_t*>(o + 16));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        send(c + 8 * k, reinterpret_cast<const uint32_t*>(o + 8 * k));
                 }
             }
             tc_before();
+            if (half) {  // neither O is written again before both have been read
+                __syncwarp();
+                if (lane == 0) bar_arrive(&x_read[x]);
+                if (!bar_wait_warp(&x_read[1 - x], pairs & 1, &s_abort)) {
+                    ok = false;
+                    break;
+                }
+                ++pairs;
+            }
         }
     }
 
