@@ -5,6 +5,9 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <stdint.h>
+
+#include <atomic>
 #include <utility>
 
 #include "wisp_b200.h"
@@ -75,6 +78,19 @@ template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block,
                        size_t smem, cudaStream_t stream, Args&&... args) {
     return launch_pdl_cluster(kern, grid, block, smem, stream, 1, std::forward<Args>(args)...);
+}
+
+// The opt-in for dynamic shared memory above 48 KB, asked for once per device: `done` is the
+// caller's own, one bit per device (devices from 64 on ask every time).
+inline cudaError_t smem_opt_in(const void* kern, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace wb

@@ -368,6 +368,9 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
 // What a row tile costs before its first KV tile, in KV tiles.
 constexpr int kLeadMma = 4, kLeadFew = 2;
 
+constexpr int kFewTiles = 4;
+constexpr double kFewBytes = 48e6;
+
 struct AttnShape {
     int rw[PLANS];  // 16-row tiles of the plan's row tiles; 0: the tensor-core kernel
     size_t bytes;
@@ -380,7 +383,9 @@ struct AttnShape {
 // rows go to tcgen05 where it takes the head dim, else to paged_attn_kernel's row tiles of two
 // or four 16-row tiles.  A batch goes by its longest sequence: single tokens beside a prompt
 // take its kernel too (they read the cache at 80% of HBM there instead of 95%; a second pair of
-// launches for them cost 12 us a call).
+// launches for them cost 12 us a call).  Up to kFewTiles 16-row tiles stay with paged_few_kernel
+// where all that the tables can name stays in L2: it needs no plan kernel before it, and reads
+// the cache again from there.
 AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     const int per = split ? 8 : 16;
@@ -394,28 +399,29 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     A.status = reinterpret_cast<int*>(ws);
     A.group = A.nh / A.nkv;
     const bool mma = paged_mma_takes(A.hd);
-    const int few = per / A.group;  // tokens whose rows fit one 16-row tile
+    const int few_tok = std::max(1, per / A.group);  // tokens of a 16-row tile
+    const double row_bytes = (double)A.table_width * A.page_size * A.nkv * A.hd * 4;
     for (int w = 0; w < PLANS; ++w) {
         PagedPlan& P = A.plan[w];
         P = PagedPlan{};
         const int n_seg = w == PLAN_PREFIX ? A.n_groups : A.n_seq;
-        long long tokens = max_q;  // of the plan's largest segment (a guess for a prefix)
-        bool on_mma = false;
-        if (w == PLAN_PREFIX) {
-            if (A.n_groups == 0) continue;
-            tokens = (A.n_tokens + n_seg - 1) / n_seg;
-            on_mma = mma && tokens > few;
-        } else {
-            on_mma = mma && max_q > few;
-            if (on_mma != (w == PLAN_MANY)) continue;
-        }
+        if (n_seg == 0) continue;
+        // tokens of the plan's largest segment (a guess for a prefix, which may have all)
+        const int tokens = w == PLAN_PREFIX ? (A.n_tokens + n_seg - 1) / n_seg : max_q;
+        const int most_tokens = w == PLAN_PREFIX ? A.n_tokens : max_q;
+        const long long tiles16 = (long long)((A.group + per - 1) / per) *
+                                  ((tokens + few_tok - 1) / few_tok);
+        // no more than this lies behind the segments' table rows: row tiles read it again out of L2
+        const bool in_l2 = n_seg * row_bytes <= kFewBytes;
+        const bool is_few = (long long)tokens * A.group <= per || (tiles16 <= kFewTiles && in_l2);
+        const bool on_mma = !is_few && mma;
+        if (w != PLAN_PREFIX && on_mma != (w == PLAN_MANY)) continue;
         P.used = 1;
-        const int most = on_mma ? paged_mma_rows(split) : 4 * per;
+        const int most = on_mma ? paged_mma_rows(split) : is_few ? per : 4 * per;
         P.gpb = std::min(A.group, most);
         P.hblocks = (A.group + P.gpb - 1) / P.gpb;
         P.heads = A.nkv * P.hblocks;
-        const int rows = (int)std::min<long long>(tokens * P.gpb, most);
-        const bool is_few = !on_mma && rows <= per;
+        const int rows = (int)std::min<long long>((long long)tokens * P.gpb, most);
         S.rw[w] = on_mma ? 0 : is_few ? 1 : paged_attn_rw(rows, split);
         P.tile = on_mma ? paged_mma_tile() : is_few ? paged_few_tile() : paged_attn_tile();
         P.rows = on_mma ? most : S.rw[w] * per;
@@ -425,9 +431,14 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
             (on_mma ? 1 : is_few ? paged_few_ctas(A.hd) : paged_attn_ctas(A.hd)) * sm_count();
         P.lead = on_mma ? kLeadMma : kLeadFew;
         P.lanes = std::min(4095, std::max(1, ctas / P.heads));
+        if (is_few && w == PLAN_PREFIX && A.plan[PLAN_FEW].used) {  // they share one launch
+            A.plan[PLAN_FEW].lanes = (A.plan[PLAN_FEW].lanes + 1) / 2;
+            P.lanes = (P.lanes + 1) / 2;
+        }
         P.max_items = A.n_tokens / P.tpt + n_seg;
-        P.inlined = is_few && n_seg <= kPagedInline &&
-                    (w == PLAN_PREFIX ? A.n_tokens : max_q) <= P.tpt;
+        P.per_seg = (most_tokens + P.tpt - 1) / P.tpt;
+        P.inlined = is_few && (long long)n_seg * P.per_seg <= kPagedInline;
+        if (P.inlined) P.max_items = n_seg * P.per_seg;
         P.n_items = reinterpret_cast<int*>(take(4));
         P.bad = reinterpret_cast<int*>(take(((size_t)P.lanes * P.heads + 1) * 4));
         P.item_off = reinterpret_cast<int*>(take((size_t)(n_seg + 1) * 4));

@@ -65,11 +65,13 @@ struct PagedPlan {
     int gpb, hblocks;   // query heads of a block, blocks of a kv head
     int lanes, heads;   // heads = kv heads * hblocks
     int max_items;
-    int inlined;           // item i is segment i: the attention CTAs find cum themselves
+    int per_seg;           // the most row tiles of a segment
+    int inlined;           // item i is tile i % per_seg of segment i / per_seg (some are empty), and
+                           // the attention CTAs find cum themselves
     int used;              // the call has this plan
 };
 
-// Segments that an attention CTA counts by itself.
+// Row tiles that an attention CTA counts by itself.
 constexpr int kPagedInline = 512;
 
 enum { PLAN_FEW = 0, PLAN_PREFIX = 1, PLAN_MANY = 2, PLANS = 3 };

@@ -499,9 +499,10 @@ paged_join2_kernel(const __grid_constant__ PagedArgs A) {
     bool redo = false;
     if (h < A.nh) {
         const PagedWhere own = A.plan[A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY].where[t];
+        const PagedWhere shared = A.plan[PLAN_PREFIX].where[t];
         const int kvh = h / A.group, hg = h - kvh * A.group;
         for (int part = 0; part < (own.alone ? 1 : 2); ++part) {
-            const PagedWhere w = part ? A.plan[PLAN_PREFIX].where[t] : own;
+            const PagedWhere w = part ? shared : own;
             if (w.plan < 0 || w.plan >= PLANS) continue;
             const PagedPlan& P = A.plan[w.plan];
             const int hb = hg / P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
@@ -526,8 +527,8 @@ template <typename T, bool SPLIT, int HD, int RW>
 cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     auto kern = paged_attn_kernel<T, SPLIT, HD, RW>;
     constexpr size_t smem = attn_smem_bytes<HD, RW, SPLIT ? PMath<T>::kFrags : 1>();
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = smem_opt_in(reinterpret_cast<const void*>(kern), smem, done);
     if (e != cudaSuccess) return e;
     const PagedPlan& P = A.plan[which];
     return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), smem, s, A, which);

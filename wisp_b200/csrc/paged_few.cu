@@ -108,22 +108,23 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         if (head_lane == 0) P.split[piece] = PagedSplit{0, 0, 0, 0, 0, 0};
         if (inlined && blockIdx.x == 0) P.bad[P.lanes * P.heads] = 0;
     }
-    const int n_items = inlined ? (prefix ? A.n_groups : A.n_seq) : *P.n_items;
+    const int n_items = inlined ? (prefix ? A.n_groups : A.n_seq) * P.per_seg : *P.n_items;
+    auto inline_item = [&](int i) { return make_item(A, P, prefix, i / P.per_seg, i % P.per_seg); };
     if (n_items == 0) return;
     const int* cum = inlined ? s_cum : P.cum;
     if (inlined) {
-        // one row tile per segment: every CTA counts the units itself, which is shorter than a
-        // kernel of its own before this one
+        // few row tiles: every CTA counts the units itself, which is shorter than a kernel of its
+        // own before this one
         __syncthreads();  // the words above are cleared
         int carry = 0;
         for (int base = 0; base < n_items; base += kThreads) {
             const int i = base + tid;
             int n = 0;
             if (i < n_items) {
-                n = item_units(P, make_item(A, P, prefix, i, 0).n_tiles);
-                if (blockIdx.x == 0 && !prefix) {
-                    const int t = A.q_start[i + 1] - A.q_start[i];
-                    if (length_too_long(A, i) || t > P.tpt)
+                n = item_units(P, inline_item(i).n_tiles);
+                if (blockIdx.x == 0 && !prefix && i % P.per_seg == 0) {
+                    const int s = i / P.per_seg, t = A.q_start[s + 1] - A.q_start[s];
+                    if (length_too_long(A, s) || t > P.tpt * P.per_seg)
                         P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
                 }
             }
@@ -200,7 +201,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 r.b = -1;
                 r.item = item0 + k + lane;
                 if (r.item < n_items && cum[r.item] < x_end) {
-                    r.it = inlined ? make_item(A, P, prefix, r.item, 0) : P.items[r.item];
+                    r.it = inlined ? inline_item(r.item) : P.items[r.item];
                     r.c0 = cum[r.item] + P.lead;
                     r.a = max(0, x0 - r.c0);
                     r.b = max(0, min(r.it.n_tiles, x_end - r.c0));
@@ -517,8 +518,8 @@ template <typename T, bool SPLIT, int HD>
 cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, cudaStream_t s) {
     auto kern = paged_few_kernel<T, SPLIT, HD>;
     constexpr size_t smem = FCfg<T, SPLIT, HD>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = smem_opt_in(reinterpret_cast<const void*>(kern), smem, done);
     if (e != cudaSuccess) return e;
     KvMaps maps;
     const int rows = kv_maps(&maps, A, std::is_same<T, __nv_bfloat16>::value,

@@ -191,7 +191,8 @@ __device__ __forceinline__ PagedSeg paged_segment(const PagedArgs& A, bool prefi
     return g;
 }
 
-// Row tile `nth` of segment `seg`.
+// Row tile `nth` of segment `seg`; WARP: by a whole warp, whose lanes share the sequences.
+template <bool WARP = false>
 __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bool prefix, int seg,
                                       int nth) {
     const PagedSeg g = paged_segment(A, prefix, seg);
@@ -212,13 +213,19 @@ __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bo
         it.pmax = -0x7fffffff;
         reach = 0;
 #pragma unroll 4
-        for (int s = g.s0; s < g.s1; ++s) {  // the tile's tokens of each sequence
+        for (int s = g.s0 + (WARP ? (int)(threadIdx.x & 31) : 0); s < g.s1; s += WARP ? 32 : 1) {
+            // the tile's tokens of each sequence
             const int end = A.q_start[s + 1], n = cached_positions(A, s);
             const int a = max(A.q_start[s], it.tok0), b = min(end, it.tok0 + it.ntok);
             if (a >= b) continue;
             it.pmin = min(it.pmin, n - (end - a));
             it.pmax = max(it.pmax, n - (end - b) - 1);
             reach = max(reach, n);
+        }
+        if (WARP) {
+            it.pmin = __reduce_min_sync(0xffffffffu, it.pmin);
+            it.pmax = __reduce_max_sync(0xffffffffu, it.pmax);
+            reach = __reduce_max_sync(0xffffffffu, reach);
         }
     }
     it.kv_lo = 0;

@@ -876,8 +876,8 @@ template <typename T, int PARTS, int HD>
 cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     auto kern = paged_mma_kernel<T, PARTS, HD>;
     constexpr int smem = MCfg<HD, PARTS>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = smem_opt_in(reinterpret_cast<const void*>(kern), smem, done);
     if (e != cudaSuccess) return e;
     KvMaps maps;
     const bool bf16 = std::is_same<T, __nv_bfloat16>::value;

@@ -73,20 +73,37 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         *P.n_items = n_items;
     }
     __syncthreads();
+    auto segment_of = [&](int i) {  // the last segment with item_off <= i
+        int lo = 0, hi = n_seg;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (P.item_off[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    if (prefix) {  // a group's row tile has many sequences: a warp each
+        for (int i = tid / 32; i < n_items; i += kPlanThreads / 32) {
+            const int seg = segment_of(i);
+            const PagedItem it = make_item<true>(A, P, true, seg, i - P.item_off[seg]);
+            if (tid % 32 == 0) P.items[i] = it;
+        }
+        __syncthreads();
+    }
     carry = 0;
     for (int base = 0; base < n_items; base += kPlanThreads) {
         const int i = base + tid;
         int tiles = 0;
         if (i < n_items) {
-            int lo = 0, hi = n_seg;  // the last segment with item_off <= i
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (P.item_off[mid] <= i) lo = mid;
-                else hi = mid;
+            PagedItem it;
+            if (prefix) {
+                it = P.items[i];
+            } else {
+                const int seg = segment_of(i);
+                it = make_item(A, P, false, seg, i - P.item_off[seg]);
             }
-            const PagedItem it = make_item(A, P, prefix, lo, i - P.item_off[lo]);
             tiles = item_units(P, it.n_tiles);
-            P.items[i] = it;
+            if (!prefix) P.items[i] = it;
         }
         const int at = carry + block_scan(tiles, &total, sums);
         if (i < n_items) P.cum[i] = at;
