@@ -1,0 +1,170 @@
+"""A batch of sequences through a decoder stack: the paged cache's operators around the MoE block.
+
+``BatchDecoder`` is the batched form of the engine's one-sequence decoder step (GQA / MHA
+attention, MoE feed-forward): each ``step`` takes new tokens of any number of sequences (a
+prompt, a chunk, a single token each, in one batch) through
+
+    x = embed[token]
+    per layer:  q, k, v = projections of rmsnorm(x);  rotary positions, k and v to the pages
+                x += o_proj(attention over the pages)
+                x += MoE(rmsnorm(x))
+    logits = lm_head . rmsnorm(x) of each sequence's last token
+
+Sequences share pages: ``fork`` continues one sequence in several ways, and a step whose
+neighbouring sequences begin with the same pages reads those once (``prefix_attention``).  The
+projections are plain fp16 matrix products; everything else runs in this library's kernels.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import paged
+from .moe import MoEStack
+
+
+@dataclass
+class AttnWeights:
+    """One layer's attention, fp16 row-major as the engine's dense file holds it."""
+    input_norm: torch.Tensor | None  # [H]
+    q_proj: torch.Tensor             # [heads * dim, H]
+    k_proj: torch.Tensor             # [kv_heads * dim, H]
+    v_proj: torch.Tensor             # [kv_heads * dim, H]
+    o_proj: torch.Tensor             # [H, heads * dim]
+
+
+def rmsnorm(x: torch.Tensor, w: torch.Tensor | None, eps: float) -> torch.Tensor:
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
+    return y if w is None else y * w.float()
+
+
+class BatchDecoder:
+    #: tokens from which a layer's MoE block takes the tensor-core path
+    PREFILL_TOKENS = 96
+    #: shared positions from which neighbouring sequences' prefix is read once
+    SHARED_POSITIONS = 256
+
+    def __init__(self, stack: MoEStack, layers: list[AttnWeights], embed: torch.Tensor,
+                 final_norm: torch.Tensor | None, lm_head: torch.Tensor, n_heads: int,
+                 n_kv_heads: int, *, theta: float = 10000.0, scaling: str | None = None,
+                 factor: float = 1.0, n_pages: int = 1024, page_size: int = 16, window: int = 0,
+                 sinks: int = 0):
+        if len(layers) != stack.L:
+            raise ValueError(f"{len(layers)} attention layers for a stack of {stack.L}")
+        H = stack.shape.hidden
+        if embed.shape[1] != H or H % n_heads or n_heads % n_kv_heads:
+            raise ValueError(f"hidden {H}, embedding {list(embed.shape)}, {n_heads} heads, "
+                             f"{n_kv_heads} kv heads")
+        self.stack, self.embed, self.lm_head, self.final_norm = stack, embed, lm_head, final_norm
+        self.nh, self.nkv, self.dim = n_heads, n_kv_heads, H // n_heads
+        self.window, self.sinks, self.eps = window, sinks, stack.shape.rms_eps
+        self.device = stack.device
+        self.layers = layers
+        self._qkv = [torch.cat((w.q_proj, w.k_proj, w.v_proj)) for w in layers]
+        self.pool = paged.PagePool(n_pages, page_size)
+        shape = (stack.L, n_pages, page_size, n_kv_heads, self.dim)
+        self.k = torch.zeros(shape, dtype=torch.float16, device=self.device)
+        self.v = torch.zeros_like(self.k)
+        self.freq, self.gain = paged.rope_frequencies(self.dim, theta, scaling=scaling,
+                                                      factor=factor, device=self.device)
+
+    # ------------------------------------------------------------------ sequences
+    def open(self) -> int:
+        return self.pool.open()
+
+    def fork(self, seq: int) -> int:
+        return self.pool.fork(seq)
+
+    def close(self, seq: int) -> None:
+        self.pool.close(seq)
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Forget the positions from ``length`` on (rejected drafts, an edited prompt)."""
+        self.pool.truncate(seq, length)
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pools; how many are in use."""
+        used = self.pool.compact()
+        self.pool.apply(self.k, self.v)
+        return used
+
+    def _shared(self, seqs: list[int]) -> tuple[list[int], list[int]]:
+        """(first sequence of each group and the end, shared positions of each group): runs of
+        neighbouring sequences that begin with the same pages."""
+        pages = [self.pool.pages(s) for s in seqs]
+        page = self.pool.page_size
+        starts, lens, i = [0], [], 0
+        while i < len(seqs):
+            # positions that are in whole pages before every new token: nobody writes them
+            common, j = min(len(pages[i]), self.pool.length(seqs[i]) // page), i + 1
+            while j < len(seqs):
+                n = 0
+                while n < min(common, len(pages[j])) and pages[j][n] == pages[i][n]:
+                    n += 1
+                if n * page < self.SHARED_POSITIONS:
+                    break
+                common, j = n, j + 1
+            starts.append(j)
+            lens.append(common * page if j - i > 1 else 0)
+            i = j
+        return starts, lens
+
+    # ------------------------------------------------------------------ one step
+    def step(self, batch: list[tuple[int, list[int]]]) -> torch.Tensor:
+        """Append each sequence's tokens; logits fp32 ``[len(batch), vocab]`` of the last ones."""
+        if not batch or any(not t for _, t in batch) or len({s for s, _ in batch}) != len(batch):
+            raise ValueError("step: each sequence once, with one token or more")
+        dev = self.device
+        before = [(seq, self.pool.length(seq)) for seq, _ in batch]
+        try:
+            for (seq, n), (_, toks) in zip(before, batch):
+                self.pool.extend(seq, n + len(toks))
+        except RuntimeError:  # out of pages: nothing of the step has happened
+            for seq, n in before:
+                self.pool.truncate(seq, n)
+            self.pool.apply(self.k, self.v)
+            raise
+        self.pool.apply(self.k, self.v)
+        seqs, counts = [s for s, _ in batch], [len(t) for _, t in batch]
+        starts = torch.tensor([0] + counts).cumsum(0).to(dev, torch.int32)
+        tb = paged.TokenBatch(starts, torch.tensor([self.pool.length(s) for s in seqs],
+                                                   dtype=torch.int32, device=dev),
+                              self.pool.table(seqs, device=dev), max(counts))
+        groups, shared = self._shared(seqs)
+        prefix = None
+        if any(shared):
+            prefix = [torch.tensor(x, dtype=torch.int32, device=dev) for x in (groups, shared)]
+        tokens = torch.tensor([t for _, ts in batch for t in ts], device=dev)
+        x = self.embed[tokens].float()
+        T, nh, nkv, d = x.shape[0], self.nh, self.nkv, self.dim
+        for l, w in enumerate(self.layers):
+            rows = rmsnorm(x, w.input_norm, self.eps).half() @ self._qkv[l].T
+            q, k, v = (rows[:, a * d:b * d].unflatten(1, (b - a, d)) for a, b in
+                       ((0, nh), (nh, nh + nkv), (nh + nkv, nh + 2 * nkv)))
+            q = paged.rope_append(q, k, v, self.k[l], self.v[l], tb, self.freq, gain=self.gain)
+            if prefix:
+                a = paged.prefix_attention(q, self.k[l], self.v[l], tb, *prefix,
+                                           window=self.window, sinks=self.sinks)
+            else:
+                a = paged.attention(q, self.k[l], self.v[l], tb, window=self.window,
+                                    sinks=self.sinks)
+            x += (a.reshape(T, nh * d) @ w.o_proj.T).float()
+            if T < self.PREFILL_TOKENS:
+                self.stack.stack(x, layers=1, layer0=l)
+            else:
+                x += self.stack.prefill(l, rmsnorm(x, self.stack.layers[l].norm, self.eps))
+        last = x[starts[1:].long() - 1]
+        return (rmsnorm(last, self.final_norm, self.eps).half() @ self.lm_head.T).float()
+
+    def generate(self, seqs: list[int], logits: torch.Tensor, n: int) -> list[list[int]]:
+        """``n`` greedy tokens of each sequence, from the logits of its last step on."""
+        out: list[list[int]] = [[] for _ in seqs]
+        for i in range(n):
+            nxt = logits.argmax(-1).tolist()
+            for o, t in zip(out, nxt):
+                o.append(t)
+            if i + 1 < n:
+                logits = self.step([(s, [t]) for s, t in zip(seqs, nxt)])
+        return out
