@@ -333,6 +333,78 @@ def test_python_refusals(cuda):
         paged.copy_pages(k, v, [0], [2, 3])
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (F32, 128), (F16, 40)])
+def test_scales_below_and_at_zero(cuda, scale, dtype, dim):
+    """A negative scale is the positive one on the negated rows (whose bound A the check takes)."""
+    for lens, window, sinks in ((DECODE + [(3, 40)], 0, 0), (PROMPT, 60, 2)):
+        q, k, v, batch = make(lens, dim=dim, dtype=dtype)
+        out, lse = paged.attention(q, k, v, batch, window=window, sinks=sinks, scale=scale,
+                                   return_lse=True)
+        same = restate(q if scale >= 0 else -q, k, v, batch, window, sinks, abs(scale))
+        check(out, lse, same, dtype, k.dtype)
+
+
+@pytest.mark.parametrize("n", [511, 513, 1500])
+def test_many_sequences(cuda, n):
+    """More sequences than the attention kernel counts by itself, than a plan's block has threads."""
+    run(make([(1, 1 + 7 * i % 90) for i in range(n)], heads=(4, 2)))
+    run(make([(1 + i % 20, 20 + 7 * i % 90) for i in range(n)], heads=(4, 2)))
+
+
+@pytest.mark.parametrize("heads", [(160, 160), (300, 150)])
+def test_more_heads_than_sms(cuda, heads):
+    run(make([(1, 70), (1, 300)], heads=heads))
+    run(make([(40, 70), (2, 300)], heads=heads))
+
+
+def test_a_table_that_is_part_of_a_wider_one(cuda):
+    q, k, v, batch = make(DECODE + [(20, 90)], dim=128)
+    n, w = batch.table.shape
+    wide = torch.full((n, w + 9), 1 << 30, dtype=torch.int32, device="cuda")
+    wide[:, 4:4 + w] = batch.table
+    other = paged.TokenBatch(batch.q_start, batch.kv_len, wide[:, 4:4 + w], batch.max_q)
+    assert torch.equal(paged.attention(q, k, v, other), paged.attention(q, k, v, batch))
+    batch.kv_len[4] = 1 << 20  # the longest: cut to the table's width, not to its stride
+    ws = torch.empty(paged.workspace_bytes(q, k, v, other), dtype=torch.uint8, device="cuda")
+    paged.attention(q, k, v, other, workspace=ws)
+    assert paged.status(ws) == 2
+
+
+@pytest.mark.parametrize("lens", [[(30, 300), (70, 500)], [(20, 4000)]])
+def test_a_captured_prompt_follows_the_lengths(cuda, lens):
+    q, k, v, batch = make(lens, dim=128)
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    paged.attention(q, k, v, batch, out=out, workspace=ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.attention(q, k, v, batch, out=out, workspace=ws)
+    batch.kv_len.sub_(9)
+    graph.replay()
+    check(out, None, restate(q, k, v, batch), F16, F16)
+    batch.q_start[-1] -= 5  # five rows of padding at the end
+    graph.replay()
+    check(out[:-5], None, tuple(x[:-5] if isinstance(x, torch.Tensor) else x for x in
+                                restate(q, k, v, batch)), F16, F16)
+
+
+def test_no_tokens(cuda):
+    q, k, v, batch = make(DECODE)
+    none = paged.TokenBatch(batch.q_start[:1], batch.kv_len[:0], batch.table[:0], 0)
+    assert paged.attention(q[:0], k, v, none).shape == (0, 8, 64)
+    f, _ = paged.rope_frequencies(64, device="cuda")
+    assert paged.rope_append(q[:0], q[:0, :2], q[:0, :2], k, v, none, f).shape == (0, 8, 64)
+
+
+def test_rows_that_ask_for_a_gradient_are_refused(cuda):
+    q, k, v, batch = make(DECODE)
+    with pytest.raises(ValueError, match="gradient"):
+        paged.attention(q.requires_grad_(), k, v, batch)
+    with torch.no_grad():
+        paged.attention(q, k, v, batch)
+
+
 # ------------------------------------------------------------------------ shared prefixes
 def prefix_run(args, groups, prefix, window=0, sinks=0):
     q, k, v, batch = args
@@ -452,6 +524,24 @@ def test_rope_of_many_tokens_and_strided_rows(cuda):
     assert (got.double() - want).abs().max().item() <= 2.0 ** -8 * want.abs().max().item()
 
 
+@pytest.mark.parametrize("heads,dim,tokens", [((80, 16), 256, 40), ((6, 2), 64, 3001), ((64, 8), 128, 1700)])
+def test_rope_of_wide_rows_and_long_batches(cuda, heads, dim, tokens):
+    """More units than a CTA's threads hold, more tokens than CTAs, and many sequences."""
+    lens = [(1, 9)] * 40 + [(tokens - 40, tokens - 30)] if tokens > 40 else [(tokens, tokens)]
+    q, k, v, batch = make(lens, heads=heads, dim=dim, dtype=F32)
+    T = q.shape[0]
+    rows = torch.randn(T, heads[1], dim, device="cuda")
+    f, _ = paged.rope_frequencies(dim // 2, 10000.0, device="cuda")
+    got = paged.rope_append(q, rows, rows, k, v, batch, f, offset=dim // 2)
+    pos = torch.cat([torch.arange(kv - n, kv) for n, kv in lens]).cuda()
+    want = rope64(q, pos, f, dim // 2, False, 1.0)
+    assert (got.double() - want).abs().max().item() <= 2.0 ** -20 * want.abs().max().item()
+    seq = torch.searchsorted(batch.q_start, torch.arange(T, device="cuda", dtype=torch.int32),
+                             right=True) - 1
+    page = batch.table.long()[seq, pos // 16]
+    assert torch.equal(v[page, pos % 16], rows.half())
+
+
 # ------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("layers,shape", [(1, (5, 8, 1, 8)), (3, (40, 16, 2, 64)),
                                           (2, (1300, 8, 1, 16)), (4, (9, 48, 8, 128))])
@@ -469,6 +559,16 @@ def test_copy_pages(cuda, layers, shape, dtype):
     assert torch.equal(k, wk) and torch.equal(v, wv)
     paged.copy_pages(k[0], v[0], [], [])
     assert torch.equal(k, wk)
+
+
+def test_more_moves_than_one_launch_carries(cuda):
+    k = torch.randn(2, 2300, 8, 1, 16, device="cuda").half()
+    v = torch.randn(2, 2300, 8, 1, 16, device="cuda").half()
+    src, dst = list(range(1, 2300, 2)), list(range(0, 2300, 2))
+    wk, wv = k.clone(), v.clone()
+    wk[:, dst], wv[:, dst] = k[:, src], v[:, src]
+    paged.copy_pages(k, v, src, dst)
+    assert torch.equal(k, wk) and torch.equal(v, wv)
 
 
 def test_one_source_to_many_pages(cuda):

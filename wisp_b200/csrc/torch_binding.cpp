@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -61,7 +62,6 @@ int dtype_of(const at::Tensor& t, const char* name) {
     }
 }
 
-int index_of(const at::Tensor& t) { return t.device().index(); }
 
 const int* ints(const at::Tensor& t, const char* name, int dim) {
     if (t.scalar_type() != at::kInt || t.dim() != dim || !t.is_cuda() || t.stride(dim - 1) != 1)
@@ -104,6 +104,8 @@ WispRows rows(const at::Tensor& x, const char* name, int64_t n, int64_t dim, con
     if (x.stride(2) != 1 || (heads > 1 && x.stride(1) != dim))
         refuse("%s: a row's heads must be contiguous", name);
     if (x.device() != dev) refuse("%s is not on the pages' device", name);
+    if (x.requires_grad() && c10::GradMode::is_enabled())
+        refuse("%s asks for a gradient: these calls have none (use torch.no_grad())", name);
     if (heads > 65535) refuse("%s: %lld heads", name, (long long)heads);
     WispRows R;
     R.base = x.data_ptr();
