@@ -635,11 +635,52 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
             const int all_hi = min(it.kv_hi, it.pmin + 1);
             const int all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
+            auto is_whole = [&](int j0) {  // nothing of the tile is hidden from any row
+                return j0 >= it.kv_lo && j0 + kN <= all_hi && (j0 >= all_lo || j0 + kN <= sinks);
+            };
+            // V of a partly hidden tile: no infinity or NaN may meet a zero weight.
+            auto look_through = [&](int j, int j0) {
+                const uint32_t rv = ring + 2 * (first + j * step) + 1;
+                if (!bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort)) return false;
+                char* vt = sKV + (rv % kSlots) * C::kSlot;
+                uint32_t found = 0;
+#pragma unroll
+                for (int c = 0; c < kN * HD / 8 / kM; ++c) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(vt + (c * kM + r) * 16);
+                    found |= odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
+                             odd_halves<T>(v.w);
+                }
+                if (found) {
+                    for (int c = r; c < kN * HD / 8; c += kM) {
+                        uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
+                        const uint4 v = *at;
+                        if (!(odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
+                              odd_halves<T>(v.w)))
+                            continue;
+                        const int p = j0 + ((c / 8) & (kN - 1));
+                        if (p >= it.kv_lo && p < any_hi && (p >= any_lo || p < sinks))
+                            P.redo[(size_t)(W.item - 1) * P.heads + head_lane] = 1;
+                        *at = make_uint4(0, 0, 0, 0);
+                    }
+                    async_fence();
+                }
+                return true;
+            };
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < own; ++j, ++cnt) {
+            // A warp without rows only keeps step: what P holds for it reaches no row that is read.
+            // (In a loop of its own: as a branch of the next one it cost prompts 5%.)
+            const bool idle = row0 + (warp & 3) * 32 >= n_rows;
+            for (int j = 0; idle && j < own; ++j, ++cnt) {
                 const int b = cnt & 1, j0 = W.tile(W.a + first + j * step) * kN;
-                const bool whole = j0 >= it.kv_lo && j0 + kN <= all_hi &&
-                                   (j0 >= all_lo || j0 + kN <= sinks);
+                ok = bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort) &&
+                     (is_whole(j0) || look_through(j, j0));
+                if (!ok) break;
+                __syncwarp();
+                if (lane == 0) bar_arrive(&p_full[x][b]);
+            }
+            for (int j = 0; !idle && j < own; ++j, ++cnt) {
+                const int b = cnt & 1, j0 = W.tile(W.a + first + j * step) * kN;
+                const bool whole = is_whole(j0);
                 if (!bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort)) {
                     ok = false;
                     break;
@@ -656,33 +697,9 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 #pragma unroll
                     for (int i = 0; i < kN; ++i)
                         if (!((w[i / 32] >> (i % 32)) & 1u)) s[i] = -INFINITY;
-                    // V of a partly hidden tile: no infinity or NaN may meet a zero weight
-                    const uint32_t rv = ring + 2 * (first + j * step) + 1;
-                    if (!bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort)) {
+                    if (!look_through(j, j0)) {
                         ok = false;
                         break;
-                    }
-                    char* vt = sKV + (rv % kSlots) * C::kSlot;
-                    uint32_t found = 0;
-#pragma unroll
-                    for (int c = 0; c < kN * HD / 8 / kM; ++c) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(vt + (c * kM + r) * 16);
-                        found |= odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
-                                 odd_halves<T>(v.w);
-                    }
-                    if (found) {
-                        for (int c = r; c < kN * HD / 8; c += kM) {
-                            uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
-                            const uint4 v = *at;
-                            if (!(odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
-                                  odd_halves<T>(v.w)))
-                                continue;
-                            const int p = j0 + ((c / 8) & (kN - 1));
-                            if (p >= it.kv_lo && p < any_hi && (p >= any_lo || p < sinks))
-                                P.redo[(size_t)(W.item - 1) * P.heads + head_lane] = 1;
-                            *at = make_uint4(0, 0, 0, 0);
-                        }
-                        async_fence();
                     }
                 }
                 float mx4[4];
