@@ -1,5 +1,5 @@
-// paged_attn.cu -- causal attention of a batch's tokens over a paged fp16 / bf16 cache, with
-// a sliding window and sinks, and its form for sequences that share a prefix.
+// paged_attn.cu -- causal attention of a batch's tokens over a paged fp16 / bf16 cache: the kernel
+// for many rows of heads wider than 128, and the join of what pieces share for all kernels.
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j)
 //   over cached j <= i with (window == 0 or i - j < window or j < sinks)
@@ -15,8 +15,12 @@
 // 16-bit parts (x ~= hi + lo, 22 bits in fp16) that fill the two halves of a
 // 16-row tile, so 8 rows cost one instruction and their two sums meet in one thread; the
 // weights p are split the same way.  bf16 parts hold 8 bits each, so there it takes three and a
-// second instruction (two parts left the results 2.8e-6 off, ten times the fp32 rounding).  In fp16, p is scaled by 2^kPShift so that small weights
-// of long contexts stay above the subnormals (the factor cancels in the quotient).
+// second instruction (two parts left the results 2.8e-6 off, ten times the fp32 rounding).  In
+// fp16, p is scaled by 2^kPShift so that small weights of long contexts stay above the subnormals
+// (the factor cancels in the quotient).
+//
+// The join reads each split row tile's partial sums (fp32) and their maxima; with its loads in
+// flight together it takes 4 us for a row over 37 pieces (21 us one piece after another).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -47,8 +51,7 @@ constexpr size_t attn_smem_bytes() {
 
 // ------------------------------------------------------------------------
 // Row tile of 16 * RW MMA rows: warp w owns rows 16 * (w % RW) .. and the positions
-// (w / RW) * kTile * RW / 4 .. of every KV tile.  With RW == 1 the warps never wait for one
-// another inside the loop (each loads what it reads).
+// (w / RW) * kTile * RW / 4 .. of every KV tile.
 // ------------------------------------------------------------------------
 template <typename T, bool SPLIT, int HD, int RW>
 __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs A, int which) {
@@ -542,9 +545,7 @@ cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
 
 template <typename T, bool SPLIT>
 cudaError_t launch_t(const PagedArgs& A, int which, int rw, cudaStream_t s) {
-    // (64 to 128 dims are the tensor-core kernel's)
-    return A.hd < 64 ? launch_rw<T, SPLIT, 64>(A, which, rw, s)
-                     : launch_rw<T, SPLIT, 256>(A, which, rw, s);
+    return launch_rw<T, SPLIT, 256>(A, which, rw, s);  // (up to 128 dims are the tcgen05 kernel's)
 }
 
 template <typename T, bool SPLIT>
@@ -571,7 +572,7 @@ int paged_attn_tile() { return kTile; }
 int paged_attn_rw(int rows, bool split) { return rows <= (split ? 16 : 32) ? 2 : 4; }
 
 // CTAs of one SM: what the ring leaves room for.
-int paged_attn_ctas(int hd) { return hd <= 64 ? 3 : 1; }
+int paged_attn_ctas() { return 1; }
 
 cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
                               cudaStream_t s) {

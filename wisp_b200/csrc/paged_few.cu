@@ -10,7 +10,10 @@
 // scores 16 of a tile's positions; the row maxima and the weights go through shared memory, and
 // then each warp adds all 64 weighted positions to a quarter of the head's dims.
 //
-// Before: each warp kept all dims for its own positions (64 accumulators a thread, a join of four
+// Measured (B200): 64 sequences with a window of 4096 and four sinks, 32 heads of 128 over 8 kv
+// heads, 175 us = 6.1 TB/s (95% of the measured copy); 14 ragged sequences of up to 4096 positions
+// 31 us (61%: starting, the tables' and the first tiles' latency and the join are 10 us of it);
+// one sequence of 1024 12 us.  Before: each warp kept all dims for its own positions (64 accumulators a thread, a join of four
 // 16 x head_dim tiles and an empty ring at the end of every row tile: 39.7 us for 14 ragged
 // sequences of up to 4096 positions); the same split with cp.async issued by the working warps
 // (486 instructions a warp and tile: 35.7 us, but long windows fell from 6.4 to 5.6 TB/s).
