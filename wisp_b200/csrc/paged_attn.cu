@@ -37,34 +37,30 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kTile = 64;  // positions of a KV tile
 
-template <int HD>
-struct Cfg {
-    static constexpr int kStages = HD <= 128 ? 3 : 2;
-    static constexpr int kCh = HD / 8;            // 16-byte pieces of a row
-    static constexpr int kStage = 2 * kTile * HD;  // elements: K then V
-};
+constexpr int HD = 256;   // dims in shared memory; narrower heads are filled up with zeros
+constexpr int kStages = 2;
+constexpr int kStage = 2 * kTile * HD;  // elements: K then V
 
-template <int HD, int RW, int FRAGS>
+template <int RW, int FRAGS>
 constexpr size_t attn_smem_bytes() {
-    return (size_t)Cfg<HD>::kStages * Cfg<HD>::kStage * 2 + (size_t)16 * RW * HD * 2 * FRAGS;
+    return (size_t)kStages * kStage * 2 + (size_t)16 * RW * HD * 2 * FRAGS;
 }
 
 // ------------------------------------------------------------------------
 // Row tile of 16 * RW MMA rows: warp w owns rows 16 * (w % RW) .. and the positions
 // (w / RW) * kTile * RW / 4 .. of every KV tile.
 // ------------------------------------------------------------------------
-template <typename T, bool SPLIT, int HD, int RW>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs A, int which) {
-    using C = Cfg<HD>;
-    constexpr int kCh = C::kCh, kS = C::kStages;
+template <typename T, bool SPLIT, int RW>
+__global__ void __launch_bounds__(kThreads)
+paged_attn_kernel(const __grid_constant__ PagedArgs A, int which) {
+    constexpr int kS = kStages;
     constexpr int kNP = kTile * RW / 4;       // positions per warp and tile
     constexpr int kNT = kNP / 8;              // score tiles of 8 positions
     constexpr int kRows = SPLIT ? 8 : 16;     // real rows per warp
     constexpr int kF = SPLIT ? PMath<T>::kFrags : 1;  // 16-row fragments that hold a row's parts
-    constexpr bool kQRegs = HD <= 128 && kF == 1;
     extern __shared__ __align__(128) char smem[];
     T* ring = reinterpret_cast<T*>(smem);
-    T* qs = ring + (size_t)kS * C::kStage;    // [kF][16 * RW][HD], swizzled like the cache rows
+    T* qs = ring + (size_t)kS * kStage;    // [kF][16 * RW][HD], swizzled like the cache rows
     __shared__ int s_pos[16 * RW];            // position of each real row (INT_MIN: no row)
     __shared__ float s_fac[16 * RW];          // SPLIT: the row's power-of-two factor
     __shared__ int s_bad;
@@ -136,24 +132,17 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             return seen ? page_offset(A, it.seq, j, kvh, &s_bad) : -1;
         };
         auto load_tile = [&](int st, long long off) {
-            T* kd = ring + (size_t)st * C::kStage;
+            T* kd = ring + (size_t)st * kStage;
             T* vd = kd + kTile * HD;
-            constexpr int kPer = 32 / kCh > 0 ? 32 / kCh : 1;   // rows per pass of the warp
-            constexpr int kCol = kCh > 32 ? kCh / 32 : 1;
 #pragma unroll
-            for (int p = 0; p < 16 / kPer; ++p) {
-                const int r = p * kPer + (kCh >= 32 ? 0 : lane / kCh);
-                const long long o = __shfl_sync(0xffffffffu, off, r);
-                const int row = warp * 16 + r;
-#pragma unroll
-                for (int cc = 0; cc < kCol; ++cc) {
-                    const int c = (kCh >= 32 ? lane : lane % kCh) + cc * 32;
-                    const bool in = o >= 0 && c * 8 < A.hd;
-                    const size_t src = in ? (size_t)o + c * 8 : 0;
-                    const int dst = row * HD + ((c ^ (row & 7)) * 8);
-                    cp16(kd + dst, Kc + src, in);
-                    cp16(vd + dst, Vc + src, in);
-                }
+            for (int rr = 0; rr < 16; ++rr) {  // a row a pass: 32 lanes of 16 bytes
+                const long long at = __shfl_sync(0xffffffffu, off, rr);
+                const int row = warp * 16 + rr;
+                const bool in = at >= 0 && lane * 8 < A.hd;
+                const size_t src = in ? (size_t)at + lane * 8 : 0;
+                const int dst = row * HD + ((lane ^ (row & 7)) * 8);
+                cp16(kd + dst, Kc + src, in);
+                cp16(vd + dst, Vc + src, in);
             }
         };
 
@@ -187,16 +176,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             lo_row[u] = A.window > 0 && prow[u] != INT_MIN ? prow[u] - A.window + 1 : INT_MIN;
         }
         const float fac = SPLIT ? s_fac[rw * 16 + g] * sl2 : sl2;
-        uint32_t qf[kQRegs ? HD / 16 : 1][4];
         auto load_q = [&](int n, int kk, uint32_t (&f)[4]) {
             const int r = rw * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
             ldsm4(f, qs + (size_t)(n * 16 * RW + r) * HD + ((c ^ (r & 7)) * 8));
         };
-        if (kQRegs) {
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) load_q(0, kk, qf[kQRegs ? kk : 0]);
-        }
-
         float o[HD / 8][4];
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i)
@@ -214,7 +197,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
                 cp_commit();
                 if (i + kS < b) off = row_offset(i + kS);
             }
-            const T* kd = ring + (size_t)st * C::kStage;
+            const T* kd = ring + (size_t)st * kStage;
             const T* vd = kd + kTile * HD;
             st = st + 1 == kS ? 0 : st + 1;
             const int j0 = tile_at(i) * kTile, jw = j0 + pw * kNP;
@@ -230,12 +213,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             for (int kk = 0; kk < HD / 16; ++kk) {
                 uint32_t qv[kF][4];
 #pragma unroll
-                for (int n = 0; n < kF; ++n) {
-                    if (!kQRegs) load_q(n, kk, qv[n]);
-                    else
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) qv[n][u] = qf[kQRegs ? kk : 0][u];
-                }
+                for (int n = 0; n < kF; ++n) load_q(n, kk, qv[n]);
 #pragma unroll
                 for (int t = 0; t < kNT; t += 2) {
                     const int r = pw * kNP + t * 8 + ((lane >> 4) & 1) * 8 + (lane & 7);
@@ -295,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             // that the usual loop stays short.
             bool odd = false;
             if (!full && it.pmin != it.pmax) {
-                for (int i = lane; i < kNP * kCh; i += 32) {
+                for (int i = lane; i < kNP * HD / 8; i += 32) {
                     const uint4 w = *reinterpret_cast<const uint4*>(vd + (size_t)pw * kNP * HD + i * 8);
                     odd |= PMath<T>::not_finite(w.x) || PMath<T>::not_finite(w.y) ||
                            PMath<T>::not_finite(w.z) || PMath<T>::not_finite(w.w);
@@ -526,10 +504,10 @@ paged_join2_kernel(const __grid_constant__ PagedArgs A) {
     }
 }
 
-template <typename T, bool SPLIT, int HD, int RW>
+template <typename T, bool SPLIT, int RW>
 cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
-    auto kern = paged_attn_kernel<T, SPLIT, HD, RW>;
-    constexpr size_t smem = attn_smem_bytes<HD, RW, SPLIT ? PMath<T>::kFrags : 1>();
+    auto kern = paged_attn_kernel<T, SPLIT, RW>;
+    constexpr size_t smem = attn_smem_bytes<RW, SPLIT ? PMath<T>::kFrags : 1>();
     static std::atomic<uint64_t> done{0};
     cudaError_t e = smem_opt_in(reinterpret_cast<const void*>(kern), smem, done);
     if (e != cudaSuccess) return e;
@@ -537,15 +515,9 @@ cudaError_t launch_one(const PagedArgs& A, int which, cudaStream_t s) {
     return launch_pdl(kern, dim3(P.heads * P.lanes), dim3(kThreads), smem, s, A, which);
 }
 
-template <typename T, bool SPLIT, int HD>
-cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
-    return rw == 2 ? launch_one<T, SPLIT, HD, 2>(A, which, s)
-                   : launch_one<T, SPLIT, HD, 4>(A, which, s);
-}
-
 template <typename T, bool SPLIT>
-cudaError_t launch_t(const PagedArgs& A, int which, int rw, cudaStream_t s) {
-    return launch_rw<T, SPLIT, 256>(A, which, rw, s);  // (up to 128 dims are the tcgen05 kernel's)
+cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
+    return rw == 2 ? launch_one<T, SPLIT, 2>(A, which, s) : launch_one<T, SPLIT, 4>(A, which, s);
 }
 
 template <typename T, bool SPLIT>
@@ -578,10 +550,10 @@ cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype
                               cudaStream_t s) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     if (kv_dtype == WISP_DTYPE_F16)
-        return split ? launch_t<__half, true>(A, which, rw, s)
-                     : launch_t<__half, false>(A, which, rw, s);
-    return split ? launch_t<__nv_bfloat16, true>(A, which, rw, s)
-                 : launch_t<__nv_bfloat16, false>(A, which, rw, s);
+        return split ? launch_rw<__half, true>(A, which, rw, s)
+                     : launch_rw<__half, false>(A, which, rw, s);
+    return split ? launch_rw<__nv_bfloat16, true>(A, which, rw, s)
+                 : launch_rw<__nv_bfloat16, false>(A, which, rw, s);
 }
 
 cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s) {
