@@ -417,49 +417,146 @@ paged_attn_kernel(const __grid_constant__ PagedArgs A, int which) {
 }
 
 // ------------------------------------------------------------------------
-// Joins the pieces of split items.  CTA (piece, block of heads, 8 / WARPS rows): the item that
-// begins in the piece and ends after it.  WARPS warps per row take every WARPS-th piece, in
-// batches whose loads are in flight together, and meet in shared memory in their order.
-// Items that the tensor-core kernel marked are worked out here without tiles.
+// Joins the pieces of split items.  CTA (piece, block of heads, ...): the item that begins in the
+// piece and ends after it.  Items that the tensor-core kernel marked are worked out here without
+// tiles.
 // ------------------------------------------------------------------------
-template <typename T, bool SPLIT, int WARPS>
+struct JoinPlace {
+    int piece, head_lane, h0, gpb;
+    __device__ __forceinline__ JoinPlace(const PagedArgs& A, const PagedPlan& P) {
+        head_lane = blockIdx.x % P.heads;
+        piece = blockIdx.x / P.heads;
+        const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
+        h0 = kvh * A.group + hb * P.gpb;
+        gpb = min(P.gpb, A.group - hb * P.gpb);
+    }
+};
+
+// By the whole CTA: the marked ones of the items whose first KV tile lies in the piece.
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void join_marked(const PagedArgs& A, const PagedPlan& P,
+                                            const PagedSplit& sp, const JoinPlace& at) {
+    int marked = 0;
+    for (int i = sp.item0 + (int)threadIdx.x; i < sp.item1; i += kJoinThreads)
+        marked |= P.redo[(size_t)i * P.heads + at.head_lane];
+    if (!__syncthreads_or(marked)) return;
+    for (int i = sp.item0; i < sp.item1; ++i) {
+        if (!P.redo[(size_t)i * P.heads + at.head_lane]) continue;
+        const PagedItem it = P.items[i];
+        for (int r = threadIdx.x / 32; r < it.ntok * at.gpb; r += kJoinThreads / 32) {
+            Joined J;
+            J.restate<T, SPLIT>(A, it.tok0 + r / at.gpb, at.h0 + r % at.gpb);
+            J.write<T, SPLIT>(A, it.tok0 + r / at.gpb, at.h0 + r % at.gpb);
+        }
+    }
+}
+
+// Items of few rows, usually in many pieces: two rows a CTA, four warps per row take every fourth
+// piece, in batches whose loads are in flight together, and meet in shared memory in their order.
+template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ PagedArgs A, int which) {
     __shared__ JoinShared S;
-    constexpr int kRows = 8 / WARPS;
+    constexpr int kWarps = 4, kRows = 2;
     const PagedPlan& P = A.plan[which];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
-    const int head_lane = blockIdx.x % P.heads, piece = blockIdx.x / P.heads;
-    const PagedSplit sp = P.split[piece];
-    const int kvh = head_lane / P.hblocks, hb = head_lane - kvh * P.hblocks;
-    const int h0 = kvh * A.group + hb * P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
-    const int warp = threadIdx.x / 32;
+    const JoinPlace at(A, P);
+    const PagedSplit sp = P.split[at.piece];
+    if (P.redo && blockIdx.y == 0) join_marked<T, SPLIT>(A, P, sp, at);
+    const int n_rows = sp.n_rows / P.gpb * at.gpb;  // (counted with full blocks of heads)
+    if ((int)blockIdx.y * kRows >= n_rows) return;
+    if (P.redo && P.redo[(size_t)sp.item * P.heads + at.head_lane]) return;
+    const int warp = threadIdx.x / 32, row = blockIdx.y * kRows + warp / kWarps;
     Joined J;
-    int marked = 0;
-    if (P.redo && blockIdx.y == 0)
-        for (int i = sp.item0 + (int)threadIdx.x; i < sp.item1; i += kJoinThreads)
-            marked |= P.redo[(size_t)i * P.heads + head_lane];
-    if (P.redo && blockIdx.y == 0 && __syncthreads_or(marked)) {
-        for (int i = sp.item0; i < sp.item1; ++i) {
-            if (!P.redo[(size_t)i * P.heads + head_lane]) continue;
-            const PagedItem it = P.items[i];
-            for (int r = warp; r < it.ntok * gpb; r += kJoinThreads / 32) {
-                J.restate<T, SPLIT>(A, it.tok0 + r / gpb, h0 + r % gpb);
-                J.write<T, SPLIT>(A, it.tok0 + r / gpb, h0 + r % gpb);
+    J.init();
+    if (row < n_rows) J.add_range(A, P, at.piece, sp.last, at.head_lane, row, warp % kWarps, kWarps);
+    J.meet(S, warp % kWarps, kWarps);
+    if (row < n_rows && warp % kWarps == 0)
+        J.write<T, SPLIT>(A, sp.tok0 + row / at.gpb, at.h0 + row % at.gpb);
+}
+
+// Items of many rows, mostly in two pieces: a thread takes four dims of kJoinRows rows, so that
+// the loads of all of them are in flight together whatever the head's size.
+constexpr int kJoinRows = 2, kJoinBatch = 2;
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kJoinThreads)
+paged_join_rows_kernel(const __grid_constant__ PagedArgs A, int which) {
+    const PagedPlan& P = A.plan[which];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
+    const JoinPlace at(A, P);
+    const PagedSplit sp = P.split[at.piece];
+    if (P.redo && blockIdx.y == 0) join_marked<T, SPLIT>(A, P, sp, at);
+    const int n_rows = sp.n_rows / P.gpb * at.gpb, quads = A.hd / 4;
+    const int e0 = blockIdx.y * (kJoinRows * kJoinThreads) + threadIdx.x;
+    if (e0 >= n_rows * quads) return;
+    if (P.redo && P.redo[(size_t)sp.item * P.heads + at.head_lane]) return;
+    int row[kJoinRows], d[kJoinRows];
+    float M[kJoinRows], L[kJoinRows];
+    float4 acc[kJoinRows];
+#pragma unroll
+    for (int u = 0; u < kJoinRows; ++u) {
+        const int e = min(e0 + u * kJoinThreads, n_rows * quads - 1);
+        row[u] = e / quads;
+        d[u] = (e - row[u] * quads) * 4;
+        M[u] = -INFINITY;
+        L[u] = 0.f;
+        acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int p = at.piece; p <= sp.last; p += kJoinBatch) {
+        float4 v[kJoinRows][kJoinBatch];
+        float2 w[kJoinRows][kJoinBatch];
+#pragma unroll
+        for (int u = 0; u < kJoinRows; ++u)
+#pragma unroll
+            for (int k = 0; k < kJoinBatch; ++k) {
+                v[u][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                w[u][k] = make_float2(-INFINITY, 0.f);
+                if (p + k > sp.last) continue;
+                const size_t id = part_row(P, p + k, at.head_lane, p + k == at.piece, row[u]);
+                v[u][k] = __ldcg(reinterpret_cast<const float4*>(P.part_o + id * A.hd + d[u]));
+                w[u][k] = __ldcg(reinterpret_cast<const float2*>(P.part_ml + id * 2));
+            }
+#pragma unroll
+        for (int u = 0; u < kJoinRows; ++u) {
+            float to = M[u];
+#pragma unroll
+            for (int k = 0; k < kJoinBatch; ++k) to = fmaxf(to, w[u][k].x);
+            const float base = to == -INFINITY ? 0.f : to, old = ex2(M[u] - base);
+            M[u] = to;
+            L[u] *= old;
+            acc[u].x *= old, acc[u].y *= old, acc[u].z *= old, acc[u].w *= old;
+#pragma unroll
+            for (int k = 0; k < kJoinBatch; ++k) {
+                if (p + k > sp.last) break;
+                const float e = ex2(w[u][k].x - base);
+                L[u] = fmaf(w[u][k].y, e, L[u]);
+                acc[u].x = fmaf(v[u][k].x, e, acc[u].x);
+                acc[u].y = fmaf(v[u][k].y, e, acc[u].y);
+                acc[u].z = fmaf(v[u][k].z, e, acc[u].z);
+                acc[u].w = fmaf(v[u][k].w, e, acc[u].w);
             }
         }
     }
-    const int n_rows = sp.n_rows / P.gpb * gpb;  // (counted with full blocks of heads)
-    if ((int)blockIdx.y * kRows >= n_rows) return;
-    if (P.redo && P.redo[(size_t)sp.item * P.heads + head_lane]) return;
-    const int row = blockIdx.y * kRows + warp / WARPS;
-    J.init();
-    if (row < n_rows) J.add_range(A, P, piece, sp.last, head_lane, row, warp % WARPS, WARPS);
-    J.meet(S, warp % WARPS, WARPS);
-    if (row < n_rows && warp % WARPS == 0)
-        J.write<T, SPLIT>(A, sp.tok0 + row / gpb, h0 + row % gpb);
+#pragma unroll
+    for (int u = 0; u < kJoinRows; ++u) {
+        if (e0 + u * kJoinThreads >= n_rows * quads) break;
+        const int t = sp.tok0 + row[u] / at.gpb, h = at.h0 + row[u] % at.gpb;
+        const size_t to = (size_t)t * A.out_stride + (size_t)h * A.hd + d[u];
+        const float inv = 1.f / L[u];
+        const float4 o = L[u] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                     : make_float4(acc[u].x * inv, acc[u].y * inv, acc[u].z * inv,
+                                                   acc[u].w * inv);
+        if (SPLIT)
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(A.out) + to) = o;
+        else
+            *reinterpret_cast<uint2*>(reinterpret_cast<T*>(A.out) + to) =
+                make_uint2(PMath<T>::pack(o.x, o.y), PMath<T>::pack(o.z, o.w));
+        if (d[u] == 0 && A.lse) A.lse[(size_t)t * A.nh + h] = row_lse(M[u], L[u]);
+    }
 }
 
 // Prefix mode: the same for CTA (token, two of its heads), over the pieces of the shared prefix
@@ -527,13 +624,14 @@ cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
                           dim3(kJoinThreads), 0, s, A);
     const int w = A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY;
     const PagedPlan& P = A.plan[w];
-    // few rows: four warps each; many: as many rows as warps, most items are in few pieces
     if (P.used_rows <= 32)
-        return launch_pdl(paged_join_kernel<T, SPLIT, 4>,
+        return launch_pdl(paged_join_kernel<T, SPLIT>,
                           dim3(P.heads * P.lanes, (P.used_rows + 1) / 2), dim3(kJoinThreads), 0, s, A,
                           w);
-    return launch_pdl(paged_join_kernel<T, SPLIT, 1>,
-                      dim3(P.heads * P.lanes, (P.used_rows + 7) / 8), dim3(kJoinThreads), 0, s, A, w);
+    constexpr int kPer = kJoinRows * kJoinThreads;
+    return launch_pdl(paged_join_rows_kernel<T, SPLIT>,
+                      dim3(P.heads * P.lanes, (P.used_rows * (A.hd / 4) + kPer - 1) / kPer),
+                      dim3(kJoinThreads), 0, s, A, w);
 }
 
 }  // namespace
