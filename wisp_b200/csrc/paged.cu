@@ -17,8 +17,8 @@
 namespace wb {
 
 cudaError_t launch_paged_plan(const PagedArgs& A, cudaStream_t s);
-cudaError_t launch_paged_few(const PagedArgs& A, int which, bool both, int q_dtype, int kv_dtype,
-                             cudaStream_t s);
+cudaError_t launch_paged_few(const PagedArgs& A, int which, bool both, bool behind, int q_dtype,
+                             int kv_dtype, cudaStream_t s);
 int paged_few_tile();
 int paged_few_ctas(int hd);
 cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
@@ -464,9 +464,9 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
 }
 
 cudaError_t launch_plan_kernel(const PagedArgs& A, const AttnShape& S, int which, bool both,
-                               int q_dtype, int kv_dtype, cudaStream_t s) {
+                               bool behind, int q_dtype, int kv_dtype, cudaStream_t s) {
     return S.rw[which] == 0   ? launch_paged_mma(A, which, q_dtype, kv_dtype, s)
-           : S.rw[which] == 1 ? launch_paged_few(A, which, both, q_dtype, kv_dtype, s)
+           : S.rw[which] == 1 ? launch_paged_few(A, which, both, behind, q_dtype, kv_dtype, s)
                               : launch_paged_attn(A, which, S.rw[which], q_dtype, kv_dtype, s);
 }
 
@@ -536,9 +536,12 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     const bool both = A.plan[PLAN_PREFIX].used && A.plan[PLAN_FEW].used &&
                       S.rw[PLAN_PREFIX] == 1 && S.rw[PLAN_FEW] == 1;
     const int order[PLANS] = {PLAN_PREFIX, PLAN_MANY, PLAN_FEW};
+    bool behind = false;
     for (int w : order) {
         if (!A.plan[w].used || (w == PLAN_PREFIX && both)) continue;
-        WB_CUDA_RET(launch_plan_kernel(A, S, w, both && w == PLAN_FEW, q->dtype, P->dtype, s), err);
+        WB_CUDA_RET(launch_plan_kernel(A, S, w, both && w == PLAN_FEW, behind, q->dtype, P->dtype, s),
+                    err);
+        behind = true;
     }
     WB_CUDA_RET(launch_paged_join(A, q->dtype, P->dtype, s), err);
     return WISP_OK;

@@ -444,7 +444,7 @@ __device__ __forceinline__ void join_marked(const PagedArgs& A, const PagedPlan&
         if (!P.redo[(size_t)i * P.heads + at.head_lane]) continue;
         const PagedItem it = P.items[i];
         for (int r = threadIdx.x / 32; r < it.ntok * at.gpb; r += kJoinThreads / 32) {
-            Joined J;
+            Joined<4> J;
             J.restate<T, SPLIT>(A, it.tok0 + r / at.gpb, at.h0 + r % at.gpb);
             J.write<T, SPLIT>(A, it.tok0 + r / at.gpb, at.h0 + r % at.gpb);
         }
@@ -453,10 +453,10 @@ __device__ __forceinline__ void join_marked(const PagedArgs& A, const PagedPlan&
 
 // Items of few rows, usually in many pieces: two rows a CTA, four warps per row take every fourth
 // piece, in batches whose loads are in flight together, and meet in shared memory in their order.
-template <typename T, bool SPLIT>
+template <typename T, bool SPLIT, int VECS>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ PagedArgs A, int which) {
-    __shared__ JoinShared S;
+    __shared__ JoinShared<VECS> S;
     constexpr int kWarps = 4, kRows = 2;
     const PagedPlan& P = A.plan[which];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -469,12 +469,12 @@ paged_join_kernel(const __grid_constant__ PagedArgs A, int which) {
     if ((int)blockIdx.y * kRows >= n_rows) return;
     if (P.redo && P.redo[(size_t)sp.item * P.heads + at.head_lane]) return;
     const int warp = threadIdx.x / 32, row = blockIdx.y * kRows + warp / kWarps;
-    Joined J;
+    Joined<VECS> J;
     J.init();
     if (row < n_rows) J.add_range(A, P, at.piece, sp.last, at.head_lane, row, warp % kWarps, kWarps);
     J.meet(S, warp % kWarps, kWarps);
     if (row < n_rows && warp % kWarps == 0)
-        J.write<T, SPLIT>(A, sp.tok0 + row / at.gpb, at.h0 + row % at.gpb);
+        J.template write<T, SPLIT>(A, sp.tok0 + row / at.gpb, at.h0 + row % at.gpb);
 }
 
 // Items of many rows, mostly in two pieces: a thread takes four dims of kJoinRows rows, so that
@@ -559,45 +559,65 @@ paged_join_rows_kernel(const __grid_constant__ PagedArgs A, int which) {
     }
 }
 
-// Prefix mode: the same for CTA (token, two of its heads), over the pieces of the shared prefix
-// and of the sequence's own part.
-template <typename T, bool SPLIT>
+// Prefix mode: CTA (token, two of its heads), over the records of the shared prefix and of the
+// sequence's own part: pieces, or one whole record.
+template <typename T, bool SPLIT, int VECS>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join2_kernel(const __grid_constant__ PagedArgs A) {
-    __shared__ JoinShared S;
-    constexpr int kWarps = 4, kRows = 2;
+    __shared__ JoinShared<VECS> S;
+    constexpr int kWarps = 4, kRows = 2, kBatch = 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
-    const int t = blockIdx.x, warp = threadIdx.x / 32;
-    const int h = blockIdx.y * kRows + warp / kWarps;
+    const int t = blockIdx.x, warp = threadIdx.x / 32 % kWarps;
+    const int h = blockIdx.y * kRows + threadIdx.x / 32 / kWarps;
     if (t < A.q_start[0] || t >= A.q_start[A.n_seq]) return;  // nobody's token
-    Joined J;
+    Joined<VECS> J;
     J.init();
     bool redo = false;
     if (h < A.nh) {
-        const PagedWhere own = A.plan[A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY].where[t];
-        const PagedWhere shared = A.plan[PLAN_PREFIX].where[t];
+        PagedWhere w[2] = {A.plan[A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY].where[t],
+                           A.plan[PLAN_PREFIX].where[t]};
         const int kvh = h / A.group, hg = h - kvh * A.group;
-        for (int part = 0; part < (own.alone ? 1 : 2); ++part) {
-            const PagedWhere w = part ? shared : own;
-            if (w.plan < 0 || w.plan >= PLANS) continue;
-            const PagedPlan& P = A.plan[w.plan];
+        int n[2], lane[2], row[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            n[k] = 0;
+            if ((k && w[0].alone) || w[k].plan < 0 || w[k].plan >= PLANS) continue;
+            const PagedPlan& P = A.plan[w[k].plan];
             const int hb = hg / P.gpb, gpb = min(P.gpb, A.group - hb * P.gpb);
-            const int head_lane = kvh * P.hblocks + hb, row = w.row0 / P.gpb * gpb + hg - hb * P.gpb;
+            lane[k] = kvh * P.hblocks + hb;
+            row[k] = w[k].row0 / P.gpb * gpb + hg - hb * P.gpb;
             // (a malformed q_start leaves tokens without a record)
-            if (w.first < 0 || w.last < w.first || w.last >= P.lanes || row < 0 || row >= P.rows ||
-                w.item < 0 || w.item >= P.max_items)
+            if (w[k].first < 0 || w[k].last < w[k].first || w[k].last >= P.lanes || row[k] < 0 ||
+                row[k] >= P.rows || w[k].item < 0 || w[k].item >= P.max_items)
                 continue;
-            if (P.redo && P.redo[(size_t)w.item * P.heads + head_lane]) redo = true;
-            if (w.first == w.last) J.add_full(A, part != 0, (size_t)t * A.nh + h, warp % kWarps);
-            else J.add_range(A, P, w.first, w.last, head_lane, row, warp % kWarps, kWarps);
+            if (P.redo && P.redo[(size_t)w[k].item * P.heads + lane[k]]) redo = true;
+            n[k] = w[k].last - w[k].first + 1;
+        }
+        for (int i = warp; i < n[0] + n[1]; i += kBatch * kWarps) {
+            const float *o[kBatch], *ml[kBatch];
+            int have = 0;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int j = min(i + b * kWarps, n[0] + n[1] - 1), k = j >= n[0];
+                const PagedPlan& P = A.plan[k ? w[1].plan : w[0].plan];
+                const int c = k ? n[1] : n[0], first = k ? w[1].first : w[0].first;
+                const int p = first + (k ? j - n[0] : j);
+                const size_t id =
+                    c == 1 ? (size_t)k * A.n_tokens * A.nh + (size_t)t * A.nh + h
+                           : part_row(P, p, k ? lane[1] : lane[0], p == first, k ? row[1] : row[0]);
+                o[b] = (c == 1 ? A.full_o : P.part_o) + id * A.hd;
+                ml[b] = (c == 1 ? A.full_ml : P.part_ml) + id * 2;
+                have += i + b * kWarps < n[0] + n[1];
+            }
+            J.template add<kBatch>(A, o, ml, have);
         }
     }
-    J.meet(S, warp % kWarps, kWarps);
-    if (h < A.nh && warp % kWarps == 0) {
-        if (redo) J.restate<T, SPLIT>(A, t, h);
-        J.write<T, SPLIT>(A, t, h);
+    J.meet(S, warp, kWarps);
+    if (h < A.nh && warp == 0) {
+        if (redo) J.template restate<T, SPLIT>(A, t, h);
+        J.template write<T, SPLIT>(A, t, h);
     }
 }
 
@@ -617,15 +637,15 @@ cudaError_t launch_rw(const PagedArgs& A, int which, int rw, cudaStream_t s) {
     return rw == 2 ? launch_one<T, SPLIT, 2>(A, which, s) : launch_one<T, SPLIT, 4>(A, which, s);
 }
 
-template <typename T, bool SPLIT>
+template <typename T, bool SPLIT, int VECS>
 cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
     if (A.n_groups > 0)
-        return launch_pdl(paged_join2_kernel<T, SPLIT>, dim3(A.n_tokens, (A.nh + 1) / 2),
+        return launch_pdl(paged_join2_kernel<T, SPLIT, VECS>, dim3(A.n_tokens, (A.nh + 1) / 2),
                           dim3(kJoinThreads), 0, s, A);
     const int w = A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY;
     const PagedPlan& P = A.plan[w];
     if (P.used_rows <= 32)
-        return launch_pdl(paged_join_kernel<T, SPLIT>,
+        return launch_pdl(paged_join_kernel<T, SPLIT, VECS>,
                           dim3(P.heads * P.lanes, (P.used_rows + 1) / 2), dim3(kJoinThreads), 0, s, A,
                           w);
     constexpr int kPer = kJoinRows * kJoinThreads;
@@ -655,11 +675,13 @@ cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype
 }
 
 cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s) {
-    const bool split = q_dtype == WISP_DTYPE_F32;
-    if (kv_dtype == WISP_DTYPE_F16)
-        return split ? launch_join<__half, true>(A, s) : launch_join<__half, false>(A, s);
-    return split ? launch_join<__nv_bfloat16, true>(A, s)
-                 : launch_join<__nv_bfloat16, false>(A, s);
+    const bool split = q_dtype == WISP_DTYPE_F32, wide = A.hd > 128;
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        return split ? (wide ? launch_join<T, true, 4>(A, s) : launch_join<T, true, 2>(A, s))
+                     : (wide ? launch_join<T, false, 4>(A, s) : launch_join<T, false, 2>(A, s));
+    };
+    return kv_dtype == WISP_DTYPE_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
 
 }  // namespace wb

@@ -66,7 +66,7 @@ __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, 128;" ::
 template <typename T, bool SPLIT, int HD>
 __global__ void __launch_bounds__(kThreads, (FCfg<T, SPLIT, HD>::kCtas))
 paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ KvMaps maps, int which0,
-                 int box_rows) {
+                 int box_rows, int behind) {
     using C = FCfg<T, SPLIT, HD>;
     constexpr int kF = C::kF, kS = C::kStages, kRows = SPLIT ? 8 : 16;
     constexpr int kDW = HD / 4;  // dims of a warp
@@ -101,7 +101,10 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // Behind the shared prefixes' kernel of this call, which has waited for all that is read here,
+    // the SMs that it leaves start on this one: only the end waits for it (for the join's sake).
+    auto wait_before = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+    if (!behind) wait_before();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const bool inlined = P.inlined != 0, prefix = which == PLAN_PREFIX;
@@ -113,7 +116,10 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     }
     const int n_items = inlined ? (prefix ? A.n_groups : A.n_seq) * P.per_seg : *P.n_items;
     auto inline_item = [&](int i) { return make_item(A, P, prefix, i / P.per_seg, i % P.per_seg); };
-    if (n_items == 0) return;
+    if (n_items == 0) {
+        if (behind) wait_before();
+        return;
+    }
     const int* cum = inlined ? s_cum : P.cum;
     if (inlined) {
         // few row tiles: every CTA counts the units itself, which is shorter than a kernel of its
@@ -153,7 +159,10 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     }
     const int total = cum[n_items];
     const Pieces pieces(P, max(total, 1));
-    if (total == 0 || piece >= pieces.n) return;
+    if (total == 0 || piece >= pieces.n) {
+        if (behind) wait_before();
+        return;
+    }
     const int x0 = pieces.start(piece), x_end = pieces.start(piece + 1);
     const int item0 = block_last_le(cum, n_items, x0);
 
@@ -515,10 +524,12 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     }
     __syncthreads();
     if (tid == 0 && (s_bad || s_abort)) P.bad[blockIdx.x] = s_bad | (s_abort ? PG_TIMEOUT : 0);
+    if (behind) wait_before();
 }
 
 template <typename T, bool SPLIT, int HD>
-cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, cudaStream_t s) {
+cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, bool behind,
+                       cudaStream_t s) {
     auto kern = paged_few_kernel<T, SPLIT, HD>;
     constexpr size_t smem = FCfg<T, SPLIT, HD>::kSmem;
     static std::atomic<uint64_t> done{0};
@@ -530,14 +541,14 @@ cudaError_t launch_one(const PagedArgs& A, int which, bool with_prefix, cudaStre
     if (rows == 0) return cudaErrorInvalidValue;
     const PagedPlan& P = A.plan[which];
     return launch_pdl(kern, dim3(P.heads * P.lanes, with_prefix ? 2 : 1), dim3(kThreads), smem, s, A,
-                      maps, which, rows);
+                      maps, which, rows, (int)behind);
 }
 
 template <typename T, bool SPLIT>
-cudaError_t launch_t(const PagedArgs& A, int which, bool both, cudaStream_t s) {
-    return A.hd <= 64    ? launch_one<T, SPLIT, 64>(A, which, both, s)
-           : A.hd <= 128 ? launch_one<T, SPLIT, 128>(A, which, both, s)
-                         : launch_one<T, SPLIT, 256>(A, which, both, s);
+cudaError_t launch_t(const PagedArgs& A, int which, bool both, bool behind, cudaStream_t s) {
+    return A.hd <= 64    ? launch_one<T, SPLIT, 64>(A, which, both, behind, s)
+           : A.hd <= 128 ? launch_one<T, SPLIT, 128>(A, which, both, behind, s)
+                         : launch_one<T, SPLIT, 256>(A, which, both, behind, s);
 }
 
 }  // namespace
@@ -547,15 +558,16 @@ int paged_few_ctas(int hd) {
     return hd <= 64 ? FCfg<__half, false, 64>::kCtas : hd <= 128 ? FCfg<__half, false, 128>::kCtas : 1;
 }
 
-// both: the shared prefixes' plan in the same launch.
-cudaError_t launch_paged_few(const PagedArgs& A, int which, bool both, int q_dtype, int kv_dtype,
-                             cudaStream_t s) {
+// both: the shared prefixes' plan in the same launch.  behind: the launch before it on the stream
+// is another attention kernel of this call.
+cudaError_t launch_paged_few(const PagedArgs& A, int which, bool both, bool behind, int q_dtype,
+                             int kv_dtype, cudaStream_t s) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     if (kv_dtype == WISP_DTYPE_F16)
-        return split ? launch_t<__half, true>(A, which, both, s)
-                     : launch_t<__half, false>(A, which, both, s);
-    return split ? launch_t<__nv_bfloat16, true>(A, which, both, s)
-                 : launch_t<__nv_bfloat16, false>(A, which, both, s);
+        return split ? launch_t<__half, true>(A, which, both, behind, s)
+                     : launch_t<__half, false>(A, which, both, behind, s);
+    return split ? launch_t<__nv_bfloat16, true>(A, which, both, behind, s)
+                 : launch_t<__nv_bfloat16, false>(A, which, both, behind, s);
 }
 
 }  // namespace wb

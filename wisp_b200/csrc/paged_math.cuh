@@ -490,18 +490,21 @@ struct RowOut {
 
 // The join of one row's partial records by W warps.
 constexpr int kJoinThreads = 256;
+template <int VECS>
 struct JoinShared {
-    float2 acc[8][128];
+    float2 acc[8][32 * VECS];
     float m[8], l[8];
 };
+// A lane holds dims (i * 32 + lane) * 2 and the next for i < VECS: heads of up to 64 VECS dims.
+template <int VECS>
 struct Joined {
     float M, L;
-    float2 acc[4];  // dims (i * 32 + lane) * 2
+    float2 acc[VECS];
     __device__ __forceinline__ void init() {
         M = -INFINITY;
         L = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = make_float2(0.f, 0.f);
+        for (int i = 0; i < VECS; ++i) acc[i] = make_float2(0.f, 0.f);
     }
     __device__ __forceinline__ void rebase(float m) {
         const float base = m == -INFINITY ? 0.f : m;
@@ -509,7 +512,7 @@ struct Joined {
         M = m;
         L *= e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < VECS; ++i) {
             acc[i].x *= e;
             acc[i].y *= e;
         }
@@ -519,13 +522,13 @@ struct Joined {
     __device__ __forceinline__ void add(const PagedArgs& A, const float* const (&o)[N],
                                         const float* const (&ml)[N], int n) {
         const int lane = threadIdx.x & 31;
-        float2 v[N][4], w[N];
+        float2 v[N][VECS], w[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             w[k] = k < n ? __ldcg(reinterpret_cast<const float2*>(ml[k]))
                          : make_float2(-INFINITY, 0.f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VECS; ++i) {
                 const int d = (i * 32 + lane) * 2;
                 v[k][i] = k < n && d < A.hd ? __ldcg(reinterpret_cast<const float2*>(o[k] + d))
                                             : make_float2(0.f, 0.f);
@@ -542,18 +545,11 @@ struct Joined {
             const float e = ex2(w[k].x - base);
             L = fmaf(w[k].y, e, L);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VECS; ++i) {
                 acc[i].x = fmaf(v[k][i].x, e, acc[i].x);
                 acc[i].y = fmaf(v[k][i].y, e, acc[i].y);
             }
         }
-    }
-    __device__ __forceinline__ void add_full(const PagedArgs& A, bool prefix, size_t id, int warp) {
-        if (warp != 0) return;
-        id += (size_t)prefix * A.n_tokens * A.nh;
-        const float* const o[1] = {A.full_o + id * A.hd};
-        const float* const ml[1] = {A.full_ml + id * 2};
-        add<1>(A, o, ml, 1);
     }
     __device__ __forceinline__ void add_range(const PagedArgs& A, const PagedPlan& P, int first,
                                               int last, int head_lane, int row, int warp,
@@ -574,11 +570,11 @@ struct Joined {
         }
     }
     // All warps of the block: a row's warps (consecutive ones) hand their sums to the first.
-    __device__ __forceinline__ void meet(JoinShared& S, int warp, int warps) {
+    __device__ __forceinline__ void meet(JoinShared<VECS>& S, int warp, int warps) {
         if (warps == 1) return;
         const int lane = threadIdx.x & 31, me = threadIdx.x / 32;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S.acc[me][i * 32 + lane] = acc[i];
+        for (int i = 0; i < VECS; ++i) S.acc[me][i * 32 + lane] = acc[i];
         if (lane == 0) {
             S.m[me] = M;
             S.l[me] = L;
@@ -591,7 +587,7 @@ struct Joined {
             const float e = ex2(m - (M == -INFINITY ? 0.f : M));
             L = fmaf(S.l[w], e, L);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VECS; ++i) {
                 const float2 v = S.acc[w][i * 32 + lane];
                 acc[i].x = fmaf(v.x, e, acc[i].x);
                 acc[i].y = fmaf(v.y, e, acc[i].y);
@@ -608,9 +604,9 @@ struct Joined {
         const int sinks = A.window > 0 ? A.sinks : 0;
         const int lo = A.window > 0 ? max(0, pos - A.window + 1) : 0;
         const size_t at = (size_t)t * A.q_stride + (size_t)h * A.hd;
-        float2 q[4];
+        float2 q[VECS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < VECS; ++i) {
             const int d = (i * 32 + lane) * 2;
             q[i] = make_float2(0.f, 0.f);
             if (d >= A.hd) continue;
@@ -626,9 +622,9 @@ struct Joined {
             const size_t row = (size_t)page * A.page_stride +
                                ((size_t)(j - p * A.page_size) * A.nkv + kvh) * A.hd;
             float dot = 0.f;
-            float2 v[4];
+            float2 v[VECS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VECS; ++i) {
                 const int d = (i * 32 + lane) * 2;
                 v[i] = make_float2(0.f, 0.f);
                 if (d >= A.hd) continue;
@@ -645,7 +641,7 @@ struct Joined {
             const float e = ex2(x - (M == -INFINITY ? 0.f : M));
             L += e;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VECS; ++i) {
                 acc[i].x = fmaf(v[i].x, e, acc[i].x);
                 acc[i].y = fmaf(v[i].y, e, acc[i].y);
             }
@@ -656,7 +652,7 @@ struct Joined {
         const int lane = threadIdx.x & 31;
         const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < VECS; ++i) {
             const int d = (i * 32 + lane) * 2;
             if (d >= A.hd) break;
             const size_t at = (size_t)t * A.out_stride + (size_t)h * A.hd + d;

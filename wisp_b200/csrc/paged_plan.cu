@@ -45,7 +45,7 @@ __device__ int block_scan(int v, int* total, int* warp_sums) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PagedArgs A) {
-    __shared__ int sums[32];
+    __shared__ int sums[32], s_off[kPlanThreads];  // (item_off of the first segments)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const bool prefix = blockIdx.x == PLAN_PREFIX;
@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         }
         const int at = carry + block_scan(n, &total, sums);
         if (i < n_seg) P.item_off[i] = at;
+        if (base == 0) s_off[tid] = at;
         carry += total;
     }
     const int n_items = min(carry, P.max_items);
@@ -73,11 +74,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         *P.n_items = n_items;
     }
     __syncthreads();
+    const int* off = n_seg <= kPlanThreads ? s_off : P.item_off;
     auto segment_of = [&](int i) {  // the last segment with item_off <= i
         int lo = 0, hi = n_seg;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (P.item_off[mid] <= i) lo = mid;
+            if (off[mid] <= i) lo = mid;
             else hi = mid;
         }
         return lo;
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     if (prefix) {  // a group's row tile has many sequences: a warp each
         for (int i = tid / 32; i < n_items; i += kPlanThreads / 32) {
             const int seg = segment_of(i);
-            const PagedItem it = make_item<true>(A, P, true, seg, i - P.item_off[seg]);
+            const PagedItem it = make_item<true>(A, P, true, seg, i - off[seg]);
             if (tid % 32 == 0) P.items[i] = it;
         }
         __syncthreads();
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
                 it = P.items[i];
             } else {
                 const int seg = segment_of(i);
-                it = make_item(A, P, false, seg, i - P.item_off[seg]);
+                it = make_item(A, P, false, seg, i - off[seg]);
             }
             tiles = item_units(P, it.n_tiles);
             if (!prefix) P.items[i] = it;
