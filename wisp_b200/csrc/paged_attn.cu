@@ -477,8 +477,10 @@ paged_join_kernel(const __grid_constant__ PagedArgs A, int which) {
         J.template write<T, SPLIT>(A, sp.tok0 + row / at.gpb, at.h0 + row % at.gpb);
 }
 
-// Items of many rows, mostly in two pieces: a thread takes four dims of kJoinRows rows, so that
-// the loads of all of them are in flight together whatever the head's size.
+// Items of many rows, mostly in two pieces: a thread takes four dims of two rows and two pieces at a
+// time, so that all lanes load whatever the head's size.  Measured (B200): ragged chunks of 7652
+// tokens, 16 heads of 64, 121 us a call against 133 us with a warp per row and four pieces in
+// flight (80 registers, eight rows a CTA); four rows or four pieces at a time 124 to 125 us.
 constexpr int kJoinRows = 2, kJoinBatch = 2;
 template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(kJoinThreads)
@@ -561,6 +563,8 @@ paged_join_rows_kernel(const __grid_constant__ PagedArgs A, int which) {
 
 // Prefix mode: CTA (token, two of its heads), over the records of the shared prefix and of the
 // sequence's own part: pieces, or one whole record.
+// (Both parts' records in one batch of loads: 64 sequences behind 32768 and 16384 positions 102 us a
+// call, one part after the other with room for 256 dims 107 us.)
 template <typename T, bool SPLIT, int VECS>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join2_kernel(const __grid_constant__ PagedArgs A) {

@@ -13,10 +13,11 @@
 // Measured (B200): 64 sequences with a window of 4096 and four sinks, 32 heads of 128 over 8 kv
 // heads, 175 us = 6.1 TB/s (95% of the measured copy); 14 ragged sequences of up to 4096 positions
 // 31 us (61%: starting, the tables' and the first tiles' latency and the join are 10 us of it);
-// one sequence of 1024 12 us.  Before: each warp kept all dims for its own positions (64 accumulators a thread, a join of four
-// 16 x head_dim tiles and an empty ring at the end of every row tile: 39.7 us for 14 ragged
-// sequences of up to 4096 positions); the same split with cp.async issued by the working warps
-// (486 instructions a warp and tile: 35.7 us, but long windows fell from 6.4 to 5.6 TB/s).
+// one sequence of 1024 12 us.  Before: each warp kept all dims for its own positions (64
+// accumulators a thread, a join of four 16 x head_dim tiles and an empty ring at the end of every
+// row tile: 39.7 us for 14 ragged sequences of up to 4096 positions); the same split with cp.async
+// issued by the working warps (486 instructions a warp and tile: 35.7 us, but long windows fell
+// from 6.4 to 5.6 TB/s).
 //
 // 32-bit rows are split into 16-bit parts (two in fp16, 22 bits, three in bf16) that share the
 // 16 rows of a fragment, 8 rows each; their sums meet in one thread.  The weights are split the
@@ -103,6 +104,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     }
     // Behind the shared prefixes' kernel of this call, which has waited for all that is read here,
     // the SMs that it leaves start on this one: only the end waits for it (for the join's sake).
+    // (64 sequences behind two long prefixes: 98 us a call, 102 us with the wait here.)
     auto wait_before = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
     if (!behind) wait_before();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
