@@ -367,11 +367,14 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
 // ------------------------------------------------------------------------
 // Attention: what runs, and its workspace
 // ------------------------------------------------------------------------
-// What a row tile costs before its first KV tile, in KV tiles.
+// What a row tile costs before its first KV tile, in KV tiles (a prompt of 8192 tokens took 816 us
+// with 0 and 694 us with 4; 14 single tokens behind up to 4096 positions 32.6 us with 0 and 30.9 us
+// with 2).
 constexpr int kLeadMma = 4, kLeadFew = 2;
-
-constexpr int kFewTiles = 4;
-constexpr double kFewBytes = 48e6;
+// Up to so many 16-row tiles stay with paged_few_kernel, where all that they read again (for wide
+// heads: all that the tables can name) is at most so large.
+constexpr int kFewTiles = 4, kFewTilesWide = 8;
+constexpr double kFewBytes = 50e6, kFewBytesWide = 100e6;
 
 struct AttnShape {
     int rw[PLANS];  // 16-row tiles of the plan's row tiles; 0: the tensor-core kernel
@@ -385,9 +388,16 @@ struct AttnShape {
 // rows go to tcgen05 where it takes the head dim, else to paged_attn_kernel's row tiles of two
 // or four 16-row tiles.  A batch goes by its longest sequence: single tokens beside a prompt
 // take its kernel too (they read the cache at 80% of HBM there instead of 95%; a second pair of
-// launches for them cost 12 us a call).  Up to kFewTiles 16-row tiles stay with paged_few_kernel
-// where all that the tables can name stays in L2: it needs no plan kernel before it, and reads
-// the cache again from there.
+// launches for them cost 12 us a call).  A few 16-row tiles stay with paged_few_kernel where they are
+// few enough to read the cache again out of L2: it needs no plan kernel before it.  Measured
+// (B200, 8 kv heads; paged_few_kernel against the other):
+//   128 dims, 4 sequences of 1024: 32 rows 19.6 and 22.2 us, 64 rows 25.0 and 20.4 us
+//             2 of 4096: 32 rows 23.2 and 23.1 us, 64 rows 31.1 and 24.5 us
+//             8 of 8192: 32 rows 98 and 67 us
+//     64 rows behind a shared prefix of 2048: 27.5 and 31.4 us, of 8192: 50.2 and 36.9 us
+//   256 dims, 4 of 1024: 32 rows 24.0 and 31.2 us, 128 rows 51 and 59 us
+//             2 of 4096: 32 rows 30.7 and 38.5 us, 128 rows 80 and 92 us
+//             8 of 8192: 32 rows 170 and 153 us, 128 rows 624 and 437 us
 AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     const int per = split ? 8 : 16;
@@ -413,9 +423,11 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         const int most_tokens = w == PLAN_PREFIX ? A.n_tokens : max_q;
         const long long tiles16 = (long long)((A.group + per - 1) / per) *
                                   ((tokens + few_tok - 1) / few_tok);
-        // no more than this lies behind the segments' table rows: row tiles read it again out of L2
-        const bool in_l2 = n_seg * row_bytes <= kFewBytes;
-        const bool is_few = (long long)tokens * A.group <= per || (tiles16 <= kFewTiles && in_l2);
+        const double bytes = n_seg * row_bytes;  // no more lies behind the segments' table rows
+        const bool is_few =
+            (long long)tokens * A.group <= per ||
+            (mma ? tiles16 <= kFewTiles && tiles16 * bytes <= kFewBytes
+                 : tiles16 <= kFewTilesWide && bytes <= kFewBytesWide);
         const bool on_mma = !is_few && mma;
         if (w != PLAN_PREFIX && on_mma != (w == PLAN_MANY)) continue;
         P.used = 1;

@@ -662,7 +662,9 @@ cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
 
 int paged_attn_tile() { return kTile; }
 
-// 16-row MMA tiles of a row tile with `rows` rows.
+// 16-row MMA tiles of a row tile with `rows` rows: two take half the registers and the sums, four
+// read the cache half as often.  Measured (B200, 8 sequences of 8192, 8 kv heads of 256): 32 rows
+// 153 us with two and 235 us with four, 64 rows 272 and 246 us, 128 rows 512 and 437 us.
 int paged_attn_rw(int rows, bool split) { return rows <= (split ? 16 : 32) ? 2 : 4; }
 
 // CTAs of one SM: what the ring leaves room for.
