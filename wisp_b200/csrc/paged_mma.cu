@@ -30,15 +30,18 @@
 // sees one, the row tile is marked and the join kernel works it out again without tiles.
 //
 // Measured (B200): a prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 550 us = 1.0 PFLOP/s
-// of the visible pairs (59% of the measured bf16 rate), tensor pipe 60% and exponential unit 60%
-// busy at 1.6 GHz under the power limit; four drafted tokens behind 64K to 128K positions, 64
+// of the visible pairs (59% of the measured bf16 rate), tensor pipe and exponential unit 55% busy
+// each at 1.67 GHz under the power limit; chunks of 7652 tokens behind up to 9000 positions, 16 heads
+// of 64, window 1024, 121 us; four drafted tokens behind 64K to 128K positions, 64
 // heads, 300 us = 6.0 TB/s (93% of the measured copy).  Steps of the prompt: mma.sync row tiles
 // of 64 rows 4.57 ms; this kernel with one thread issuing all products 1.15 ms (it was bound by
 // 80 to 115 cycles an instruction); a warp per row tile with warp-uniform operands 816 us; pieces
 // that count what beginning a row tile costs 694 us; Q by TMA behind the last product 551 us.
 // Measured and not kept: Q double buffered with a ring of three KV tiles (817 us), registers moved
 // to the softmax warps (no gain), one softmax warp of a pair waiting for the other's exponentials
-// (no gain), skipping hidden tiles warp by warp inside the loop (prompts 10% slower).
+// (no gain), skipping hidden tiles warp by warp inside the loop (prompts 10% slower), a quarter to
+// a half of the exponentials as polynomials (no gain; with five eighths 8% slower), deciding per
+// 128 rows what is hidden (chunks 3% faster, prompts 2 to 5% slower).
 //
 // TMEM (512 columns): S buffers of 64 columns, P over them (or beside them when it has several
 // parts), O of head_dim columns per row tile.  Every wait is bounded; on a timeout all roles
