@@ -241,6 +241,12 @@ __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bo
         it.alone = gr < 0;
         if (prefix) it.kv_hi = min(reach, pl);
         else it.kv_lo = min(reach, pl);
+        if (it.mixed && A.window == 0 && it.kv_hi <= it.pmin + 1) {
+            // every row sees the whole prefix: any positions from pmin on say so (looking each
+            // token's up is a search and two loads behind one another)
+            it.mixed = 0;
+            it.pos0 = it.pmin;
+        }
     }
     const int end = min(it.kv_hi, it.pmax + 1), begin = it.kv_lo;
     const int wlo = A.window > 0 ? max(begin, it.pmin - A.window + 1) : begin;
