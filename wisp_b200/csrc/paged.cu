@@ -446,8 +446,8 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.lead = on_mma ? kLeadMma : kLeadFew;
         P.lanes = std::min(4095, std::max(1, ctas / P.heads));
         if (is_few && w == PLAN_PREFIX && A.plan[PLAN_FEW].used) {  // they share one launch
-            A.plan[PLAN_FEW].lanes = (A.plan[PLAN_FEW].lanes + 1) / 2;
-            P.lanes = (P.lanes + 1) / 2;
+            A.plan[PLAN_FEW].lanes = std::max(1, A.plan[PLAN_FEW].lanes / 2);
+            P.lanes = std::max(1, P.lanes / 2);
         }
         P.max_items = A.n_tokens / P.tpt + n_seg;
         P.per_seg = (most_tokens + P.tpt - 1) / P.tpt;

@@ -72,7 +72,7 @@ struct PagedPlan {
 };
 
 // Row tiles that an attention CTA counts by itself.
-constexpr int kPagedInline = 512;
+constexpr int kPagedInline = 160;
 
 enum { PLAN_FEW = 0, PLAN_PREFIX = 1, PLAN_MANY = 2, PLANS = 3 };
 

@@ -41,12 +41,14 @@ namespace {
 constexpr int kWork = 128;             // working threads
 constexpr int kThreads = kWork + 32;  // and the loading warp
 constexpr int kTile = 64;
-constexpr int kRecs = 32;
+constexpr long long kPrefetchTable = 65536;  // entries of the page table
+constexpr int kRecs = 16;
+static_assert(kPagedInline <= kThreads, "a thread per row tile");
 
 template <typename T, bool SPLIT, int HD>
 struct FCfg {
     static constexpr int kF = SPLIT ? PMath<T>::kFrags : 1;  // 16-row fragments of a row's parts
-    static constexpr int kStages = HD == 64 ? 4 : HD == 128 && kF == 1 ? 3 : 2;
+    static constexpr int kStages = HD == 64 ? (kF == 1 ? 4 : 3) : HD == 128 && kF == 1 ? 3 : 2;
     static constexpr int kCtas = HD == 64 ? 3 : HD == 128 ? 2 : 1;
     static constexpr int kHalves = HD / 64;
     static constexpr int kTen = kTile * HD * 2;      // bytes of a K or V tile
@@ -54,6 +56,8 @@ struct FCfg {
     // converted q (fp32 rows only) or the tile's weights, elements
     static constexpr int kBuf = std::max(kF * 16 * kTile, SPLIT ? kF * 16 * HD : 0);
     static constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kTen + 2 * kQBytes + kBuf * 2;
+    // (4 KB for what is declared in the kernel, 1 KB of the system's for each CTA of the SM's 228)
+    static_assert((kSmem + 4096 + 1024) * kCtas <= 228 * 1024, "kCtas do not fit");
 };
 
 struct Rec {  // a row tile of this piece and its KV tiles [a, b); b < 0: there are no more
@@ -61,6 +65,26 @@ struct Rec {  // a row tile of this piece and its KV tiles [a, b); b < 0: there 
     int a, b;
     int item, c0;
 };
+__device__ __forceinline__ Rec make_rec(const PagedPlan& P, const PagedItem& it, int item, int cum,
+                                        int x0, int x_end) {
+    const int c0 = cum + P.lead;
+    return Rec{it, max(0, x0 - c0), max(0, min(it.n_tiles, x_end - c0)), item, c0};
+}
+
+// What every CTA's plan and page look-ups read, into L2 while the kernel before this one runs (small
+// tables only: each thread of the grid takes a line of 128 bytes).
+__device__ __forceinline__ void prefetch_batch(const PagedArgs& A) {
+    auto fetch = [](const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); };
+    const int tid = threadIdx.x;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid * 32 <= A.n_seq) {
+        fetch(A.q_start + tid * 32);
+        if (tid * 32 < A.n_seq) fetch(A.kv_len + tid * 32);
+    }
+    const long long at = ((long long)blockIdx.x * kThreads + tid) * 32;
+    if (blockIdx.y == 0 && at < kPrefetchTable &&
+        at < (long long)(A.n_seq - 1) * A.table_stride + A.table_width)
+        fetch(A.table + at);
+}
 
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -80,7 +104,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     __shared__ volatile int s_abort;
     __shared__ Rec s_rec[kRecs], s_cur[2];
     __shared__ int s_cum[kPagedInline + 1];
-    __shared__ int s_sum[kThreads / 32], s_bad, s_pos[16];
+    __shared__ int s_sum[kThreads / 32], s_bad, s_item0, s_pos[16];
     __shared__ float s_fac[16], s_max[4][16], s_l[4][16];
     const int which = blockIdx.y ? PLAN_PREFIX : which0;
     const PagedPlan& P = A.plan[which];
@@ -106,7 +130,10 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     // the SMs that it leaves start on this one: only the end waits for it (for the join's sake).
     // (64 sequences behind two long prefixes: 98 us a call, 102 us with the wait here.)
     auto wait_before = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
-    if (!behind) wait_before();
+    if (!behind) {
+        prefetch_batch(A);
+        wait_before();
+    }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const bool inlined = P.inlined != 0, prefix = which == PLAN_PREFIX;
@@ -117,56 +144,62 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         if (inlined && blockIdx.x == 0) P.bad[P.lanes * P.heads] = 0;
     }
     const int n_items = inlined ? (prefix ? A.n_groups : A.n_seq) * P.per_seg : *P.n_items;
-    auto inline_item = [&](int i) { return make_item(A, P, prefix, i / P.per_seg, i % P.per_seg); };
     if (n_items == 0) {
         if (behind) wait_before();
         return;
     }
     const int* cum = inlined ? s_cum : P.cum;
+    PagedItem mine;
+    int units = 0, before = 0, total = 0;
     if (inlined) {
-        // few row tiles: every CTA counts the units itself, which is shorter than a kernel of its
-        // own before this one
+        // few row tiles: every CTA counts the units itself, a thread per row tile, which is shorter
+        // than a kernel of its own before this one
+        if (tid < kRecs) s_rec[tid].a = 0, s_rec[tid].b = -1;
         __syncthreads();  // the words above are cleared
-        int carry = 0;
-        for (int base = 0; base < n_items; base += kThreads) {
-            const int i = base + tid;
-            int n = 0;
-            if (i < n_items) {
-                n = item_units(P, inline_item(i).n_tiles);
-                if (blockIdx.x == 0 && !prefix && i % P.per_seg == 0) {
-                    const int s = i / P.per_seg, t = A.q_start[s + 1] - A.q_start[s];
-                    if (length_too_long(A, s) || t > P.tpt * P.per_seg)
-                        P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
-                }
+        if (tid < n_items) {
+            mine = make_item(A, P, prefix, tid / P.per_seg, tid % P.per_seg);
+            units = item_units(P, mine.n_tiles);
+            if (blockIdx.x == 0 && !prefix && tid % P.per_seg == 0) {
+                const int s = tid / P.per_seg, t = A.q_start[s + 1] - A.q_start[s];
+                if (length_too_long(A, s) || t > P.tpt * P.per_seg)
+                    P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
             }
-            int v = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += y;
-            }
-            if (lane == 31) s_sum[warp] = v;
-            __syncthreads();
-            int before = carry;
-#pragma unroll
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) before += s_sum[w];
-                carry += s_sum[w];
-            }
-            if (i < n_items) s_cum[i] = before + v - n;
-            __syncthreads();
         }
-        if (tid == 0) s_cum[n_items] = carry;
+        int v = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += y;
+        }
+        if (lane == 31) s_sum[warp] = v;
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) before += s_sum[w];
+            total += s_sum[w];
+        }
+        before += v - units;
+        if (tid < n_items) s_cum[tid] = before;
+        if (tid == 0) s_cum[n_items] = total;
+    } else {
+        total = P.cum[n_items];
     }
-    const int total = cum[n_items];
     const Pieces pieces(P, max(total, 1));
     if (total == 0 || piece >= pieces.n) {
         if (behind) wait_before();
         return;
     }
     const int x0 = pieces.start(piece), x_end = pieces.start(piece + 1);
-    const int item0 = block_last_le(cum, n_items, x0);
+    int item0;
+    if (inlined) {  // the first records of this piece are at hand
+        if (before <= x0 && x0 < before + units) s_item0 = tid;
+        __syncthreads();
+        item0 = s_item0;
+        if (tid >= item0 && tid < item0 + kRecs && tid < n_items && before < x_end)
+            s_rec[tid - item0] = make_rec(P, mine, tid, before, x0, x_end);
+    } else {
+        item0 = block_last_le(cum, n_items, x0);
+    }
 
     __syncthreads();  // the barriers are there (a plan that is not inlined had no barrier yet)
     const int sinks = A.window > 0 ? A.sinks : 0;
@@ -208,19 +241,18 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             return true;
         };
         for (int k = 0; ok; ++k) {
-            if (k % kRecs == 0) {  // the next records, one a lane
+            if (k % kRecs == 0 && !(inlined && k == 0)) {  // the next records, one a lane
                 __syncwarp();
-                Rec r;
-                r.a = 0;
-                r.b = -1;
-                r.item = item0 + k + lane;
-                if (r.item < n_items && cum[r.item] < x_end) {
-                    r.it = inlined ? inline_item(r.item) : P.items[r.item];
-                    r.c0 = cum[r.item] + P.lead;
-                    r.a = max(0, x0 - r.c0);
-                    r.b = max(0, min(r.it.n_tiles, x_end - r.c0));
+                const int i = item0 + k + lane;
+                if (lane < kRecs) {
+                    s_rec[lane].a = 0;
+                    s_rec[lane].b = -1;
+                    if (i < n_items && cum[i] < x_end)
+                        s_rec[lane] =
+                            make_rec(P, inlined ? make_item(A, P, prefix, i / P.per_seg, i % P.per_seg)
+                                                : P.items[i],
+                                     i, cum[i], x0, x_end);
                 }
-                s_rec[lane] = r;
                 __syncwarp();
             }
             const Rec& r = s_rec[k % kRecs];
