@@ -19,17 +19,14 @@ namespace wb {
 cudaError_t launch_paged_plan(const PagedArgs& A, cudaStream_t s);
 cudaError_t launch_paged_few(const PagedArgs& A, int which, bool both, bool behind, int q_dtype,
                              int kv_dtype, cudaStream_t s);
-int paged_few_tile();
 int paged_few_ctas(int hd);
 cudaError_t launch_paged_attn(const PagedArgs& A, int which, int rw, int q_dtype, int kv_dtype,
                               cudaStream_t s);
 cudaError_t launch_paged_mma(const PagedArgs& A, int which, int q_dtype, int kv_dtype,
                              cudaStream_t s);
 bool paged_mma_takes(int hd);
-int paged_mma_tile();
 int paged_mma_rows(bool split);
 cudaError_t launch_paged_join(const PagedArgs& A, int q_dtype, int kv_dtype, cudaStream_t s);
-int paged_attn_tile();
 int paged_attn_rw(int rows, bool split);
 int paged_attn_ctas();
 
@@ -437,7 +434,6 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.heads = A.nkv * P.hblocks;
         const int rows = (int)std::min<long long>((long long)tokens * P.gpb, most);
         S.rw[w] = on_mma ? 0 : is_few ? 1 : paged_attn_rw(rows, split);
-        P.tile = on_mma ? paged_mma_tile() : is_few ? paged_few_tile() : paged_attn_tile();
         P.rows = on_mma ? most : S.rw[w] * per;
         P.tpt = std::max(1, P.rows / P.gpb);
         P.used_rows = w == PLAN_PREFIX ? P.rows : std::min(rows, P.rows);

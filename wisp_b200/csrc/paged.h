@@ -14,7 +14,7 @@ namespace wb {
 enum { PG_BAD_PAGE = 1, PG_BAD_LENGTH = 2, PG_TIMEOUT = 8 };
 
 // One row tile: consecutive tokens whose rows (token, query head of the kv head) go through
-// the same cached positions.  Positions come in tiles of `tile` from 0: the item's list is
+// the same cached positions.  Positions come in tiles of kPagedTile from 0: the item's list is
 // [sink0, sink0 + n_sink) and then n_tiles - n_sink tiles from `first` on.
 struct PagedItem {
     int tok0, ntok;    // tokens
@@ -57,7 +57,6 @@ struct PagedPlan {
     PagedSplit* split;  // [lanes]
     PagedWhere* where;  // prefix mode: [n_tokens]
     int* redo;          // [max_items][heads], set for items to be worked out without tiles
-    int tile;           // positions of a KV tile
     int lead;
     int tpt;            // tokens of a row tile
     int rows;           // rows of a row tile
@@ -70,6 +69,8 @@ struct PagedPlan {
                            // the attention CTAs find cum themselves
     int used;              // the call has this plan
 };
+
+constexpr int kPagedTile = 64;  // positions of a KV tile
 
 // Row tiles that an attention CTA counts by itself.
 constexpr int kPagedInline = 160;

@@ -35,7 +35,7 @@ namespace wb {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kTile = 64;  // positions of a KV tile
+constexpr int kTile = kPagedTile;  // positions of a KV tile
 
 constexpr int HD = 256;   // dims in shared memory; narrower heads are filled up with zeros
 constexpr int kStages = 2;
@@ -659,8 +659,6 @@ cudaError_t launch_join(const PagedArgs& A, cudaStream_t s) {
 }
 
 }  // namespace
-
-int paged_attn_tile() { return kTile; }
 
 // 16-row MMA tiles of a row tile with `rows` rows: two take half the registers and the sums, four
 // read the cache half as often.  Measured (B200, 8 sequences of 8192, 8 kv heads of 256): 32 rows

@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kWork = 128;             // working threads
 constexpr int kThreads = kWork + 32;  // and the loading warp
-constexpr int kTile = 64;
+constexpr int kTile = kPagedTile;
 constexpr long long kPrefetchTable = 65536;  // entries of the page table
 constexpr int kRecs = 16;
 static_assert(kPagedInline <= kThreads, "a thread per row tile");
@@ -157,11 +157,12 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         if (tid < kRecs) s_rec[tid].a = 0, s_rec[tid].b = -1;
         __syncthreads();  // the words above are cleared
         if (tid < n_items) {
-            mine = make_item(A, P, prefix, tid / P.per_seg, tid % P.per_seg);
+            const int seg = P.per_seg == 1 ? tid : tid / P.per_seg;
+            mine = make_item(A, P, prefix, seg, tid - seg * P.per_seg);
             units = item_units(P, mine.n_tiles);
-            if (blockIdx.x == 0 && !prefix && tid % P.per_seg == 0) {
-                const int s = tid / P.per_seg, t = A.q_start[s + 1] - A.q_start[s];
-                if (length_too_long(A, s) || t > P.tpt * P.per_seg)
+            if (blockIdx.x == 0 && !prefix && tid == seg * P.per_seg) {
+                const int t = A.q_start[seg + 1] - A.q_start[seg];
+                if (length_too_long(A, seg) || t > P.tpt * P.per_seg)
                     P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
             }
         }
@@ -587,7 +588,6 @@ cudaError_t launch_t(const PagedArgs& A, int which, bool both, bool behind, cuda
 
 }  // namespace
 
-int paged_few_tile() { return kTile; }
 int paged_few_ctas(int hd) {
     return hd <= 64 ? FCfg<__half, false, 64>::kCtas : hd <= 128 ? FCfg<__half, false, 128>::kCtas : 1;
 }

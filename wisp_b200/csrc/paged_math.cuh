@@ -251,15 +251,15 @@ __device__ inline PagedItem make_item(const PagedArgs& A, const PagedPlan& P, bo
     const int end = min(it.kv_hi, it.pmax + 1), begin = it.kv_lo;
     const int wlo = A.window > 0 ? max(begin, it.pmin - A.window + 1) : begin;
     it.sink0 = it.n_sink = 0;
-    it.first = begin / P.tile;
+    it.first = begin / kPagedTile;
     it.n_tiles = 1;
     if (end > begin) {
-        const int last = (end + P.tile - 1) / P.tile;  // exclusive
-        int f = min(wlo, end - 1) / P.tile;
+        const int last = (end + kPagedTile - 1) / kPagedTile;  // exclusive
+        int f = min(wlo, end - 1) / kPagedTile;
         const int send = min(A.window > 0 ? A.sinks : 0, end);
         if (send > begin) {
-            it.sink0 = begin / P.tile;
-            const int se = (send + P.tile - 1) / P.tile;
+            it.sink0 = begin / kPagedTile;
+            const int se = (send + kPagedTile - 1) / kPagedTile;
             if (se >= f) f = it.sink0;  // they meet: one list
             else it.n_sink = se - it.sink0;
         }

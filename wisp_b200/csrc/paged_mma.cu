@@ -60,7 +60,7 @@
 namespace wb {
 namespace {
 
-constexpr int kN = 64;          // positions of a KV tile
+constexpr int kN = kPagedTile;          // positions of a KV tile
 constexpr int kM = 128;         // rows of a row tile
 constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kRowWarp = 11;
@@ -933,7 +933,6 @@ cudaError_t launch_hd(const PagedArgs& A, int which, cudaStream_t s) {
 
 // Head dims that the tensor-core kernel takes: one or two boxes of 64, the last possibly cut.
 bool paged_mma_takes(int hd) { return hd <= 128; }
-int paged_mma_tile() { return kN; }
 int paged_mma_rows(bool split) { return split ? kM : 2 * kM; }
 
 cudaError_t launch_paged_mma(const PagedArgs& A, int which, int q_dtype, int kv_dtype,
