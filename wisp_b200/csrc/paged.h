@@ -43,9 +43,10 @@ struct PagedWhere {
 };
 
 // A plan covers the row tiles of one kind.  On the line of their work an item is `lead` units
-// (what it costs to begin one, in KV tiles) and its KV tiles; cum[i] units lie before item i.
-// The line is cut into at most `lanes` equal pieces; one CTA takes a piece for one block of
-// query heads.
+// (what it costs to begin one) and its KV tiles of `grain` units each (one unit where items of at
+// most kPagedHalf rows cost half); cum[i] units lie before item i.  The line is cut into at most
+// `lanes` equal pieces of at least `grain` units; a KV tile belongs to the piece that its first
+// unit lies in.  One CTA takes a piece for one block of query heads.
 struct PagedPlan {
     int* n_items;
     int* bad;       // [lanes * heads + 1] status bits of each CTA, then of the plan
@@ -57,7 +58,7 @@ struct PagedPlan {
     PagedSplit* split;  // [lanes]
     PagedWhere* where;  // prefix mode: [n_tokens]
     int* redo;          // [max_items][heads], set for items to be worked out without tiles
-    int lead;
+    int lead, grain;
     int tpt;            // tokens of a row tile
     int rows;           // rows of a row tile
     int used_rows;      // of them at most so many are used
@@ -71,6 +72,8 @@ struct PagedPlan {
 };
 
 constexpr int kPagedTile = 64;  // positions of a KV tile
+// Rows up to which both of the tensor-core kernel's row tiles work on one item.
+constexpr int kPagedHalf = 128;
 
 // Row tiles that an attention CTA counts by itself.
 constexpr int kPagedInline = 160;

@@ -159,7 +159,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         if (tid < n_items) {
             const int seg = P.per_seg == 1 ? tid : tid / P.per_seg;
             mine = make_item(A, P, prefix, seg, tid - seg * P.per_seg);
-            units = item_units(P, mine.n_tiles);
+            units = item_units(P, mine);
             if (blockIdx.x == 0 && !prefix && tid == seg * P.per_seg) {
                 const int t = A.q_start[seg + 1] - A.q_start[seg];
                 if (length_too_long(A, seg) || t > P.tpt * P.per_seg)

@@ -407,8 +407,12 @@ __device__ __forceinline__ void gather_status(const PagedArgs& A) {
     if (threadIdx.x == 0) *A.status = any | len | late;
 }
 
-__device__ __forceinline__ int item_units(const PagedPlan& P, int tiles) {
-    return tiles ? tiles + P.lead : 0;
+// A KV tile of the item is 2^item_shift units.
+__device__ __forceinline__ int item_shift(const PagedPlan& P, const PagedItem& it) {
+    return P.grain > 1 && it.ntok * P.gpb > kPagedHalf;
+}
+__device__ __forceinline__ int item_units(const PagedPlan& P, const PagedItem& it) {
+    return it.n_tiles ? (it.n_tiles << item_shift(P, it)) + P.lead : 0;
 }
 
 // The last i in [0, n) with cum[i] <= x (cum[0] <= x), by the whole block.
@@ -428,7 +432,9 @@ __device__ __forceinline__ int block_last_le(const int* cum, int n, int x) {
 // Piece p starts at unit start(p); unit x lies in piece of(x).
 struct Pieces {
     int total, n;
-    __device__ Pieces(const PagedPlan& P, int total_) : total(total_), n(min(P.lanes, total_)) {}
+    __device__ Pieces(const PagedPlan& P, int total_) : total(total_) {
+        n = min(P.lanes, P.grain > 1 ? max(total_ / P.grain, 1) : total_);
+    }
     __device__ __forceinline__ int start(int p) const {
         if (total <= 1 << 20) return (int)((unsigned)p * (unsigned)total / (unsigned)n);
         return (int)((unsigned long long)p * total / n);

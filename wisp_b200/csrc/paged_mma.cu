@@ -61,7 +61,7 @@ namespace wb {
 namespace {
 
 constexpr int kN = kPagedTile;          // positions of a KV tile
-constexpr int kM = 128;         // rows of a row tile
+constexpr int kM = kPagedHalf;  // rows of a row tile
 constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kRowWarp = 11;
 
@@ -246,19 +246,25 @@ struct Walk {
     int item, x, x_end;
     int a, b;  // KV tiles [a, b) of the item
     int c0;    // the item's first KV tile on the line
+    int sh;    // its KV tiles are 2^sh units
     PagedItem it;
     __device__ __forceinline__ bool next(const PagedPlan& P) {
         while (x < x_end) {
             it = P.items[item];
             c0 = P.cum[item] + P.lead;
+            sh = item_shift(P, it);
             ++item;
             if (it.n_tiles == 0) continue;
-            a = max(0, x - c0);
-            b = min(it.n_tiles, x_end - c0);
-            x = c0 + max(b, 0);
-            return b > 0;  // (not: the piece ends before the item's first tile)
+            a = (max(0, x - c0) + sh) >> sh;
+            b = min(it.n_tiles, (max(0, x_end - c0) + sh) >> sh);
+            x = min(c0 + (it.n_tiles << sh), x_end);
+            if (a < b) return true;  // (else: the piece has none of the item's tiles)
         }
         return false;
+    }
+    // The piece of the item's last KV tile.
+    __device__ __forceinline__ static int last_piece(const Pieces& pieces, int c0, int sh, int n_tiles) {
+        return pieces.of(c0 + ((n_tiles - 1) << sh));
     }
     __device__ __forceinline__ int tile(int i) const {
         return i < it.n_sink ? it.sink0 + i : it.first + i - it.n_sink;
@@ -434,10 +440,14 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                     sp.item1 = max(sp.item0, last + 1);
                     if (last >= sp.item0 && P.cum[last + 1] > W.x_end && A.n_groups == 0) {
                         const PagedItem it = P.items[last];
-                        sp.tok0 = it.tok0;
-                        sp.n_rows = it.ntok * P.gpb;
-                        sp.last = pieces.of(P.cum[last + 1] - 1);
-                        sp.item = last;
+                        const int to = Walk::last_piece(pieces, P.cum[last] + P.lead,
+                                                        item_shift(P, it), it.n_tiles);
+                        if (to > piece) {
+                            sp.tok0 = it.tok0;
+                            sp.n_rows = it.ntok * P.gpb;
+                            sp.last = to;
+                            sp.item = last;
+                        }
                     }
                 }
                 P.split[piece] = sp;
@@ -828,7 +838,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                         make_float2(M, l);
             }
             if (A.n_groups > 0 && W.a == 0 && head_lane == 0 && real && tells && h == h0) {
-                const int last = Pieces(P, P.cum[*P.n_items]).of(W.c0 + it.n_tiles - 1);
+                const int last =
+                    Walk::last_piece(Pieces(P, P.cum[*P.n_items]), W.c0, W.sh, it.n_tiles);
                 P.where[tok] = PagedWhere{piece, last, row, it.alone, which, W.item - 1};
             }
             // 32 bytes of each row at a time through shared memory, so that two lanes write a row's

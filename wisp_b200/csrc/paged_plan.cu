@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     carry = 0;
     for (int base = 0; base < n_items; base += kPlanThreads) {
         const int i = base + tid;
-        int tiles = 0;
+        int units = 0;
         if (i < n_items) {
             PagedItem it;
             if (prefix) {
@@ -104,10 +104,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
                 const int seg = segment_of(i);
                 it = make_item(A, P, false, seg, i - off[seg]);
             }
-            tiles = item_units(P, it.n_tiles);
+            units = item_units(P, it);
             if (!prefix) P.items[i] = it;
         }
-        const int at = carry + block_scan(tiles, &total, sums);
+        const int at = carry + block_scan(units, &total, sums);
         if (i < n_items) P.cum[i] = at;
         carry += total;
     }
