@@ -75,8 +75,7 @@ struct MCfg {
     // dims it does not: a ring of three tiles cost more than Q's early loads gave)
     static constexpr int kQBufs = HD == 64 ? 2 : 1;
     static constexpr int kSlots = HD == 64 ? (PARTS == 3 ? 8 : 12) : PARTS == 3 ? 7 : 9;
-    static constexpr int kStage = 4 * kRT * 1024;  // 32 bytes of each row on their way out
-    static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot + kStage;
+    static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot;
     // TMEM columns
     static constexpr int kPCols = 32 * PARTS;
     static __host__ __device__ constexpr int s_col(int x, int b) { return (x * 2 + b) * 64; }
@@ -227,6 +226,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+
+// 32 bytes to a 32-byte boundary.
+__device__ __forceinline__ void store32(void* to, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 
 // The low n bits (none for n <= 0, all for n >= 64).
@@ -842,29 +848,20 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                     Walk::last_piece(Pieces(P, P.cum[*P.n_items]), W.c0, W.sh, it.n_tiles);
                 P.where[tok] = PagedWhere{piece, last, row, it.alone, which, W.item - 1};
             }
-            // 32 bytes of each row at a time through shared memory, so that two lanes write a row's
-            // whole sectors.  The 16-byte pieces are XORed with the row to keep both sides free of
-            // bank conflicts.
-            char* stage = sKV + kSlots * C::kSlot + warp * 1024;
+            // A lane writes whole sectors of its own row (32 bytes in one store: 3350 cycles an item
+            // of 256 rows of 128, 4850 through shared memory with two lanes to a sector).
             const bool halves = !SPLIT && last_word;
-            auto send = [&](int col, const uint32_t* w) {  // 8 words of this row from dim `col` on
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    *reinterpret_cast<uint4*>(stage + lane * 32 + ((c ^ ((lane >> 2) & 1)) * 16)) =
-                        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-                __syncwarp();
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int rr = k * 16 + lane / 2, c = lane & 1;
-                    char* to = reinterpret_cast<char*>(
-                        __shfl_sync(kAll, reinterpret_cast<unsigned long long>(dst), rr));
-                    const int d = col + c * (halves ? 8 : 4);
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 32 +
-                                                                    ((c ^ ((rr >> 2) & 1)) * 16));
-                    if (row0 + (warp & 3) * 32 + rr < n_rows && d < A.hd)
-                        *reinterpret_cast<uint4*>(to + d * (halves ? 2 : 4)) = v;
+            const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
+            auto send = [&](int d, const uint32_t* w) {  // 8 words of this row from dim d on
+                if (!real || d >= A.hd) return;
+                char* to = dst + d * (halves ? 2 : 4);
+                if (wide && d + (halves ? 16 : 8) <= A.hd) {
+                    store32(to, w);
+                } else {
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (!halves || d + 8 < A.hd)
+                        *reinterpret_cast<uint4*>(to + 16) = make_uint4(w[4], w[5], w[6], w[7]);
                 }
-                __syncwarp();
             };
 #pragma unroll 1
             for (int c = half ? x * (HD / 2) : 0; c < (half ? (x + 1) * (HD / 2) : HD); c += 32) {
