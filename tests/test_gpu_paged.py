@@ -352,6 +352,69 @@ def test_many_sequences(cuda, n):
     run(make([(1 + i % 20, 20 + 7 * i % 90) for i in range(n)], heads=(4, 2)))
 
 
+@pytest.mark.parametrize("n,heads", [(15, (160, 160)), (33, (160, 160)), (40, (160, 160)),
+                                     (159, (4, 2)), (160, (4, 2)), (161, (4, 2))])
+def test_many_short_sequences_in_one_piece(cuda, n, heads):
+    """With 160 kv heads a CTA takes half of the line: more row tiles than it holds records of at a
+    time; and about as many row tiles as a CTA counts by itself."""
+    run(make([(1, 1 + 13 * i % 150) for i in range(n)], heads=heads, dim=16))
+    run(make([(1, 13 * i % 150) for i in range(n)], heads=heads, dim=16), window=20, sinks=2)
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (2, 2), (4, 1), (12, 3)])
+@pytest.mark.parametrize("lens", [[(300, 300), (100, 900), (257, 700), (5, 3000)],
+                                  [(20, 4000), (129, 129), (128, 2000)],
+                                  [(257, 257)], [(33, 33), (600, 2500), (1, 1), (31, 5000)]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 5)])
+def test_row_tiles_of_full_and_half_size_on_one_line(cuda, heads, lens, window, sinks):
+    """Few heads: many short pieces, whose ends fall between and inside the row tiles."""
+    run(make(lens, heads=heads, dim=128, page=32), window=window, sinks=sinks)
+    run(make(lens, heads=heads, dim=64, cache=BF16, page=16), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dim", [64, 72, 128, 256])
+@pytest.mark.parametrize("n,tokens", [(3, 8), (4, 16), (2, 33)])
+def test_few_row_tiles_behind_small_and_large_tables(cuda, dim, n, tokens):
+    """Both sides of the choice between the kernels for few and for many rows."""
+    args = make([(tokens, 40 + 300 * i) for i in range(n)], heads=(8, 2), dim=dim)
+    run(args)
+    q, k, v, batch = args
+    wide = torch.zeros(n, 9000, dtype=torch.int32, device="cuda")
+    wide[:, :batch.table.shape[1]] = batch.table
+    run((q, k, v, paged.TokenBatch(batch.q_start, batch.kv_len, wide, batch.max_q)))
+
+
+@pytest.mark.parametrize("tokens,heads,dim", [(1, (2, 2), 128), (1, (1, 1), 256), (20, (16, 2), 128),
+                                              (20, (16, 2), 64), (5, (40, 2), 256)])
+@pytest.mark.parametrize("cache", [F16, BF16])
+def test_fp32_rows_keep_their_size_over_long_caches(cuda, tokens, heads, dim, cache):
+    """Sums that are cut off instead of rounded shrink with every instruction.  v = 1 + a small part:
+    all of a row's outputs are near one, and what they miss on average is the shrinking.  With 12
+    instructions (three parts of 64 positions) times four KV tiles a sum loses at most
+    48 * 2^-23, a score of size A 24 * 2^-23 A more in the exponent's unit."""
+    q, k, v, batch = make([(tokens, 12000)], heads=heads, dim=dim, page=64, cache=cache, dtype=F32)
+    v = (1 + v.double().nan_to_num() / 64).to(cache)
+    q = q * 0.01
+    want, _, A, _ = restate(q, k, v, batch)
+    got = paged.attention(q, k, v, batch).double()
+    assert A < 0.5
+    assert abs(((got - want) / want).mean().item()) < (48 + 24 * A) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (F16, 40), (F32, 64), (F16, 128)])
+def test_rows_that_leave_at_odd_places(cuda, dtype, dim):
+    """Outputs at 16 bytes past a 32-byte boundary."""
+    q, k, v, batch = make([(150, 200), (40, 700)], heads=(6, 2), dim=dim, dtype=dtype)
+    n, nh = q.shape[:2]
+    skip = 16 // q.element_size()
+    flat = torch.empty(n * nh * dim + 2 * skip, dtype=q.dtype, device="cuda")
+    out = flat[skip:skip + n * nh * dim].view(n, nh, dim)
+    assert out.data_ptr() % 32 == 16
+    got, lse = paged.attention(q, k, v, batch, return_lse=True, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check(out, lse, restate(q, k, v, batch), q.dtype, k.dtype)
+
+
 @pytest.mark.parametrize("heads", [(160, 160), (300, 150)])
 def test_more_heads_than_sms(cuda, heads):
     run(make([(1, 70), (1, 300)], heads=heads))

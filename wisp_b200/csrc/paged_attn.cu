@@ -328,11 +328,7 @@ paged_attn_kernel(const __grid_constant__ PagedArgs A, int which) {
                                 vf[2 * n + 1] = f.b1;
                             }
                         }
-#pragma unroll
-                        for (int n = 0; n < kF; ++n) {
-                            PMath<T>::mma(o[d], pf[n], vf[0], vf[1]);
-                            PMath<T>::mma(o[d + 1], pf[n], vf[2], vf[3]);
-                        }
+                        add_products<T, SPLIT, kF>(o[d], o[d + 1], pf, vf);
                     }
                 }
             };

@@ -11,9 +11,10 @@
 // then each warp adds all 64 weighted positions to a quarter of the head's dims.
 //
 // Measured (B200): 64 sequences with a window of 4096 and four sinks, 32 heads of 128 over 8 kv
-// heads, 175 us = 6.1 TB/s (95% of the measured copy); 14 ragged sequences of up to 4096 positions
-// 31 us (61%: starting, the tables' and the first tiles' latency and the join are 10 us of it);
-// one sequence of 1024 12 us.  Before: each warp kept all dims for its own positions (64
+// heads, 171 us = 6.3 TB/s (97% of the measured copy); 14 ragged sequences of up to 4096 positions
+// 30 us (63%: the first tile is there after 5 us, the join takes 4.5 us); one sequence of 1024
+// 10.6 us (11.9 us with the row tiles of a piece worked out twice and shared memory for one CTA
+// an SM where two were counted on).  Before: each warp kept all dims for its own positions (64
 // accumulators a thread, a join of four 16 x head_dim tiles and an empty ring at the end of every
 // row tile: 39.7 us for 14 ragged sequences of up to 4096 positions); the same split with cp.async
 // issued by the working warps (486 instructions a warp and tile: 35.7 us, but long windows fell
@@ -505,11 +506,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                             vf[2 * n + 1] = f.b1;
                         }
                     }
-#pragma unroll
-                    for (int n = 0; n < kF; ++n) {
-                        PMath<T>::mma(o[d], pf[n], vf[0], vf[1]);
-                        PMath<T>::mma(o[d + 1], pf[n], vf[2], vf[3]);
-                    }
+                    add_products<T, SPLIT, kF>(o[d], o[d + 1], pf, vf);
                 }
             }
         };

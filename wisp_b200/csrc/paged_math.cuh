@@ -154,6 +154,26 @@ __device__ __noinline__ SpecialFrag specials(SpecialFrag f, uint32_t a0, uint32_
     return f;
 }
 
+// o0, o1 += p V for 16 positions and 16 dims.  The tensor core cuts its sums off (they shrink by
+// half a unit of their last place each time: 5e-7 of rows over 2668 positions, 1e-6 over 16000), so
+// fp32 rows take the products by themselves and add them rounded.
+template <typename T, bool SPLIT, int F>
+__device__ __forceinline__ void add_products(float (&o0)[4], float (&o1)[4],
+                                             const uint32_t (&p)[F][4], const uint32_t (&v)[4]) {
+    float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < F; ++n) {
+        PMath<T>::mma(SPLIT ? t0 : o0, p[n], v[0], v[1]);
+        PMath<T>::mma(SPLIT ? t1 : o1, p[n], v[2], v[3]);
+    }
+    if (!SPLIT) return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        o0[u] += t0[u];
+        o1[u] += t1[u];
+    }
+}
+
 // The last i in [0, n) with a[i] <= x (0 when there is none).
 __device__ __forceinline__ int last_le(const int* __restrict__ a, int n, int x) {
     int lo = 0, hi = n;

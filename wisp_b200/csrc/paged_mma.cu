@@ -29,14 +29,15 @@
 // NaNs before the product: those that no row sees are zeroed in shared memory; where some row
 // sees one, the row tile is marked and the join kernel works it out again without tiles.
 //
-// Measured (B200): a prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 550 us = 1.0 PFLOP/s
-// of the visible pairs (59% of the measured bf16 rate), tensor pipe and exponential unit 55% busy
+// Measured (B200): a prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 540 us = 1.0 PFLOP/s
+// of the visible pairs (60% of the measured bf16 rate), tensor pipe and exponential unit 55% busy
 // each at 1.67 GHz under the power limit; chunks of 7652 tokens behind up to 9000 positions, 16 heads
-// of 64, window 1024, 121 us; four drafted tokens behind 64K to 128K positions, 64
+// of 64, window 1024, 118 us; four drafted tokens behind 64K to 128K positions, 64
 // heads, 300 us = 6.0 TB/s (93% of the measured copy).  Steps of the prompt: mma.sync row tiles
 // of 64 rows 4.57 ms; this kernel with one thread issuing all products 1.15 ms (it was bound by
 // 80 to 115 cycles an instruction); a warp per row tile with warp-uniform operands 816 us; pieces
-// that count what beginning a row tile costs 694 us; Q by TMA behind the last product 551 us.
+// that count what beginning a row tile costs 694 us; Q by TMA behind the last product 551 us;
+// pieces balanced by what a row tile costs to begin (six KV tiles) and by its rows 540 us.
 // Measured and not kept: Q double buffered with a ring of three KV tiles (817 us), registers moved
 // to the softmax warps (no gain), one softmax warp of a pair waiting for the other's exponentials
 // (no gain), skipping hidden tiles warp by warp inside the loop (prompts 10% slower), a quarter to
@@ -63,6 +64,11 @@ namespace {
 constexpr int kN = kPagedTile;          // positions of a KV tile
 constexpr int kM = kPagedHalf;  // rows of a row tile
 constexpr int kThreads = 384;
+// fp32 rows: O is added to a rounded sum after so many KV tiles.  The tensor core cuts its sums off,
+// which shrinks a long row by half a unit of the last place an instruction: 40 tokens behind 16000
+// positions were 3.6e-6 off (plain fp32 0.7e-6), with 8 tiles 1.7e-6, with 4 1.25e-6, with 1 0.9e-6;
+// 3 x 500 tokens behind 4000 took 178, 182, 204 and 218 us.
+constexpr int kFlush = 4;
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kRowWarp = 11;
 
 template <int HD, int PARTS>
@@ -76,13 +82,17 @@ struct MCfg {
     static constexpr int kQBufs = HD == 64 ? 2 : 1;
     static constexpr int kSlots = HD == 64 ? (PARTS == 3 ? 8 : 12) : PARTS == 3 ? 7 : 9;
     static constexpr int kSmem = 1024 + kQBufs * kRT * PARTS * kQ + kSlots * kSlot;
-    // TMEM columns
-    static constexpr int kPCols = 32 * PARTS;
+    // TMEM columns: S in two buffers, part p of P over them or (two parts, and the third) behind
     static __host__ __device__ constexpr int s_col(int x, int b) { return (x * 2 + b) * 64; }
-    static __host__ __device__ constexpr int p_col(int x, int b) {
-        return PARTS == 1 ? s_col(x, b) : 128 + b * kPCols;
+    static __host__ __device__ constexpr int p_col(int x, int b, int p) {
+        return PARTS == 1   ? s_col(x, b)
+               : PARTS == 2 ? 128 + b * 64 + p * 32
+               : p < 2      ? s_col(x, b) + p * 32
+                            : 128 + b * 32;
     }
     static __host__ __device__ constexpr int o_col(int x) { return 512 - (kRT - x) * HD; }
+    // fp32 rows: what O held every kFlush KV tiles, added rounded
+    static constexpr int kSumCol = 512 - 2 * HD;
 };
 
 // Shared-memory descriptors, 128-byte swizzle.  K-major (Q, K): 64 elements per row of 128 B,
@@ -572,15 +582,17 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) && arrive_full(rv);
                 if (!ok) break;
                 tc_after();
-                const uint32_t d = tmem + C::o_col(x), a0 = tmem + C::p_col(x, 0) +
-                                                            (cnt & 1) * (C::p_col(x, 1) - C::p_col(x, 0));
+                const uint32_t d = tmem + C::o_col(x);
                 const uint32_t v0 = vd + (rv % kSlots) * (C::kSlot >> 4);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
+                for (int p = 0; p < PARTS; ++p) {
+                    const uint32_t a0 = tmem + C::p_col(x, 0, p) +
+                                        (cnt & 1) * (C::p_col(x, 1, p) - C::p_col(x, 0, p));
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
-                        mma_ts(d, a0 + p * 32 + k * 8, v0 + ((k * 16 * 128) >> 4),
-                               idesc(kType, HD, 1), p || k ? 1u : (uint32_t)(j > 0), leader);
+                        mma_ts(d, a0 + k * 8, v0 + ((k * 16 * 128) >> 4), idesc(kType, HD, 1),
+                               p || k ? 1u : (uint32_t)(SPLIT ? j % kFlush > 0 : j > 0), leader);
+                }
                 commit(&o_done[x][cnt & 1]);
                 commit(&empty[rv % kSlots]);
             }
@@ -743,7 +755,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 const float mx =
                     max3(max3(mx4[0], s[kN - 4], s[kN - 3]), max3(mx4[1], s[kN - 2], s[kN - 1]),
                          fmaxf(mx4[2], mx4[3])) * fac;
-                if (__any_sync(kAll, mx > m + 8.f)) {
+                const bool flush = SPLIT && j > 0 && j % kFlush == 0;
+                if (flush || __any_sync(kAll, mx > m + 8.f)) {
                     const float to = fmaxf(m, mx);
                     const float al = ex2(m - (to == -INFINITY ? 0.f : to));
                     m = to;
@@ -760,7 +773,17 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                             tmem_ld32(lanes + C::o_col(x) + c, o);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] *= al;
-                            tmem_st32(lanes + C::o_col(x) + c, reinterpret_cast<uint32_t*>(o));
+                            if (!flush)
+                                tmem_st32(lanes + C::o_col(x) + c, reinterpret_cast<uint32_t*>(o));
+                            if (SPLIT && (flush || j > kFlush)) {
+                                // the sums up to the last multiple of kFlush, and O at the next
+                                float sum[32];
+                                if (j > kFlush) tmem_ld32(lanes + C::kSumCol + c, sum);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    sum[i] = (j > kFlush ? sum[i] * al : 0.f) + (flush ? o[i] : 0.f);
+                                tmem_st32(lanes + C::kSumCol + c, reinterpret_cast<uint32_t*>(sum));
+                            }
                         }
                     }
                 }
@@ -792,7 +815,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                             s[2 * i + 1] -= f.y;
                         }
                     }
-                    tmem_st32(lanes + C::p_col(x, b) + p * 32, w);
+                    tmem_st32(lanes + C::p_col(x, b, p), w);
                 }
                 tmem_wait_st();
                 tc_before();
@@ -867,6 +890,12 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             for (int c = half ? x * (HD / 2) : 0; c < (half ? (x + 1) * (HD / 2) : HD); c += 32) {
                 float o[32];
                 tmem_ld32(lanes + C::o_col(x) + c, o);
+                if (SPLIT && own > kFlush) {
+                    float sum[32];
+                    tmem_ld32(lanes + C::kSumCol + c, sum);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] += sum[i];
+                }
                 if (half) {
                     float p[32];
                     tmem_ld32(lanes + C::o_col(kRT - 1 - x) + c, p);
