@@ -166,11 +166,12 @@ __device__ __forceinline__ void add_products(float (&o0)[4], float (&o1)[4],
         PMath<T>::mma(SPLIT ? t0 : o0, p[n], v[0], v[1]);
         PMath<T>::mma(SPLIT ? t1 : o1, p[n], v[2], v[3]);
     }
-    if (!SPLIT) return;
+    if constexpr (SPLIT) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        o0[u] += t0[u];
-        o1[u] += t1[u];
+        for (int u = 0; u < 4; ++u) {
+            o0[u] += t0[u];
+            o1[u] += t1[u];
+        }
     }
 }
 
