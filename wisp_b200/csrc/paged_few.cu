@@ -42,7 +42,6 @@ namespace {
 constexpr int kWork = 128;             // working threads
 constexpr int kThreads = kWork + 32;  // and the loading warp
 constexpr int kTile = kPagedTile;
-constexpr long long kPrefetchTable = 65536;  // entries of the page table
 constexpr int kRecs = 16;
 static_assert(kPagedInline <= kThreads, "a thread per row tile");
 
@@ -70,21 +69,6 @@ __device__ __forceinline__ Rec make_rec(const PagedPlan& P, const PagedItem& it,
                                         int x0, int x_end) {
     const int c0 = cum + P.lead;
     return Rec{it, max(0, x0 - c0), max(0, min(it.n_tiles, x_end - c0)), item, c0};
-}
-
-// What every CTA's plan and page look-ups read, into L2 while the kernel before this one runs (small
-// tables only: each thread of the grid takes a line of 128 bytes).
-__device__ __forceinline__ void prefetch_batch(const PagedArgs& A) {
-    auto fetch = [](const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); };
-    const int tid = threadIdx.x;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid * 32 <= A.n_seq) {
-        fetch(A.q_start + tid * 32);
-        if (tid * 32 < A.n_seq) fetch(A.kv_len + tid * 32);
-    }
-    const long long at = ((long long)blockIdx.x * kThreads + tid) * 32;
-    if (blockIdx.y == 0 && at < kPrefetchTable &&
-        at < (long long)(A.n_seq - 1) * A.table_stride + A.table_width)
-        fetch(A.table + at);
 }
 
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -131,10 +115,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     // the SMs that it leaves start on this one: only the end waits for it (for the join's sake).
     // (64 sequences behind two long prefixes: 98 us a call, 102 us with the wait here.)
     auto wait_before = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
-    if (!behind) {
-        prefetch_batch(A);
-        wait_before();
-    }
+    if (!behind) wait_before();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const bool inlined = P.inlined != 0, prefix = which == PLAN_PREFIX;

@@ -15,8 +15,10 @@
 //   warps 8 and 9        issue the MMAs of one row tile each (an elected thread)
 //   warp 10              loads K and V: TMA boxes of up to 64 positions out of one page, lane
 //                        per box, 128-byte swizzle, ring of 16-KB slots
-//   warp 11              loads the rows of Q (TMA where a row tile is whole tokens) as soon as
-//                        the last product that reads the previous ones is done
+//   warp 11              loads the rows of Q (TMA where a row tile is whole tokens) as soon as the
+//                        last product that reads the previous ones is done; 32-bit rows, which
+//                        have one row tile, are loaded and split by warps 4-7 (one prompt of 2048
+//                        fp32 tokens 222 us, 641 us with one warp)
 // A row's running maximum is only moved when a score passes it by more than 2^8 (the weights
 // then still fit 16 bits and the sums are fp32), so that O is rarely rescaled; the warp that
 // needs it does so itself, behind the previous product.
@@ -287,10 +289,11 @@ struct Walk {
     }
 };
 
-// By one warp: n rows of Q from row `row0` of the item on into a 128-row tile (zeros below them).
+// n rows of Q from row `row0` of the item on into a 128-row tile (zeros below them): all of it by
+// one warp, of fp32 rows 32 from row `part` on.
 template <typename T, int PARTS, int HD>
 __device__ __forceinline__ void load_q_tile(const PagedArgs& A, int tok0, int row0, int n, int h0,
-                                            int gpb, bool flip, char* tile, float* s_fac) {
+                                            int gpb, bool flip, char* tile, float* s_fac, int part) {
     const int lane = threadIdx.x & 31;
     using C = MCfg<HD, PARTS>;
     auto source = [&](int r) {
@@ -323,8 +326,8 @@ __device__ __forceinline__ void load_q_tile(const PagedArgs& A, int tok0, int ro
         // largest exponent
         constexpr int kV = HD / 32;  // 2 or 4
         const int d = lane * kV, c = d / 8;
-#pragma unroll 4
-        for (int r = 0; r < kM; ++r) {
+#pragma unroll 8
+        for (int r = part; r < part + 32; ++r) {
             const bool in = r < n && d < A.hd;
             const float* from = reinterpret_cast<const float*>(A.q) + (in ? source(r) + d : 0);
             float v[kV], mx = 0.f;
@@ -402,7 +405,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         }
         for (int x = 0; x < kRT; ++x) {
             for (int b = 0; b < kQB; ++b) {
-                bar_init(&q_full[x][b], 1);
+                bar_init(&q_full[x][b], SPLIT ? 4 : 1);
                 bar_init(&q_empty[x][b], SPLIT ? 5 : 1);
             }
             for (int b = 0; b < 2; ++b) {
@@ -601,7 +604,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         commit(&drain[x]);
         if (lane == 0) bar_drain(&drain[x], 0);
         __syncwarp();
-    } else if (warp == kRowWarp) {
+    } else if (SPLIT ? warp >= 4 && warp < 8 : warp == kRowWarp) {
         // ------------------------------------------------------------- rows of Q
         const bool flip = A.scale_log2 < 0.f;  // q takes the sign, so that the factor is >= 0
         uint32_t seg[kRT] = {};
@@ -628,7 +631,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 }
                 const int n = min(kM, n_rows - row0);
                 load_q_tile<T, PARTS, HD>(A, W.it.tok0, row0, n, h0, gpb, flip,
-                                          sQ + (qb * kRT + x) * PARTS * C::kQ, s_fac[x][qb]);
+                                          sQ + (qb * kRT + x) * PARTS * C::kQ, s_fac[x][qb],
+                                          SPLIT ? (warp - 4) * 32 : 0);
                 async_fence();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&q_full[x][qb]);
