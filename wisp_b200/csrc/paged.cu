@@ -366,9 +366,10 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
 // ------------------------------------------------------------------------
 // What a row tile costs before its first KV tile, in KV tiles (a prompt of 8192 tokens took 816 us
 // with 0 and 694 us with 4, later 560 us with 4 and 540 us with 6, where a KV tile took 0.94 us
-// and a beginning 5.4 us; 14 single tokens behind up to 4096 positions 32.6 us with 0 and 30.9 us
-// with 2).
-constexpr int kLeadMma = 6, kLeadFew = 2;
+// and a beginning 5.4 us; fp32 rows, which are split first: 2048 tokens 280 us with 3, 212 with 6,
+// 179 with 12, 191 with 16, and 3 x 500 tokens behind 4000 116 us with 3 and 118 with 12; 14 single
+// tokens behind up to 4096 positions 32.6 us with 0 and 30.9 us with 2).
+constexpr int kLeadMma = 6, kLeadMma32 = 12, kLeadFew = 2;
 // Up to so many 16-row tiles stay with paged_few_kernel, where all that they read again (for wide
 // heads: all that the tables can name) is at most so large.
 constexpr int kFewTiles = 4, kFewTilesWide = 8;
@@ -441,7 +442,7 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         const int ctas =
             (on_mma ? 1 : is_few ? paged_few_ctas(A.hd) : paged_attn_ctas()) * sm_count();
         P.grain = on_mma && !split ? 2 : 1;
-        P.lead = (on_mma ? kLeadMma : kLeadFew) * P.grain;
+        P.lead = on_mma ? (split ? kLeadMma32 : kLeadMma * P.grain) : kLeadFew;
         P.lanes = std::min(4095, std::max(1, ctas / P.heads));
         if (is_few && w == PLAN_PREFIX && A.plan[PLAN_FEW].used) {  // they share one launch
             A.plan[PLAN_FEW].lanes = std::max(1, A.plan[PLAN_FEW].lanes / 2);
