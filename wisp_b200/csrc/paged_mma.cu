@@ -18,7 +18,9 @@
 //   warp 11              loads the rows of Q (TMA where a row tile is whole tokens) as soon as the
 //                        last product that reads the previous ones is done; 32-bit rows, which
 //                        have one row tile, are loaded and split by warps 4-7 (one prompt of 2048
-//                        fp32 tokens 222 us then, 641 us with one warp)
+//                        fp32 tokens 222 us then, 641 us with one warp).  It also looks V of partly
+//                        hidden tiles through for infinities and NaNs, for both row tiles: their
+//                        products with V wait for it
 // A row's running maximum is only moved when a score passes it by more than 2^8 (the weights
 // then still fit 16 bits and the sums are fp32), so that O is rarely rescaled; the warp that
 // needs it does so itself, behind the previous product.
@@ -265,14 +267,17 @@ struct Walk {
     int a, b;  // KV tiles [a, b) of the item
     int c0;    // the item's first KV tile on the line
     int sh;    // its KV tiles are 2^sh units
+    int all_hi, all_lo;  // every row sees the positions between (and the sinks)
     PagedItem it;
-    __device__ __forceinline__ bool next(const PagedPlan& P) {
+    __device__ __forceinline__ bool next(const PagedArgs& A, const PagedPlan& P) {
         while (x < x_end) {
             it = P.items[item];
             c0 = P.cum[item] + P.lead;
             sh = item_shift(P, it);
             ++item;
             if (it.n_tiles == 0) continue;
+            all_hi = min(it.kv_hi, it.pmin + 1);
+            all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
             a = (max(0, x - c0) + sh) >> sh;
             b = min(it.n_tiles, (max(0, x_end - c0) + sh) >> sh);
             x = min(c0 + (it.n_tiles << sh), x_end);
@@ -383,7 +388,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     constexpr int kQB = C::kQBufs;
     char* sQ = base;                                // [kQB][kRT][PARTS][kH][128 rows][128 B]
     char* sKV = base + kQB * kRT * PARTS * C::kQ;   // [kSlots][kH][64 rows][128 B]
-    __shared__ uint64_t full[kSlots], empty[kSlots];
+    __shared__ uint64_t full[kSlots], empty[kSlots], v_load[kSlots], v_seen[kSlots];
     __shared__ uint64_t q_full[kRT][kQB], q_empty[kRT][kQB], s_full[kRT][2], p_full[kRT][2], o_done[kRT][2], drain[kRT];
     __shared__ uint32_t s_tmem;
     __shared__ uint64_t x_done[2], x_read[2];  // both halves of an item: sums there, O read
@@ -402,6 +407,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         for (int i = 0; i < kSlots; ++i) {
             bar_init(&full[i], 1);
             bar_init(&empty[i], kRT);
+            bar_init(&v_load[i], 1);
+            bar_init(&v_seen[i], 1);
         }
         for (int x = 0; x < kRT; ++x) {
             for (int b = 0; b < kQB; ++b) {
@@ -482,12 +489,25 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     // Whether both row tiles' roles work on one item of at most kM rows (even and odd KV tiles).
     auto halved = [&]() { return kRT == 2 && W.it.ntok * gpb <= kM && W.b - W.a >= 2; };
     uint32_t ring = 0;  // K / V tiles so far: slot ring % kSlots, phase (ring / kSlots) & 1
+    // Is some of KV tile i of the item hidden from some row?  V of these tiles is looked through.  The
+    // c-th such tile of the piece has its load behind it with v_load[c % kSlots] (a wait for `full`
+    // any earlier could meet an older phase of its parity) and its look with v_seen[c % kSlots].
+    // Its slot is released only behind both, and the tile kSlots before has been when it is loaded.
+    const int sinks = A.window > 0 ? A.sinks : 0;
+    auto hides = [&](int i) {
+        const int j0 = W.tile(i) * kN;
+        return !(j0 >= W.it.kv_lo && j0 + kN <= W.all_hi && (j0 >= W.all_lo || j0 + kN <= sinks));
+    };
+    uint32_t looks = 0;  // such tiles so far
+    auto looked = [&]() {
+        return bar_wait_warp(&v_seen[looks % kSlots], (looks / kSlots) & 1, &s_abort);
+    };
     if (warp == kLoadWarp) {
         // ------------------------------------------------------------- K / V tiles
         const int per_half = kN / box_rows, boxes = per_half * kH;
         const int half = lane / per_half, rb = lane - half * per_half;
         bool ok = true;
-        while (ok && W.next(P)) {
+        while (ok && W.next(A, P)) {
             // this lane's page and row of a tile's box
             auto place = [&](int i) {
                 return lane < boxes
@@ -510,6 +530,10 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                     if (lane < boxes)
                         tma4d(smem_addr(sKV + s * C::kSlot + half * (kN * 128) + rb * box_rows * 128),
                               kv ? &maps.v : &maps.k, half * 64, kvh, cur.y, cur.x, &full[s]);
+                }
+                if (ok && hides(i)) {
+                    if (lane == 0) bar_arrive(&v_load[looks % kSlots]);
+                    ++looks;
                 }
             }
         }
@@ -552,10 +576,11 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             }
             return true;
         };
-        for (; ok && W.next(P); ring += 2 * (W.b - W.a)) {
+        for (; ok && W.next(A, P); ring += 2 * (W.b - W.a)) {
             const int n = W.b - W.a;
             const bool half = halved();
             if (!half && x * kM >= W.it.ntok * gpb) {  // no rows here
+                for (int i = W.a; i < W.b; ++i) looks += hides(i);
                 ok = release(ring, 2 * n);
                 continue;
             }
@@ -567,6 +592,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                  (cnt < 2 || __all_sync(kAll, pv_done(x, cnt - 2)));
             if (!ok) break;
             ++seg;
+            if (first) looks += hides(W.a);
             tc_after();
             issue_s(r0 % kSlots, cnt, qb);
             commit(&empty[r0 % kSlots]);
@@ -582,8 +608,12 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                     commit(&empty[rk % kSlots]);
                     if (j + 2 == own) commit(&q_empty[x][qb]);
                 }
-                ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) && arrive_full(rv);
+                const int i = W.a + first + j * step;
+                const bool hidden = hides(i);
+                ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) &&
+                     arrive_full(rv) && (!hidden || looked());
                 if (!ok) break;
+                looks += hidden + (half && i + 1 < W.b && hides(i + 1));
                 tc_after();
                 const uint32_t d = tmem + C::o_col(x);
                 const uint32_t v0 = vd + (rv % kSlots) * (C::kSlot >> 4);
@@ -604,17 +634,19 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         commit(&drain[x]);
         if (lane == 0) bar_drain(&drain[x], 0);
         __syncwarp();
-    } else if (SPLIT ? warp >= 4 && warp < 8 : warp == kRowWarp) {
-        // ------------------------------------------------------------- rows of Q
+    } else if (warp == kRowWarp || (SPLIT && warp >= 4 && warp < 8)) {
+        // ------------------------------------------------------------- rows of Q, a look at V
+        const bool rows = !SPLIT || warp < 8;
         const bool flip = A.scale_log2 < 0.f;  // q takes the sign, so that the factor is >= 0
         uint32_t seg[kRT] = {};
         bool ok = true;
-        while (ok && W.next(P)) {
-            const int n_rows = W.it.ntok * gpb;
+        for (; ok && W.next(A, P); ring += 2 * (W.b - W.a)) {
+            const PagedItem& it = W.it;
+            const int n_rows = it.ntok * gpb;
 #pragma unroll
             for (int x = 0; x < kRT; ++x) {
                 const int row0 = halved() ? 0 : x * kM;
-                if (!ok || row0 >= n_rows) continue;
+                if (!ok || !rows || row0 >= n_rows) continue;
                 const uint32_t qb = seg[x] % kQB;
                 ok = bar_wait_warp(&q_empty[x][qb], ((seg[x] / kQB) & 1) ^ 1, &s_abort);
                 if (!ok) continue;
@@ -625,17 +657,57 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 #pragma unroll
                         for (int h = 0; h < kH; ++h)
                             tma3d(smem_addr(sQ + (qb * kRT + x) * C::kQ + h * (kM * 128)), &q_map,
-                                  h * 64, h0, W.it.tok0 + row0 / gpb, &q_full[x][qb]);
+                                  h * 64, h0, it.tok0 + row0 / gpb, &q_full[x][qb]);
                     }
                     continue;
                 }
                 const int n = min(kM, n_rows - row0);
-                load_q_tile<T, PARTS, HD>(A, W.it.tok0, row0, n, h0, gpb, flip,
+                load_q_tile<T, PARTS, HD>(A, it.tok0, row0, n, h0, gpb, flip,
                                           sQ + (qb * kRT + x) * PARTS * C::kQ, s_fac[x][qb],
                                           SPLIT ? (warp - 4) * 32 : 0);
                 async_fence();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&q_full[x][qb]);
+            }
+            if (warp != kRowWarp) continue;
+            // No infinity or NaN of a partly hidden tile may meet a zero weight: zeros take their
+            // places, and where some row sees one the join works the item out again without tiles.
+            // (One warp for both row tiles: with each of them looking for itself nothing ordered the
+            // zeros that one had written before the other's product.)
+            const int any_hi = min(it.kv_hi, it.pmax + 1);
+            const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
+            for (int i = W.a; i < W.b; ++i) {
+                if (!hides(i)) continue;
+                const uint32_t rv = ring + 2 * (i - W.a) + 1;
+                ok = bar_wait_warp(&v_load[looks % kSlots], (looks / kSlots) & 1, &s_abort) &&
+                     bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort);
+                if (!ok) break;
+                const int j0 = W.tile(i) * kN;
+                char* vt = sKV + (rv % kSlots) * C::kSlot;
+                uint32_t found = 0;
+#pragma unroll 8
+                for (int c = lane; c < kN * HD / 8; c += 32) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(vt + c * 16);
+                    found |= odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
+                             odd_halves<T>(v.w);
+                }
+                if (found) {
+                    for (int c = lane; c < kN * HD / 8; c += 32) {
+                        uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
+                        const uint4 v = *at;
+                        if (!(odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
+                              odd_halves<T>(v.w)))
+                            continue;
+                        const int p = j0 + ((c / 8) & (kN - 1));
+                        if (p >= it.kv_lo && p < any_hi && (p >= any_lo || p < sinks))
+                            P.redo[(size_t)(W.item - 1) * P.heads + head_lane] = 1;
+                        *at = make_uint4(0, 0, 0, 0);
+                    }
+                    async_fence();
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&v_seen[looks % kSlots]);
+                ++looks;
             }
         }
         if (q_boxes && lane == 0)  // (only after a timeout can some of these still be in flight)
@@ -651,7 +723,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         constexpr float kShift = MShift<T>::value;
         uint32_t cnt = 0, seg = 0, pairs = 0;
         bool ok = true;
-        for (; ok && W.next(P); ring += 2 * (W.b - W.a)) {
+        while (ok && W.next(A, P)) {
             const PagedItem& it = W.it;
             const int n_rows = it.ntok * gpb, n = W.b - W.a;
             const bool half = halved();
@@ -677,57 +749,20 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             fac = fmaxf(fac, 1e-37f);  // (0 would make NaNs of hidden scores)
             const int hi_row = real ? min(it.kv_hi, pos + 1) : 0;
             const int lo_row = real && A.window > 0 ? pos - A.window + 1 : INT_MIN;
-            const int sinks = A.window > 0 ? A.sinks : 0;
-            const int any_hi = min(it.kv_hi, it.pmax + 1);
-            const int any_lo = A.window > 0 ? it.pmin - A.window + 1 : INT_MIN;
-            const int all_hi = min(it.kv_hi, it.pmin + 1);
-            const int all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
-            auto is_whole = [&](int j0) {  // nothing of the tile is hidden from any row
-                return j0 >= it.kv_lo && j0 + kN <= all_hi && (j0 >= all_lo || j0 + kN <= sinks);
-            };
-            // V of a partly hidden tile: no infinity or NaN may meet a zero weight.
-            auto look_through = [&](int j, int j0) {
-                const uint32_t rv = ring + 2 * (first + j * step) + 1;
-                if (!bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort)) return false;
-                char* vt = sKV + (rv % kSlots) * C::kSlot;
-                uint32_t found = 0;
-#pragma unroll
-                for (int c = 0; c < kN * HD / 8 / kM; ++c) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vt + (c * kM + r) * 16);
-                    found |= odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
-                             odd_halves<T>(v.w);
-                }
-                if (found) {
-                    for (int c = r; c < kN * HD / 8; c += kM) {
-                        uint4* at = reinterpret_cast<uint4*>(vt + c * 16);
-                        const uint4 v = *at;
-                        if (!(odd_halves<T>(v.x) | odd_halves<T>(v.y) | odd_halves<T>(v.z) |
-                              odd_halves<T>(v.w)))
-                            continue;
-                        const int p = j0 + ((c / 8) & (kN - 1));
-                        if (p >= it.kv_lo && p < any_hi && (p >= any_lo || p < sinks))
-                            P.redo[(size_t)(W.item - 1) * P.heads + head_lane] = 1;
-                        *at = make_uint4(0, 0, 0, 0);
-                    }
-                    async_fence();
-                }
-                return true;
-            };
             float m = -INFINITY, l = 0.f;
             // A warp without rows only keeps step: what P holds for it reaches no row that is read.
             // (In a loop of its own: as a branch of the next one it cost prompts 5%.)
             const bool idle = row0 + (warp & 3) * 32 >= n_rows;
             for (int j = 0; idle && j < own; ++j, ++cnt) {
-                const int b = cnt & 1, j0 = W.tile(W.a + first + j * step) * kN;
-                ok = bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort) &&
-                     (is_whole(j0) || look_through(j, j0));
+                const int b = cnt & 1;
+                ok = bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort);
                 if (!ok) break;
                 __syncwarp();
                 if (lane == 0) bar_arrive(&p_full[x][b]);
             }
             for (int j = 0; !idle && j < own; ++j, ++cnt) {
-                const int b = cnt & 1, j0 = W.tile(W.a + first + j * step) * kN;
-                const bool whole = is_whole(j0);
+                const int b = cnt & 1, i0 = W.a + first + j * step, j0 = W.tile(i0) * kN;
+                const bool whole = !hides(i0);
                 if (!bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort)) {
                     ok = false;
                     break;
@@ -744,10 +779,6 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 #pragma unroll
                     for (int i = 0; i < kN; ++i)
                         if (!((w[i / 32] >> (i % 32)) & 1u)) s[i] = -INFINITY;
-                    if (!look_through(j, j0)) {
-                        ok = false;
-                        break;
-                    }
                 }
                 float mx4[4];
 #pragma unroll
