@@ -559,7 +559,8 @@ WispError wisp_rope_append(const WispRows* q, const WispRows* k, const WispRows*
  * the plain call up to rounding.
  * The workspace's first word is the call's status (wisp_moe_status reads it;
  * bit 0: a page number outside the pool, its positions read as zeros; bit 1: a
- * kv_len beyond the table, cut to it; bit 3: a bounded wait timed out). */
+ * kv_len beyond the table, cut to it; bit 3: a bounded wait timed out, the rows
+ * are not valid). */
 size_t wisp_paged_attention_workspace_bytes(const WispKvPages* pages, const WispTokenBatch* batch,
                                             int n_heads, int q_dtype, int n_groups);
 WispError wisp_paged_attention(const WispRows* q, const WispRows* out, float* lse,
@@ -571,6 +572,11 @@ WispError wisp_prefix_attention(const WispRows* q, const WispRows* out, float* l
                                 const int* groups, const int* prefix_len, int n_groups,
                                 float scale, int window, int sinks, void* workspace,
                                 size_t workspace_bytes, cudaStream_t stream, WispErrCtx* err);
+
+/* How long a wait inside an attention kernel may take, in nanoseconds of wall time (2 s at first),
+ * for the calls made from now on in this process; the limit before.  A GPU that is shared in time
+ * slices may need more. */
+unsigned long long wisp_paged_wait_limit(unsigned long long ns);
 
 /* Pages src[i] -> dst[i] (host arrays, n pairs) in every layer: layer l's page
  * p of the keys is k + l * layer_stride + p * page_stride elements.  All source

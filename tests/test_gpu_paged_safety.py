@@ -28,3 +28,34 @@ def test_two_row_tiles_behind_one_tile_of_hidden_nans(cuda, dim, cache, heads, w
         for _ in range(20):
             again = paged.attention(*args, window=window, sinks=sinks)
             assert torch.equal(again, first)
+
+
+# ------------------------------------------------------------------------ waits that run out
+def test_a_call_whose_waits_run_out_returns_and_says_so(cuda):
+    """With no time to wait every role of the kernels gives up at some point of its work, whichever
+    comes first: the call still ends, its status says it (or its result is right), and the next
+    call with time finds everything in order."""
+    decode = make([(1, 40000), (1, 17), (1, 9000), (3, 500)], heads=(32, 8), dim=128)
+    rows32 = make([(1, 20000), (2, 300)], heads=(8, 2), dim=64, dtype=F32)
+    prompt = make([(900, 3000), (70, 333), (4, 20000)], heads=(32, 8), dim=128, cache=BF16)
+    split = make([(300, 2000)], heads=(8, 2), dim=64, dtype=F32, cache=BF16)
+    seen = set()
+    for args in (decode, rows32, prompt, split):
+        q, k, v, batch = args
+        ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+        want = restate(q, k, v, batch)
+        before = paged.wait_limit(0)
+        assert before == 2.0
+        try:
+            for _ in range(4):
+                out, lse = paged.attention(q, k, v, batch, return_lse=True, workspace=ws)
+                seen.add(paged.status(ws))
+                if paged.status(ws) == 0:
+                    check(out, lse, want, q.dtype, k.dtype)
+        finally:
+            assert paged.wait_limit(before) == 0.0
+        run(args)
+    assert seen <= {0, 8} and 8 in seen
+    for bad in (-1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="wait_limit"):
+            paged.wait_limit(bad)

@@ -7,6 +7,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <new>
 #include <vector>
 
@@ -481,6 +482,8 @@ cudaError_t launch_plan_kernel(const PagedArgs& A, const AttnShape& S, int which
                               : launch_paged_attn(A, which, S.rw[which], q_dtype, kv_dtype, s);
 }
 
+std::atomic<unsigned long long> g_wait_ns{2000000000ull};
+
 PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_heads, int n_groups) {
     PagedArgs A{};
     A.k = P->k;
@@ -500,6 +503,7 @@ PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_he
     A.nh = n_heads;
     A.nkv = P->n_kv_heads;
     A.hd = P->head_dim;
+    A.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     return A;
 }
 
@@ -562,6 +566,10 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
 }  // namespace wb
 
 using namespace wb;
+
+extern "C" unsigned long long wisp_paged_wait_limit(unsigned long long ns) {
+    return g_wait_ns.exchange(ns, std::memory_order_relaxed);
+}
 
 extern "C" size_t wisp_paged_attention_workspace_bytes(const WispKvPages* P, const WispTokenBatch* B,
                                                        int n_heads, int q_dtype, int n_groups) {

@@ -98,6 +98,7 @@ struct PagedArgs {
     int n_seq, n_tokens, n_groups, table_stride, table_width, n_pages, page_size, page_shift;
     int nh, nkv, group, hd, window, sinks;
     float scale_log2;
+    unsigned long long wait_ns;  // how long a wait in a kernel may take
     // the sequences' own part, of few or of many rows (one of the two), and the shared prefixes
     PagedPlan plan[PLANS];
 };

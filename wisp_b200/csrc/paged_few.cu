@@ -72,6 +72,17 @@ __device__ __forceinline__ Rec make_rec(const PagedPlan& P, const PagedItem& it,
 }
 
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The same; whether any thread has `x` set.
+__device__ __forceinline__ bool work_any(bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, 1, 128, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)x)
+        : "memory");
+    return any != 0;
+}
 
 template <typename T, bool SPLIT, int HD>
 __global__ void __launch_bounds__(kThreads, (FCfg<T, SPLIT, HD>::kCtas))
@@ -86,7 +97,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     char* qraw = ring + kS * 2 * C::kTen;  // [2] rows of q as they are
     T* work = reinterpret_cast<T*>(qraw + 2 * C::kQBytes);
     __shared__ uint64_t full[kS], empty[kS], q_full[2], q_empty[2];
-    __shared__ volatile int s_abort;
+    __shared__ Waits s_wait;
     __shared__ Rec s_rec[kRecs], s_cur[2];
     __shared__ int s_cum[kPagedInline + 1];
     __shared__ int s_sum[kThreads / 32], s_bad, s_item0, s_pos[16];
@@ -108,7 +119,8 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             bar_init(&q_full[i], 33);
             bar_init(&q_empty[i], 4);
         }
-        s_abort = 0;
+        s_wait.out = 0;
+        s_wait.limit = A.wait_ns;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Behind the shared prefixes' kernel of this call, which has waited for all that is read here,
@@ -195,7 +207,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         // hands a record (and with it the rows of q) over
         auto hand = [&](const Rec& r) {
             const int b = rows & 1;
-            if (!bar_wait_warp(&q_empty[b], ((rows >> 1) & 1) ^ 1, &s_abort)) return false;
+            if (!bar_wait_warp(&q_empty[b], ((rows >> 1) & 1) ^ 1, &s_wait)) return false;
             ++rows;
             if (lane == 0) {
                 s_cur[b] = r;
@@ -251,7 +263,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 const int2 cur = at;
                 if (i + 1 < r.b) at = place(i + 1);
                 const int st = tiles % kS;
-                ok = bar_wait_warp(&empty[st], ((tiles / kS) & 1) ^ 1, &s_abort);
+                ok = bar_wait_warp(&empty[st], ((tiles / kS) & 1) ^ 1, &s_wait);
                 if (!ok) break;
                 if (lane == 0) bar_expect(&full[st], 2 * C::kTen);
                 __syncwarp();
@@ -277,7 +289,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 bar_drain(&full[i % kS], (i / kS) & 1);
     } else {
     // ---------------------------------------------------------------- work
-    Rec cur;
+    Rec cur{};
     int hi_row[2] = {0, 0}, lo_row[2] = {INT_MIN, INT_MIN};
     int all_hi = 0, all_lo = 0, n_rows = 0;
     float fac = A.scale_log2;
@@ -288,32 +300,36 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     bool begins = true;
 
     for (;;) {
+        // A warp whose wait ran out goes on to the next barrier of the four, where all leave together:
+        // one that left alone would keep the others there.
+        bool late = false;
         if (begins) {
             const int b = rows & 1;
-            if (!__all_sync(kAll, bar_wait(&q_full[b], (rows >> 1) & 1, &s_abort))) break;
-            cur = s_cur[b];
-            if (cur.b < 0) break;
+            late = !bar_wait_warp(&q_full[b], (rows >> 1) & 1, &s_wait);
+            if (!late) cur = s_cur[b];
             ci = cur.a;
         }
-        if (!__all_sync(kAll, bar_wait(&full[done % kS], (done / kS) & 1, &s_abort))) break;
+        if (!late && !(begins && cur.b < 0))
+            late = !bar_wait_warp(&full[done % kS], (done / kS) & 1, &s_wait);
         const PagedItem& it = cur.it;
         if (begins) {
-            n_rows = it.ntok * gpb;
-            all_hi = min(it.kv_hi, it.pmin + 1);
-            all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
-            if (tid < 16) {
+            if (tid < 16 && !late && cur.b >= 0) {
                 int pos = INT_MIN;
-                if (tid < kRows && tid < n_rows)
+                if (tid < kRows && tid < it.ntok * gpb)
                     pos = it.mixed ? token_position(A, it.tok0 + tid / gpb) : it.pos0 + tid / gpb;
                 s_pos[tid] = pos;
             }
+            // (behind it the last tile's weights have been read, too)
+            if (work_any(late) || cur.b < 0) break;
+            n_rows = it.ntok * gpb;
+            all_hi = min(it.kv_hi, it.pmin + 1);
+            all_lo = A.window > 0 ? it.pmax - A.window + 1 : INT_MIN;
             const T* q = reinterpret_cast<const T*>(qraw + (rows & 1) * C::kQBytes);
             if (SPLIT) {
-                work_sync();  // the last tile's weights have been read
                 split_rows<T, HD>(A, reinterpret_cast<const float*>(q), n_rows, work, s_fac);
                 q = work;
+                work_sync();
             }
-            work_sync();
 #pragma unroll
             for (int n = 0; n < kF; ++n)
 #pragma unroll
@@ -388,7 +404,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
             if (c4 == 0) s_max[warp][g + 8 * u] = mx[u];
         }
-        work_sync();
+        if (work_any(late)) break;
         float al[2] = {1.f, 1.f};
 #pragma unroll
         for (int u = 0; u < (SPLIT ? 1 : 2); ++u) {
@@ -536,7 +552,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     }
     }
     __syncthreads();
-    if (tid == 0 && (s_bad || s_abort)) P.bad[blockIdx.x] = s_bad | (s_abort ? PG_TIMEOUT : 0);
+    if (tid == 0 && (s_bad || s_wait.out)) P.bad[blockIdx.x] = s_bad | (s_wait.out ? PG_TIMEOUT : 0);
     if (behind) wait_before();
 }
 

@@ -394,7 +394,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     __shared__ uint64_t x_done[2], x_read[2];  // both halves of an item: sums there, O read
     __shared__ float2 s_ml[2][kM];
     __shared__ float s_fac[kRT][kQB][kM];  // fp32 rows: score factors
-    __shared__ volatile int s_abort;
+    __shared__ Waits s_wait;
     __shared__ int s_bad;
     // (the shuffle tells the compiler that the warp number is the same for all lanes)
     const int tid = threadIdx.x, warp = __shfl_sync(kAll, tid >> 5, 0), lane = tid & 31;
@@ -426,7 +426,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             bar_init(&x_done[x], 4);
             bar_init(&x_read[x], 4);
         }
-        s_abort = 0;
+        s_wait.out = 0;
+        s_wait.limit = A.wait_ns;
         s_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -484,7 +485,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     // The product with V of row tile x's c-th KV tile is done.  (A barrier for odd and one for
     // even tiles: a waiter may be two tiles ahead, where one barrier's parity would repeat.)
     auto pv_done = [&](int x, uint32_t c) {
-        return bar_wait(&o_done[x][c & 1], (c >> 1) & 1, &s_abort);
+        return bar_wait(&o_done[x][c & 1], (c >> 1) & 1, &s_wait);
     };
     // Whether both row tiles' roles work on one item of at most kM rows (even and odd KV tiles).
     auto halved = [&]() { return kRT == 2 && W.it.ntok * gpb <= kM && W.b - W.a >= 2; };
@@ -500,7 +501,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
     };
     uint32_t looks = 0;  // such tiles so far
     auto looked = [&]() {
-        return bar_wait_warp(&v_seen[looks % kSlots], (looks / kSlots) & 1, &s_abort);
+        return bar_wait_warp(&v_seen[looks % kSlots], (looks / kSlots) & 1, &s_wait);
     };
     if (warp == kLoadWarp) {
         // ------------------------------------------------------------- K / V tiles
@@ -521,7 +522,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++ring) {
                     const int s = ring % kSlots;
-                    if (!bar_wait_warp(&empty[s], ((ring / kSlots) & 1) ^ 1, &s_abort)) {
+                    if (!bar_wait_warp(&empty[s], ((ring / kSlots) & 1) ^ 1, &s_wait)) {
                         ok = false;
                         break;
                     }
@@ -551,7 +552,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
         bool ok = true;
         uint32_t seg = 0, cnt = 0;  // segments, KV tiles of this row tile so far
         auto arrive_full = [&](uint32_t i) {
-            return bar_wait_warp(&full[i % kSlots], (i / kSlots) & 1, &s_abort);
+            return bar_wait_warp(&full[i % kSlots], (i / kSlots) & 1, &s_wait);
         };
         auto commit = [&](uint64_t* bar) {
             if (leader) mma_commit(bar);
@@ -588,7 +589,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             const uint32_t qb = seg % kQB, r0 = ring + 2 * first;
             // S of tile c takes the buffer of tile c - 2's P
             ok = (first == 0 || release(ring, 2)) &&
-                 bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_abort) && arrive_full(r0) &&
+                 bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_wait) && arrive_full(r0) &&
                  (cnt < 2 || __all_sync(kAll, pv_done(x, cnt - 2)));
             if (!ok) break;
             ++seg;
@@ -610,7 +611,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 }
                 const int i = W.a + first + j * step;
                 const bool hidden = hides(i);
-                ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_abort) &&
+                ok = bar_wait_warp(&p_full[x][cnt & 1], (cnt >> 1) & 1, &s_wait) &&
                      arrive_full(rv) && (!hidden || looked());
                 if (!ok) break;
                 looks += hidden + (half && i + 1 < W.b && hides(i + 1));
@@ -648,7 +649,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 const int row0 = halved() ? 0 : x * kM;
                 if (!ok || !rows || row0 >= n_rows) continue;
                 const uint32_t qb = seg[x] % kQB;
-                ok = bar_wait_warp(&q_empty[x][qb], ((seg[x] / kQB) & 1) ^ 1, &s_abort);
+                ok = bar_wait_warp(&q_empty[x][qb], ((seg[x] / kQB) & 1) ^ 1, &s_wait);
                 if (!ok) continue;
                 ++seg[x];
                 if (q_boxes) {
@@ -679,8 +680,8 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             for (int i = W.a; i < W.b; ++i) {
                 if (!hides(i)) continue;
                 const uint32_t rv = ring + 2 * (i - W.a) + 1;
-                ok = bar_wait_warp(&v_load[looks % kSlots], (looks / kSlots) & 1, &s_abort) &&
-                     bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_abort);
+                ok = bar_wait_warp(&v_load[looks % kSlots], (looks / kSlots) & 1, &s_wait) &&
+                     bar_wait_warp(&full[rv % kSlots], (rv / kSlots) & 1, &s_wait);
                 if (!ok) break;
                 const int j0 = W.tile(i) * kN;
                 char* vt = sKV + (rv % kSlots) * C::kSlot;
@@ -737,7 +738,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             float fac = fabsf(A.scale_log2);
             if (SPLIT) {
                 const uint32_t qb = seg % kQB;
-                if (!bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_abort)) {
+                if (!bar_wait_warp(&q_full[x][qb], (seg / kQB) & 1, &s_wait)) {
                     ok = false;
                     break;
                 }
@@ -755,7 +756,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             const bool idle = row0 + (warp & 3) * 32 >= n_rows;
             for (int j = 0; idle && j < own; ++j, ++cnt) {
                 const int b = cnt & 1;
-                ok = bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort);
+                ok = bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_wait);
                 if (!ok) break;
                 __syncwarp();
                 if (lane == 0) bar_arrive(&p_full[x][b]);
@@ -763,7 +764,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             for (int j = 0; !idle && j < own; ++j, ++cnt) {
                 const int b = cnt & 1, i0 = W.a + first + j * step, j0 = W.tile(i0) * kN;
                 const bool whole = !hides(i0);
-                if (!bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_abort)) {
+                if (!bar_wait_warp(&s_full[x][b], (cnt >> 1) & 1, &s_wait)) {
                     ok = false;
                     break;
                 }
@@ -872,7 +873,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
                 tc_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&x_done[x]);
-                if (!bar_wait_warp(&x_done[1 - x], pairs & 1, &s_abort)) {
+                if (!bar_wait_warp(&x_done[1 - x], pairs & 1, &s_wait)) {
                     ok = false;
                     break;
                 }
@@ -957,7 +958,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             if (half) {  // neither O is written again before both have been read
                 __syncwarp();
                 if (lane == 0) bar_arrive(&x_read[x]);
-                if (!bar_wait_warp(&x_read[1 - x], pairs & 1, &s_abort)) {
+                if (!bar_wait_warp(&x_read[1 - x], pairs & 1, &s_wait)) {
                     ok = false;
                     break;
                 }
@@ -968,7 +969,7 @@ paged_mma_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
 
     tc_before();
     __syncthreads();
-    if (tid == 0 && (s_bad || s_abort)) P.bad[blockIdx.x] = s_bad | (s_abort ? PG_TIMEOUT : 0);
+    if (tid == 0 && (s_bad || s_wait.out)) P.bad[blockIdx.x] = s_bad | (s_wait.out ? PG_TIMEOUT : 0);
     if (warp == kMmaWarp) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem)

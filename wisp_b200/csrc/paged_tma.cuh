@@ -12,7 +12,12 @@
 namespace wb {
 namespace {
 
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr unsigned long long kDrainNs = 2000000000ull;
+// How long a wait may take, and whether one of the CTA has run out.
+struct Waits {
+    unsigned long long limit;  // ns
+    volatile int out;
+};
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ uint64_t now_ns() {
@@ -43,30 +48,30 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait; false when it ran out here or in another role.
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, Waits* w) {
     if (bar_try(b, parity)) return true;
     uint64_t t0 = 0;
     for (uint32_t it = 0;; ++it) {
         if (bar_try(b, parity)) return true;
-        if ((it & 63) == 63) {
-            if (*abort_flag) return false;
+        if ((it & 63) == 3) {
+            if (w->out) return false;
             const uint64_t t = now_ns();
             if (t0 == 0) t0 = t;
-            else if (t - t0 > kWaitNs) {
-                *abort_flag = 1;
+            if (t - t0 >= w->limit) {
+                w->out = 1;
                 return false;
             }
         }
     }
 }
-__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, uint32_t parity,
-                                              volatile int* abort_flag) {
-    return __all_sync(kAll, bar_wait(b, parity, abort_flag));
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, uint32_t parity, Waits* w) {
+    return __all_sync(kAll, bar_wait(b, parity, w));
 }
+// For a copy or a product that has been issued and will arrive.
 __device__ __forceinline__ void bar_drain(uint64_t* b, uint32_t parity) {
     const uint64_t t0 = now_ns();
     while (!bar_try(b, parity))
-        if (now_ns() - t0 > kWaitNs) return;
+        if (now_ns() - t0 > kDrainNs) return;
 }
 
 __device__ __forceinline__ void tma4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,

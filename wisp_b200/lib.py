@@ -149,6 +149,7 @@ _SIGS = {
                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_float,
                                         C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
                                         C.c_void_p]),
+    "wisp_paged_wait_limit": (C.c_ulonglong, [C.c_ulonglong]),
     "wisp_rope_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "wisp_pages_copy": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p,

@@ -156,6 +156,14 @@ def status(workspace: torch.Tensor) -> int:
                                      torch.cuda.current_stream(workspace.device).cuda_stream))
 
 
+def wait_limit(seconds: float) -> float:
+    """How long a wait inside an attention kernel may take (2 s at first) before the call gives up
+    with bit 3 of its status; for the calls made from now on.  Returns the limit before."""
+    if not 0 <= seconds < 1e9:
+        raise ValueError(f"wait_limit: {seconds} seconds")
+    return lib().wisp_paged_wait_limit(int(seconds * 1e9)) / 1e9
+
+
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst) -> None:
     """Copy pages ``src[i]`` to ``dst[i]`` (host integers) in every layer of pools
     ``[n_layers, n_pages, page_size, n_kv_heads, head_dim]`` (or one layer's four dimensions).
