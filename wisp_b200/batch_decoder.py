@@ -18,6 +18,7 @@ projections are plain fp16 matrix products; everything else runs in this library
 from __future__ import annotations
 
 from dataclasses import dataclass
+from operator import index
 
 import torch
 
@@ -116,6 +117,10 @@ class BatchDecoder:
         """Append each sequence's tokens; logits fp32 ``[len(batch), vocab]`` of the last ones."""
         if not batch or any(not t for _, t in batch) or len({s for s, _ in batch}) != len(batch):
             raise ValueError("step: each sequence once, with one token or more")
+        tokens = [index(t) for _, ts in batch for t in ts]
+        for t in tokens:  # (a row that the embedding does not have would fault the GPU)
+            if not 0 <= t < self.embed.shape[0]:
+                raise ValueError(f"step: token {t} of a vocabulary of {self.embed.shape[0]}")
         dev = self.device
         before = [(seq, self.pool.length(seq)) for seq, _ in batch]
         try:
@@ -136,8 +141,7 @@ class BatchDecoder:
         prefix = None
         if any(shared):
             prefix = [torch.tensor(x, dtype=torch.int32, device=dev) for x in (groups, shared)]
-        tokens = torch.tensor([t for _, ts in batch for t in ts], device=dev)
-        x = self.embed[tokens].float()
+        x = self.embed[torch.tensor(tokens, device=dev)].float()
         T, nh, nkv, d = x.shape[0], self.nh, self.nkv, self.dim
         for l, w in enumerate(self.layers):
             rows = rmsnorm(x, w.input_norm, self.eps).half() @ self._qkv[l].T
