@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from test_gpu_batch_decoder import close, decoder, model, prompt  # noqa: F401 (a fixture)
 from test_gpu_paged import BF16, F16, F32, check, make, restate, run
 from wisp_b200 import paged
 from wisp_b200.lib import WispError
@@ -59,3 +60,31 @@ def test_a_call_whose_waits_run_out_returns_and_says_so(cuda):
     for bad in (-1.0, math.inf, math.nan):
         with pytest.raises(ValueError, match="wait_limit"):
             paged.wait_limit(bad)
+
+
+# ------------------------------------------------------------------------ a step that fails
+@pytest.mark.parametrize("where", ["attention", "rope_append", "stack"])
+def test_a_step_that_failed_can_be_repeated(model, monkeypatch, where):  # noqa: F811
+    """A failure in the second layer: the repeated step gives what a decoder gives that never failed."""
+    p, q = prompt(40, 21), prompt(9, 22)
+    fresh, dec = decoder(model), decoder(model)
+    a, b = fresh.open(), fresh.open()
+    fresh.step([(a, p[:20]), (b, q[:5])])
+    want = fresh.step([(a, p[20:]), (b, q[5:])])
+    a, b = dec.open(), dec.open()
+    dec.step([(a, p[:20]), (b, q[:5])])
+    owner = dec.stack if where == "stack" else paged
+    real, calls = getattr(owner, where), []
+
+    def fail(*args, **kw):
+        calls.append(0)
+        if len(calls) == 2:
+            raise torch.cuda.OutOfMemoryError("no memory left")
+        return real(*args, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(owner, where, fail)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            dec.step([(a, p[20:]), (b, q[5:])])
+    assert len(calls) == 2 and dec.pool.length(a) == 20 and dec.pool.length(b) == 5
+    close(dec.step([(a, p[20:]), (b, q[5:])]), want)

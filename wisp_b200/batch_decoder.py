@@ -17,6 +17,7 @@ projections are plain fp16 matrix products; everything else runs in this library
 
 from __future__ import annotations
 
+from contextlib import suppress
 from dataclasses import dataclass
 from operator import index
 
@@ -58,8 +59,12 @@ class BatchDecoder:
         if embed.shape[1] != H or H % n_heads or n_heads % n_kv_heads:
             raise ValueError(f"hidden {H}, embedding {list(embed.shape)}, {n_heads} heads, "
                              f"{n_kv_heads} kv heads")
+        dim = H // n_heads
+        if dim % 16 or dim > 256 or page_size <= 0 or page_size % 8 or window < 0 or sinks < 0:
+            raise ValueError(f"heads of {dim} (a multiple of 16 up to 256), page_size {page_size} (of "
+                             f"8), window {window}, sinks {sinks} (not negative)")
         self.stack, self.embed, self.lm_head, self.final_norm = stack, embed, lm_head, final_norm
-        self.nh, self.nkv, self.dim = n_heads, n_kv_heads, H // n_heads
+        self.nh, self.nkv, self.dim = n_heads, n_kv_heads, dim
         self.window, self.sinks, self.eps = window, sinks, stack.shape.rms_eps
         self.device = stack.device
         self.layers = layers
@@ -121,17 +126,22 @@ class BatchDecoder:
         for t in tokens:  # (a row that the embedding does not have would fault the GPU)
             if not 0 <= t < self.embed.shape[0]:
                 raise ValueError(f"step: token {t} of a vocabulary of {self.embed.shape[0]}")
-        dev = self.device
         before = [(seq, self.pool.length(seq)) for seq, _ in batch]
         try:
             for (seq, n), (_, toks) in zip(before, batch):
                 self.pool.extend(seq, n + len(toks))
-        except RuntimeError:  # out of pages: nothing of the step has happened
+            self.pool.apply(self.k, self.v)
+            return self._run(batch, tokens)
+        except BaseException:
+            # whatever failed: the lengths must not stand ahead of what has been written
             for seq, n in before:
                 self.pool.truncate(seq, n)
-            self.pool.apply(self.k, self.v)
+            with suppress(Exception):  # pages that got copies keep them
+                self.pool.apply(self.k, self.v)
             raise
-        self.pool.apply(self.k, self.v)
+
+    def _run(self, batch: list[tuple[int, list[int]]], tokens: list[int]) -> torch.Tensor:
+        dev = self.device
         seqs, counts = [s for s, _ in batch], [len(t) for _, t in batch]
         starts = torch.tensor([0] + counts).cumsum(0).to(dev, torch.int32)
         tb = paged.TokenBatch(starts, torch.tensor([self.pool.length(s) for s in seqs],
