@@ -612,7 +612,10 @@ int wisp_page_pool_compact(WispPagePool* pool, WispErrCtx* err);
 int wisp_page_pool_length(const WispPagePool* pool, int seq, WispErrCtx* err);
 /* The sequence's page numbers (at most cap); how many it has, -1 on failure. */
 int wisp_page_pool_pages(const WispPagePool* pool, int seq, int* pages, int cap, WispErrCtx* err);
-/* Drain up to cap queued moves; how many were written. */
+/* The queued moves (at most cap), which stay queued; how many there are. */
+int wisp_page_pool_queued(const WispPagePool* pool, int* src, int* dst, int cap);
+/* Drain up to cap queued moves, whose copies the caller has launched or launches before anything
+ * else; how many were written. */
 int wisp_page_pool_moves(WispPagePool* pool, int* src, int* dst, int cap);
 
 /* ====================================================================== *

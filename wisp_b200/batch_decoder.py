@@ -92,6 +92,7 @@ class BatchDecoder:
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pools; how many are in use."""
+        self.pool.apply(self.k, self.v)  # (what a failed step may have left queued)
         used = self.pool.compact()
         self.pool.apply(self.k, self.v)
         return used

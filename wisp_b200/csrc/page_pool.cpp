@@ -240,6 +240,15 @@ extern "C" int wisp_page_pool_pages(const WispPagePool* p, int seq, int* pages, 
     return (int)v.size();
 }
 
+extern "C" int wisp_page_pool_queued(const WispPagePool* p, int* src, int* dst, int cap) {
+    if (!p) return 0;
+    for (int i = 0; src && dst && i < std::min(cap, (int)p->moves.size()); ++i) {
+        src[i] = p->moves[i].first;
+        dst[i] = p->moves[i].second;
+    }
+    return (int)p->moves.size();
+}
+
 extern "C" int wisp_page_pool_moves(WispPagePool* p, int* src, int* dst, int cap) {
     if (!p || !src || !dst || cap <= 0) return 0;
     const int n = std::min(cap, (int)p->moves.size());

@@ -165,6 +165,7 @@ _SIGS = {
     "wisp_page_pool_compact": (C.c_int, [C.c_void_p, C.c_void_p]),
     "wisp_page_pool_length": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
     "wisp_page_pool_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
+    "wisp_page_pool_queued": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]),
     "wisp_page_pool_moves": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]),
     "wisp_gpu_embed_lookup": (None, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
     "wisp_gpu_rope": (None, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float,

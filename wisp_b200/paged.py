@@ -247,18 +247,24 @@ class PagePool:
         return s, d
 
     def apply(self, k_pages: torch.Tensor, v_pages: torch.Tensor) -> int:
-        """Run the queued moves on the pools of all layers; how many there were."""
-        s, d = self.moves()
+        """Run the queued moves on the pools of all layers; how many there were.  What a refused
+        copy leaves undone stays queued, for another call."""
+        n = lib().wisp_page_pool_queued(self._h, None, None, 0)
+        src, dst = (C.c_int * n)(), (C.c_int * n)()
+        lib().wisp_page_pool_queued(self._h, src, dst, n)
+        s, d = src[:n], dst[:n]
         at, touched, written = 0, set(), set()
-        for i, (a, b) in enumerate(zip(s, d)):
-            if b in touched or a in written:  # a page was freed and taken again in between
-                copy_pages(k_pages, v_pages, s[at:i], d[at:i])
+        for i in range(n + 1):
+            # (a destination met before: the page was freed and taken again in between)
+            if i == n or d[i] in touched or s[i] in written:
+                if i > at:
+                    copy_pages(k_pages, v_pages, s[at:i], d[at:i])
+                    lib().wisp_page_pool_moves(self._h, src, dst, i - at)
                 at, touched, written = i, set(), set()
-            touched |= {a, b}
-            written.add(b)
-        if s:
-            copy_pages(k_pages, v_pages, s[at:], d[at:])
-        return len(s)
+            if i < n:
+                touched |= {s[i], d[i]}
+                written.add(d[i])
+        return n
 
     def table(self, seqs, width: int | None = None, device=None) -> torch.Tensor:
         """The sequences' page numbers, int32 ``[len(seqs), width]`` (0 where a row is shorter)."""
