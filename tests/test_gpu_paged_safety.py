@@ -88,3 +88,47 @@ def test_a_step_that_failed_can_be_repeated(model, monkeypatch, where):  # noqa:
             dec.step([(a, p[20:]), (b, q[5:])])
     assert len(calls) == 2 and dec.pool.length(a) == 20 and dec.pool.length(b) == 5
     close(dec.step([(a, p[20:]), (b, q[5:])]), want)
+
+
+# ------------------------------------------------------------------------ bounds that are too small
+@pytest.mark.parametrize("dim,heads,lens,max_q", [
+    (64, (8, 2), [(1, 200 + 13 * i) for i in range(180)] + [(4, 9000)], 1),  # few rows, planned
+    (64, (8, 2), [(1, 300), (4, 9000), (2, 40)], 1),                         # few rows
+    (128, (8, 2), [(60, 20000), (3, 100)], 20),                              # tcgen05
+    (128, (8, 2), [(300, 9000)], 33),
+    (256, (8, 2), [(60, 20000), (3, 100)], 20),                              # wide heads
+    (256, (8, 8), [(64, 9000)], 24)])
+def test_more_tokens_than_max_q_are_done_or_reported(cuda, dim, heads, lens, max_q):
+    q, k, v, good = make(lens, heads=heads, dim=dim)
+    want = restate(q, k, v, good)
+    batch = paged.TokenBatch(good.q_start, good.kv_len, good.table, max_q)
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, math.nan)
+    _, lse = paged.attention(q, k, v, batch, out=out, return_lse=True, workspace=ws)
+    assert paged.status(ws) in (0, 2)
+    if paged.status(ws) == 0:
+        check(out, lse, want, q.dtype, k.dtype)
+    # what lies within the bound is done in any case
+    starts = good.q_start.tolist()
+    for s, (n, kv) in enumerate(lens):
+        if n <= max_q:
+            a, b = starts[s], starts[s + 1]
+            check(out[a:b], lse[a:b], (want[0][a:b], want[1][a:b], *want[2:]), q.dtype, k.dtype)
+
+
+def test_a_replayed_step_whose_tokens_pass_max_q_says_so(cuda):
+    q, k, v, batch = make([(20, 9000), (20, 9000), (20, 9000)], heads=(8, 2), dim=128)
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, math.nan)
+    graph = torch.cuda.CUDAGraph()
+    paged.attention(q, k, v, batch, out=out, workspace=ws)
+    with torch.cuda.graph(graph):
+        paged.attention(q, k, v, batch, out=out, workspace=ws)
+    graph.replay()
+    assert paged.status(ws) == 0
+    batch.q_start.copy_(torch.tensor([0, 1, 2, 60], dtype=torch.int32))
+    graph.replay()
+    if paged.status(ws) == 0:
+        check(out, None, restate(q, k, v, batch), F16, F16)
+    else:
+        assert paged.status(ws) == 2

@@ -156,7 +156,7 @@ paged_few_kernel(const __grid_constant__ PagedArgs A, const __grid_constant__ Kv
             units = item_units(P, mine);
             if (blockIdx.x == 0 && !prefix && tid == seg * P.per_seg) {
                 const int t = A.q_start[seg + 1] - A.q_start[seg];
-                if (length_too_long(A, seg) || t > P.tpt * P.per_seg)
+                if (length_too_long(A, seg) || t > P.tpt * P.per_seg || left_out(A, P, t))
                     P.bad[P.lanes * P.heads] = PG_BAD_LENGTH;
             }
         }

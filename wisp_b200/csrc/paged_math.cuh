@@ -197,6 +197,12 @@ __device__ __forceinline__ bool length_too_long(const PagedArgs& A, int s) {
     return A.kv_len[s] > (long long)A.table_width * A.page_size;
 }
 
+// May rows of a sequence with so many tokens be left out (it has more than the call's bound)?  The
+// joins of split items take used_rows of each; in prefix mode they go by tokens.
+__device__ __forceinline__ bool left_out(const PagedArgs& A, const PagedPlan& P, int tokens) {
+    return A.n_groups == 0 && min(tokens, P.tpt) * P.gpb > P.used_rows;
+}
+
 struct PagedSeg {
     int t0, t1;  // tokens
     int s0, s1;  // sequences

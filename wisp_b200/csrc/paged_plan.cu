@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
         if (i < n_seg) {
             const PagedSeg g = paged_segment(A, prefix, i);
             n = (g.t1 - g.t0 + P.tpt - 1) / P.tpt;
-            bad |= !prefix && length_too_long(A, i);
+            bad |= !prefix && (length_too_long(A, i) || left_out(A, P, g.t1 - g.t0));
         }
         const int at = carry + block_scan(n, &total, sums);
         if (i < n_seg) P.item_off[i] = at;
