@@ -502,7 +502,8 @@ typedef struct WispKvPages {
  * replayed after they changed.  max_q: no sequence has more tokens (a bound
  * for the choice of kernels; tokens beyond it may be left out, with bit 1 of
  * the status set).  A sequence with kv_len 0 (an unused slot) or
- * with more tokens than positions has tokens that see nothing. */
+ * with more tokens than positions has tokens that see nothing; so do tokens
+ * outside [q_start[0], q_start[n_seq]), which are nobody's. */
 typedef struct WispTokenBatch {
     const int* q_start; /* [n_seq + 1] */
     const int* kv_len;  /* [n_seq] */

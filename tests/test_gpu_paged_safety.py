@@ -132,3 +132,45 @@ def test_a_replayed_step_whose_tokens_pass_max_q_says_so(cuda):
         check(out, None, restate(q, k, v, batch), F16, F16)
     else:
         assert paged.status(ws) == 2
+
+
+# ------------------------------------------------------------------------ tokens of nobody
+@pytest.mark.parametrize("lens,dim,dtype", [
+    ([(1, 30), (1, 2000)], 128, F32), ([(3, 90), (2, 700)], 64, F16), ([(70, 90), (200, 3000)], 128, F16),
+    ([(70, 90), (200, 3000)], 64, F32), ([(70, 90), (40, 3000)], 256, F16)])
+@pytest.mark.parametrize("groups", [False, True])
+def test_rows_that_no_sequence_owns_are_zeros(cuda, lens, dim, dtype, groups):
+    q, k, v, batch = make(lens, dim=dim, dtype=dtype)
+    n = q.shape[0]
+    q = torch.cat([q.new_full((3, *q.shape[1:]), math.nan), q, q.new_full((70, *q.shape[1:]), math.inf)])
+    res = torch.full((n + 73, 10 * dim), 7.0, dtype=dtype, device="cuda")
+    out = res[:, dim:9 * dim].unflatten(1, (8, dim))
+    batch.q_start.add_(3)
+    kw = {}
+    call = paged.attention
+    if groups:
+        call = paged.prefix_attention
+        kw = dict(groups=torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+                  prefix_len=torch.tensor([16], dtype=torch.int32, device="cuda"))
+    _, lse = call(q, k, v, batch, out=out, return_lse=True, **kw)
+    for rows in (slice(0, 3), slice(n + 3, None)):
+        assert not out[rows].any() and (lse[rows] == -math.inf).all()
+    batch.q_start.sub_(3)
+    check(out[3:n + 3], lse[3:n + 3], restate(q[3:n + 3], k, v, batch), dtype, k.dtype)
+    assert (res[:, :dim] == 7).all() and (res[:, 9 * dim:] == 7).all()
+
+
+def test_a_replayed_step_with_fewer_tokens_clears_the_rest(cuda):
+    q, k, v, batch = make([(30, 300), (70, 500)], dim=128)
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    paged.attention(q, k, v, batch, out=out, workspace=ws)
+    with torch.cuda.graph(graph):
+        paged.attention(q, k, v, batch, out=out, workspace=ws)
+    graph.replay()
+    batch.q_start[-1] -= 45
+    graph.replay()
+    assert paged.status(ws) == 0 and not out[55:].any()
+    want = restate(q, k, v, batch)
+    check(out[:55], None, (want[0][:55], want[1][:55], *want[2:]), F16, F16)

@@ -447,6 +447,28 @@ __device__ __forceinline__ void join_marked(const PagedArgs& A, const PagedPlan&
     }
 }
 
+// Rows of tokens that no sequence owns, as of rows that see nothing: [0, lo) and [hi, n_tokens), by
+// the CTAs of the first row.
+struct Owned {
+    int lo, hi;
+    __device__ __forceinline__ explicit Owned(const PagedArgs& A) {
+        lo = min(max(A.q_start[0], 0), A.n_tokens);
+        hi = min(max(A.q_start[A.n_seq], lo), A.n_tokens);
+    }
+};
+template <bool SPLIT>
+__device__ __forceinline__ void clear_rest(const PagedArgs& A, const Owned& own) {
+    const int rest = A.n_tokens - (own.hi - own.lo), size = SPLIT ? 4 : 2;
+    for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+        const size_t t = i < own.lo ? i : own.hi + (i - own.lo);
+        uint4* row = reinterpret_cast<uint4*>(static_cast<char*>(A.out) + t * A.out_stride * size);
+        for (int d = threadIdx.x; d < A.nh * A.hd * size / 16; d += kJoinThreads)
+            row[d] = make_uint4(0, 0, 0, 0);
+        for (int h = threadIdx.x; A.lse && h < A.nh; h += kJoinThreads)
+            A.lse[t * A.nh + h] = -INFINITY;
+    }
+}
+
 // Items of few rows, usually in many pieces: two rows a CTA, four warps per row take every fourth
 // piece, in batches whose loads are in flight together, and meet in shared memory in their order.
 template <typename T, bool SPLIT, int VECS>
@@ -459,7 +481,9 @@ paged_join_kernel(const __grid_constant__ PagedArgs A, int which) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
     const JoinPlace at(A, P);
+    const Owned own(A);
     const PagedSplit sp = P.split[at.piece];
+    if (blockIdx.y == 0) clear_rest<SPLIT>(A, own);
     if (P.redo && blockIdx.y == 0) join_marked<T, SPLIT>(A, P, sp, at);
     const int n_rows = sp.n_rows / P.gpb * at.gpb;  // (counted with full blocks of heads)
     if ((int)blockIdx.y * kRows >= n_rows) return;
@@ -486,7 +510,9 @@ paged_join_rows_kernel(const __grid_constant__ PagedArgs A, int which) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
     const JoinPlace at(A, P);
+    const Owned own(A);
     const PagedSplit sp = P.split[at.piece];
+    if (blockIdx.y == 0) clear_rest<SPLIT>(A, own);
     if (P.redo && blockIdx.y == 0) join_marked<T, SPLIT>(A, P, sp, at);
     const int n_rows = sp.n_rows / P.gpb * at.gpb, quads = A.hd / 4;
     const int e0 = blockIdx.y * (kJoinRows * kJoinThreads) + threadIdx.x;
@@ -571,11 +597,11 @@ paged_join2_kernel(const __grid_constant__ PagedArgs A) {
     if (blockIdx.x == 0 && blockIdx.y == 0) gather_status(A);
     const int t = blockIdx.x, warp = threadIdx.x / 32 % kWarps;
     const int h = blockIdx.y * kRows + threadIdx.x / 32 / kWarps;
-    if (t < A.q_start[0] || t >= A.q_start[A.n_seq]) return;  // nobody's token
+    const bool owned = t >= A.q_start[0] && t < A.q_start[A.n_seq];  // (else: zeros)
     Joined<VECS> J;
     J.init();
     bool redo = false;
-    if (h < A.nh) {
+    if (h < A.nh && owned) {
         PagedWhere w[2] = {A.plan[A.plan[PLAN_FEW].used ? PLAN_FEW : PLAN_MANY].where[t],
                            A.plan[PLAN_PREFIX].where[t]};
         const int kvh = h / A.group, hg = h - kvh * A.group;
