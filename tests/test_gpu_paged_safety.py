@@ -174,3 +174,15 @@ def test_a_replayed_step_with_fewer_tokens_clears_the_rest(cuda):
     assert paged.status(ws) == 0 and not out[55:].any()
     want = restate(q, k, v, batch)
     check(out[:55], None, (want[0][:55], want[1][:55], *want[2:]), F16, F16)
+
+
+def test_a_call_without_tokens_has_a_status_of_its_own(cuda):
+    q, k, v, batch = make([(1, 300), (70, 200)])
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    batch.table[0, 3] = -1
+    paged.attention(q, k, v, batch, workspace=ws)
+    assert paged.status(ws) == 1
+    none = paged.TokenBatch(batch.q_start[:1], batch.kv_len[:0], batch.table[:0], 0)
+    paged.attention(q[:0], k, v, none, workspace=ws)
+    assert paged.status(ws) == 0
+    paged.attention(q[:0], k, v, none, workspace=ws[:0])

@@ -513,7 +513,10 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
                          void* ws, size_t ws_bytes, cudaStream_t s, WispErrCtx* err) {
     WispError rc;
     if ((rc = check_pages(who, P, err)) || (rc = check_batch(who, B, err))) return rc;
-    if (B->n_tokens == 0) return WISP_OK;
+    if (B->n_tokens == 0) {  // nothing can go wrong: the status word says so
+        if (ws && al16(ws) && ws_bytes >= 4) WB_CUDA_RET(cudaMemsetAsync(ws, 0, 4, s), err);
+        return WISP_OK;
+    }
     if ((rc = check_rows(who, "q", q, P->head_dim, err)) ||
         (rc = check_rows(who, "out", out, P->head_dim, err)))
         return rc;
