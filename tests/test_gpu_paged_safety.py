@@ -186,3 +186,25 @@ def test_a_call_without_tokens_has_a_status_of_its_own(cuda):
     paged.attention(q[:0], k, v, none, workspace=ws)
     assert paged.status(ws) == 0
     paged.attention(q[:0], k, v, none, workspace=ws[:0])
+
+
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (128, 200), (128, 3), (256, 40)])
+@pytest.mark.parametrize("seen_inf", [False, True])
+def test_positions_of_a_bad_page_read_as_zeros(cuda, dim, tokens, seen_inf):
+    """The same for every kernel, and where a visible infinity has an item worked out again."""
+    q, k, v, batch = make([(tokens, 700), (tokens, 333)], dim=dim)
+    page = k.shape[1]
+    k[-1], v[-1] = 0, 0
+    spare = k.shape[0] - 1
+    if (batch.table == spare).any():
+        batch.table[batch.table == spare] = batch.table[0, 0].clone()
+    if seen_inf:
+        v[batch.table[0, 690 // page], 690 % page, 0, 3] = math.inf
+    zeros = batch.table.clone()
+    zeros[0, 3] = zeros[1, 1] = spare
+    want = restate(q, k, v, paged.TokenBatch(batch.q_start, batch.kv_len, zeros, batch.max_q))
+    batch.table[0, 3], batch.table[1, 1] = -1, 1 << 30
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    out, lse = paged.attention(q, k, v, batch, return_lse=True, workspace=ws)
+    assert paged.status(ws) == 1
+    check(out, lse, want, F16, F16)

@@ -657,8 +657,8 @@ struct Joined {
             if (j >= sinks && j < lo) j = lo;
             const int p = A.page_shift >= 0 ? j >> A.page_shift : j / A.page_size;
             const int page = A.table[(size_t)s * A.table_stride + p];
-            if ((unsigned)page >= (unsigned)A.n_pages) continue;
-            const size_t row = (size_t)page * A.page_stride +
+            const bool in = (unsigned)page < (unsigned)A.n_pages;  // (else: zeros)
+            const size_t row = (size_t)(in ? page : 0) * A.page_stride +
                                ((size_t)(j - p * A.page_size) * A.nkv + kvh) * A.hd;
             float dot = 0.f;
             float2 v[VECS];
@@ -666,7 +666,7 @@ struct Joined {
             for (int i = 0; i < VECS; ++i) {
                 const int d = (i * 32 + lane) * 2;
                 v[i] = make_float2(0.f, 0.f);
-                if (d >= A.hd) continue;
+                if (d >= A.hd || !in) continue;
                 const float2 k = PMath<T>::unpack(*reinterpret_cast<const uint32_t*>(
                     reinterpret_cast<const T*>(A.k) + row + d));
                 v[i] = PMath<T>::unpack(*reinterpret_cast<const uint32_t*>(
