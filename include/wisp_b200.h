@@ -551,7 +551,7 @@ WispError wisp_rope_append(const WispRows* q, const WispRows* k, const WispRows*
  * A row that sees nothing gets zeros and lse -infinity.  What a row does not
  * see never reaches it, infinities and NaNs included.  q and out: fp32 (products
  * to fp32 precision: the rows and weights are split into two 16-bit parts), or
- * the pages' dtype; q.n_heads a multiple of n_kv_heads.
+ * the pages' dtype; out must not overlap q; q.n_heads a multiple of n_kv_heads.
  * wisp_prefix_attention: groups of consecutive sequences
  * [groups[g], groups[g + 1]) whose first prefix_len[g] positions lie in the
  * same pages: these are read once for all rows of the group (through the table

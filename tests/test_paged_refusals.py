@@ -1,0 +1,45 @@
+"""Arguments of the paged cache's calls that are refused before any GPU work (no GPU)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from wisp_b200 import paged
+from wisp_b200.lib import WispErrCtx, WispKvPages, WispRows, WispTokenBatch, lib
+
+
+def attention(q, out, tokens=7, **batch):
+    """The refusal of a call without a workspace, which is looked at last."""
+    P = WispKvPages(1024, 2048, 16 * 2 * 64, 4, 16, 2, 64, 1)
+    B = WispTokenBatch(**dict(dict(q_start=64, kv_len=64, table=64, n_seq=2, n_tokens=tokens, max_q=7,
+                                   table_stride=4), **batch))
+    err = WispErrCtx()
+    rc = lib().wisp_paged_attention(C.byref(q), C.byref(out), None, C.byref(P), C.byref(B),
+                                    C.c_float(0.1), 0, 0, None, 0, None, C.byref(err))
+    assert rc == 4
+    return err.message.decode()
+
+
+ROW = 8 * 64  # elements of a row of 8 heads
+
+
+@pytest.mark.parametrize("at,stride,tokens,over", [
+    (0, ROW, 7, True), (ROW, ROW, 7, True), (6 * ROW, ROW, 7, True), (7 * ROW, ROW, 7, False),
+    (-7 * ROW, ROW, 7, False), (-7 * ROW + 8, ROW, 7, True), (0, ROW, 1, True), (ROW, ROW, 1, False),
+    (ROW, 2 * ROW, 7, True)])
+def test_out_must_not_overlap_q(built_lib, at, stride, tokens, over):
+    base = 1 << 20
+    msg = attention(WispRows(base, ROW, 8, 1), WispRows(base + 2 * at, stride, 8, 1), tokens)
+    assert ("overlap" if over else "workspace") in msg, msg
+
+
+@pytest.mark.parametrize("at,width,out_stride,over", [
+    (ROW, 3 * ROW, 3 * ROW, False), (2 * ROW, 3 * ROW, 3 * ROW, False), (ROW - 8, 3 * ROW, 3 * ROW, True),
+    (2 * ROW + 8, 3 * ROW, 3 * ROW, True), (ROW, 2 * ROW, 4 * ROW, False), (ROW, 4 * ROW, 2 * ROW, False),
+    (ROW, 2 * ROW, 3 * ROW, True)])
+def test_out_and_q_may_lie_beside_each_other(built_lib, at, width, out_stride, over):
+    """Columns of one buffer of rows (a fused projection), and rows between rows."""
+    base = 1 << 20
+    msg = attention(WispRows(base, width, 8, 1), WispRows(base + 2 * at, out_stride, 8, 1))
+    assert ("overlap" if over else "workspace") in msg, msg

@@ -362,6 +362,21 @@ WispError check_rows(const char* who, const char* name, const WispRows* R, int h
     return WISP_OK;
 }
 
+// Do the rows of n tokens (the same number of heads and dtype) share memory?
+bool overlap(const WispRows& a, const WispRows& b, int n, int hd) {
+    const long long size = a.dtype == WISP_DTYPE_F32 ? 4 : 2, w = (long long)a.n_heads * hd * size;
+    const long long sa = (long long)a.stride * size, sb = (long long)b.stride * size;
+    const long long d = static_cast<char*>(b.base) - static_cast<char*>(a.base);
+    if (d >= (n - 1) * sa + w || -d >= (n - 1) * sb + w) return false;
+    for (long long t = 0; t < n; ++t) {
+        // the first row of b that ends behind the begin of row t of a
+        const long long gap = t * sa - d - w;
+        const long long u = gap < 0 ? 0 : gap / sb + 1;
+        if (u < n && d + u * sb < t * sa + w) return true;
+    }
+    return false;
+}
+
 // ------------------------------------------------------------------------
 // Attention: what runs, and its workspace
 // ------------------------------------------------------------------------
@@ -526,6 +541,8 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     if (q->n_heads != out->n_heads || q->n_heads % P->n_kv_heads)
         PG_REFUSE("%s: %d heads of q, %d of out (a multiple of the %d kv heads, both the same)", who,
                   q->n_heads, out->n_heads, P->n_kv_heads);
+    if (overlap(*q, *out, B->n_tokens, P->head_dim))
+        PG_REFUSE("%s: out overlaps q, whose rows may be read again behind the results", who);
     if (!(fabsf(scale) <= 3e38f) || window < 0 || sinks < 0)
         PG_REFUSE("%s: scale %g, window %d, sinks %d (finite; not negative)", who, (double)scale,
                   window, sinks);

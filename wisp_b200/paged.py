@@ -125,7 +125,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bat
     token i sees position j when i - j < window or j < ``sinks``.  ``scale`` defaults to
     dim ** -0.5.  ``return_lse``: also the rows' log-sum-exp, fp32 ``[T, heads]`` (-inf for a row
     that sees nothing; its result is zero).  ``workspace``: uint8, at least
-    ``workspace_bytes``; by default taken from torch's allocator for the call."""
+    ``workspace_bytes``; by default taken from torch's allocator for the call.  ``out`` must not
+    overlap q."""
     return (_binding or _torch()).attend(
         q, k_pages, v_pages, batch, None, None, out, scale, window, sinks, return_lse, workspace)
 
