@@ -43,3 +43,28 @@ def test_out_and_q_may_lie_beside_each_other(built_lib, at, width, out_stride, o
     base = 1 << 20
     msg = attention(WispRows(base, width, 8, 1), WispRows(base + 2 * at, out_stride, 8, 1))
     assert ("overlap" if over else "workspace") in msg, msg
+
+
+# ------------------------------------------------------------------------ gradients
+def test_pages_that_ask_for_a_gradient_are_refused():
+    plain = torch.zeros(4, 16, 2, 64, dtype=torch.float16)
+    asks = plain.clone().requires_grad_()
+    q = torch.zeros(2, 8, 64, dtype=torch.float16)
+    for k, v, name in ((asks, plain, "k_pages"), (plain, asks, "v_pages")):
+        for call in (lambda: paged.attention(q, k, v, None), lambda: paged.copy_pages(k, v, [0], [1])):
+            with pytest.raises(ValueError, match=name + " asks for a gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+                call()
+
+
+def test_forward_mode_tangents_are_refused():
+    plain = torch.zeros(4, 16, 2, 64, dtype=torch.float16)
+    q = torch.zeros(2, 8, 64, dtype=torch.float16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(plain, torch.ones_like(plain))
+        for k, v, name in ((dual, plain, "k_pages"), (plain, dual, "v_pages")):
+            with torch.no_grad(), pytest.raises(ValueError, match=name + " has a forward-mode tangent"):
+                paged.attention(q, k, v, None)
+    with pytest.raises(ValueError, match="CUDA device"):
+        paged.attention(q, plain, plain, None)

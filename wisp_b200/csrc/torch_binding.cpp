@@ -69,11 +69,21 @@ const int* ints(const at::Tensor& t, const char* name, int dim) {
     return static_cast<const int*>(t.data_ptr());
 }
 
+// These calls have no derivative, backward or forward.
+void no_derivative(const at::Tensor& x, const char* name) {
+    if (x.requires_grad() && c10::GradMode::is_enabled())
+        refuse("%s asks for a gradient: these calls have none (use torch.no_grad())", name);
+    if (x._fw_grad(/*level=*/0).defined())
+        refuse("%s has a forward-mode tangent: these calls have none", name);
+}
+
 WispKvPages pages(const at::Tensor& k, const at::Tensor& v, int dim0) {
     if (k.dim() != dim0 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() ||
         k.strides() != v.strides())
         refuse("k_pages and v_pages: two [%sn_pages, page_size, n_kv_heads, head_dim] tensors of one "
                "shape, layout and dtype are wanted", dim0 == 5 ? "n_layers, " : "");
+    no_derivative(k, "k_pages");
+    no_derivative(v, "v_pages");
     const int o = dim0 - 4;
     const int64_t n = k.size(o), page = k.size(o + 1), heads = k.size(o + 2), dim = k.size(o + 3);
     const bool one = page > 0 && heads > 0 && dim > 0;
@@ -104,8 +114,7 @@ WispRows rows(const at::Tensor& x, const char* name, int64_t n, int64_t dim, con
     if (x.stride(2) != 1 || (heads > 1 && x.stride(1) != dim))
         refuse("%s: a row's heads must be contiguous", name);
     if (x.device() != dev) refuse("%s is not on the pages' device", name);
-    if (x.requires_grad() && c10::GradMode::is_enabled())
-        refuse("%s asks for a gradient: these calls have none (use torch.no_grad())", name);
+    no_derivative(x, name);
     if (heads > 65535) refuse("%s: %lld heads", name, (long long)heads);
     WispRows R;
     R.base = x.data_ptr();
