@@ -510,6 +510,9 @@ typedef struct WispTokenBatch {
     const int* table;   /* [n_seq][table_width], rows table_stride apart */
     int n_seq, n_tokens, max_q, table_stride;
     int table_width; /* pages in a row of the table (0: table_stride) */
+    /* device word that gets the status bits of the batch's attention calls
+     * OR-ed in (those of a call's workspace, below), or NULL */
+    int* status;
 } WispTokenBatch;
 
 /* Rows of the batch's tokens: token t's head h starts at base + t * stride +

@@ -208,3 +208,48 @@ def test_positions_of_a_bad_page_read_as_zeros(cuda, dim, tokens, seen_inf):
     out, lse = paged.attention(q, k, v, batch, return_lse=True, workspace=ws)
     assert paged.status(ws) == 1
     check(out, lse, want, F16, F16)
+
+
+# ------------------------------------------------------------------------ failures that are seen
+@pytest.mark.parametrize("lens,dim", [([(1, 300), (1, 40)], 64), ([(70, 300), (1, 200)], 128),
+                                      ([(40, 300)], 256)])
+def test_a_status_word_collects_the_bits_of_calls(cuda, lens, dim):
+    q, k, v, batch = make(lens, dim=dim)
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.attention(q, k, v, batch, status=word)
+    groups = dict(groups=torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+                  prefix_len=torch.tensor([16], dtype=torch.int32, device="cuda"))
+    paged.prefix_attention(q, k, v, batch, status=word, **groups)
+    assert word.item() == 0
+    keep = batch.table[0, 3].clone()
+    batch.table[0, 3] = -1
+    paged.prefix_attention(q, k, v, batch, status=word, **groups)
+    assert word.item() == 1
+    batch.table[0, 3] = keep
+    batch.kv_len[0] = 1 << 20
+    paged.attention(q, k, v, batch, status=word)
+    assert word.item() == 3
+    for bad in (word.long(), word.cpu(), torch.zeros(2, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError, match="status"):
+            paged.attention(q, k, v, batch, status=bad)
+
+
+def test_a_step_over_a_bad_page_raises(model, monkeypatch):  # noqa: F811
+    dec, fresh = decoder(model), decoder(model)
+    p = prompt(50, 31)
+    a, b = dec.open(), fresh.open()
+    dec.step([(a, p[:30])])
+    fresh.step([(b, p[:30])])
+    real = dec.pool.table
+
+    def table(*args, **kw):
+        t = real(*args, **kw)
+        t[0, 1] = 1 << 20
+        return t
+
+    with monkeypatch.context() as m:
+        m.setattr(dec.pool, "table", table)
+        with pytest.raises(RuntimeError, match="page number outside the pool"):
+            dec.step([(a, p[30:])])
+    assert dec.pool.length(a) == 30
+    close(dec.step([(a, p[30:])]), fresh.step([(b, p[30:])]))

@@ -120,7 +120,10 @@ class BatchDecoder:
 
     # ------------------------------------------------------------------ one step
     def step(self, batch: list[tuple[int, list[int]]]) -> torch.Tensor:
-        """Append each sequence's tokens; logits fp32 ``[len(batch), vocab]`` of the last ones."""
+        """Append each sequence's tokens; logits fp32 ``[len(batch), vocab]`` of the last ones.
+
+        Waits for the step, and raises where a kernel reported a failure; the sequences are then as
+        they were before."""
         if not batch or any(not t for _, t in batch) or len({s for s, _ in batch}) != len(batch):
             raise ValueError("step: each sequence once, with one token or more")
         tokens = [index(t) for _, ts in batch for t in ts]
@@ -154,24 +157,31 @@ class BatchDecoder:
             prefix = [torch.tensor(x, dtype=torch.int32, device=dev) for x in (groups, shared)]
         x = self.embed[torch.tensor(tokens, device=dev)].float()
         T, nh, nkv, d = x.shape[0], self.nh, self.nkv, self.dim
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
         for l, w in enumerate(self.layers):
             rows = rmsnorm(x, w.input_norm, self.eps).half() @ self._qkv[l].T
             q, k, v = (rows[:, a * d:b * d].unflatten(1, (b - a, d)) for a, b in
                        ((0, nh), (nh, nh + nkv), (nh + nkv, nh + 2 * nkv)))
-            q = paged.rope_append(q, k, v, self.k[l], self.v[l], tb, self.freq, gain=self.gain)
+            q = paged.rope_append(q, k, v, self.k[l], self.v[l], tb, self.freq, gain=self.gain,
+                                  status=status)
             if prefix:
                 a = paged.prefix_attention(q, self.k[l], self.v[l], tb, *prefix,
-                                           window=self.window, sinks=self.sinks)
+                                           window=self.window, sinks=self.sinks, status=status)
             else:
                 a = paged.attention(q, self.k[l], self.v[l], tb, window=self.window,
-                                    sinks=self.sinks)
+                                    sinks=self.sinks, status=status)
             x += (a.reshape(T, nh * d) @ w.o_proj.T).float()
             if T < self.PREFILL_TOKENS:
                 self.stack.stack(x, layers=1, layer0=l)
             else:
                 x += self.stack.prefill(l, rmsnorm(x, self.stack.layers[l].norm, self.eps))
         last = x[starts[1:].long() - 1]
-        return (rmsnorm(last, self.final_norm, self.eps).half() @ self.lm_head.T).float()
+        logits = (rmsnorm(last, self.final_norm, self.eps).half() @ self.lm_head.T).float()
+        if bad := status.item():
+            raise RuntimeError("step: " + ", ".join(m for b, m in (
+                (1, "a page number outside the pool"), (2, "a length beyond the page table"),
+                (8, "a wait ran out (paged.wait_limit)")) if bad & b))
+        return logits
 
     def generate(self, seqs: list[int], logits: torch.Tensor, n: int) -> list[list[int]]:
         """``n`` greedy tokens of each sequence, from the logits of its last step on."""

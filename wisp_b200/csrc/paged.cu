@@ -506,6 +506,7 @@ PagedArgs attention_args(const WispKvPages* P, const WispTokenBatch* B, int n_he
     A.q_start = B->q_start;
     A.kv_len = B->kv_len;
     A.table = B->table;
+    A.all_status = B->status;
     A.page_stride = P->page_stride;
     A.n_seq = B->n_seq;
     A.n_tokens = B->n_tokens;

@@ -94,6 +94,7 @@ struct PagedArgs {
     float* full_o;          // prefix mode: [own, shared][n_tokens * n_heads][hd], whole items
     float* full_ml;  // the same [2]: M and the sum of weights 2^(score - M), score in log2 units
     int* status;
+    int* all_status;  // the caller's word, or NULL
     size_t q_stride, out_stride, page_stride;
     int n_seq, n_tokens, n_groups, table_stride, table_width, n_pages, page_size, page_shift;
     int nh, nkv, group, hd, window, sinks;

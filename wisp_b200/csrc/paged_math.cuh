@@ -431,7 +431,10 @@ __device__ __forceinline__ void gather_status(const PagedArgs& A) {
     const int any = __syncthreads_or(bits & PG_BAD_PAGE) ? PG_BAD_PAGE : 0;
     const int len = __syncthreads_or(bits & PG_BAD_LENGTH) ? PG_BAD_LENGTH : 0;
     const int late = __syncthreads_or(bits & PG_TIMEOUT) ? PG_TIMEOUT : 0;
-    if (threadIdx.x == 0) *A.status = any | len | late;
+    if (threadIdx.x == 0) {
+        *A.status = any | len | late;
+        if (A.all_status && (any | len | late)) atomicOr(A.all_status, any | len | late);
+    }
 }
 
 // A KV tile of the item is 2^item_shift units.

@@ -128,7 +128,7 @@ WispRows rows(const at::Tensor& x, const char* name, int64_t n, int64_t dim, con
 WispTokenBatch batch_parts(PyObject* const* a, int64_t n_tokens, at::Device* dev) {
     const at::Tensor &qs = tensor(a[0], "q_start"), &kl = tensor(a[1], "kv_len"),
                      &tb = tensor(a[2], "table");
-    WispTokenBatch B;
+    WispTokenBatch B{};
     B.q_start = ints(qs, "q_start", 1);
     B.kv_len = ints(kl, "kv_len", 1);
     B.table = ints(tb, "table", 2);
@@ -166,6 +166,15 @@ WispTokenBatch batch_of(PyObject* batch, int64_t n_tokens, at::Device* dev) {
     for (int i = 0; i < 4; ++i)
         if (!(a[i] = PyObject_GetAttr(batch, g_names[i]))) throw Refused();
     return batch_parts(a, n_tokens, dev);
+}
+
+int* status_word(PyObject* o, const at::Device& dev) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor& w = tensor(o, "status");
+    const int* p = ints(w, "status", 1);
+    if (w.size(0) != 1 || w.device() != dev)
+        refuse("status: one int32 value on the pages' device is wanted");
+    return const_cast<int*>(p);
 }
 
 cudaStream_t stream_on(const at::Device& dev) {
@@ -234,9 +243,9 @@ PyObject* workspace_bytes(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 }
 
 // attend(q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks, return_lse,
-//        workspace)
+//        workspace, status)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-    WANT_ARGS("attend", 12)
+    WANT_ARGS("attend", 13)
     return guarded([&]() -> PyObject* {
         const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_pages"),
                          &v = tensor(a[2], "v_pages");
@@ -245,8 +254,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         const int64_t T = q.dim() ? q.size(0) : 0;
         const WispRows rq = rows(q, "q", T, P.head_dim, dev);
         at::Device bdev(at::kCUDA);
-        const WispTokenBatch B = batch_of(a[3], T, &bdev);
+        WispTokenBatch B = batch_of(a[3], T, &bdev);
         if (bdev != dev) refuse("the batch is not on the pages' device");
+        B.status = status_word(a[12], dev);
         const cudaStream_t s = stream_on(dev);
         int n_groups = 0;
         const int *groups = nullptr, *prefix = nullptr;
@@ -337,19 +347,13 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         const double gain = PyFloat_AsDouble(a[10]);
         if (R.interleaved < 0 || (gain == -1.0 && PyErr_Occurred())) throw Refused();
         R.gain = (float)gain;
-        int* status = nullptr;
         if (a[11] != Py_None) {
             const at::Tensor& p = tensor(a[11], "positions");
             R.positions = ints(p, "positions", 1);
             if (p.size(0) != T || p.device() != dev)
                 refuse("positions: %lld int32 values on the pages' device are wanted", (long long)T);
         }
-        if (a[12] != Py_None) {
-            const at::Tensor& w = tensor(a[12], "status");
-            status = const_cast<int*>(ints(w, "status", 1));
-            if (w.size(0) != 1 || w.device() != dev)
-                refuse("status: one int32 value on the pages' device is wanted");
-        }
+        int* status = status_word(a[12], dev);
         WispErrCtx err{};
         checked(p_rope(&rq, &rk, &rv, &ro, &P, &B, &R, status, s, &err), err);
         return THPVariable_Wrap(out);

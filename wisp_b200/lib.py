@@ -47,7 +47,7 @@ class WispKvPages(C.Structure):
 class WispTokenBatch(C.Structure):
     _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p),
                 ("n_seq", C.c_int), ("n_tokens", C.c_int), ("max_q", C.c_int),
-                ("table_stride", C.c_int), ("table_width", C.c_int)]
+                ("table_stride", C.c_int), ("table_width", C.c_int), ("status", C.c_void_p)]
 
 
 class WispRows(C.Structure):

@@ -118,7 +118,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, batch: TokenBatch, *,
               out: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
-              sinks: int = 0, return_lse: bool = False, workspace: torch.Tensor | None = None):
+              sinks: int = 0, return_lse: bool = False, workspace: torch.Tensor | None = None,
+              status: torch.Tensor | None = None):
     """Causal attention of the batch's tokens over their sequences' cached positions.
 
     q ``[T, heads, dim]`` in fp32 or the pages' dtype; the result has q's dtype.  ``window`` > 0:
@@ -126,21 +127,25 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bat
     dim ** -0.5.  ``return_lse``: also the rows' log-sum-exp, fp32 ``[T, heads]`` (-inf for a row
     that sees nothing; its result is zero).  ``workspace``: uint8, at least
     ``workspace_bytes``; by default taken from torch's allocator for the call.  ``out`` must not
-    overlap q."""
+    overlap q.  ``status``: an int32 word that gets the bits of ``paged.status`` OR-ed in; without it
+    (and without a workspace to ask) a bad page, a cut length or a wait that ran out stays unseen."""
     return (_binding or _torch()).attend(
-        q, k_pages, v_pages, batch, None, None, out, scale, window, sinks, return_lse, workspace)
+        q, k_pages, v_pages, batch, None, None, out, scale, window, sinks, return_lse, workspace,
+        status)
 
 
 def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                      batch: TokenBatch, groups: torch.Tensor, prefix_len: torch.Tensor, *,
                      out: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
                      sinks: int = 0, return_lse: bool = False,
-                     workspace: torch.Tensor | None = None):
+                     workspace: torch.Tensor | None = None,
+                     status: torch.Tensor | None = None):
     """``attention`` for sequences that share prefixes: the sequences ``groups[g]`` to
     ``groups[g + 1]`` hold their first ``prefix_len[g]`` positions in the same pages, which are
     read once for all of the group.  Both int32 on the device."""
     return (_binding or _torch()).attend(
-        q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks, return_lse, workspace)
+        q, k_pages, v_pages, batch, groups, prefix_len, out, scale, window, sinks, return_lse,
+        workspace, status)
 
 
 def workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
