@@ -70,3 +70,8 @@ def test_an_interrupted_step_keeps_a_fork_apart(built_lib, monkeypatch):
 def test_shapes_that_the_operators_refuse_are_refused_at_once(built_lib, kw, msg):
     with pytest.raises(ValueError, match=msg):
         decoder(**kw)
+
+
+def test_rows_of_other_types_are_refused(built_lib):
+    with pytest.raises(ValueError, match="rows of torch.bfloat16"):
+        decoder(rows=torch.bfloat16)

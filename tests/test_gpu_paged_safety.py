@@ -253,3 +253,28 @@ def test_a_step_over_a_bad_page_raises(model, monkeypatch):  # noqa: F811
             dec.step([(a, p[30:])])
     assert dec.pool.length(a) == 30
     close(dec.step([(a, p[30:])]), fresh.step([(b, p[30:])]))
+
+
+# ------------------------------------------------------------------------ bits kept by the decoder
+def test_logits_are_the_products_in_fp32(model, monkeypatch):  # noqa: F811
+    """Products of 16-bit values are exact in fp32 and summed there: 2^-20 of the sum of sizes."""
+    from wisp_b200 import batch_decoder
+    dec, seen = decoder(model), []
+    real = batch_decoder.rmsnorm
+    monkeypatch.setattr(batch_decoder, "rmsnorm", lambda *a: seen.append(real(*a)) or seen[-1])
+    got = dec.step([(dec.open(), prompt(30, 41)), (dec.open(), prompt(5, 42))]).double()
+    y, w = seen[-1].half().double(), dec.lm_head.double()
+    assert ((got - y @ w.T).abs() <= 2.0 ** -20 * (y.abs() @ w.abs().T)).all()
+
+
+def test_fp32_rows_stay_near_the_one_sequence_step(model):  # noqa: F811
+    """What is left is the rounding of the products' inputs: three in each of two layers and one in
+    front of the logits, and the weights' own precision; eight times 2^-11."""
+    from test_gpu_batch_decoder import one_by_one
+    p, q = prompt(150, 51), prompt(33, 52)
+    dec = decoder(model, rows=torch.float32)
+    a, b = dec.open(), dec.open()
+    dec.step([(a, p[:100]), (b, q[:32])])
+    got = dec.step([(a, p[100:]), (b, q[32:])])
+    want = torch.stack((one_by_one(model, p)[-1], one_by_one(model, q)[-1]))
+    assert (got - want).norm() <= 8 * 2.0 ** -11 * want.norm()

@@ -13,6 +13,11 @@ prompt, a chunk, a single token each, in one batch) through
 Sequences share pages: ``fork`` continues one sequence in several ways, and a step whose
 neighbouring sequences begin with the same pages reads those once (``prefix_attention``).  The
 projections are plain fp16 matrix products; everything else runs in this library's kernels.
+
+The one-sequence step keeps 32 bits everywhere but in the cache.  Here the inputs of the matrix
+products are rounded to fp16, the weights' type, so that they run on the tensor cores; their sums,
+the residual and the logits are fp32.  q, k, v and the attention rows are fp16 by default, which is
+what prompts are fast in; ``rows=torch.float32`` keeps them in fp32.
 """
 
 from __future__ import annotations
@@ -52,7 +57,7 @@ class BatchDecoder:
                  final_norm: torch.Tensor | None, lm_head: torch.Tensor, n_heads: int,
                  n_kv_heads: int, *, theta: float = 10000.0, scaling: str | None = None,
                  factor: float = 1.0, n_pages: int = 1024, page_size: int = 16, window: int = 0,
-                 sinks: int = 0):
+                 sinks: int = 0, rows: torch.dtype = torch.float16):
         if len(layers) != stack.L:
             raise ValueError(f"{len(layers)} attention layers for a stack of {stack.L}")
         H = stack.shape.hidden
@@ -63,6 +68,9 @@ class BatchDecoder:
         if dim % 16 or dim > 256 or page_size <= 0 or page_size % 8 or window < 0 or sinks < 0:
             raise ValueError(f"heads of {dim} (a multiple of 16 up to 256), page_size {page_size} (of "
                              f"8), window {window}, sinks {sinks} (not negative)")
+        if rows not in (torch.float16, torch.float32):
+            raise ValueError(f"rows of {rows} (fp16 or fp32)")
+        self.rows = rows
         self.stack, self.embed, self.lm_head, self.final_norm = stack, embed, lm_head, final_norm
         self.nh, self.nkv, self.dim = n_heads, n_kv_heads, dim
         self.window, self.sinks, self.eps = window, sinks, stack.shape.rms_eps
@@ -159,7 +167,8 @@ class BatchDecoder:
         T, nh, nkv, d = x.shape[0], self.nh, self.nkv, self.dim
         status = torch.zeros(1, dtype=torch.int32, device=dev)
         for l, w in enumerate(self.layers):
-            rows = rmsnorm(x, w.input_norm, self.eps).half() @ self._qkv[l].T
+            rows = torch.mm(rmsnorm(x, w.input_norm, self.eps).half(), self._qkv[l].T,
+                            out_dtype=self.rows)
             q, k, v = (rows[:, a * d:b * d].unflatten(1, (b - a, d)) for a, b in
                        ((0, nh), (nh, nh + nkv), (nh + nkv, nh + 2 * nkv)))
             q = paged.rope_append(q, k, v, self.k[l], self.v[l], tb, self.freq, gain=self.gain,
@@ -170,13 +179,14 @@ class BatchDecoder:
             else:
                 a = paged.attention(q, self.k[l], self.v[l], tb, window=self.window,
                                     sinks=self.sinks, status=status)
-            x += (a.reshape(T, nh * d) @ w.o_proj.T).float()
+            x += torch.mm(a.reshape(T, nh * d).half(), w.o_proj.T, out_dtype=torch.float32)
             if T < self.PREFILL_TOKENS:
                 self.stack.stack(x, layers=1, layer0=l)
             else:
                 x += self.stack.prefill(l, rmsnorm(x, self.stack.layers[l].norm, self.eps))
         last = x[starts[1:].long() - 1]
-        logits = (rmsnorm(last, self.final_norm, self.eps).half() @ self.lm_head.T).float()
+        logits = torch.mm(rmsnorm(last, self.final_norm, self.eps).half(), self.lm_head.T,
+                          out_dtype=torch.float32)
         if bad := status.item():
             raise RuntimeError("step: " + ", ".join(m for b, m in (
                 (1, "a page number outside the pool"), (2, "a length beyond the page table"),
