@@ -48,3 +48,11 @@ def test_a_copy_refused_half_way_keeps_the_rest(built_lib, monkeypatch):
     refuse[:] = [False]
     assert p.apply(None, None) == 1 and made == [([0], [1])] * 2
     assert p.apply(None, None) == 0
+
+
+def test_a_pool_that_outlives_the_modules_is_quiet(built_lib, monkeypatch):
+    """At the interpreter's end a pool may go after the names that its module uses."""
+    p = paged.PagePool(4, 8)
+    monkeypatch.setattr(paged, "lib", None)
+    p.__del__()
+    p.__del__()

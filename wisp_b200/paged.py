@@ -192,11 +192,12 @@ class PagePool:
         self._h = lib().wisp_page_pool_create(n_pages, page_size, C.byref(err))
         if not self._h:
             raise WispError(err)
+        self._destroy = lib().wisp_page_pool_destroy  # (`lib` may be gone when the pool goes)
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None
         if h:
-            lib().wisp_page_pool_destroy(h)
+            self._destroy(h)
 
     def _id(self, rc: int, err: WispErrCtx) -> int:
         if rc < 0:
