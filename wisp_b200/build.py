@@ -19,6 +19,8 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -104,28 +106,47 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         lib_stamp.write_text(link_key)
-    binding.result()
+    try:
+        binding.result()
+    except BindingUnavailable as e:  # the C library stands without it
+        warnings.warn(f"built without the torch binding of wisp_b200.paged: {e}", RuntimeWarning)
     return LIB
+
+
+class BindingUnavailable(RuntimeError):
+    """What the torch binding is built against is not installed."""
 
 
 def build_binding(verbose: bool = False) -> Path:
     """``_paged_torch.so`` (host code only), rebuilt when its source, the ABI header, torch or
     the flags change."""
-    import sysconfig
-
-    import torch
-    from torch.utils import cpp_extension
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    src, torch_lib = CSRC / BINDING_SRC, Path(torch.__file__).parent / "lib"
+    src, stamp = CSRC / BINDING_SRC, BINDING.with_suffix(".so.sha256")
+    src_key = hashlib.sha256(src.read_bytes() +
+                             (ROOT / "include" / "wisp_b200.h").read_bytes()).hexdigest()
+
+    def missing(what: str):
+        # (a binding of another source does not fit the library: it must not be loaded)
+        if BINDING.exists() and not (stamp.exists() and stamp.read_text().startswith(src_key + " ")):
+            BINDING.unlink()
+        return BindingUnavailable(what)
+
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError as e:
+        raise missing(f"no torch ({e})") from None
+    torch_lib = Path(torch.__file__).parent / "lib"
     inc = [*cpp_extension.include_paths(device_type="cuda"), sysconfig.get_paths()["include"],
            str(ROOT / "include")]
+    for header in ("Python.h", "ATen/ATen.h"):
+        if not any((Path(i) / header).exists() for i in inc):
+            raise missing(f"no {header}")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{i}" for i in inc), str(src), "-o", str(BINDING), f"-L{torch_lib}",
            f"-Wl,-rpath,{torch_lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    key = hashlib.sha256(src.read_bytes() + (ROOT / "include" / "wisp_b200.h").read_bytes() +
-                         torch.__version__.encode() + " ".join(cmd).encode()).hexdigest()
-    stamp = BINDING.with_suffix(".so.sha256")
+    key = src_key + " " + hashlib.sha256((torch.__version__ + " ".join(cmd)).encode()).hexdigest()
     if BINDING.exists() and stamp.exists() and stamp.read_text() == key:
         return BINDING
     if verbose:
