@@ -68,3 +68,18 @@ def test_forward_mode_tangents_are_refused():
                 paged.attention(q, k, v, None)
     with pytest.raises(ValueError, match="CUDA device"):
         paged.attention(q, plain, plain, None)
+
+
+# ------------------------------------------------------------------------ calls too long for 32 bits
+@pytest.mark.parametrize("tokens,heads,window,long", [
+    (1 << 20, 64, 0, True), (1 << 20, 64, 4096, False), (1 << 20, 8, 0, False), (8192, 64, 0, False),
+    (1 << 22, 64, 1 << 20, True)])
+def test_a_prompt_whose_work_passes_31_bits_is_refused(built_lib, tokens, heads, window, long):
+    """One kv head, a table of 2^20 positions: the row tiles' KV tiles are counted in 32 bits."""
+    P = WispKvPages(1024, 2048, 16 * 64, 1 << 20, 16, 1, 64, 1)
+    B = WispTokenBatch(64, 64, 64, 1, tokens, tokens, 1 << 16, 0)
+    q, out = WispRows(1 << 20, heads * 64, heads, 1), WispRows(1 << 40, heads * 64, heads, 1)
+    err = WispErrCtx()
+    rc = lib().wisp_paged_attention(C.byref(q), C.byref(out), None, C.byref(P), C.byref(B),
+                                    C.c_float(0.1), window, 0, None, 0, None, C.byref(err))
+    assert rc == 4 and ("in one call" if long else "workspace") in err.message.decode(), err.message

@@ -394,6 +394,7 @@ constexpr double kFewBytes = 50e6, kFewBytesWide = 100e6;
 struct AttnShape {
     int rw[PLANS];  // 16-row tiles of the plan's row tiles; 0: the tensor-core kernel
     size_t bytes;
+    double units;  // no plan's line of work is longer
 };
 
 // Fills the geometry, plans and (with a workspace) pointers of a call.
@@ -468,6 +469,12 @@ AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
         P.per_seg = (most_tokens + P.tpt - 1) / P.tpt;
         P.inlined = is_few && (long long)n_seg * P.per_seg <= kPagedInline;
         if (P.inlined) P.max_items = n_seg * P.per_seg;
+        // KV tiles of a row tile: of the positions that a table row holds or, of consecutive tokens
+        // with a window, of the window and the sinks
+        double tiles = (double)A.table_width * A.page_size / kPagedTile + 1;
+        if (A.window > 0 && w != PLAN_PREFIX)
+            tiles = std::min(tiles, ((double)A.window + P.tpt + A.sinks) / kPagedTile + 4);
+        S.units = std::max(S.units, P.max_items * (tiles * P.grain + P.lead));
         P.n_items = reinterpret_cast<int*>(take(4));
         P.bad = reinterpret_cast<int*>(take(((size_t)P.lanes * P.heads + 1) * 4));
         P.item_off = reinterpret_cast<int*>(take((size_t)(n_seg + 1) * 4));
@@ -562,6 +569,9 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     A.scale_log2 = scale * 1.4426950408889634f;
     const AttnShape S = attention_layout(A, q->dtype, std::min(B->max_q, B->n_tokens),
                                          static_cast<char*>(ws));
+    if (S.units >= 2147483648.0)  // (they are counted in 32 bits)
+        PG_REFUSE("%s: up to %.2g KV tiles in one call, the limit is 2^31: fewer tokens at a time or a "
+                  "narrower table", who, S.units);
     if (!ws || !al16(ws) || ws_bytes < S.bytes)
         PG_REFUSE("%s: workspace of %zu bytes, need %zu (16-byte aligned)", who, ws ? ws_bytes : 0,
                   S.bytes);
