@@ -278,3 +278,26 @@ def test_fp32_rows_stay_near_the_one_sequence_step(model):  # noqa: F811
     got = dec.step([(a, p[100:]), (b, q[32:])])
     want = torch.stack((one_by_one(model, p)[-1], one_by_one(model, q)[-1]))
     assert (got - want).norm() <= 8 * 2.0 ** -11 * want.norm()
+
+
+def test_the_status_of_a_call_without_tokens_comes_after_the_call_before_it(cuda):
+    """Both words are written by kernels in the stream's order, captured ones included."""
+    q, k, v, batch = make([(1, 300), (70, 200)])
+    ws = torch.empty(paged.workspace_bytes(q, k, v, batch), dtype=torch.uint8, device="cuda")
+    none = paged.TokenBatch(batch.q_start[:1], batch.kv_len[:0], batch.table[:0], 0)
+    batch.table[0, 3] = -1
+    graph = torch.cuda.CUDAGraph()
+    paged.attention(q, k, v, batch, workspace=ws)
+    with torch.cuda.graph(graph):
+        paged.attention(q, k, v, batch, workspace=ws)
+        paged.attention(q[:0], k, v, none, workspace=ws)
+    for _ in range(20):
+        graph.replay()
+        assert paged.status(ws) == 0
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other):
+        paged.attention(q[:0], k, v, none, workspace=ws)
+        paged.attention(q, k, v, batch, workspace=ws)
+    for _ in range(20):
+        other.replay()
+        assert paged.status(ws) == 1

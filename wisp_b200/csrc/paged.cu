@@ -537,7 +537,8 @@ WispError attention_call(const char* who, const WispRows* q, const WispRows* out
     WispError rc;
     if ((rc = check_pages(who, P, err)) || (rc = check_batch(who, B, err))) return rc;
     if (B->n_tokens == 0) {  // nothing can go wrong: the status word says so
-        if (ws && al16(ws) && ws_bytes >= 4) WB_CUDA_RET(cudaMemsetAsync(ws, 0, 4, s), err);
+        if (ws && al16(ws) && ws_bytes >= 4)
+            WB_CUDA_RET(launch_zero_words(static_cast<int*>(ws), 1, s), err);
         return WISP_OK;
     }
     if ((rc = check_rows(who, "q", q, P->head_dim, err)) ||
