@@ -383,7 +383,7 @@ bool overlap(const WispRows& a, const WispRows& b, int n, int hd) {
 // What a row tile costs before its first KV tile, in KV tiles (a prompt of 8192 tokens took 816 us
 // with 0 and 694 us with 4, later 560 us with 4 and 540 us with 6, where a KV tile took 0.94 us
 // and a beginning 5.4 us; fp32 rows, which are split first: 2048 tokens 280 us with 3, 212 with 6,
-// 179 with 12, 191 with 16, and 3 x 500 tokens behind 4000 116 us with 3 and 118 with 12; 14 single
+// 179 with 12 (205 when measured again), 191 with 16, and 3 x 500 tokens behind 4000 116 us with 3 and 118 with 12; 14 single
 // tokens behind up to 4096 positions 32.6 us with 0 and 30.9 us with 2).
 constexpr int kLeadMma = 6, kLeadMma32 = 12, kLeadFew = 2;
 // Up to so many 16-row tiles stay with paged_few_kernel, where all that they read again (for wide
@@ -405,15 +405,17 @@ struct AttnShape {
 // or four 16-row tiles.  A batch goes by its longest sequence: single tokens beside a prompt
 // take its kernel too (they read the cache at 80% of HBM there instead of 95%; a second pair of
 // launches for them cost 12 us a call).  A few 16-row tiles stay with paged_few_kernel where they are
-// few enough to read the cache again out of L2: it needs no plan kernel before it.  Measured
-// (B200, 8 kv heads; paged_few_kernel against the other):
+// few enough to read the cache again out of L2: it needs no plan kernel before it.  The lengths
+// are not known here, so what a batch reads again is bounded by its table's width: a table wider
+// than its sequences need (a captured step's) leaves this choice early.  Measured with tables as
+// wide as the longest sequence (B200, 8 kv heads; paged_few_kernel against the other):
 //   128 dims, 4 sequences of 1024: 32 rows 19.6 and 22.2 us, 64 rows 25.0 and 20.4 us
 //             2 of 4096: 32 rows 23.2 and 23.1 us, 64 rows 31.1 and 24.5 us
 //             8 of 8192: 32 rows 98 and 67 us
 //     64 rows behind a shared prefix of 2048: 27.5 and 31.4 us, of 8192: 50.2 and 36.9 us
 //   256 dims, 4 of 1024: 32 rows 24.0 and 31.2 us, 128 rows 51 and 59 us
 //             2 of 4096: 32 rows 30.7 and 38.5 us, 128 rows 80 and 92 us
-//             8 of 8192: 32 rows 170 and 153 us, 128 rows 624 and 437 us
+//             8 of 8192: 32 rows 170 and 153 us, 128 rows 624 and 437 to 460 us
 AttnShape attention_layout(PagedArgs& A, int q_dtype, int max_q, char* ws) {
     const bool split = q_dtype == WISP_DTYPE_F32;
     const int per = split ? 8 : 16;

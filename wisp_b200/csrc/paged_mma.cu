@@ -18,7 +18,7 @@
 //   warp 11              loads the rows of Q (TMA where a row tile is whole tokens) as soon as the
 //                        last product that reads the previous ones is done; 32-bit rows, which
 //                        have one row tile, are loaded and split by warps 4-7 (one prompt of 2048
-//                        fp32 tokens 222 us then, 641 us with one warp).  It also looks V of partly
+//                        fp32 tokens 222 us at that step, 641 us with one warp).  It also looks V of partly
 //                        hidden tiles through for infinities and NaNs, for both row tiles: their
 //                        products with V wait for it
 // A row's running maximum is only moved when a score passes it by more than 2^8 (the weights
@@ -29,15 +29,16 @@
 // product each into the same accumulator; one tile of 128 rows then.
 //
 // Hidden values.  A box outside what the tile's rows see is loaded from outside the tensor map
-// (zeros).  In tiles that are partly hidden the softmax warps look V through for infinities and
-// NaNs before the product: those that no row sees are zeroed in shared memory; where some row
-// sees one, the row tile is marked and the join kernel works it out again without tiles.
+// (zeros).  In tiles that are partly hidden V is looked through for infinities and NaNs before
+// the product: those that no row sees are zeroed in shared memory; where some row sees one, the
+// row tile is marked and the join kernel works it out again without tiles.
 //
-// Measured (B200): a prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 540 us = 1.0 PFLOP/s
-// of the visible pairs (60% of the measured bf16 rate), tensor pipe and exponential unit 55% busy
-// each at 1.67 GHz under the power limit; chunks of 7652 tokens behind up to 9000 positions, 16 heads
-// of 64, window 1024, 118 us; four drafted tokens behind 64K to 128K positions, 64
-// heads, 300 us = 6.0 TB/s (93% of the measured copy).  Steps of the prompt: mma.sync row tiles
+// Measured (B200; ranges: the best and the middle of long replays, under the power limit): a prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 515 to 590 us = 1.07 to 0.93
+// PFLOP/s of the visible pairs (63 to 55% of the measured bf16 rate), tensor pipe and exponential
+// unit 56% busy each at 1.66 GHz; chunks of 7652 tokens behind up to 9000 positions, 16 heads of 64,
+// window 1024, 117 us; four drafted tokens behind 64K to 128K positions, 64 heads, 302 to 345 us = 6.0
+// to 5.2 TB/s (92 to 81% of the measured copy); 2048 fp32 tokens 205 us.  Steps of the prompt, at
+// their best: mma.sync row tiles
 // of 64 rows 4.57 ms; this kernel with one thread issuing all products 1.15 ms (it was bound by
 // 80 to 115 cycles an instruction); a warp per row tile with warp-uniform operands 816 us; pieces
 // that count what beginning a row tile costs 694 us; Q by TMA behind the last product 551 us;

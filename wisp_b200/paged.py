@@ -76,8 +76,10 @@ def rope_frequencies(dim: int, theta: float = 10000.0, *, scaling: str | None = 
     ``scaling``: None; ``"linear"`` (every frequency / factor); ``"base"`` (theta raised so
     that the slowest pair is stretched by factor and the fastest kept); ``"by_parts"``: pairs
     that make fewer than ``low`` turns in ``original`` positions are divided by factor, those of
-    more than ``high`` kept, those between blended, and the rows scaled by
-    ``0.1 ln(factor) + 1``."""
+    more than ``high`` kept, those between blended in proportion to their turns, and the rows
+    scaled by ``0.1 ln(factor) + 1``.  Models were also trained with blends that are linear in the
+    pair's index, with other bounds or without the gain: give the operators frequencies and a gain
+    of your own for those."""
     if dim <= 0 or dim % 2 or factor < 1.0 or theta <= 0:
         raise ValueError(f"rope_frequencies: dim {dim} (even), theta {theta}, factor {factor} (>= 1)")
     i = torch.arange(dim // 2, dtype=torch.float64)
