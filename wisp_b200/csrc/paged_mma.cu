@@ -33,11 +33,12 @@
 // the product: those that no row sees are zeroed in shared memory; where some row sees one, the
 // row tile is marked and the join kernel works it out again without tiles.
 //
-// Measured (B200; ranges: the best and the middle of long replays, under the power limit): a prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 515 to 590 us = 1.07 to 0.93
-// PFLOP/s of the visible pairs (63 to 55% of the measured bf16 rate), tensor pipe and exponential
-// unit 56% busy each at 1.66 GHz; chunks of 7652 tokens behind up to 9000 positions, 16 heads of 64,
-// window 1024, 117 us; four drafted tokens behind 64K to 128K positions, 64 heads, 302 to 345 us = 6.0
-// to 5.2 TB/s (92 to 81% of the measured copy); 2048 fp32 tokens 205 us.  Steps of the prompt, at
+// Measured (B200; ranges: the best and the middle of long replays, under the power limit): a
+// prompt of 8192 tokens, 32 heads of 128 over 8 kv heads, 515 to 590 us = 1.07 to 0.93 PFLOP/s of
+// the visible pairs (63 to 55% of the measured bf16 rate), tensor pipe and exponential unit 56%
+// busy each at 1.66 GHz; chunks of 7652 tokens behind up to 9000 positions, 16 heads of 64, window
+// 1024, 117 us; four drafted tokens behind 64K to 128K positions, 64 heads, 302 to 345 us = 6.0 to
+// 5.2 TB/s (92 to 81% of the measured copy); 2048 fp32 tokens 205 us.  Steps of the prompt, at
 // their best: mma.sync row tiles
 // of 64 rows 4.57 ms; this kernel with one thread issuing all products 1.15 ms (it was bound by
 // 80 to 115 cycles an instruction); a warp per row tile with warp-uniform operands 816 us; pieces
