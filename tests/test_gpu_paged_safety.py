@@ -11,7 +11,6 @@ import torch
 from test_gpu_batch_decoder import close, decoder, model, prompt  # noqa: F401 (a fixture)
 from test_gpu_paged import BF16, F16, F32, check, make, restate, run
 from wisp_b200 import paged
-from wisp_b200.lib import WispError
 
 pytestmark = pytest.mark.gpu
 
